@@ -47,6 +47,14 @@ extern "C" {
 #define DH_ERR_SCRATCH_LIMIT 106u
 #define DH_ERR_NCCL 107u
 
+/* Element types of the entry points that take several. */
+#define DH_TYPE_F32 0u
+#define DH_TYPE_BF16 1u
+#define DH_TYPE_F16 2u
+
+/* No token (mask_token_id of the scoring entry points). */
+#define DH_NO_TOKEN 0xFFFFFFFFu
+
 /* RNG family -- same values as RngKernelStatus (philox_rng.hpp:29-33). */
 #define DH_RNG_INVALID_POSITION_COUNT 1u
 #define DH_RNG_INVALID_VOCABULARY_SIZE 2u
@@ -522,6 +530,64 @@ uint32_t dh_output_head_int8(const int8_t* hidden, const int8_t* weights,
                              uint32_t vocabulary_size, uint32_t mask_token_id,
                              uint32_t evaluation_id, uint32_t stream_id, uint32_t seed_low,
                              uint32_t seed_high, uint64_t* workspace, void* stream);
+
+/* ---------------------------------------------------------------- scoring */
+
+/* The W8A8 linear of any width (fixed_mlp.quantized_linear, fixed_mlp.py:65-136):
+ *   out[r, c] = (sum_k a[r, k] w[c, k]) * fp32(a_scale[r] * w_scale[c]) + bias[c]
+ * a [m, k] and w [n, k] int8 rows lda / ldw bytes apart (16-byte aligned, lda
+ * and ldw multiples of 16, k any up to 131,071), a_scale [m], w_scale [n],
+ * bias [n] or NULL fp32; out [m, n] of out_type (DH_TYPE_*), rows ldo >= n
+ * elements apart, aligned to its elements.  fp32 outputs are evaluated in
+ * float64 and rounded once (the reference's values bit for bit, as
+ * dh_head_argmax_i8 computes its logits); 16-bit outputs in fp32 and rounded.
+ * Status: DH_ERR_*. */
+uint32_t dh_gemm_i8_scaled(const int8_t* a, uint64_t lda, const float* a_scale, const int8_t* w, uint64_t ldw,
+                           const float* w_scale, const float* bias, void* out, uint64_t ldo, uint32_t out_type,
+                           uint32_t m, uint32_t n, uint32_t k, void* stream);
+
+/* Scores of rows of logits in one pass: log probabilities of given tokens
+ * under softmax(logits), entropy (nats), logsumexp and the top_k best tokens
+ * (mdlm._mdlm_log_probabilities, mdlm.py:851-858, without the [rows, vocab]
+ * array of them).
+ *   logits        [rows, vocabulary_size] of logits_type (DH_TYPE_*), rows
+ *                 row_stride elements apart, aligned to its elements
+ *   mask_token_id excluded: its logit counts as -inf; DH_NO_TOKEN for none
+ *   targets       int32 (target_bytes 4) or int64 (8) [rows, targets_per_row]
+ *                 token ids, targets_per_row 0 for none; a negative id stands
+ *                 for "no token"
+ *   logprobs      [rows, targets_per_row]: 0 for a negative id, NaN for one
+ *                 past the vocabulary
+ *   entropy, logsumexp [rows], either may be NULL
+ *   top_ids, top_logprobs [rows, top_k], 0 <= top_k <= 32: the tokens of
+ *                 largest logit in descending order, the lower id first among
+ *                 equals; tokens whose logit is -inf are none, and missing
+ *                 entries hold -1 and -inf
+ * A row whose logits are all -inf has logsumexp and logprobs -inf, entropy 0
+ * and no best tokens.  A row with a NaN or +inf (other than the mask token's)
+ * has NaN for all of them and ids -1.  At least one output is asked for.
+ * Status: DH_ERR_*. */
+uint32_t dh_token_logprobs(const void* logits, uint32_t logits_type, uint64_t row_stride, uint32_t rows,
+                           uint32_t vocabulary_size, uint32_t mask_token_id, const void* targets,
+                           uint32_t target_bytes, uint32_t targets_per_row, uint32_t top_k, float* logprobs,
+                           float* entropy, float* logsumexp, int32_t* top_ids, float* top_logprobs, void* stream);
+
+/* The scores of dh_token_logprobs for the logits of an int8 output head,
+ *   x[r, v] = fp32(acc[r, v] * fp32(a_scale[r] * w_scale[v]) + bias[v]),
+ * which never reach memory (mlx_mdlm._FinalLayer, mlx_mdlm.py:456-498, then
+ * mdlm.py:851-858).  hidden [rows, hidden_size] and weights [vocabulary_size,
+ * hidden_size] int8 as in dh_gemm_i8_scaled, bias NULL or [vocabulary_size];
+ * the rest as in dh_token_logprobs.  workspace: 256-byte aligned device
+ * memory of the size the query returns for these rows and this top_k on the
+ * current device; calls that may overlap need one each.  Status: head family
+ * codes, then DH_ERR_*. */
+size_t dh_head_logprobs_workspace_size(uint32_t rows, uint32_t vocabulary_size, uint32_t top_k);
+uint32_t dh_head_logprobs_i8(const int8_t* hidden, uint64_t ld_hidden, const float* a_scale, const int8_t* weights,
+                             uint64_t ld_weights, const float* w_scale, const float* bias, uint32_t rows,
+                             uint32_t hidden_size, uint32_t vocabulary_size, uint32_t mask_token_id,
+                             const void* targets, uint32_t target_bytes, uint32_t targets_per_row, uint32_t top_k,
+                             float* logprobs, float* entropy, float* logsumexp, int32_t* top_ids,
+                             float* top_logprobs, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------ model loop (selected-row head) state */
 /*
