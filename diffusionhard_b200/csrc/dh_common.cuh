@@ -48,6 +48,15 @@ inline cudaError_t smem_optin_once(Kernel kernel, uint32_t bytes, std::atomic<ui
     return e;
 }
 
+// Host: streaming multiprocessors of the current device.
+inline uint32_t device_sms() {
+    int dev = 0, v = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess &&
+        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0)
+        return static_cast<uint32_t>(v);
+    return kNumSMs;
+}
+
 DH_DEVINL uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }

@@ -439,7 +439,7 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p) {
         float part = lane_max[0][lane];
 #pragma unroll
         for (uint32_t w = 1; w < kRowWarps; ++w) part = fmaxf(part, lane_max[w][lane]);
-        const float bound = kth_largest_of_lanes(part, k, lane);
+        const float bound = kth_largest_of_pairs(part, -CUDART_INF_F, k, lane);
         for (uint32_t todo = __ballot_sync(kFullMask, m >= bound && m > -CUDART_INF_F); todo; todo &= todo - 1) {
             const uint32_t owner = warp * 32 + (__ffs(todo) - 1);
             for (uint32_t v0 = owner; v0 < pitch / 4; v0 += 32 * kRowThreads) {
@@ -517,14 +517,6 @@ HeadSplit split_of(uint32_t rows, uint32_t vocab, uint32_t sms) {
     // a span of ceil(total / grid) tiles touches at most this many row tiles
     s.max_segs = static_cast<uint32_t>(((s.total + s.grid - 1) / s.grid + s.n_tiles - 2) / s.n_tiles + 1);
     return s;
-}
-
-uint32_t device_sms() {
-    int sms = kNumSMs, dev = 0, v = 0;
-    if (cudaGetDevice(&dev) == cudaSuccess &&
-        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0)
-        sms = v;
-    return static_cast<uint32_t>(sms);
 }
 
 uint64_t partial_bytes(const HeadSplit& s) {

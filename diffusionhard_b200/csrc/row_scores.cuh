@@ -93,19 +93,78 @@ DH_DEVINL void list_insert(uint64_t& list, uint64_t cand, uint32_t k, uint32_t l
     }
 }
 
-// The k-th largest of the 32 lanes' values (1 <= k <= 32).  Whole warp.
-DH_DEVINL float kth_largest_of_lanes(float v, uint32_t k, uint32_t lane) {
-#pragma unroll
-    for (uint32_t size = 2; size <= 32; size <<= 1) {
-#pragma unroll
-        for (uint32_t stride = size >> 1; stride > 0; stride >>= 1) {
-            const float o = __shfl_xor_sync(kFullMask, v, stride);
-            const bool desc = (lane & size) == 0 || size == 32;
-            const bool upper = (lane & stride) != 0;
-            v = (upper != desc) ? fmaxf(v, o) : fminf(v, o);
+// The k best of the list and a batch of up to 32 keys in shared memory, which
+// serves as scratch.  A first batch (`fresh`) is sorted: a key's place is the
+// number of keys above it.  Out of line: a row's end runs once a row, and its
+// code size costs more than the call.  Whole warp.
+static __device__ __noinline__ uint64_t list_merge(uint64_t list, bool fresh, uint64_t* batch, uint32_t count,
+                                                   uint32_t k, uint32_t lane) {
+    __syncwarp();
+    const uint64_t key = lane < count ? batch[lane] : 0ull;
+    if (!fresh) {
+        list_insert(list, key, k, lane);
+        __syncwarp();
+        return list;
+    }
+    uint32_t place = 0;
+#pragma unroll 4
+    for (uint32_t i = 0; i < count; ++i) place += batch[i] > key;
+    __syncwarp();
+    if (lane >= count) batch[lane] = 0;
+    __syncwarp();
+    if (key) batch[place] = key;
+    __syncwarp();
+    list = lane < k ? batch[lane] : 0ull;
+    __syncwarp();
+    return list;
+}
+
+// The k best of a stream of candidates, gathered 32 at a time.  Whole warp.
+struct TopList {
+    uint64_t list;       // lane i: the i-th best so far
+    uint64_t* batch;     // 32 words of shared memory
+    uint32_t count, k, lane;
+    bool fresh;          // nothing merged yet
+    DH_DEVINL TopList(uint64_t* batch, uint32_t k, uint32_t lane)
+        : list(0), batch(batch), count(0), k(k), lane(lane), fresh(true) {}
+    DH_DEVINL void flush() {
+        list = list_merge(list, fresh, batch, count, k, lane);
+        fresh = false;
+        count = 0;
+    }
+    // each lane's candidate (0: none)
+    DH_DEVINL void add(uint64_t key) {
+        const uint32_t mask = __ballot_sync(kFullMask, key != 0);
+        const uint32_t n = __popc(mask);
+        if (count + n > 32) flush();
+        if (key) batch[count + __popc(mask & ((1u << lane) - 1u))] = key;
+        count += n;
+    }
+};
+
+// The largest of the lanes' values (no NaN).  Whole warp.
+DH_DEVINL float lanes_max(float v) {
+    float y;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(v));
+    return y;
+}
+// The k-th largest of the lanes' pairs a >= b (1 <= k <= 64, no NaN).  Whole warp.
+DH_DEVINL float kth_largest_of_pairs(float a, float b, uint32_t k, uint32_t lane) {
+    float y = 0.f;
+#pragma unroll 1
+    for (uint32_t i = 0; i < k; ++i) {
+        y = lanes_max(a);
+        if (lane == __ffs(__ballot_sync(kFullMask, a == y)) - 1) {
+            a = b;
+            b = -CUDART_INF_F;
         }
     }
-    return __shfl_sync(kFullMask, v, k - 1);
+    return y;
+}
+// v joins the two largest of a set, a >= b.
+DH_DEVINL void two_largest(float& a, float& b, float v) {
+    b = fmaxf(b, fminf(a, v));
+    a = fmaxf(a, v);
 }
 
 // ------------------------------------------------------------- outputs
