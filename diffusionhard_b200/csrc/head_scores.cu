@@ -9,12 +9,14 @@
 //    these into running softmax statistics (row_scores.cuh).  A CTA walks a
 //    contiguous span of tiles in (row tile, column tile) order, so that a
 //    thread's statistics stay in registers until the row tile changes.  For
-//    the k best tokens it stores only the maximum of each group of 16 logits:
-//    the k best lie in the k groups of largest maximum (earlier group first
-//    among equals), since each of those holds a logit at least as good.
-// 2. head_rows_kernel: joins a row's partial statistics, picks the k groups,
-//    and computes their 16 logits again (dp4a, the same fp32 expression, so
-//    the same bits), like the given tokens' logits.
+//    the k best tokens it stores only maxima: of each group of 16 logits and
+//    of each 128 (half a tile).  The k best lie in the k groups of largest
+//    maximum (earlier group first among equals), since each of those holds a
+//    logit at least as good.
+// 2. head_rows_kernel: joins a row's partial statistics, picks the k groups
+//    through the larger maxima, and computes their 16 logits again (the same
+//    fp32 expression of the same integer sum, so the same bits), like the given
+//    tokens' logits.
 #include "dequant.cuh"
 #include "row_scores.cuh"
 #include "tc_ptx.cuh"
@@ -38,6 +40,7 @@ constexpr uint32_t kHeadThreads = 64 + 32 * kEpiWarps;
 constexpr uint32_t kHalfCols = kBN / 2;                 // columns of an epilogue warp
 constexpr uint32_t kGroup = 16;                         // logits per stored maximum
 constexpr uint32_t kGroupsPerTile = kBN / kGroup;
+constexpr uint32_t kGroupsPerHalf = kHalfCols / kGroup;
 constexpr uint32_t kBarBytes = 1024;
 constexpr uint32_t kStagePerWarp = kHalfCols * 8;       // bias and w_scale of the warp's columns
 constexpr uint32_t kHeadSmem =
@@ -63,7 +66,8 @@ struct HeadScoreParams {
     const float* w_scale;
     const float* bias;   // or null
     float4* partials;    // [grid][max_segs][4][128]: base, s, t of a row's part
-    float* group_max;    // [rows][n_tiles * 16], or null
+    float* group_max;    // [rows][n_tiles * 16], or null: none asked for
+    float* half_max;     // [rows][n_tiles * 2]
 };
 
 // The logit of one accumulator.  kWide: k > kExactK, where float(acc) would
@@ -304,6 +308,7 @@ head_stats_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             float* gm = p.group_max && row_ok
                             ? p.group_max + row * pitch + nt * kGroupsPerTile + half * (kHalfCols / kGroup)
                             : nullptr;
+            float hm = -CUDART_INF_F;
             const uint32_t taddr = tmem_base + ((quad * 32u) << 16) + group * kBN + half * kHalfCols;
 #pragma unroll 1
             for (uint32_t c = 0; c < kHalfCols; c += 32) {
@@ -312,8 +317,10 @@ head_stats_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                 tc::tmem_ld_wait();
                 const float2 g = odd ? add_chunk<kWide, true>(st, seen, v, ab, ws + c, bs + c)
                                      : add_chunk<kWide, false>(st, seen, v, ab, ws + c, bs + c);
+                hm = fmaxf(hm, fmaxf(g.x, g.y));
                 if (gm) *reinterpret_cast<float2*>(gm + c / kGroup) = g;
             }
+            if (gm) p.half_max[row * static_cast<uint64_t>(n_tiles * 2) + nt * 2 + half] = hm;
             tc::tc_fence_before();
             tc::mbar_arrive(&acce_bar[group]);
             phase ^= 1;
@@ -343,6 +350,7 @@ struct HeadRowParams {
     const float* bias;
     const float4* partials;
     const float* group_max;
+    const float* half_max;
     ScoreOutputs out;
 };
 
@@ -363,20 +371,87 @@ DH_DEVINL int32_t dot_share(const int8_t* h, const int8_t* w, uint32_t k, uint32
     return acc;
 }
 
-constexpr uint32_t kRowThreads = 256;
-constexpr uint32_t kRowWarps = kRowThreads / 32;
+DH_DEVINL void mma_s8(int32_t (&c)[4], int32_t a0, int32_t a1, int32_t a2, int32_t a3, int32_t b0, int32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 
-// One CTA per row.
-template <bool kWide>
-__global__ void __launch_bounds__(kRowThreads)
+// Integer sums of the 16 tokens of a group with the hidden row, by a warp: a
+// 16 x 8 x 32 MMA whose 16 rows are the tokens and whose first column is the
+// hidden row (the other 7 are 0).  Any order of the k dimension serves as long
+// as both operands share it, so a lane loads 16 consecutive bytes of token
+// lane / 4 and of the one 8 further on, and feeds them to two MMAs.  Lanes with
+// lane % 4 == 0 return the sums of tokens lane / 4 (x) and lane / 4 + 8 (y).
+DH_DEVINL int2 group_sums(const int8_t* h, const int8_t* w, uint64_t ldw, uint32_t first, uint32_t vocab, uint32_t k,
+                          uint32_t lane) {
+    const uint32_t g = lane / 4, t = lane % 4;
+    const int8_t* wa = w + min(first + g, vocab - 1) * ldw;
+    const int8_t* wb = w + min(first + g + 8, vocab - 1) * ldw;
+    const int4 none = make_int4(0, 0, 0, 0);
+    int32_t c[4] = {0, 0, 0, 0};
+    const uint32_t whole = k & ~15u;
+    constexpr uint32_t kUnroll = 4;  // of 64 bytes a row: 8 loads a lane in flight
+#pragma unroll 1
+    for (uint32_t at = t * 16; at < whole + t * 16; at += 64 * kUnroll) {
+        int4 a[kUnroll], b[kUnroll], x[kUnroll];
+#pragma unroll
+        for (uint32_t u = 0; u < kUnroll; ++u) {
+            const uint32_t o = at + 64 * u;
+            const bool in = o < whole;
+            a[u] = in ? __ldg(reinterpret_cast<const int4*>(wa + o)) : none;
+            b[u] = in ? __ldg(reinterpret_cast<const int4*>(wb + o)) : none;
+            x[u] = in && g == 0 ? __ldg(reinterpret_cast<const int4*>(h + o)) : none;
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kUnroll; ++u) {
+            mma_s8(c, a[u].x, b[u].x, a[u].y, b[u].y, x[u].x, x[u].y);
+            mma_s8(c, a[u].z, b[u].z, a[u].w, b[u].w, x[u].z, x[u].w);
+        }
+    }
+    if (whole < k) {  // the bytes past the last whole 16
+        int4 a = none, b = none, x = none;
+        if (t == 0) {
+#pragma unroll 1
+            for (uint32_t o = whole; o < k; ++o) {
+                const uint32_t sh = 8 * (o % 4), i = (o - whole) / 4;
+                const int32_t va = static_cast<int32_t>(static_cast<uint8_t>(wa[o])) << sh;
+                const int32_t vb = static_cast<int32_t>(static_cast<uint8_t>(wb[o])) << sh;
+                const int32_t vx = g == 0 ? static_cast<int32_t>(static_cast<uint8_t>(h[o])) << sh : 0;
+                if (i == 0) { a.x |= va; b.x |= vb; x.x |= vx; }
+                else if (i == 1) { a.y |= va; b.y |= vb; x.y |= vx; }
+                else if (i == 2) { a.z |= va; b.z |= vb; x.z |= vx; }
+                else { a.w |= va; b.w |= vb; x.w |= vx; }
+            }
+        }
+        mma_s8(c, a.x, b.x, a.y, b.y, x.x, x.y);
+        mma_s8(c, a.z, b.z, a.w, b.w, x.z, x.w);
+    }
+    return make_int2(c[0], c[2]);
+}
+
+constexpr uint32_t kRowWarps = 8;
+constexpr uint32_t kTeamRows = 2048;  // fewer rows: a CTA each
+
+// kTeam warps a row: 1 when there are rows enough for every warp of the GPU,
+// all of a CTA's when there are few.
+template <bool kWide, uint32_t kTeam>
+__global__ void __launch_bounds__(32 * kRowWarps, 3)
 head_rows_kernel(const __grid_constant__ HeadRowParams p) {
-    __shared__ float lane_max[kRowWarps][32];
-    __shared__ float part_max[kRowWarps], sum_s[kRowWarps], sum_t[kRowWarps];
-    __shared__ uint64_t lists[kRowWarps][32];
-    __shared__ uint64_t best_groups[32];
+    constexpr uint32_t kTeams = kRowWarps / kTeam;
+    __shared__ float part_base[kRowWarps], part_s[kRowWarps], part_t[kRowWarps];
+    __shared__ uint64_t keys[kRowWarps][32], lists[kRowWarps][32];
+    __shared__ uint64_t groups[kTeams][32];
+    __shared__ uint32_t halves[kTeams][64];
 
-    const uint32_t tid = threadIdx.x, warp = warp_id(), lane = lane_id();
-    const uint64_t row = blockIdx.x;
+    const uint32_t warp = warp_id(), lane = lane_id();
+    const uint32_t team = warp / kTeam, member = warp % kTeam;
+    auto team_sync = [] {
+        if (kTeam == 1) __syncwarp();
+        else __syncthreads();
+    };
+    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * kTeams + team;
+    if (kTeam == 1 && row >= p.split.rows) return;  // (otherwise the grid is the rows)
     const uint32_t k = p.out.top_k, targets = p.out.targets_per_row;
     const int8_t* h = p.hidden + row * p.ld_hidden;
     const float ab = __ldg(p.a_scale + row);
@@ -392,16 +467,19 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p) {
         const int32_t acc = __reduce_add_sync(kFullMask, dot_share(h, p.weights + t * p.ld_weights, p.k, lane, 32));
         return token_logit(static_cast<uint32_t>(t), acc);
     };
+    // the last members take the first given tokens, the first the k best
+    const uint32_t first_target = kTeam - 1 - member;
     int64_t target = -1;
     float target_x = 0.f;
-    if (warp < targets) target_x = target_logit(warp, target);
+    if (first_target < targets) target_x = target_logit(first_target, target);
 
-    // join the row's partial statistics
+    // the row's partial statistics
     const uint32_t mt = static_cast<uint32_t>(row / kBM), r_in = static_cast<uint32_t>(row % kBM);
     const uint64_t t0 = static_cast<uint64_t>(mt) * p.split.n_tiles;
     const uint32_t c_lo = p.split.cta_of(t0), c_hi = p.split.cta_of(t0 + p.split.n_tiles - 1);
     RowStats st{-CUDART_INF_F, 0.f, 0.f};
-    for (uint32_t i = tid; i < (c_hi - c_lo + 1) * 4; i += kRowThreads) {
+#pragma unroll 4
+    for (uint32_t i = member * 32 + lane; i < (c_hi - c_lo + 1) * 4; i += kTeam * 32) {
         const uint32_t c = c_lo + i / 4;
         const uint32_t seg = mt - static_cast<uint32_t>(p.split.first_tile(c) / p.split.n_tiles);
         const float4 q = __ldg(p.partials + ((static_cast<uint64_t>(c) * p.split.max_segs + seg) * 4 + i % 4) * kBM + r_in);
@@ -412,98 +490,92 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p) {
         st.s += o.s;
         st.t += o.t;
     }
-    // the largest group maximum of each thread
-    const uint32_t pitch = p.split.n_tiles * kGroupsPerTile;
-    const float4* gm = reinterpret_cast<const float4*>(p.group_max + row * pitch);
-    float m = -CUDART_INF_F;
-    if (k) {
-        for (uint32_t v = tid; v < pitch / 4; v += kRowThreads) {
-            const float4 g = __ldg(gm + v);
-            m = fmaxf(m, fmaxf(fmaxf(g.x, g.y), fmaxf(g.z, g.w)));
-        }
-        lane_max[warp][lane] = m;
-    }
-    const float wm = warp_max_f32(st.base);
-    if (lane == 0) part_max[warp] = wm;
-    __syncthreads();
-    const float top = warp_max_f32(lane < kRowWarps ? part_max[lane] : -CUDART_INF_F);
+    float top = lanes_max(st.base);
     rebase(st, top);
-    const float ss = warp_sum_f32(st.s), tt = warp_sum_f32(st.t);
-    if (lane == 0) {
-        sum_s[warp] = ss;
-        sum_t[warp] = tt;
+    st.s = warp_sum_f32(st.s);
+    st.t = warp_sum_f32(st.t);
+    if (kTeam > 1 && lane == 0) {
+        part_base[warp] = top;
+        part_s[warp] = st.s;
+        part_t[warp] = st.t;
     }
-    uint64_t list = 0;
-    if (k) {
-        // the k best groups, as token_scores.cu finds the k best tokens
-        float part = lane_max[0][lane];
-#pragma unroll
-        for (uint32_t w = 1; w < kRowWarps; ++w) part = fmaxf(part, lane_max[w][lane]);
-        const float bound = kth_largest_of_pairs(part, -CUDART_INF_F, k, lane);
-        for (uint32_t todo = __ballot_sync(kFullMask, m >= bound && m > -CUDART_INF_F); todo; todo &= todo - 1) {
-            const uint32_t owner = warp * 32 + (__ffs(todo) - 1);
-            for (uint32_t v0 = owner; v0 < pitch / 4; v0 += 32 * kRowThreads) {
-                const uint32_t v = v0 + lane * kRowThreads;
-                const bool in = v < pitch / 4;
-                float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (in) g = __ldg(gm + v);
-                const float f[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) {
-                    const bool c = in && f[e] >= bound && f[e] > -CUDART_INF_F;
-                    if (__any_sync(kFullMask, c)) list_insert(list, c ? token_key(f[e], v * 4 + e) : 0ull, k, lane);
+
+    if (k && member == 0) {
+        // the k best groups: those of the half tiles that reach the k-th
+        // largest of the lanes' maxima (the two largest of each)
+        const uint32_t n_half = p.split.n_tiles * 2;
+        const float* hm = p.half_max + row * n_half;
+        const float* gm = p.group_max + row * n_half * kGroupsPerHalf;
+        float a = -CUDART_INF_F, b = -CUDART_INF_F;
+#pragma unroll 8
+        for (uint32_t i = lane; i < n_half; i += 32) two_largest(a, b, __ldg(hm + i));
+        const float bound = kth_largest_of_pairs(a, b, k, lane);
+        TopList best(keys[warp], k, lane);
+        uint32_t n = 0;
+#pragma unroll 1
+        for (uint32_t i0 = 0; i0 < n_half; i0 += 32) {
+            const float v = i0 + lane < n_half ? __ldg(hm + i0 + lane) : -CUDART_INF_F;
+            const uint32_t who = __ballot_sync(kFullMask, v >= bound && v > -CUDART_INF_F);
+            if ((who >> lane) & 1u) halves[team][n + __popc(who & ((1u << lane) - 1u))] = i0 + lane;
+            n += __popc(who);
+            if (n > 32 || i0 + 32 >= n_half) {
+                __syncwarp();
+                // 8 groups of 4 half tiles at a time
+#pragma unroll 1
+                for (uint32_t j = lane / 8; j < n + lane / 8; j += 4) {
+                    const uint32_t id = j < n ? halves[team][j] * kGroupsPerHalf + lane % 8 : 0u;
+                    const float y = j < n ? __ldg(gm + id) : -CUDART_INF_F;
+                    best.add(y >= bound && y > -CUDART_INF_F ? token_key(y, id) : 0ull);
                 }
+                n = 0;
+                __syncwarp();
             }
         }
-        lists[warp][lane] = list;
+        best.flush();
+        groups[team][lane] = best.list;
     }
-    __syncthreads();
-    if (k) {
-        if (warp == 0) {
-            list = lists[0][lane];
+    team_sync();
+    if (kTeam > 1) {
+        st = lane < kRowWarps ? RowStats{part_base[lane], part_s[lane], part_t[lane]} : RowStats{-CUDART_INF_F, 0.f, 0.f};
+        top = lanes_max(st.base);
+        rebase(st, top);
+        st.s = warp_sum_f32(st.s);
+        st.t = warp_sum_f32(st.t);
+    }
+    const RowResult r = row_result(top, st.s, st.t);
+    if (member == 0 && lane == 0) store_row(p.out, row, r);
+    for (uint32_t i = first_target; i < targets; i += kTeam) {
+        if (i != first_target) target_x = target_logit(i, target);
+        if (lane == 0) p.out.logprobs[row * targets + i] = given_logprob(r, target, p.vocab, target_x);
+    }
+    if (!k) return;
+    // the groups' logits; the k-th group's maximum bounds the k-th best
+    const uint64_t least = groups[team][k - 1];
+    const float bound = least ? key_logit(least) : -CUDART_INF_F;
+    TopList best(keys[warp], k, lane);
+    for (uint32_t i = member; i < k && groups[team][i]; i += kTeam) {
+        const uint32_t first = packed_id(groups[team][i]) * kGroup;
+        const int2 acc = group_sums(h, p.weights, p.ld_weights, first, p.vocab, p.k, lane);
 #pragma unroll
-            for (uint32_t w = 1; w < kRowWarps; ++w) list_insert(list, lists[w][lane], k, lane);
-            best_groups[lane] = list;
+        for (uint32_t e = 0; e < 2; ++e) {
+            const uint32_t c = first + lane / 4 + 8 * e;
+            const float x = lane % 4 == 0 && c < p.vocab ? token_logit(c, e ? acc.y : acc.x) : -CUDART_INF_F;
+            best.add(x >= bound && x > -CUDART_INF_F ? token_key(x, c) : 0ull);
         }
+    }
+    best.flush();
+    if (kTeam > 1) {
+        lists[warp][lane] = best.list;
         __syncthreads();
-        // their logits: half a warp a token, 8 tokens each
-        list = 0;
-        for (uint32_t i = warp; i < k && best_groups[i]; i += kRowWarps) {
-            const uint32_t c0 = packed_id(best_groups[i]) * kGroup + (lane / 16) * 8;
-            int32_t mine = 0;
-#pragma unroll 4
-            for (uint32_t e = 0; e < 8; ++e) {
-                const uint32_t c = min(c0 + e, p.vocab - 1);
-                int32_t acc = dot_share(h, p.weights + c * p.ld_weights, p.k, lane % 16, 16);
-#pragma unroll
-                for (uint32_t o = 8; o > 0; o >>= 1) acc += __shfl_xor_sync(kFullMask, acc, o);
-                if (lane % 16 == e) mine = acc;
-            }
-            const uint32_t c = c0 + lane % 16;
-            const float x = lane % 16 < 8 && c < p.vocab ? token_logit(c, mine) : -CUDART_INF_F;
-            list_insert(list, x > -CUDART_INF_F ? token_key(x, c) : 0ull, k, lane);
-        }
-        lists[warp][lane] = list;
-        __syncthreads();
+        if (member != 0) return;
+        uint64_t least_of = 0;
+        for (uint32_t w = 0; w < kTeam; ++w) least_of = lists[w][k - 1] > least_of ? lists[w][k - 1] : least_of;
+        TopList all(keys[warp], k, lane);
+        for (uint32_t w = 0; w < kTeam; ++w) all.add(lists[w][lane] >= least_of ? lists[w][lane] : 0ull);
+        all.flush();
+        best.list = all.list;
     }
-    const float s = warp_sum_f32(lane < kRowWarps ? sum_s[lane] : 0.f);
-    const float t = warp_sum_f32(lane < kRowWarps ? sum_t[lane] : 0.f);
-    const RowResult r = row_result(top, s, t);
-    if (warp == 0) {
-        if (lane == 0) store_row(p.out, row, r);
-        if (k) {
-            list = lists[0][lane];
-#pragma unroll
-            for (uint32_t w = 1; w < kRowWarps; ++w) list_insert(list, lists[w][lane], k, lane);
-            store_top(p.out, row, r, list, lane);
-        }
-    }
-    for (uint32_t i = warp; i < targets; i += kRowWarps) {
-        if (i != warp) target_x = target_logit(i, target);
-        if (lane == 0)
-            p.out.logprobs[row * targets + i] =
-                target < 0 ? 0.f : (target >= p.vocab ? CUDART_NAN_F : row_logprob(r, target_x));
-    }
+    store_top(p.out, row, r, best.list, lane);
 }
 
 constexpr uint64_t align256(uint64_t v) { return (v + 255) / 256 * 256; }
@@ -523,6 +595,13 @@ uint64_t partial_bytes(const HeadSplit& s) {
     return align256(static_cast<uint64_t>(s.grid) * s.max_segs * 4 * kBM * sizeof(float4));
 }
 
+uint64_t group_bytes(const HeadSplit& s) {
+    return align256(static_cast<uint64_t>(s.rows) * s.n_tiles * kGroupsPerTile * sizeof(float));
+}
+uint64_t half_bytes(const HeadSplit& s) {
+    return align256(static_cast<uint64_t>(s.rows) * s.n_tiles * 2 * sizeof(float));
+}
+
 }  // namespace
 }  // namespace dh
 
@@ -531,8 +610,7 @@ using namespace dh;
 extern "C" size_t dh_head_logprobs_workspace_size(uint32_t rows, uint32_t vocabulary_size, uint32_t top_k) {
     if (rows == 0 || vocabulary_size == 0) return 0;
     const HeadSplit s = split_of(rows, vocabulary_size, device_sms());
-    return partial_bytes(s) +
-           (top_k ? static_cast<uint64_t>(rows) * s.n_tiles * kGroupsPerTile * sizeof(float) : 0u);
+    return partial_bytes(s) + (top_k ? group_bytes(s) + half_bytes(s) : 0u);
 }
 
 extern "C" uint32_t dh_head_logprobs_i8(const int8_t* hidden, uint64_t ld_hidden, const float* a_scale,
@@ -566,20 +644,23 @@ extern "C" uint32_t dh_head_logprobs_i8(const int8_t* hidden, uint64_t ld_hidden
     if (st != DH_OK) return st;
     const bool wide = hidden_size > kExactK;
     auto stats = wide ? head_stats_kernel<true> : head_stats_kernel<false>;
-    auto rows_kernel = wide ? head_rows_kernel<true> : head_rows_kernel<false>;
     static std::atomic<uint64_t> configured[2];
     if (smem_optin_once(stats, kHeadSmem, configured[wide]) != cudaSuccess) return DH_ERR_CUDA;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     float4* partials = static_cast<float4*>(workspace);
-    float* group_max = top_k ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + partial_bytes(split))
-                             : nullptr;
+    uint8_t* maxima = static_cast<uint8_t*>(workspace) + partial_bytes(split);
+    float* group_max = top_k ? reinterpret_cast<float*>(maxima) : nullptr;
+    float* half_max = top_k ? reinterpret_cast<float*>(maxima + group_bytes(split)) : nullptr;
     const HeadScoreParams sp{split, vocabulary_size, mask_token_id, hidden_size, a_scale, w_scale, bias,
-                             partials, group_max};
+                             partials, group_max, half_max};
     stats<<<split.grid, kHeadThreads, kHeadSmem, s>>>(ta, tb, sp);
     DH_LAUNCH_CHECK();
     const HeadRowParams rp{split, vocabulary_size, mask_token_id, hidden_size, hidden, ld_hidden, weights,
-                           ld_weights, a_scale, w_scale, bias, partials, group_max, out};
-    rows_kernel<<<rows, kRowThreads, 0, s>>>(rp);
+                           ld_weights, a_scale, w_scale, bias, partials, group_max, half_max, out};
+    const bool team = rows < kTeamRows;
+    auto rows_kernel = wide ? (team ? head_rows_kernel<true, kRowWarps> : head_rows_kernel<true, 1>)
+                            : (team ? head_rows_kernel<false, kRowWarps> : head_rows_kernel<false, 1>);
+    rows_kernel<<<team ? rows : (rows + kRowWarps - 1) / kRowWarps, 32 * kRowWarps, 0, s>>>(rp);
     DH_LAUNCH_CHECK();
     return DH_OK;
 }

@@ -204,6 +204,10 @@ DH_DEVINL float row_logprob(const RowResult& r, float x) {
     if (r.empty) return -CUDART_INF_F;
     return (x - r.m) - r.log_s;
 }
+// The answer for given token t of a row (x: its logit).
+DH_DEVINL float given_logprob(const RowResult& r, int64_t t, uint32_t vocab, float x) {
+    return t < 0 ? 0.f : (t >= vocab ? CUDART_NAN_F : row_logprob(r, x));
+}
 DH_DEVINL void store_row(const ScoreOutputs& o, uint64_t row, const RowResult& r) {
     if (o.entropy) o.entropy[row] = r.entropy;
     if (o.logsumexp) o.logsumexp[row] = r.bad ? CUDART_NAN_F : (r.empty ? -CUDART_INF_F : r.m + r.log_s);

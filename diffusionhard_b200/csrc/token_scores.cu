@@ -258,11 +258,6 @@ DH_DEVINL void collect(TopList& best, const RowView<T>& r, float bound, const ui
     }
 }
 
-// The answer for given token t of a row (x: its logit).
-DH_DEVINL float given_logprob(const RowResult& r, int64_t t, uint32_t vocab, float x) {
-    return t < 0 ? 0.f : (t >= vocab ? CUDART_NAN_F : row_logprob(r, x));
-}
-
 DH_DEVINL void bulk_load(void* smem, const void* gmem, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                      smem_u32(smem)),
