@@ -10,13 +10,12 @@
 //    contiguous span of tiles in (row tile, column tile) order, so that a
 //    thread's statistics stay in registers until the row tile changes.  For
 //    the k best tokens it stores only maxima: of each group of 16 logits and
-//    of each 128 (half a tile).  The k best lie in the k groups of largest
-//    maximum (earlier group first among equals), since each of those holds a
-//    logit at least as good.
-// 2. head_rows_kernel: joins a row's partial statistics, picks the k groups
-//    through the larger maxima, and computes their 16 logits again (the same
-//    fp32 expression of the same integer sum, so the same bits), like the given
-//    tokens' logits.
+//    of each part of 64 (4 groups).
+// 2. head_rows_kernel: joins a row's partial statistics, bounds the k-th best
+//    logit from below by the k-th largest of maxima of disjoint parts, and
+//    computes the logits of the groups that reach the bound (about k) again (the
+//    same fp32 expression of the same integer sum, so the same bits), like the
+//    given tokens' logits.
 #include "dequant.cuh"
 #include "row_scores.cuh"
 #include "tc_ptx.cuh"
@@ -33,41 +32,60 @@ uint32_t make_i8_operand_maps(CUtensorMap* ta, CUtensorMap* tb, const int8_t* a,
 namespace {
 
 constexpr uint32_t kBM = 128, kBN = 256, kBK = 128;
-constexpr uint32_t kHeadStages = 4;
+constexpr uint32_t kMaxStages = 6;
 constexpr uint32_t kABytes = kBM * kBK, kBBytes = kBN * kBK;
-constexpr uint32_t kEpiWarps = 16;                      // two groups of 8, one per TMEM buffer
+constexpr uint32_t kEpiWarps = 16;                      // 4 for each lane quadrant of TMEM
 constexpr uint32_t kHeadThreads = 64 + 32 * kEpiWarps;
-constexpr uint32_t kHalfCols = kBN / 2;                 // columns of an epilogue warp
-constexpr uint32_t kGroup = 16;                         // logits per stored maximum
+constexpr uint32_t kParts = kEpiWarps / 4;              // of a tile's columns, one for each of those
+constexpr uint32_t kPartCols = kBN / kParts;
+constexpr uint32_t kGroup = 16;                         // logits per stored maximum: of a part's 64, every
+                                                        // 8 (i) the two at 2 (group % 4)
 constexpr uint32_t kGroupsPerTile = kBN / kGroup;
-constexpr uint32_t kGroupsPerHalf = kHalfCols / kGroup;
+constexpr uint32_t kGroupsPerPart = kPartCols / kGroup;
+static_assert(kPartCols == 64, "two blocks of 32 columns");
 constexpr uint32_t kBarBytes = 1024;
-constexpr uint32_t kStagePerWarp = kHalfCols * 8;       // bias and w_scale of the warp's columns
-constexpr uint32_t kHeadSmem =
-    1024 + kHeadStages * (kABytes + kBBytes) + kBarBytes + kEpiWarps * kStagePerWarp;
+constexpr uint32_t kStagePerWarp = kPartCols * 8;       // bias and w_scale of the warp's columns
+// Shared memory: with k <= kResidentK the row tile's A stays for all its column
+// tiles and the ring holds B alone (the copies into shared memory compete with
+// the MMA's and the epilogue's reads of it); otherwise a stage holds both.
+constexpr uint32_t kSmemLimit = 227 * 1024;
+constexpr uint32_t kSmemFixed = 1024 + kBarBytes + kEpiWarps * kStagePerWarp;
+constexpr uint32_t kResidentK = 768;
+constexpr uint32_t kStreamedStages = 4;
+constexpr uint32_t resident_stages(uint32_t k_blocks) {
+    const uint32_t n = (kSmemLimit - kSmemFixed - k_blocks * kABytes) / kBBytes;
+    return n < kMaxStages ? n : kMaxStages;
+}
+static_assert(resident_stages(kResidentK / kBK) >= 3, "room for a ring beside A");
+static_assert(kSmemFixed + kStreamedStages * (kABytes + kBBytes) <= kSmemLimit, "room for the streamed ring");
 // float(acc) is exact up to 2^24: k products of magnitude 127 * 127 (128 * 128)
 constexpr uint32_t kExactK = 1024;
+constexpr uint64_t kMaxTiles = 1u << 30;
 
-// How a launch splits the work: shared by the two kernels.
+// How a launch splits the work, shared by the two kernels: CTA c takes `each`
+// tiles, and one more if c < more, after those of the CTAs before it.
 struct HeadSplit {
-    uint32_t rows, n_tiles, grid, max_segs;
-    uint64_t total;  // row tiles * n_tiles
-    __host__ __device__ uint64_t first_tile(uint32_t cta) const { return total * cta / grid; }
-    // the CTA that holds tile t: the last with first_tile <= t
-    __host__ __device__ uint32_t cta_of(uint64_t t) const {
-        return static_cast<uint32_t>(((t + 1) * grid - 1) / total);
+    uint32_t rows, n_tiles, grid, max_segs, each, more;
+    __host__ __device__ uint32_t first_tile(uint32_t cta) const { return cta * each + (cta < more ? cta : more); }
+    // the CTA that holds tile t
+    __host__ __device__ uint32_t cta_of(uint32_t t) const {
+        const uint32_t longer = more * (each + 1);
+        return t < longer ? t / (each + 1) : more + (t - longer) / each;
     }
+    // where a row's maximum of a part lies
+    __host__ __device__ uint64_t padded_rows() const { return (static_cast<uint64_t>(rows) + kBM - 1) / kBM * kBM; }
+    __host__ __device__ uint64_t slot(uint32_t part, uint32_t row) const { return part * padded_rows() + row; }
 };
 
 struct HeadScoreParams {
     HeadSplit split;
-    uint32_t vocab, mask_id, k;
+    uint32_t vocab, mask_id, k, stages;
     const float* a_scale;
     const float* w_scale;
     const float* bias;   // or null
-    float4* partials;    // [grid][max_segs][4][128]: base, s, t of a row's part
-    float* group_max;    // [rows][n_tiles * 16], or null: none asked for
-    float* half_max;     // [rows][n_tiles * 2]
+    float4* partials;    // [grid][max_segs][kParts][128]: base, s, t of a row's part
+    float* group_max;    // [n_tiles * kParts][rows][4], or null: none asked for
+    float* part_max;     // [n_tiles * kParts][rows]; rows rounded up to row tiles
 };
 
 // The logit of one accumulator.  kWide: k > kExactK, where float(acc) would
@@ -84,92 +102,121 @@ DH_DEVINL float max3(float a, float b, float c) {
     return y;
 }
 
-// 32 accumulators of one row: add to the statistics, return the maxima of
-// the two groups.  kClamp: some logit may be -inf (or NaN).
-template <bool kWide, bool kClamp>
-DH_DEVINL float2 add_chunk(RowStats& st, bool& seen, const uint32_t* v, float ab, const float* ws, const float* bs) {
-    float2 x[16];
-    const float2 ab2 = make_float2(ab, ab);
+// A row's running statistics in this kernel: pairs of sums of e = 2^z and of
+// e z, z = (x - base) log2 e.
+struct PairStats {
+    float base;  // -inf before the first logit above it
+    float2 s, t;
+    DH_DEVINL void clear() {
+        base = -CUDART_INF_F;
+        s = t = make_float2(0.f, 0.f);
+    }
+    // a new maximum (rare once a row has begun)
+    DH_DEVINL void raise(float m) {
+        const float z = base == -CUDART_INF_F ? 0.f : max_nan((base - m) * kLog2E, -1e30f), f = exp2_fast(z);
+        s = make_float2(s.x * f, s.y * f);
+        t = make_float2(__fmaf_rn(s.x, z, f * t.x), __fmaf_rn(s.y, z, f * t.y));
+        base = m;
+    }
+    DH_DEVINL RowStats sum() const { return RowStats{base, s.x + s.y, (t.x + t.y) * kLn2}; }
+};
+
+// 32 columns of 4 rows (8 logits of each): accumulators to logits, to the rows'
+// statistics, and their maxima to g.  kClamp: some logit may be -inf (or NaN),
+// or so far below the others that a difference overflows.
+template <bool kWide, bool kTop, bool kClamp>
+DH_DEVINL void add_block(PairStats (&st)[4], float (&g)[4], const uint32_t (&v)[2][16], const float (&ab)[4],
+                         const float2 (&w)[4], const float2 (&b)[4]) {
+    float2 x[4][4];
 #pragma unroll
-    for (uint32_t j = 0; j < 16; j += 2) {
-        const float4 w = *reinterpret_cast<const float4*>(ws + 2 * j);
-        const float4 b = *reinterpret_cast<const float4*>(bs + 2 * j);
-        if (kWide) {
-            x[j] = make_float2(ref_logit(static_cast<int32_t>(v[2 * j]), ab, w.x, b.x),
-                               ref_logit(static_cast<int32_t>(v[2 * j + 1]), ab, w.y, b.y));
-            x[j + 1] = make_float2(ref_logit(static_cast<int32_t>(v[2 * j + 2]), ab, w.z, b.z),
-                                   ref_logit(static_cast<int32_t>(v[2 * j + 3]), ab, w.w, b.w));
-        } else {
-            const float2 a0 = make_float2(static_cast<float>(static_cast<int32_t>(v[2 * j])),
-                                          static_cast<float>(static_cast<int32_t>(v[2 * j + 1])));
-            const float2 a1 = make_float2(static_cast<float>(static_cast<int32_t>(v[2 * j + 2])),
-                                          static_cast<float>(static_cast<int32_t>(v[2 * j + 3])));
-            x[j] = __ffma2_rn(a0, __fmul2_rn(ab2, make_float2(w.x, w.y)), make_float2(b.x, b.y));
-            x[j + 1] = __ffma2_rn(a1, __fmul2_rn(ab2, make_float2(w.z, w.w)), make_float2(b.z, b.w));
+    for (uint32_t r = 0; r < 4; ++r) {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            const int32_t v0 = static_cast<int32_t>(v[r / 2][4 * j + r % 2 * 2]);
+            const int32_t v1 = static_cast<int32_t>(v[r / 2][4 * j + r % 2 * 2 + 1]);
+            if (kWide)
+                x[r][j] = make_float2(ref_logit(v0, ab[r], w[j].x, b[j].x), ref_logit(v1, ab[r], w[j].y, b[j].y));
+            else
+                x[r][j] = __ffma2_rn(make_float2(static_cast<float>(v0), static_cast<float>(v1)),
+                                     __fmul2_rn(make_float2(ab[r], ab[r]), w[j]), b[j]);
         }
     }
-    float gm[2];
+    bool above = false;
+    float m[4];
 #pragma unroll
-    for (uint32_t g = 0; g < 2; ++g) {
-        float a = fmaxf(x[8 * g].x, x[8 * g].y), b = fmaxf(x[8 * g + 1].x, x[8 * g + 1].y);
+    for (uint32_t r = 0; r < 4; ++r) {
+        m[r] = max3(fmaxf(x[r][0].x, x[r][0].y), x[r][1].x, x[r][1].y);
+        m[r] = fmaxf(m[r], max3(fmaxf(x[r][2].x, x[r][2].y), x[r][3].x, x[r][3].y));
+        if (kTop) g[r] = fmaxf(g[r], m[r]);
+        above = above || m[r] > st[r].base + kBaseSlack;
+    }
+    // (one branch for the four rows: what follows is one block of independent work)
+    if (above) {
 #pragma unroll
-        for (uint32_t j = 2; j < 8; j += 2) {
-            a = max3(a, x[8 * g + j].x, x[8 * g + j].y);
-            b = max3(b, x[8 * g + j + 1].x, x[8 * g + j + 1].y);
-        }
-        gm[g] = fmaxf(a, b);
+        for (uint32_t r = 0; r < 4; ++r)
+            if (m[r] > st[r].base + kBaseSlack) st[r].raise(m[r]);
     }
-    const float cm = fmaxf(gm[0], gm[1]);
-    if (cm > st.base + kBaseSlack || (!seen && cm > -CUDART_INF_F)) {
-        rebase(st, cm);
-        seen = true;
-    }
-    // the chunk's own sums first: a thread adds thousands of logits, and one
-    // long chain of fp32 additions would lose two digits
-    const float2 nb = make_float2(-st.base, -st.base);
     const float2 c2 = make_float2(kLog2E, kLog2E);
-    float2 s = make_float2(0.f, 0.f), t = make_float2(0.f, 0.f);
+    float2 nb[4];  // z is one FMA: the product of base and log2 e is rounded once for all logits
 #pragma unroll
-    for (uint32_t j = 0; j < 16; ++j) {
-        float2 d = __fadd2_rn(x[j], nb);
-        if (kClamp) d = make_float2(max_nan(d.x, -1e30f), max_nan(d.y, -1e30f));
-        const float2 z = __fmul2_rn(d, c2);
-        const float2 e = make_float2(exp2_fast(z.x), exp2_fast(z.y));
-        s = __fadd2_rn(s, e);
-        t = __ffma2_rn(e, d, t);
+    for (uint32_t r = 0; r < 4; ++r) {
+        float y = -st[r].base;
+        if (kClamp) y = st[r].base == -CUDART_INF_F ? 0.f : y;
+        else y = __fmul_rn(y, kLog2E);
+        nb[r] = make_float2(y, y);
     }
-    st.s += s.x + s.y;
-    st.t += t.x + t.y;
-    return make_float2(gm[0], gm[1]);
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+#pragma unroll
+        for (uint32_t r = 0; r < 4; ++r) {
+            float2 z;
+            if (kClamp) {
+                z = __fmul2_rn(__fadd2_rn(x[r][j], nb[r]), c2);
+                z = make_float2(max_nan(z.x, -1e30f), max_nan(z.y, -1e30f));
+            } else {
+                z = __ffma2_rn(x[r][j], c2, nb[r]);
+            }
+            const float2 e = make_float2(exp2_fast(z.x), exp2_fast(z.y));
+            st[r].s = __fadd2_rn(st[r].s, e);
+            st[r].t = __ffma2_rn(e, z, st[r].t);
+        }
+    }
 }
 
-template <bool kWide>
+// kTop: some alternatives are asked for.
+template <bool kWide, bool kResident, bool kTop>
 __global__ void __launch_bounds__(kHeadThreads, 1)
 head_stats_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                   const __grid_constant__ HeadScoreParams p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~static_cast<uintptr_t>(1023));
+    const uint32_t n_tiles = p.split.n_tiles, stages = p.stages;
+    const uint32_t k_blocks = (p.k + kBK - 1) / kBK;
     uint8_t* a_smem = smem;
-    uint8_t* b_smem = smem + kHeadStages * kABytes;
-    uint64_t* full_bar = reinterpret_cast<uint64_t*>(b_smem + kHeadStages * kBBytes);
-    uint64_t* empty_bar = full_bar + kHeadStages;
-    uint64_t* accf_bar = empty_bar + kHeadStages;  // [2]
+    uint8_t* b_smem = smem + (kResident ? k_blocks : stages) * kABytes;
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(b_smem + stages * kBBytes);
+    uint64_t* empty_bar = full_bar + kMaxStages;
+    uint64_t* accf_bar = empty_bar + kMaxStages;   // [2]
     uint64_t* acce_bar = accf_bar + 2;             // [2]
-    uint64_t* drain_bar = acce_bar + 2;            // [1]
+    uint64_t* a_full = acce_bar + 2;               // resident A is there
+    uint64_t* a_free = a_full + 1;                 // and was multiplied for the last time
+    uint64_t* drain_bar = a_free + 1;              // [1]
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain_bar + 1);
     uint8_t* staging = reinterpret_cast<uint8_t*>(full_bar) + kBarBytes;
 
     const uint32_t warp = warp_id(), lane = lane_id();
     if (warp == 0 && lane == 0) {
-        for (uint32_t s = 0; s < kHeadStages; ++s) {
+        for (uint32_t s = 0; s < kMaxStages; ++s) {
             tc::mbar_init(&full_bar[s], 1);
             tc::mbar_init(&empty_bar[s], 1);
         }
         for (uint32_t b = 0; b < 2; ++b) {
             tc::mbar_init(&accf_bar[b], 1);
-            tc::mbar_init(&acce_bar[b], 8 * 32);  // one group of 8 warps drains a buffer
+            tc::mbar_init(&acce_bar[b], kEpiWarps);
         }
+        tc::mbar_init(a_full, 1);
+        tc::mbar_init(a_free, 1);
         tc::mbar_init(drain_bar, 1);
         tc::fence_barrier_init();
         tc::prefetch_tmap(&tmap_a);
@@ -181,52 +228,60 @@ head_stats_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     tc::tc_fence_after();
     const uint32_t tmem_base = *tmem_holder;
 
-    const uint32_t n_tiles = p.split.n_tiles;
-    const uint32_t k_blocks = (p.k + kBK - 1) / kBK;
-    const uint32_t tile0 = static_cast<uint32_t>(p.split.first_tile(blockIdx.x));
-    const uint32_t tile1 = static_cast<uint32_t>(p.split.first_tile(blockIdx.x + 1));
+    const uint32_t tile0 = p.split.first_tile(blockIdx.x), tile1 = p.split.first_tile(blockIdx.x + 1);
 
     if (warp == 0) {
         // ------------------------------------------------------ TMA producer
         if (tc::elect_one()) {
-            uint32_t stage = 0, phase = 0, issued = 0;
-            uint32_t issued_parity[kHeadStages];
+            uint32_t stage = 0, phase = 0, issued = 0, issued_parity = 0, a_phase = 0, a_loads = 0;
             bool ok = true;
             for (uint32_t tile = tile0; tile < tile1 && ok; ++tile) {
                 const uint32_t m0 = (tile / n_tiles) * kBM, n0 = (tile % n_tiles) * kBN;
+                if (kResident && (tile == tile0 || n0 == 0)) {
+                    if (!tc::mbar_wait(a_free, a_phase ^ 1, tc::kErrTimeoutEmpty)) break;
+                    a_phase ^= 1;
+                    ++a_loads;
+                    tc::mbar_arrive_expect_tx(a_full, k_blocks * kABytes);
+                    for (uint32_t kb = 0; kb < k_blocks; ++kb)
+                        tc::tma_load_2d(a_smem + kb * kABytes, &tmap_a, a_full, static_cast<int32_t>(kb * kBK),
+                                        static_cast<int32_t>(m0));
+                }
                 for (uint32_t kb = 0; kb < k_blocks; ++kb) {
                     if (!tc::mbar_wait(&empty_bar[stage], phase ^ 1, tc::kErrTimeoutEmpty)) {
                         ok = false;
                         break;
                     }
-                    tc::mbar_arrive_expect_tx(&full_bar[stage], kABytes + kBBytes);
-                    tc::tma_load_2d(a_smem + stage * kABytes, &tmap_a, &full_bar[stage],
-                                    static_cast<int32_t>(kb * kBK), static_cast<int32_t>(m0));
+                    tc::mbar_arrive_expect_tx(&full_bar[stage], kResident ? kBBytes : kABytes + kBBytes);
+                    if (!kResident)
+                        tc::tma_load_2d(a_smem + stage * kABytes, &tmap_a, &full_bar[stage],
+                                        static_cast<int32_t>(kb * kBK), static_cast<int32_t>(m0));
                     tc::tma_load_2d(b_smem + stage * kBBytes, &tmap_b, &full_bar[stage],
                                     static_cast<int32_t>(kb * kBK), static_cast<int32_t>(n0));
-                    issued_parity[stage] = phase;
+                    issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
                     ++issued;
-                    if (++stage == kHeadStages) {
+                    if (++stage == stages) {
                         stage = 0;
                         phase ^= 1;
                     }
                 }
             }
             // Drain: every copy this CTA issued has landed before it may exit.
-            const uint32_t last = issued < kHeadStages ? issued : kHeadStages;
-            for (uint32_t i = 0; i < last; ++i) {
-                const uint32_t s = (stage + kHeadStages - 1 - i) % kHeadStages;
-                tc::mbar_wait(&full_bar[s], issued_parity[s], tc::kErrTimeoutFull);
-            }
+            for (uint32_t s = 0; s < stages && s < issued; ++s)
+                tc::mbar_wait(&full_bar[s], (issued_parity >> s) & 1u, tc::kErrTimeoutFull);
+            if (a_loads) tc::mbar_wait(a_full, (a_loads - 1) & 1u, tc::kErrTimeoutFull);
         }
     } else if (warp == 1) {
         // ------------------------------------------------------- MMA issuer
         if (tc::elect_one()) {
             constexpr uint32_t idesc = tc::idesc_i8_s32<kBM, kBN>();
-            uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+            uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, a_phase = 0;
             bool ok = true;
             for (uint32_t tile = tile0; tile < tile1 && ok; ++tile) {
                 if (!tc::mbar_wait(&acce_bar[acc], acc_phase ^ 1, tc::kErrTimeoutAccEmpty)) break;
+                if (kResident && (tile == tile0 || tile % n_tiles == 0)) {
+                    if (!tc::mbar_wait(a_full, a_phase, tc::kErrTimeoutFull)) break;
+                    a_phase ^= 1;
+                }
                 tc::tc_fence_after();
                 const uint32_t d_tmem = tmem_base + acc * kBN;
                 for (uint32_t kb = 0; kb < k_blocks; ++kb) {
@@ -235,20 +290,21 @@ head_stats_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                         break;
                     }
                     tc::tc_fence_after();
-                    const uint64_t a_desc = tc::smem_desc_sw128(a_smem + stage * kABytes);
+                    const uint64_t a_desc = tc::smem_desc_sw128(a_smem + (kResident ? kb : stage) * kABytes);
                     const uint64_t b_desc = tc::smem_desc_sw128(b_smem + stage * kBBytes);
 #pragma unroll
                     for (uint32_t kk = 0; kk < kBK / 32; ++kk)
                         tc::mma_i8(d_tmem, tc::desc_advance(a_desc, kk * 32), tc::desc_advance(b_desc, kk * 32),
                                    idesc, (kb | kk) != 0u);
                     tc::mma_commit(&empty_bar[stage]);
-                    if (++stage == kHeadStages) {
+                    if (++stage == stages) {
                         stage = 0;
                         phase ^= 1;
                     }
                 }
                 if (!ok) break;
                 tc::mma_commit(&accf_bar[acc]);
+                if (kResident && (tile + 1) % n_tiles == 0) tc::mma_commit(a_free);
                 if (++acc == 2) {
                     acc = 0;
                     acc_phase ^= 1;
@@ -260,70 +316,131 @@ head_stats_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         }
     } else {
         // --------------------------------------------------------- epilogue
-        const uint32_t ew = warp - 2, group = ew / 8u, quad = warp & 3u, half = (ew >> 2) & 1u;
+        // All warps drain the same tile, so that none idles while its buffer is
+        // filled again (two groups of 8 warps, a buffer each: 1100 us for 32768
+        // rows).  A thread holds 4 rows (lane / 4 + 0, 8, 16, 24 of its
+        // quadrant's) and a quarter of its part's columns (2 of every 8), so that
+        // it reads a column's scale and bias once for 4 logits: with a row a
+        // thread, these reads from shared memory were what set the pace (1000
+        // against 860 us without them).  A group is the thread's 16 columns.
+        const uint32_t ew = warp - 2, quad = warp & 3u, part = ew >> 2;
         float* bs = reinterpret_cast<float*>(staging + ew * kStagePerWarp);
-        float* ws = bs + kHalfCols;
-        const uint32_t mt0 = tile0 / n_tiles;
-        const uint64_t pitch = static_cast<uint64_t>(n_tiles) * kGroupsPerTile;
-        RowStats st{0.f, 0.f, 0.f};
-        bool seen = false;
+        float* ws = bs + kPartCols;
+        const uint32_t mt0 = tile0 / n_tiles, row_in = quad * 32 + lane / 4, quarter = lane % 4;
+        PairStats st[4];
         uint32_t seg = 0;
+#pragma unroll
+        for (uint32_t r = 0; r < 4; ++r) st[r].clear();
         auto flush = [&]() {
-            float4* dst = p.partials +
-                          ((static_cast<uint64_t>(blockIdx.x) * p.split.max_segs + seg) * 4 + group * 2 + half) * kBM +
-                          quad * 32 + lane;
-            *dst = make_float4(seen ? st.base : -CUDART_INF_F, st.s, st.t, 0.f);
-            st = RowStats{0.f, 0.f, 0.f};
-            seen = false;
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r) {
+                // the 4 threads of a row
+                RowStats o = st[r].sum();
+                float top = fmaxf(o.base, __shfl_xor_sync(kFullMask, o.base, 1));
+                top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 2));
+                rebase(o, top);
+#pragma unroll
+                for (uint32_t i = 1; i < 4; i <<= 1) {
+                    o.s += __shfl_xor_sync(kFullMask, o.s, i);
+                    o.t += __shfl_xor_sync(kFullMask, o.t, i);
+                }
+                if (quarter == 0)
+                    p.partials[((static_cast<uint64_t>(blockIdx.x) * p.split.max_segs + seg) * kParts + part) * kBM +
+                               row_in + 8 * r] = make_float4(top, o.s, o.t, 0.f);
+                st[r].clear();
+            }
             ++seg;
         };
-        uint32_t phase = 0;
-        for (uint32_t tile = tile0 + group; tile < tile1; tile += 2) {
-            const uint32_t mt = tile / n_tiles, nt = tile % n_tiles;
-            while (seg < mt - mt0) flush();
-            const uint32_t row = mt * kBM + quad * 32 + lane;
-            const bool row_ok = row < p.split.rows;
-            const float ab = row_ok ? __ldg(p.a_scale + row) : 0.f;
-            // this warp's columns: excluded ones (past the vocabulary, the
-            // masked token) get a logit of -inf from a scale of 0 and that bias
-            __syncwarp();
-            bool odd = !(fabsf(ab) < 1e11f);
+        uint32_t mt = mt0, nt = tile0 % n_tiles;  // this tile
+        // the next tile's scales and biases, fetched while one is added: columns
+        // that are excluded (past the vocabulary, the masked token) get a logit
+        // of -inf from a scale of 0 and that bias
+        float w_next[kPartCols / 32], b_next[kPartCols / 32], ab[4];
+        auto fetch = [&](uint32_t n) {
 #pragma unroll
-            for (uint32_t i = 0; i < kHalfCols; i += 32) {
-                const uint32_t c = nt * kBN + half * kHalfCols + i + lane;
-                float w = 0.f, b = -CUDART_INF_F;
+            for (uint32_t i = 0; i < kPartCols / 32; ++i) {
+                const uint32_t c = n * kBN + part * kPartCols + i * 32 + lane;
+                w_next[i] = 0.f;
+                b_next[i] = -CUDART_INF_F;
                 if (c < p.vocab && c != p.mask_id) {
-                    w = __ldg(p.w_scale + c);
-                    b = p.bias ? __ldg(p.bias + c) : 0.f;
+                    w_next[i] = __ldg(p.w_scale + c);
+                    b_next[i] = p.bias ? __ldg(p.bias + c) : 0.f;
                 }
-                bs[i + lane] = b;
-                ws[i + lane] = w;
+            }
+        };
+        bool odd_row = false;
+        auto fetch_rows = [&](uint32_t m) {
+            odd_row = false;
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r) {
+                const uint32_t row = m * kBM + row_in + 8 * r;
+                ab[r] = row < p.split.rows ? __ldg(p.a_scale + row) : 0.f;
+                odd_row = odd_row || !(fabsf(ab[r]) < 1e11f);
+            }
+        };
+        fetch(nt);
+        fetch_rows(mt);
+        uint32_t acc = 0, phase = 0;
+        for (uint32_t tile = tile0; tile < tile1; ++tile) {
+            __syncwarp();
+            bool odd = odd_row;
+#pragma unroll
+            for (uint32_t i = 0; i < kPartCols / 32; ++i) {
+                bs[i * 32 + lane] = b_next[i];
+                ws[i * 32 + lane] = w_next[i];
                 // within these no logit overflows, so no difference of two is
                 // infinite or NaN
-                odd = odd || !(fabsf(b) < 1e37f && fabsf(w) < 1e18f);
+                odd = odd || !(fabsf(b_next[i]) < 1e37f && fabsf(w_next[i]) < 1e18f);
             }
             odd = __any_sync(kFullMask, odd);
-            if (!tc::mbar_wait(&accf_bar[group], phase, tc::kErrTimeoutAccFull)) break;
+            __syncwarp();
+            const bool last = nt + 1 == n_tiles;
+            if (tile + 1 < tile1) fetch(last ? 0u : nt + 1);
+            if (!tc::mbar_wait(&accf_bar[acc], phase, tc::kErrTimeoutAccFull)) break;
             tc::tc_fence_after();
-            float* gm = p.group_max && row_ok
-                            ? p.group_max + row * pitch + nt * kGroupsPerTile + half * (kHalfCols / kGroup)
-                            : nullptr;
-            float hm = -CUDART_INF_F;
-            const uint32_t taddr = tmem_base + ((quad * 32u) << 16) + group * kBN + half * kHalfCols;
-#pragma unroll 1
-            for (uint32_t c = 0; c < kHalfCols; c += 32) {
-                uint32_t v[32];
-                tc::tmem_ld_32x32b_x32(taddr + c, v);
+            const uint32_t taddr = tmem_base + ((quad * 32u) << 16) + acc * kBN + part * kPartCols;
+            float g[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {  // 32 columns at a time
+                uint32_t v[2][16];
+                tc::tmem_ld_16x256b_x4(taddr + 32 * h, v[0]);
+                tc::tmem_ld_16x256b_x4(taddr + 32 * h + (16u << 16), v[1]);
+                float2 w[4], b[4];
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    w[j] = *reinterpret_cast<const float2*>(ws + 32 * h + 8 * j + 2 * quarter);
+                    b[j] = *reinterpret_cast<const float2*>(bs + 32 * h + 8 * j + 2 * quarter);
+                }
                 tc::tmem_ld_wait();
-                const float2 g = odd ? add_chunk<kWide, true>(st, seen, v, ab, ws + c, bs + c)
-                                     : add_chunk<kWide, false>(st, seen, v, ab, ws + c, bs + c);
-                hm = fmaxf(hm, fmaxf(g.x, g.y));
-                if (gm) *reinterpret_cast<float2*>(gm + c / kGroup) = g;
+                if (h == 1) {
+                    // the accumulators are read: their buffer may be filled again
+                    tc::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&acce_bar[acc]);
+                }
+                if (odd) add_block<kWide, kTop, true>(st, g, v, ab, w, b);
+                else add_block<kWide, kTop, false>(st, g, v, ab, w, b);
             }
-            if (gm) p.half_max[row * static_cast<uint64_t>(n_tiles * 2) + nt * 2 + half] = hm;
-            tc::tc_fence_before();
-            tc::mbar_arrive(&acce_bar[group]);
-            phase ^= 1;
+            if (kTop) {
+#pragma unroll
+                for (uint32_t r = 0; r < 4; ++r) {
+                    // (rows past the last have room, and hold what nothing reads)
+                    const uint64_t at = p.split.slot(nt * kParts + part, mt * kBM + row_in + 8 * r);
+                    p.group_max[at * kGroupsPerPart + quarter] = g[r];
+                    g[r] = fmaxf(g[r], __shfl_xor_sync(kFullMask, g[r], 1));
+                    g[r] = fmaxf(g[r], __shfl_xor_sync(kFullMask, g[r], 2));
+                    if (quarter == 0) p.part_max[at] = g[r];
+                }
+            }
+            ++nt;
+            if (last) {
+                flush();
+                nt = 0;
+                ++mt;
+                if (tile + 1 < tile1) fetch_rows(mt);
+            }
+            acc ^= 1;
+            phase ^= acc == 0;
         }
         const uint32_t segs = tile1 > tile0 ? (tile1 - 1) / n_tiles - mt0 + 1 : 0u;
         while (seg < segs) flush();
@@ -350,7 +467,7 @@ struct HeadRowParams {
     const float* bias;
     const float4* partials;
     const float* group_max;
-    const float* half_max;
+    const float* part_max;
     ScoreOutputs out;
 };
 
@@ -377,37 +494,54 @@ DH_DEVINL void mma_s8(int32_t (&c)[4], int32_t a0, int32_t a1, int32_t a2, int32
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The j-th of a group's 16 tokens.
+DH_DEVINL uint32_t group_token(uint32_t group, uint32_t j) {
+    return group / kGroupsPerPart * kPartCols + j / 2 * 8 + group % kGroupsPerPart * 2 + j % 2;
+}
+
 // Integer sums of the 16 tokens of a group with the hidden row, by a warp: a
 // 16 x 8 x 32 MMA whose 16 rows are the tokens and whose first column is the
 // hidden row (the other 7 are 0).  Any order of the k dimension serves as long
-// as both operands share it, so a lane loads 16 consecutive bytes of token
-// lane / 4 and of the one 8 further on, and feeds them to two MMAs.  Lanes with
-// lane % 4 == 0 return the sums of tokens lane / 4 (x) and lane / 4 + 8 (y).
-DH_DEVINL int2 group_sums(const int8_t* h, const int8_t* w, uint64_t ldw, uint32_t first, uint32_t vocab, uint32_t k,
+// as both operands share it, so a lane loads 16 consecutive bytes of the tokens
+// lane / 4 and lane / 4 + 8, and feeds them to two MMAs.  Lanes with lane % 4 ==
+// 0 return the sums of these tokens (x and y).
+DH_DEVINL int2 group_sums(const int8_t* h, const int8_t* w, uint64_t ldw, uint32_t group, uint32_t vocab, uint32_t k,
                           uint32_t lane) {
     const uint32_t g = lane / 4, t = lane % 4;
-    const int8_t* wa = w + min(first + g, vocab - 1) * ldw;
-    const int8_t* wb = w + min(first + g + 8, vocab - 1) * ldw;
+    const int8_t* wa = w + min(group_token(group, g), vocab - 1) * ldw;
+    const int8_t* wb = w + min(group_token(group, g + 8), vocab - 1) * ldw;
     const int4 none = make_int4(0, 0, 0, 0);
     int32_t c[4] = {0, 0, 0, 0};
     const uint32_t whole = k & ~15u;
     constexpr uint32_t kUnroll = 4;  // of 64 bytes a row: 8 loads a lane in flight
+    uint32_t at = 0;
 #pragma unroll 1
-    for (uint32_t at = t * 16; at < whole + t * 16; at += 64 * kUnroll) {
+    for (; at + 64 * kUnroll <= whole; at += 64 * kUnroll) {
+        const int4* pa = reinterpret_cast<const int4*>(wa + at) + t;
+        const int4* pb = reinterpret_cast<const int4*>(wb + at) + t;
+        const int4* px = reinterpret_cast<const int4*>(h + at) + t;
         int4 a[kUnroll], b[kUnroll], x[kUnroll];
 #pragma unroll
         for (uint32_t u = 0; u < kUnroll; ++u) {
-            const uint32_t o = at + 64 * u;
-            const bool in = o < whole;
-            a[u] = in ? __ldg(reinterpret_cast<const int4*>(wa + o)) : none;
-            b[u] = in ? __ldg(reinterpret_cast<const int4*>(wb + o)) : none;
-            x[u] = in && g == 0 ? __ldg(reinterpret_cast<const int4*>(h + o)) : none;
+            a[u] = __ldg(pa + 4 * u);
+            b[u] = __ldg(pb + 4 * u);
+            x[u] = none;
+            if (g == 0) x[u] = __ldg(px + 4 * u);
         }
 #pragma unroll
         for (uint32_t u = 0; u < kUnroll; ++u) {
             mma_s8(c, a[u].x, b[u].x, a[u].y, b[u].y, x[u].x, x[u].y);
             mma_s8(c, a[u].z, b[u].z, a[u].w, b[u].w, x[u].z, x[u].w);
         }
+    }
+#pragma unroll 1
+    for (; at < whole; at += 64) {
+        const bool in = at + t * 16 < whole;
+        const int4 a = in ? __ldg(reinterpret_cast<const int4*>(wa + at) + t) : none;
+        const int4 b = in ? __ldg(reinterpret_cast<const int4*>(wb + at) + t) : none;
+        const int4 x = in && g == 0 ? __ldg(reinterpret_cast<const int4*>(h + at) + t) : none;
+        mma_s8(c, a.x, b.x, a.y, b.y, x.x, x.y);
+        mma_s8(c, a.z, b.z, a.w, b.w, x.z, x.w);
     }
     if (whole < k) {  // the bytes past the last whole 16
         int4 a = none, b = none, x = none;
@@ -431,18 +565,22 @@ DH_DEVINL int2 group_sums(const int8_t* h, const int8_t* w, uint64_t ldw, uint32
 }
 
 constexpr uint32_t kRowWarps = 8;
+constexpr uint32_t kMaxStaged = 1280;  // words of shared memory a row: vocabularies up to 81,920
+constexpr uint32_t kPicks = 96;  // groups kept for the k best (more, by ties: every group is looked at)
 constexpr uint32_t kTeamRows = 2048;  // fewer rows: a CTA each
 
 // kTeam warps a row: 1 when there are rows enough for every warp of the GPU,
 // all of a CTA's when there are few.
 template <bool kWide, uint32_t kTeam>
 __global__ void __launch_bounds__(32 * kRowWarps, 3)
-head_rows_kernel(const __grid_constant__ HeadRowParams p) {
+head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged) {
+    extern __shared__ float staged_max[];  // the part maxima of the CTA's rows, if `staged` holds them: [kTeams][staged]
     constexpr uint32_t kTeams = kRowWarps / kTeam;
     __shared__ float part_base[kRowWarps], part_s[kRowWarps], part_t[kRowWarps];
     __shared__ uint64_t keys[kRowWarps][32], lists[kRowWarps][32];
-    __shared__ uint64_t groups[kTeams][32];
-    __shared__ uint32_t halves[kTeams][64];
+    __shared__ uint32_t picks[kTeams][kPicks], pick_count[kTeams];
+    __shared__ float pick_bound[kTeams];
+    __shared__ uint32_t parts[kTeams][64];
 
     const uint32_t warp = warp_id(), lane = lane_id();
     const uint32_t team = warp / kTeam, member = warp % kTeam;
@@ -451,8 +589,24 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p) {
         else __syncthreads();
     };
     const uint64_t row = static_cast<uint64_t>(blockIdx.x) * kTeams + team;
-    if (kTeam == 1 && row >= p.split.rows) return;  // (otherwise the grid is the rows)
     const uint32_t k = p.out.top_k, targets = p.out.targets_per_row;
+    const uint32_t n_part = p.split.n_tiles * kParts;
+    if (staged) {
+        // 8 consecutive rows of a part are one 32-byte sector
+        const float4* from = reinterpret_cast<const float4*>(p.part_max) + blockIdx.x * (kTeams / 4);
+        const uint32_t pitch = static_cast<uint32_t>(p.split.padded_rows() / 4), q = threadIdx.x % 2;
+#pragma unroll 4
+        for (uint32_t i = threadIdx.x / 2; i < n_part; i += 16 * kRowWarps) {
+            const float4 v = __ldg(from + static_cast<uint64_t>(i) * pitch + q);
+            float* to = staged_max + 4 * q * staged + i;
+            to[0] = v.x;
+            to[staged] = v.y;
+            to[2 * staged] = v.z;
+            to[3 * staged] = v.w;
+        }
+        __syncthreads();
+    }
+    if (kTeam == 1 && row >= p.split.rows) return;  // (otherwise the grid is the rows)
     const int8_t* h = p.hidden + row * p.ld_hidden;
     const float ab = __ldg(p.a_scale + row);
 
@@ -475,14 +629,14 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p) {
 
     // the row's partial statistics
     const uint32_t mt = static_cast<uint32_t>(row / kBM), r_in = static_cast<uint32_t>(row % kBM);
-    const uint64_t t0 = static_cast<uint64_t>(mt) * p.split.n_tiles;
+    const uint32_t t0 = mt * p.split.n_tiles;
     const uint32_t c_lo = p.split.cta_of(t0), c_hi = p.split.cta_of(t0 + p.split.n_tiles - 1);
     RowStats st{-CUDART_INF_F, 0.f, 0.f};
 #pragma unroll 4
-    for (uint32_t i = member * 32 + lane; i < (c_hi - c_lo + 1) * 4; i += kTeam * 32) {
-        const uint32_t c = c_lo + i / 4;
-        const uint32_t seg = mt - static_cast<uint32_t>(p.split.first_tile(c) / p.split.n_tiles);
-        const float4 q = __ldg(p.partials + ((static_cast<uint64_t>(c) * p.split.max_segs + seg) * 4 + i % 4) * kBM + r_in);
+    for (uint32_t i = member * 32 + lane; i < (c_hi - c_lo + 1) * kParts; i += kTeam * 32) {
+        const uint32_t c = c_lo + i / kParts;
+        const uint32_t seg = mt - p.split.first_tile(c) / p.split.n_tiles;
+        const float4 q = __ldg(p.partials + ((static_cast<uint64_t>(c) * p.split.max_segs + seg) * kParts + i % kParts) * kBM + r_in);
         RowStats o{q.x, q.y, q.z};
         const float m = fmaxf(st.base, o.base);
         rebase(st, m);
@@ -501,38 +655,46 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p) {
     }
 
     if (k && member == 0) {
-        // the k best groups: those of the half tiles that reach the k-th
-        // largest of the lanes' maxima (the two largest of each)
-        const uint32_t n_half = p.split.n_tiles * 2;
-        const float* hm = p.half_max + row * n_half;
-        const float* gm = p.group_max + row * n_half * kGroupsPerHalf;
+        // the k-th largest of the lanes' maxima of parts (the two largest of
+        // each) bounds the k-th best logit: the groups that reach it
+        auto part_max = [&](uint32_t i) {
+            return staged ? staged_max[team * staged + i] : __ldg(p.part_max + p.split.slot(i, static_cast<uint32_t>(row)));
+        };
+        auto group_max = [&](uint32_t id) {
+            return __ldg(p.group_max + p.split.slot(id / kGroupsPerPart, static_cast<uint32_t>(row)) * kGroupsPerPart +
+                         id % kGroupsPerPart);
+        };
         float a = -CUDART_INF_F, b = -CUDART_INF_F;
 #pragma unroll 8
-        for (uint32_t i = lane; i < n_half; i += 32) two_largest(a, b, __ldg(hm + i));
+        for (uint32_t i = lane; i < n_part; i += 32) two_largest(a, b, part_max(i));
         const float bound = kth_largest_of_pairs(a, b, k, lane);
-        TopList best(keys[warp], k, lane);
-        uint32_t n = 0;
+        uint32_t n = 0, count = 0;
 #pragma unroll 1
-        for (uint32_t i0 = 0; i0 < n_half; i0 += 32) {
-            const float v = i0 + lane < n_half ? __ldg(hm + i0 + lane) : -CUDART_INF_F;
+        for (uint32_t i0 = 0; i0 < n_part; i0 += 32) {
+            const float v = i0 + lane < n_part ? part_max(i0 + lane) : -CUDART_INF_F;
             const uint32_t who = __ballot_sync(kFullMask, v >= bound && v > -CUDART_INF_F);
-            if ((who >> lane) & 1u) halves[team][n + __popc(who & ((1u << lane) - 1u))] = i0 + lane;
+            if ((who >> lane) & 1u) parts[team][n + __popc(who & ((1u << lane) - 1u))] = i0 + lane;
             n += __popc(who);
-            if (n > 32 || i0 + 32 >= n_half) {
+            if (n > 32 || i0 + 32 >= n_part) {
                 __syncwarp();
-                // 8 groups of 4 half tiles at a time
+                // the 4 groups of 8 parts at a time
 #pragma unroll 1
-                for (uint32_t j = lane / 8; j < n + lane / 8; j += 4) {
-                    const uint32_t id = j < n ? halves[team][j] * kGroupsPerHalf + lane % 8 : 0u;
-                    const float y = j < n ? __ldg(gm + id) : -CUDART_INF_F;
-                    best.add(y >= bound && y > -CUDART_INF_F ? token_key(y, id) : 0ull);
+                for (uint32_t j = lane / 4; j < n + lane / 4; j += 8) {
+                    const uint32_t id = j < n ? parts[team][j] * kGroupsPerPart + lane % 4 : 0u;
+                    const float y = j < n ? group_max(id) : -CUDART_INF_F;
+                    const uint32_t in = __ballot_sync(kFullMask, y >= bound && y > -CUDART_INF_F);
+                    const uint32_t at = count + __popc(in & ((1u << lane) - 1u));
+                    if (((in >> lane) & 1u) && at < kPicks) picks[team][at] = id;
+                    count += __popc(in);
                 }
                 n = 0;
                 __syncwarp();
             }
         }
-        best.flush();
-        groups[team][lane] = best.list;
+        if (lane == 0) {
+            pick_count[team] = count;
+            pick_bound[team] = bound;
+        }
     }
     team_sync();
     if (kTeam > 1) {
@@ -550,18 +712,24 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p) {
     }
     if (!k) return;
     // the groups' logits; the k-th group's maximum bounds the k-th best
-    const uint64_t least = groups[team][k - 1];
-    const float bound = least ? key_logit(least) : -CUDART_INF_F;
+    const float bound = pick_bound[team];
+    const bool all = pick_count[team] > kPicks;
+    const uint32_t n_pick = all ? p.split.n_tiles * kGroupsPerTile : pick_count[team];
     TopList best(keys[warp], k, lane);
-    for (uint32_t i = member; i < k && groups[team][i]; i += kTeam) {
-        const uint32_t first = packed_id(groups[team][i]) * kGroup;
-        const int2 acc = group_sums(h, p.weights, p.ld_weights, first, p.vocab, p.k, lane);
-#pragma unroll
-        for (uint32_t e = 0; e < 2; ++e) {
-            const uint32_t c = first + lane / 4 + 8 * e;
-            const float x = lane % 4 == 0 && c < p.vocab ? token_logit(c, e ? acc.y : acc.x) : -CUDART_INF_F;
-            best.add(x >= bound && x > -CUDART_INF_F ? token_key(x, c) : 0ull);
-        }
+#pragma unroll 1
+    for (uint32_t i = member; i < n_pick; i += kTeam) {
+        const uint32_t group = all ? i : picks[team][i];
+        if (all && !(__ldg(p.group_max + p.split.slot(i / kGroupsPerPart, static_cast<uint32_t>(row)) * kGroupsPerPart +
+                           i % kGroupsPerPart) >= bound))
+            continue;
+        // lanes with lane % 4 < 2 answer for token lane / 4 + 8 (lane % 4)
+        const uint32_t c = group_token(group, lane / 4 + 8 * (lane % 4 & 1u));
+        const bool in = lane % 4 < 2 && c < p.vocab && c != p.mask_id;
+        const float w = in ? __ldg(p.w_scale + c) : 0.f, b = in && p.bias ? __ldg(p.bias + c) : 0.f;
+        const int2 acc = group_sums(h, p.weights, p.ld_weights, group, p.vocab, p.k, lane);
+        const int32_t y = __shfl_sync(kFullMask, acc.y, lane & ~3u);
+        const float x = score_logit<kWide>(lane % 4 ? y : acc.x, ab, w, b);
+        best.add(in && x >= bound && x > -CUDART_INF_F ? token_key(x, c) : 0ull);
     }
     best.flush();
     if (kTeam > 1) {
@@ -580,26 +748,32 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p) {
 
 constexpr uint64_t align256(uint64_t v) { return (v + 255) / 256 * 256; }
 
+uint64_t tiles_of(uint32_t rows, uint32_t vocab) {
+    return static_cast<uint64_t>((rows + kBM - 1) / kBM) * ((vocab + kBN - 1) / kBN);
+}
+
 HeadSplit split_of(uint32_t rows, uint32_t vocab, uint32_t sms) {
     HeadSplit s{};
     s.rows = rows;
     s.n_tiles = (vocab + kBN - 1) / kBN;
-    s.total = static_cast<uint64_t>((rows + kBM - 1) / kBM) * s.n_tiles;
-    s.grid = static_cast<uint32_t>(std::min<uint64_t>(s.total, sms));
-    // a span of ceil(total / grid) tiles touches at most this many row tiles
-    s.max_segs = static_cast<uint32_t>(((s.total + s.grid - 1) / s.grid + s.n_tiles - 2) / s.n_tiles + 1);
+    const uint32_t total = static_cast<uint32_t>(tiles_of(rows, vocab));
+    s.grid = total < sms ? total : sms;
+    s.each = total / s.grid;
+    s.more = total % s.grid;
+    // a span of that many tiles touches at most this many row tiles
+    s.max_segs = (s.each + (s.more ? 1 : 0) + s.n_tiles - 2) / s.n_tiles + 1;
     return s;
 }
 
 uint64_t partial_bytes(const HeadSplit& s) {
-    return align256(static_cast<uint64_t>(s.grid) * s.max_segs * 4 * kBM * sizeof(float4));
+    return align256(static_cast<uint64_t>(s.grid) * s.max_segs * kParts * kBM * sizeof(float4));
 }
 
 uint64_t group_bytes(const HeadSplit& s) {
-    return align256(static_cast<uint64_t>(s.rows) * s.n_tiles * kGroupsPerTile * sizeof(float));
+    return align256(s.padded_rows() * s.n_tiles * kGroupsPerTile * sizeof(float));
 }
-uint64_t half_bytes(const HeadSplit& s) {
-    return align256(static_cast<uint64_t>(s.rows) * s.n_tiles * 2 * sizeof(float));
+uint64_t part_max_bytes(const HeadSplit& s) {
+    return align256(s.padded_rows() * s.n_tiles * kParts * sizeof(float));
 }
 
 }  // namespace
@@ -608,9 +782,9 @@ uint64_t half_bytes(const HeadSplit& s) {
 using namespace dh;
 
 extern "C" size_t dh_head_logprobs_workspace_size(uint32_t rows, uint32_t vocabulary_size, uint32_t top_k) {
-    if (rows == 0 || vocabulary_size == 0) return 0;
+    if (rows == 0 || vocabulary_size == 0 || tiles_of(rows, vocabulary_size) > kMaxTiles) return 0;
     const HeadSplit s = split_of(rows, vocabulary_size, device_sms());
-    return partial_bytes(s) + (top_k ? group_bytes(s) + half_bytes(s) : 0u);
+    return partial_bytes(s) + (top_k ? group_bytes(s) + part_max_bytes(s) : 0u);
 }
 
 extern "C" uint32_t dh_head_logprobs_i8(const int8_t* hidden, uint64_t ld_hidden, const float* a_scale,
@@ -632,8 +806,8 @@ extern "C" uint32_t dh_head_logprobs_i8(const int8_t* hidden, uint64_t ld_hidden
     if (st != DH_OK) return st;
     if (top_k > kMaxTopK || hidden_size > 131071 || rows > (1u << 24) || vocabulary_size > (1u << 24))
         return DH_ERR_UNSUPPORTED_SHAPE;
+    if (tiles_of(rows, vocabulary_size) > kMaxTiles) return DH_ERR_UNSUPPORTED_SHAPE;
     const HeadSplit split = split_of(rows, vocabulary_size, device_sms());
-    if (split.total > 0x7FFFFFFFull) return DH_ERR_UNSUPPORTED_SHAPE;
     if (((reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(w_scale) |
           reinterpret_cast<uintptr_t>(bias)) & 3u) || (reinterpret_cast<uintptr_t>(workspace) & 255u))
         return DH_ERR_ALIGNMENT;
@@ -643,24 +817,35 @@ extern "C" uint32_t dh_head_logprobs_i8(const int8_t* hidden, uint64_t ld_hidden
                               hidden_size, kBN);
     if (st != DH_OK) return st;
     const bool wide = hidden_size > kExactK;
-    auto stats = wide ? head_stats_kernel<true> : head_stats_kernel<false>;
-    static std::atomic<uint64_t> configured[2];
-    if (smem_optin_once(stats, kHeadSmem, configured[wide]) != cudaSuccess) return DH_ERR_CUDA;
+    const bool resident = hidden_size <= kResidentK;
+    auto stats = top_k ? (wide ? head_stats_kernel<true, false, true>
+                               : (resident ? head_stats_kernel<false, true, true> : head_stats_kernel<false, false, true>))
+                       : (wide ? head_stats_kernel<true, false, false>
+                               : (resident ? head_stats_kernel<false, true, false> : head_stats_kernel<false, false, false>));
+    const uint32_t k_blocks = (hidden_size + kBK - 1) / kBK;
+    const uint32_t stages = resident ? resident_stages(k_blocks) : kStreamedStages;
+    const uint32_t smem = kSmemFixed + (resident ? k_blocks * kABytes + stages * kBBytes : stages * (kABytes + kBBytes));
+    static std::atomic<uint64_t> configured[2][3];
+    if (smem_optin_once(stats, kSmemLimit, configured[top_k ? 1 : 0][wide ? 2 : (resident ? 1 : 0)]) != cudaSuccess) return DH_ERR_CUDA;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     float4* partials = static_cast<float4*>(workspace);
     uint8_t* maxima = static_cast<uint8_t*>(workspace) + partial_bytes(split);
     float* group_max = top_k ? reinterpret_cast<float*>(maxima) : nullptr;
-    float* half_max = top_k ? reinterpret_cast<float*>(maxima + group_bytes(split)) : nullptr;
-    const HeadScoreParams sp{split, vocabulary_size, mask_token_id, hidden_size, a_scale, w_scale, bias,
-                             partials, group_max, half_max};
-    stats<<<split.grid, kHeadThreads, kHeadSmem, s>>>(ta, tb, sp);
+    float* part_max = top_k ? reinterpret_cast<float*>(maxima + group_bytes(split)) : nullptr;
+    const HeadScoreParams sp{split, vocabulary_size, mask_token_id, hidden_size, stages, a_scale, w_scale, bias,
+                             partials, group_max, part_max};
+    stats<<<split.grid, kHeadThreads, smem, s>>>(ta, tb, sp);
     DH_LAUNCH_CHECK();
     const HeadRowParams rp{split, vocabulary_size, mask_token_id, hidden_size, hidden, ld_hidden, weights,
-                           ld_weights, a_scale, w_scale, bias, partials, group_max, half_max, out};
+                           ld_weights, a_scale, w_scale, bias, partials, group_max, part_max, out};
     const bool team = rows < kTeamRows;
     auto rows_kernel = wide ? (team ? head_rows_kernel<true, kRowWarps> : head_rows_kernel<true, 1>)
                             : (team ? head_rows_kernel<false, kRowWarps> : head_rows_kernel<false, 1>);
-    rows_kernel<<<team ? rows : (rows + kRowWarps - 1) / kRowWarps, 32 * kRowWarps, 0, s>>>(rp);
+    // the part maxima of 8 rows, each row's 1 mod 2 words apart, where they fit
+    uint32_t staged = (split.n_tiles * kParts) | 1u;
+    if (!top_k || team || staged > kMaxStaged) staged = 0;
+    rows_kernel<<<team ? rows : (rows + kRowWarps - 1) / kRowWarps, 32 * kRowWarps,
+                  staged * kRowWarps * sizeof(float), s>>>(rp, staged);
     DH_LAUNCH_CHECK();
     return DH_OK;
 }

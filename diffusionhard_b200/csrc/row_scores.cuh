@@ -18,6 +18,7 @@ namespace dh {
 
 constexpr uint32_t kMaxTopK = 32;  // a warp holds the list, one entry a lane
 constexpr float kLog2E = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kFullMask = 0xFFFFFFFFu;
 
 DH_DEVINL float exp2_fast(float x) {

@@ -203,6 +203,20 @@ DH_DEVINL void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)[32]) {
         : "r"(taddr));
 }
 
+// 16 lanes x 32 consecutive columns, spread over the warp like the accumulators
+// of a 16 x 8 MMA: for each 8 columns i, thread t receives row t / 4, columns
+// 8 i + 2 (t % 4) + {0, 1} in r[4 i], r[4 i + 1], and row t / 4 + 8 of the same
+// columns in r[4 i + 2], r[4 i + 3].
+DH_DEVINL void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
 DH_DEVINL uint32_t tmem_ld_32x32b_x1(uint32_t taddr) {
     uint32_t r;
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
@@ -210,7 +224,6 @@ DH_DEVINL uint32_t tmem_ld_32x32b_x1(uint32_t taddr) {
 }
 
 DH_DEVINL void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
 // 32 lanes x 16 consecutive columns (stores) -- used to stage P for attention.
 DH_DEVINL void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
