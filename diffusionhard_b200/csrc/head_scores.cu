@@ -567,20 +567,22 @@ DH_DEVINL int2 group_sums(const int8_t* h, const int8_t* w, uint64_t ldw, uint32
 constexpr uint32_t kRowWarps = 8;
 constexpr uint32_t kMaxStaged = 1280;  // words of shared memory a row: vocabularies up to 81,920
 constexpr uint32_t kPicks = 96;  // groups kept for the k best (more, by ties: every group is looked at)
-constexpr uint32_t kTeamRows = 2048;  // fewer rows: a CTA each
+// Rows below which each gets a CTA: 512 rows 46 / 50 us (1 / 8 alternatives)
+// against 44 / 64 with a warp each, 1001 rows 71 / 79 against 58 / 80.
+constexpr uint32_t kTeamRows = 768;
 
 // kTeam warps a row: 1 when there are rows enough for every warp of the GPU,
 // all of a CTA's when there are few.
 template <bool kWide, uint32_t kTeam>
-__global__ void __launch_bounds__(32 * kRowWarps, 3)
+__global__ void __launch_bounds__(32 * kRowWarps, 4)
 head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged) {
     extern __shared__ float staged_max[];  // the part maxima of the CTA's rows, if `staged` holds them: [kTeams][staged]
     constexpr uint32_t kTeams = kRowWarps / kTeam;
     __shared__ float part_base[kRowWarps], part_s[kRowWarps], part_t[kRowWarps];
     __shared__ uint64_t keys[kRowWarps][32], lists[kRowWarps][32];
     __shared__ uint32_t picks[kTeams][kPicks], pick_count[kTeams];
-    __shared__ float pick_bound[kTeams];
-    __shared__ uint32_t parts[kTeams][64];
+    __shared__ uint32_t parts[kRowWarps][160];
+    __shared__ float pairs[kTeam > 1 ? kRowWarps : 1][2][32];
 
     const uint32_t warp = warp_id(), lane = lane_id();
     const uint32_t team = warp / kTeam, member = warp % kTeam;
@@ -654,46 +656,28 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
         part_t[warp] = st.t;
     }
 
-    if (k && member == 0) {
-        // the k-th largest of the lanes' maxima of parts (the two largest of
-        // each) bounds the k-th best logit: the groups that reach it
-        auto part_max = [&](uint32_t i) {
-            return staged ? staged_max[team * staged + i] : __ldg(p.part_max + p.split.slot(i, static_cast<uint32_t>(row)));
-        };
-        auto group_max = [&](uint32_t id) {
-            return __ldg(p.group_max + p.split.slot(id / kGroupsPerPart, static_cast<uint32_t>(row)) * kGroupsPerPart +
-                         id % kGroupsPerPart);
-        };
-        float a = -CUDART_INF_F, b = -CUDART_INF_F;
-#pragma unroll 8
-        for (uint32_t i = lane; i < n_part; i += 32) two_largest(a, b, part_max(i));
-        const float bound = kth_largest_of_pairs(a, b, k, lane);
-        uint32_t n = 0, count = 0;
-#pragma unroll 1
-        for (uint32_t i0 = 0; i0 < n_part; i0 += 32) {
-            const float v = i0 + lane < n_part ? part_max(i0 + lane) : -CUDART_INF_F;
-            const uint32_t who = __ballot_sync(kFullMask, v >= bound && v > -CUDART_INF_F);
-            if ((who >> lane) & 1u) parts[team][n + __popc(who & ((1u << lane) - 1u))] = i0 + lane;
-            n += __popc(who);
-            if (n > 32 || i0 + 32 >= n_part) {
-                __syncwarp();
-                // the 4 groups of 8 parts at a time
-#pragma unroll 1
-                for (uint32_t j = lane / 4; j < n + lane / 4; j += 8) {
-                    const uint32_t id = j < n ? parts[team][j] * kGroupsPerPart + lane % 4 : 0u;
-                    const float y = j < n ? group_max(id) : -CUDART_INF_F;
-                    const uint32_t in = __ballot_sync(kFullMask, y >= bound && y > -CUDART_INF_F);
-                    const uint32_t at = count + __popc(in & ((1u << lane) - 1u));
-                    if (((in >> lane) & 1u) && at < kPicks) picks[team][at] = id;
-                    count += __popc(in);
-                }
-                n = 0;
-                __syncwarp();
-            }
+    // the k-th largest of the lanes' maxima of parts (the two largest of each)
+    // bounds the k-th best logit; the parts are dealt to the members
+    const float* maxima = staged ? staged_max + team * staged : p.part_max + row;
+    const uint64_t stride = staged ? 1u : p.split.padded_rows();
+    constexpr uint32_t kStep = 32 * kTeam;
+    auto four = [&](uint32_t i, float (&v)[4]) {  // 4 at a time, -inf past the last
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) v[u] = i + kStep * u < n_part ? maxima[(i + kStep * u) * stride] : -CUDART_INF_F;
+    };
+    float a = -CUDART_INF_F, b = -CUDART_INF_F, bound = -CUDART_INF_F;
+    if (k) {
+#pragma unroll 2
+        for (uint32_t i = member * 32 + lane; i < n_part; i += 4 * kStep) {
+            float v[4];
+            four(i, v);
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u) two_largest(a, b, v[u]);
         }
-        if (lane == 0) {
-            pick_count[team] = count;
-            pick_bound[team] = bound;
+        if (member == 0 && lane == 0) pick_count[team] = 0;
+        if (kTeam > 1) {
+            pairs[warp][0][lane] = a;
+            pairs[warp][1][lane] = b;
         }
     }
     team_sync();
@@ -711,8 +695,51 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
         if (lane == 0) p.out.logprobs[row * targets + i] = given_logprob(r, target, p.vocab, target_x);
     }
     if (!k) return;
-    // the groups' logits; the k-th group's maximum bounds the k-th best
-    const float bound = pick_bound[team];
+    if (kTeam > 1) {
+        a = b = -CUDART_INF_F;
+#pragma unroll
+        for (uint32_t w = 0; w < kRowWarps; ++w) {
+            two_largest(a, b, pairs[w][0][lane]);
+            two_largest(a, b, pairs[w][1][lane]);
+        }
+    }
+    bound = kth_largest_of_pairs(a, b, k, lane);
+    // the groups that reach it
+    uint32_t n = 0;
+#pragma unroll 1
+    for (uint32_t i0 = member * 32; i0 < n_part; i0 += 4 * kStep) {
+        float v[4];
+        four(i0 + lane, v);
+        const float m = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+        if (__any_sync(kFullMask, m >= bound && m > -CUDART_INF_F)) {
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u) {
+                const uint32_t who = __ballot_sync(kFullMask, v[u] >= bound && v[u] > -CUDART_INF_F);
+                if ((who >> lane) & 1u) parts[warp][n + __popc(who & ((1u << lane) - 1u))] = i0 + kStep * u + lane;
+                n += __popc(who);
+            }
+        }
+        if (n > 32 || i0 + 4 * kStep >= n_part) {
+            __syncwarp();
+            // the 4 groups of 8 parts at a time
+#pragma unroll 1
+            for (uint32_t j = lane / 4; j < n + lane / 4; j += 8) {
+                const uint32_t part = j < n ? parts[warp][j] : 0u;
+                const float y = j < n ? __ldg(p.group_max + p.split.slot(part, static_cast<uint32_t>(row)) * kGroupsPerPart +
+                                              lane % 4)
+                                      : -CUDART_INF_F;
+                const uint32_t in = __ballot_sync(kFullMask, y >= bound && y > -CUDART_INF_F);
+                uint32_t at = 0;
+                if (lane == 0 && in) at = atomicAdd(&pick_count[team], __popc(in));
+                at = __shfl_sync(kFullMask, at, 0) + __popc(in & ((1u << lane) - 1u));
+                if (((in >> lane) & 1u) && at < kPicks) picks[team][at] = part * kGroupsPerPart + lane % 4;
+            }
+            n = 0;
+            __syncwarp();
+        }
+    }
+    team_sync();
+    // their logits
     const bool all = pick_count[team] > kPicks;
     const uint32_t n_pick = all ? p.split.n_tiles * kGroupsPerTile : pick_count[team];
     TopList best(keys[warp], k, lane);
