@@ -500,33 +500,30 @@ DH_DEVINL uint32_t group_token(uint32_t group, uint32_t j) {
 }
 
 // Integer sums of the 16 tokens of a group with the hidden row, by a warp: a
-// 16 x 8 x 32 MMA whose 16 rows are the tokens and whose first column is the
-// hidden row (the other 7 are 0).  Any order of the k dimension serves as long
-// as both operands share it, so a lane loads 16 consecutive bytes of the tokens
-// lane / 4 and lane / 4 + 8, and feeds them to two MMAs.  Lanes with lane % 4 ==
-// 0 return the sums of these tokens (x and y).
+// 16 x 8 x 32 MMA whose 16 rows are the tokens and whose 8 columns are all the
+// hidden row.  Any order of the k dimension serves as long as both operands
+// share it, so a lane loads 16 consecutive bytes of the tokens lane / 4 and
+// lane / 4 + 8, and feeds them to two MMAs.  Every lane receives the sums of
+// these two tokens (x and y).
 DH_DEVINL int2 group_sums(const int8_t* h, const int8_t* w, uint64_t ldw, uint32_t group, uint32_t vocab, uint32_t k,
                           uint32_t lane) {
     const uint32_t g = lane / 4, t = lane % 4;
     const int8_t* wa = w + min(group_token(group, g), vocab - 1) * ldw;
     const int8_t* wb = w + min(group_token(group, g + 8), vocab - 1) * ldw;
-    const int4 none = make_int4(0, 0, 0, 0);
+    const int4 *pa = reinterpret_cast<const int4*>(wa) + t, *pb = reinterpret_cast<const int4*>(wb) + t;
+    const int4* px = reinterpret_cast<const int4*>(h) + t;
     int32_t c[4] = {0, 0, 0, 0};
-    const uint32_t whole = k & ~15u;
-    constexpr uint32_t kUnroll = 4;  // of 64 bytes a row: 8 loads a lane in flight
+    const uint32_t vecs = k / 16;
+    constexpr uint32_t kUnroll = 3;  // of 64 bytes a row: 6 loads a lane in flight
     uint32_t at = 0;
 #pragma unroll 1
-    for (; at + 64 * kUnroll <= whole; at += 64 * kUnroll) {
-        const int4* pa = reinterpret_cast<const int4*>(wa + at) + t;
-        const int4* pb = reinterpret_cast<const int4*>(wb + at) + t;
-        const int4* px = reinterpret_cast<const int4*>(h + at) + t;
+    for (; at + 4 * kUnroll <= vecs; at += 4 * kUnroll, pa += 4 * kUnroll, pb += 4 * kUnroll, px += 4 * kUnroll) {
         int4 a[kUnroll], b[kUnroll], x[kUnroll];
 #pragma unroll
         for (uint32_t u = 0; u < kUnroll; ++u) {
             a[u] = __ldg(pa + 4 * u);
             b[u] = __ldg(pb + 4 * u);
-            x[u] = none;
-            if (g == 0) x[u] = __ldg(px + 4 * u);
+            x[u] = __ldg(px + 4 * u);
         }
 #pragma unroll
         for (uint32_t u = 0; u < kUnroll; ++u) {
@@ -534,34 +531,21 @@ DH_DEVINL int2 group_sums(const int8_t* h, const int8_t* w, uint64_t ldw, uint32
             mma_s8(c, a[u].z, b[u].z, a[u].w, b[u].w, x[u].z, x[u].w);
         }
     }
+    const int4 none = make_int4(0, 0, 0, 0);
 #pragma unroll 1
-    for (; at < whole; at += 64) {
-        const bool in = at + t * 16 < whole;
-        const int4 a = in ? __ldg(reinterpret_cast<const int4*>(wa + at) + t) : none;
-        const int4 b = in ? __ldg(reinterpret_cast<const int4*>(wb + at) + t) : none;
-        const int4 x = in && g == 0 ? __ldg(reinterpret_cast<const int4*>(h + at) + t) : none;
+    for (; at < vecs; at += 4, pa += 4, pb += 4, px += 4) {
+        const bool in = at + t < vecs;
+        const int4 a = in ? __ldg(pa) : none, b = in ? __ldg(pb) : none, x = in ? __ldg(px) : none;
         mma_s8(c, a.x, b.x, a.y, b.y, x.x, x.y);
         mma_s8(c, a.z, b.z, a.w, b.w, x.z, x.w);
     }
-    if (whole < k) {  // the bytes past the last whole 16
-        int4 a = none, b = none, x = none;
-        if (t == 0) {
+    int2 sums = make_int2(c[0], c[2]);
 #pragma unroll 1
-            for (uint32_t o = whole; o < k; ++o) {
-                const uint32_t sh = 8 * (o % 4), i = (o - whole) / 4;
-                const int32_t va = static_cast<int32_t>(static_cast<uint8_t>(wa[o])) << sh;
-                const int32_t vb = static_cast<int32_t>(static_cast<uint8_t>(wb[o])) << sh;
-                const int32_t vx = g == 0 ? static_cast<int32_t>(static_cast<uint8_t>(h[o])) << sh : 0;
-                if (i == 0) { a.x |= va; b.x |= vb; x.x |= vx; }
-                else if (i == 1) { a.y |= va; b.y |= vb; x.y |= vx; }
-                else if (i == 2) { a.z |= va; b.z |= vb; x.z |= vx; }
-                else { a.w |= va; b.w |= vb; x.w |= vx; }
-            }
-        }
-        mma_s8(c, a.x, b.x, a.y, b.y, x.x, x.y);
-        mma_s8(c, a.z, b.z, a.w, b.w, x.z, x.w);
+    for (uint32_t o = vecs * 16; o < k; ++o) {  // the bytes past the last whole 16
+        sums.x += static_cast<int32_t>(wa[o]) * h[o];
+        sums.y += static_cast<int32_t>(wb[o]) * h[o];
     }
-    return make_int2(c[0], c[2]);
+    return sums;
 }
 
 constexpr uint32_t kRowWarps = 8;
@@ -661,16 +645,20 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
     const float* maxima = staged ? staged_max + team * staged : p.part_max + row;
     const uint64_t stride = staged ? 1u : p.split.padded_rows();
     constexpr uint32_t kStep = 32 * kTeam;
-    auto four = [&](uint32_t i, float (&v)[4]) {  // 4 at a time, -inf past the last
+    const float* mine = maxima + (member * 32 + lane) * stride;
+    const uint64_t hop = kStep * stride;
+    // 4 at a time, from `at` on, the i-th of all; -inf past the last
+    auto four = [&](const float* at, uint32_t i, float (&v)[4]) {
 #pragma unroll
-        for (uint32_t u = 0; u < 4; ++u) v[u] = i + kStep * u < n_part ? maxima[(i + kStep * u) * stride] : -CUDART_INF_F;
+        for (uint32_t u = 0; u < 4; ++u) v[u] = i + kStep * u < n_part ? at[u * hop] : -CUDART_INF_F;
     };
     float a = -CUDART_INF_F, b = -CUDART_INF_F, bound = -CUDART_INF_F;
     if (k) {
+        const float* at = mine;
 #pragma unroll 2
-        for (uint32_t i = member * 32 + lane; i < n_part; i += 4 * kStep) {
+        for (uint32_t i = member * 32 + lane; i < n_part; i += 4 * kStep, at += 4 * hop) {
             float v[4];
-            four(i, v);
+            four(at, i, v);
 #pragma unroll
             for (uint32_t u = 0; u < 4; ++u) two_largest(a, b, v[u]);
         }
@@ -706,10 +694,11 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
     bound = kth_largest_of_pairs(a, b, k, lane);
     // the groups that reach it
     uint32_t n = 0;
+    const float* at = mine;
 #pragma unroll 1
-    for (uint32_t i0 = member * 32; i0 < n_part; i0 += 4 * kStep) {
+    for (uint32_t i0 = member * 32; i0 < n_part; i0 += 4 * kStep, at += 4 * hop) {
         float v[4];
-        four(i0 + lane, v);
+        four(at, i0 + lane, v);
         const float m = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
         if (__any_sync(kFullMask, m >= bound && m > -CUDART_INF_F)) {
 #pragma unroll
@@ -729,10 +718,10 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
                                               lane % 4)
                                       : -CUDART_INF_F;
                 const uint32_t in = __ballot_sync(kFullMask, y >= bound && y > -CUDART_INF_F);
-                uint32_t at = 0;
-                if (lane == 0 && in) at = atomicAdd(&pick_count[team], __popc(in));
-                at = __shfl_sync(kFullMask, at, 0) + __popc(in & ((1u << lane) - 1u));
-                if (((in >> lane) & 1u) && at < kPicks) picks[team][at] = part * kGroupsPerPart + lane % 4;
+                uint32_t to = 0;
+                if (lane == 0 && in) to = atomicAdd(&pick_count[team], __popc(in));
+                to = __shfl_sync(kFullMask, to, 0) + __popc(in & ((1u << lane) - 1u));
+                if (((in >> lane) & 1u) && to < kPicks) picks[team][to] = part * kGroupsPerPart + lane % 4;
             }
             n = 0;
             __syncwarp();
@@ -754,8 +743,7 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
         const bool in = lane % 4 < 2 && c < p.vocab && c != p.mask_id;
         const float w = in ? __ldg(p.w_scale + c) : 0.f, b = in && p.bias ? __ldg(p.bias + c) : 0.f;
         const int2 acc = group_sums(h, p.weights, p.ld_weights, group, p.vocab, p.k, lane);
-        const int32_t y = __shfl_sync(kFullMask, acc.y, lane & ~3u);
-        const float x = score_logit<kWide>(lane % 4 ? y : acc.x, ab, w, b);
+        const float x = score_logit<kWide>(lane % 4 ? acc.y : acc.x, ab, w, b);
         best.add(in && x >= bound && x > -CUDART_INF_F ? token_key(x, c) : 0ull);
     }
     best.flush();
