@@ -38,15 +38,19 @@ struct ScaledParams {
     bool vec;              // out and its row pitch are multiples of 16 bytes
 };
 
+constexpr uint32_t kFull = 0xFFFFFFFFu;
+
 DH_DEVINL uint16_t to_bits16(float v, __nv_bfloat16) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
 DH_DEVINL uint16_t to_bits16(float v, __half) { return __half_as_ushort(__float2half_rn(v)); }
 
-// kHalf: columns of an epilogue warp, half the tile.
-template <class T, uint32_t kHalf_>
+// ------------------------------------------------------------ small products
+//
+// 128 x 64 tiles on the kernel of gemm_tc.cuh: at most one a CTA.
+template <class T>
 struct EpiScaled : EpiBase {
-    static constexpr uint32_t kHalf = kHalf_;
+    static constexpr uint32_t kHalf = 32;  // columns of an epilogue warp, half the tile
     static constexpr bool kF32 = sizeof(T) == 4;
-    static constexpr uint32_t kStages = kHalf == 128 ? 3 : 6;
+    static constexpr uint32_t kStages = 6;
     static constexpr uint32_t kChunk = 32;
     // per warp: the 32 x 32 outputs on their way to whole row segments (4 KB),
     // then its columns' biases (double for fp32 outputs) and w_scale
@@ -134,11 +138,335 @@ struct EpiScaled : EpiBase {
     static DH_DEVINL void tile_end(const Params&, TileState&, const EpiCtx&) {}
 };
 
+// ------------------------------------------------------------ large products
+//
+// 128 x 256 tiles, the TMA ring, MMA thread and double-buffered accumulators of
+// gemm_tc.cuh, but an epilogue of 16 warps that all drain the same tile (none
+// idles while its accumulators are made) and whose threads hold 4 rows and 2 of
+// every 8 columns, so that a column's scale and bias are read from shared memory
+// once for 4 outputs.  Outputs leave through shared memory as whole row
+// segments: TMA stores where the row pitch allows them.
+constexpr uint32_t kBM = 128, kBN = 256, kBK = 128;
+constexpr uint32_t kBigStages = 3;
+constexpr uint32_t kABytes = kBM * kBK, kBBytes = kBN * kBK;
+constexpr uint32_t kEpiWarps = 16, kParts = kEpiWarps / 4, kPartCols = kBN / kParts;
+constexpr uint32_t kBigThreads = 64 + 32 * kEpiWarps;
+constexpr uint32_t kOutBytes = 4096;                     // a warp's outputs on their way
+constexpr uint32_t kColBytes = kPartCols * 8;            // and its columns' scales and biases
+constexpr uint32_t kBigSmem = 1024 + kBigStages * (kABytes + kBBytes) + 1024 + kEpiWarps * (kOutBytes + kColBytes);
+static_assert(kBigSmem <= 227 * 1024, "shared memory of a CTA");
+
+struct BigParams {
+    CUtensorMap out_map;  // with `tma`: out, box 32 rows x 128 bytes, 128-byte swizzle
+    const float* a_scale;
+    const float* w_scale;
+    const float* bias;
+    void* out;
+    uint64_t ldo;
+    uint32_t m, n, k;
+    uint32_t align;       // of out and its row pitch: 16 (TMA stores) or less
+};
+
+// acc * combined + bias for positive normal `combined`, as ref_logit_bits.
+DH_DEVINL float scaled_f32(uint32_t acc, float combined, double bias) {
+    const double acc_d = __hiloint2double(0x43300000, static_cast<int32_t>(acc ^ 0x80000000u)) - 4503601774854144.0;
+    const uint32_t cb = __float_as_uint(combined);
+    const double comb_d =
+        __hiloint2double(static_cast<int32_t>((cb >> 3) + 0x38000000u), static_cast<int32_t>(cb << 29));
+    return __double2float_rn(__fma_rn(acc_d, comb_d, bias));
+}
+
+// Where 16-byte piece c of row r lies in a buffer of 128-byte rows under the
+// 128-byte swizzle of the TMA stores.
+DH_DEVINL uint32_t swz128(uint32_t r, uint32_t c) { return r * 128 + ((c ^ (r & 7u)) << 4); }
+
+// One element a time of the warp's buffer, V bytes a lane, to rows of any pitch:
+// 32 rows x 128 bytes, the first `cols` elements of those below `rows`.
+template <class T, class V>
+DH_DEVINL void store_rows(const uint8_t* buf, T* out, uint64_t ldo, uint32_t rows, uint32_t cols, uint32_t lane) {
+    constexpr uint32_t kLanes = 128 / sizeof(V), kE = sizeof(V) / sizeof(T);  // lanes a row needs
+    constexpr uint32_t kAtOnce = kLanes < 32 ? 32 / kLanes : 1;
+#pragma unroll 8
+    for (uint32_t r0 = 0; r0 < 32; r0 += kAtOnce) {
+        const uint32_t r = r0 + (kLanes < 32 ? lane / kLanes : 0u);
+#pragma unroll
+        for (uint32_t o = 0; o < (kLanes > 32 ? kLanes : 32u); o += 32) {
+            const uint32_t at = kLanes < 32 ? lane % kLanes : lane + o, e = at * kE;  // lane's first element
+            const V v = *reinterpret_cast<const V*>(buf + swz128(r, at * sizeof(V) / 16) + at * sizeof(V) % 16);
+            if (r < rows) {
+                if (e + kE <= cols) {
+                    *reinterpret_cast<V*>(out + r * ldo + e) = v;
+                } else if (kE > 1 && e < cols) {
+#pragma unroll
+                    for (uint32_t i = 0; i < kE; ++i)
+                        if (e + i < cols) out[r * ldo + e + i] = reinterpret_cast<const T*>(&v)[i];
+                }
+            }
+        }
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kBigThreads, 1)
+gemm_scaled_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                   const __grid_constant__ BigParams p) {
+    constexpr bool kF32 = sizeof(T) == 4;
+    constexpr uint32_t kSegCols = 128 / sizeof(T);  // columns of the buffer's 128-byte rows
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                               ~static_cast<uintptr_t>(1023));
+    uint8_t* a_smem = smem;
+    uint8_t* b_smem = smem + kBigStages * kABytes;
+    uint8_t* out_smem = b_smem + kBigStages * kBBytes;
+    uint8_t* col_smem = out_smem + kEpiWarps * kOutBytes;
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(col_smem + kEpiWarps * kColBytes);
+    uint64_t* empty_bar = full_bar + kBigStages;
+    uint64_t* accf_bar = empty_bar + kBigStages;  // [2]
+    uint64_t* acce_bar = accf_bar + 2;            // [2]
+    uint64_t* drain_bar = acce_bar + 2;
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain_bar + 1);
+
+    const uint32_t warp = warp_id(), lane = lane_id();
+    if (warp == 0 && lane == 0) {
+        for (uint32_t s = 0; s < kBigStages; ++s) {
+            tc::mbar_init(&full_bar[s], 1);
+            tc::mbar_init(&empty_bar[s], 1);
+        }
+        for (uint32_t b = 0; b < 2; ++b) {
+            tc::mbar_init(&accf_bar[b], 1);
+            tc::mbar_init(&acce_bar[b], kEpiWarps);
+        }
+        tc::mbar_init(drain_bar, 1);
+        tc::fence_barrier_init();
+        tc::prefetch_tmap(&tmap_a);
+        tc::prefetch_tmap(&tmap_b);
+    }
+    if (warp == 1) tc::tmem_alloc(tmem_holder, 2 * kBN);
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem_base = *tmem_holder;
+
+    const uint32_t n_tiles = (p.n + kBN - 1) / kBN, total = (p.m + kBM - 1) / kBM * n_tiles;
+    const uint32_t k_blocks = (p.k + kBK - 1) / kBK;
+
+    if (warp == 0) {
+        // ------------------------------------------------------ TMA producer
+        if (tc::elect_one()) {
+            uint32_t stage = 0, phase = 0, issued = 0, issued_parity = 0;
+            bool ok = true;
+            for (uint32_t tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+                const uint32_t m0 = tile / n_tiles * kBM, n0 = tile % n_tiles * kBN;
+                for (uint32_t kb = 0; kb < k_blocks; ++kb) {
+                    if (!tc::mbar_wait(&empty_bar[stage], phase ^ 1, tc::kErrTimeoutEmpty)) {
+                        ok = false;
+                        break;
+                    }
+                    tc::mbar_arrive_expect_tx(&full_bar[stage], kABytes + kBBytes);
+                    tc::tma_load_2d(a_smem + stage * kABytes, &tmap_a, &full_bar[stage],
+                                    static_cast<int32_t>(kb * kBK), static_cast<int32_t>(m0));
+                    tc::tma_load_2d(b_smem + stage * kBBytes, &tmap_b, &full_bar[stage],
+                                    static_cast<int32_t>(kb * kBK), static_cast<int32_t>(n0));
+                    issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
+                    ++issued;
+                    if (++stage == kBigStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+            // Drain: every copy this CTA issued has landed before it may exit.
+            for (uint32_t s = 0; s < kBigStages && s < issued; ++s)
+                tc::mbar_wait(&full_bar[s], (issued_parity >> s) & 1u, tc::kErrTimeoutFull);
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------- MMA issuer
+        if (tc::elect_one()) {
+            constexpr uint32_t idesc = tc::idesc_i8_s32<kBM, kBN>();
+            uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+            bool ok = true;
+            for (uint32_t tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+                if (!tc::mbar_wait(&acce_bar[acc], acc_phase ^ 1, tc::kErrTimeoutAccEmpty)) break;
+                tc::tc_fence_after();
+                for (uint32_t kb = 0; kb < k_blocks; ++kb) {
+                    if (!tc::mbar_wait(&full_bar[stage], phase, tc::kErrTimeoutFull)) {
+                        ok = false;
+                        break;
+                    }
+                    tc::tc_fence_after();
+                    const uint64_t a_desc = tc::smem_desc_sw128(a_smem + stage * kABytes);
+                    const uint64_t b_desc = tc::smem_desc_sw128(b_smem + stage * kBBytes);
+#pragma unroll
+                    for (uint32_t kk = 0; kk < kBK / 32; ++kk)
+                        tc::mma_i8(tmem_base + acc * kBN, tc::desc_advance(a_desc, kk * 32),
+                                   tc::desc_advance(b_desc, kk * 32), idesc, (kb | kk) != 0u);
+                    tc::mma_commit(&empty_bar[stage]);
+                    if (++stage == kBigStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+                if (!ok) break;
+                tc::mma_commit(&accf_bar[acc]);
+                acc ^= 1;
+                acc_phase ^= acc == 0;
+            }
+            // Drain: all MMAs issued by this thread complete before TMEM is freed.
+            tc::mma_commit(drain_bar);
+            tc::mbar_wait(drain_bar, 0, tc::kErrTimeoutAccFull);
+        }
+    } else {
+        // --------------------------------------------------------- epilogue
+        const uint32_t ew = warp - 2, quad = warp & 3u, part = ew >> 2, quarter = lane % 4;
+        uint8_t* buf = out_smem + ew * kOutBytes;
+        float* bs = reinterpret_cast<float*>(col_smem + ew * kColBytes);
+        float* ws = bs + kPartCols;
+        // the next tile's scales and biases, fetched while one is stored
+        float w_next[kPartCols / 32], b_next[kPartCols / 32], a_next[4];
+        auto fetch = [&](uint32_t tile) {
+            const uint32_t row = tile / n_tiles * kBM + quad * 32 + lane / 4, col = tile % n_tiles * kBN + part * kPartCols;
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r) a_next[r] = row + 8 * r < p.m ? __ldg(p.a_scale + row + 8 * r) : 1.f;
+#pragma unroll
+            for (uint32_t i = 0; i < kPartCols / 32; ++i) {
+                const uint32_t c = col + i * 32 + lane;
+                w_next[i] = c < p.n ? __ldg(p.w_scale + c) : 1.f;
+                b_next[i] = c < p.n && p.bias ? __ldg(p.bias + c) : 0.f;
+            }
+        };
+        // scales whose products are positive normal numbers
+        auto usual = [](float x) { return x > 1e-18f && x < 1e18f; };
+        if (blockIdx.x < total) fetch(blockIdx.x);
+        uint32_t acc = 0, phase = 0;
+        for (uint32_t tile = blockIdx.x; tile < total; tile += gridDim.x) {
+            const uint32_t row0 = tile / n_tiles * kBM + quad * 32, col0 = tile % n_tiles * kBN + part * kPartCols;
+            __syncwarp();
+            bool plain = true;
+            float ab[4];
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r) {
+                ab[r] = a_next[r];
+                plain = plain && usual(ab[r]);
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < kPartCols / 32; ++i) {
+                bs[i * 32 + lane] = b_next[i];
+                ws[i * 32 + lane] = w_next[i];
+                plain = plain && usual(w_next[i]);
+            }
+            if (kF32) plain = __all_sync(kFull, plain);
+            __syncwarp();
+            if (tile + gridDim.x < total) fetch(tile + gridDim.x);
+            if (!tc::mbar_wait(&accf_bar[acc], phase, tc::kErrTimeoutAccFull)) break;
+            tc::tc_fence_after();
+            const uint32_t taddr = tmem_base + ((quad * 32u) << 16) + acc * kBN + part * kPartCols;
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {  // 32 columns at a time
+                uint32_t v[2][16];
+                tc::tmem_ld_16x256b_x4(taddr + 32 * h, v[0]);
+                tc::tmem_ld_16x256b_x4(taddr + 32 * h + (16u << 16), v[1]);
+                float2 w[4], b[4];
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    w[j] = *reinterpret_cast<const float2*>(ws + 32 * h + 8 * j + 2 * quarter);
+                    b[j] = *reinterpret_cast<const float2*>(bs + 32 * h + 8 * j + 2 * quarter);
+                }
+                if (p.align == 16 && (kF32 || h == 0)) {
+                    // the last store has read the buffer
+                    if (lane == 0) tc::tma_store_wait_read<0>();
+                    __syncwarp();
+                }
+                tc::tmem_ld_wait();
+                if (h == 1) {
+                    // the accumulators are read: their buffer may be filled again
+                    tc::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&acce_bar[acc]);
+                }
+#pragma unroll
+                for (uint32_t r = 0; r < 4; ++r) {
+                    const uint32_t row = lane / 4 + 8 * r;
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        const uint32_t v0 = v[r / 2][4 * j + r % 2 * 2], v1 = v[r / 2][4 * j + r % 2 * 2 + 1];
+                        if constexpr (kF32) {
+                            float2 y;
+                            if (plain) {
+                                y.x = scaled_f32(v0, __fmul_rn(ab[r], w[j].x), static_cast<double>(b[j].x));
+                                y.y = scaled_f32(v1, __fmul_rn(ab[r], w[j].y), static_cast<double>(b[j].y));
+                            } else {
+                                y.x = ref_logit(static_cast<int32_t>(v0), ab[r], w[j].x, b[j].x);
+                                y.y = ref_logit(static_cast<int32_t>(v1), ab[r], w[j].y, b[j].y);
+                            }
+                            *reinterpret_cast<float2*>(buf + swz128(row, 2 * j + quarter / 2) + quarter % 2 * 8) = y;
+                        } else {
+                            const float2 y = __ffma2_rn(make_float2(static_cast<float>(static_cast<int32_t>(v0)),
+                                                                    static_cast<float>(static_cast<int32_t>(v1))),
+                                                        __fmul2_rn(make_float2(ab[r], ab[r]), w[j]), b[j]);
+                            *reinterpret_cast<uint32_t*>(buf + swz128(row, 4 * h + j) + quarter * 4) =
+                                to_bits16(y.x, T()) | (static_cast<uint32_t>(to_bits16(y.y, T())) << 16);
+                        }
+                    }
+                }
+                if (!kF32 && h == 0) continue;  // 64 columns of 2 bytes make a row of the buffer
+                const uint32_t col = col0 + (kF32 ? 32 * h : 0u);
+                if (p.align == 16) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0 && col < p.n && row0 < p.m) {
+                        tc::tma_store_2d(&p.out_map, buf, static_cast<int32_t>(col), static_cast<int32_t>(row0));
+                        tc::tma_store_commit();
+                    }
+                } else {
+                    __syncwarp();
+                    if (col < p.n && row0 < p.m) {
+                        T* out = static_cast<T*>(p.out) + row0 * p.ldo + col;
+                        const uint32_t rows = min(32u, p.m - row0), cols = min(kSegCols, p.n - col);
+                        if (p.align == 8) store_rows<T, uint2>(buf, out, p.ldo, rows, cols, lane);
+                        else if (p.align == 4) store_rows<T, uint32_t>(buf, out, p.ldo, rows, cols, lane);
+                        else if constexpr (!kF32) store_rows<T, uint16_t>(buf, out, p.ldo, rows, cols, lane);
+                    }
+                    __syncwarp();
+                }
+            }
+            acc ^= 1;
+            phase ^= acc == 0;
+        }
+        if (p.align == 16 && lane == 0) tc::tma_store_wait_all();
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc::tc_fence_after();
+        tc::tmem_dealloc(tmem_base, 2 * kBN);
+    }
+}
+
 template <class T>
 cudaError_t launch_scaled(const CUtensorMap& ta, const CUtensorMap& tb, const GemmShape& shape,
                           const ScaledParams& p, uint32_t bn, uint32_t tiles, cudaStream_t s) {
-    if (bn == 64) return launch_gemm_i8<64, EpiScaled<T, 32>>(ta, tb, shape, p, tiles, s);
-    return launch_gemm_i8<256, EpiScaled<T, 128>>(ta, tb, shape, p, tiles, s);
+    if (bn == 64) return launch_gemm_i8<64, EpiScaled<T>>(ta, tb, shape, p, tiles, s);
+    BigParams q{};
+    q.a_scale = p.a_scale;
+    q.w_scale = p.w_scale;
+    q.bias = p.bias;
+    q.out = p.out;
+    q.ldo = p.ldo;
+    q.m = shape.M;
+    q.n = shape.N;
+    q.k = shape.K;
+    const uint64_t at = reinterpret_cast<uintptr_t>(p.out) | (p.ldo * sizeof(T));
+    q.align = at & 15u ? (at & 7u ? (at & 3u ? 2u : 4u) : 8u) : 16u;
+    if (q.align == 16 &&
+        !make_tmap_2d(&q.out_map, p.out, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
+                      sizeof(T), shape.M, shape.N, p.ldo * sizeof(T), 32, 128 / sizeof(T)))
+        q.align = 8;  // a pitch that no map holds (2^40 bytes)
+    static std::atomic<uint64_t> configured{0};
+    const cudaError_t e = smem_optin_once(gemm_scaled_kernel<T>, kBigSmem, configured);
+    if (e != cudaSuccess) return e;
+    const uint32_t sms = device_sms();
+    gemm_scaled_kernel<T><<<tiles < sms ? tiles : sms, kBigThreads, kBigSmem, s>>>(ta, tb, q);
+    return cudaGetLastError();
 }
 
 }  // namespace

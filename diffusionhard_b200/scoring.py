@@ -19,6 +19,7 @@ before anything is launched.
 
 from __future__ import annotations
 
+import functools
 from typing import Any, NamedTuple, Optional
 
 import torch
@@ -41,23 +42,24 @@ class TokenScores(NamedTuple):
     top_logprobs: Optional[torch.Tensor]  # fp32 [rows, top_k]
 
 
-class _On:
-    """The device of a call's tensors as the current device."""
+# A call of these functions takes a few microseconds of the host, and the smallest
+# of them as little of the GPU: the checks below are ordered so that a call that
+# is as it should be passes few of them.
+_current_device = torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
-    __slots__ = ("index", "previous")
 
-    def __init__(self, index: int) -> None:
-        self.index = index
-
-    def __enter__(self) -> int:
-        self.previous = torch.cuda.current_device()
-        if self.previous != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
-
-    def __exit__(self, *exc: Any) -> None:
-        if self.previous != self.index:
-            torch.cuda.set_device(self.previous)
+def _call(name: str, device: torch.device, *args: Any) -> None:
+    """An entry point on the current stream of `device`, its last argument."""
+    index = device.index
+    if _current_device() == index:
+        status = getattr(_lib.lib(), name)(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = getattr(_lib.lib(), name)(*args, _raw_stream(index))
+    if status:
+        raise _lib.DHStatusError(name, int(status))
 
 
 def _cuda(name: str, t: torch.Tensor, device: Optional[torch.device] = None) -> torch.Tensor:
@@ -69,24 +71,30 @@ def _cuda(name: str, t: torch.Tensor, device: Optional[torch.device] = None) -> 
 
 
 def _vector(name: str, t: torch.Tensor, n: int, device: torch.device) -> torch.Tensor:
+    if t.dtype is torch.float32 and t.device == device and t.shape == (n,):
+        return t if t.is_contiguous() else t.contiguous()
     _cuda(name, t, device)
-    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n:
-        raise ValueError(f"{name} must be a float32 vector of {n}")
-    return t if t.is_contiguous() else t.contiguous()
+    raise ValueError(f"{name} must be a float32 vector of {n}")
 
 
 def _rows_i8(name: str, t: torch.Tensor, device: Optional[torch.device] = None) -> torch.Tensor:
     """int8 rows that start at 16-byte boundaries: `t`, or a copy with padded
     rows (store weights that way once: torch.nn.functional.pad)."""
     _cuda(name, t, device)
-    if t.dtype != torch.int8 or t.dim() != 2 or t.shape[1] == 0:
+    if t.dtype is not torch.int8 or t.dim() != 2 or t.shape[1] == 0:
         raise ValueError(f"{name} must be a two-dimensional int8 tensor with columns")
-    if t.stride(1) == 1 and t.stride(0) >= t.shape[1] and t.stride(0) % 16 == 0 and t.data_ptr() % 16 == 0:
+    pitch, inner = t.stride()
+    if inner == 1 and pitch >= t.shape[1] and not (pitch | t.data_ptr()) & 15:
         return t
     rows, cols = t.shape
     padded = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=t.device)
     padded[:, :cols].copy_(t)
     return padded[:, :cols]
+
+
+def _empty(shape: tuple, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    # (empty_strided parses its arguments in half the time of empty)
+    return torch.empty_strided(shape, (shape[1], 1) if len(shape) == 2 else (1,), dtype=dtype, device=device)
 
 
 def linear_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -110,35 +118,42 @@ def linear_i8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     if bias is not None:
         bias = _vector("bias", bias, n, dev)
     if out is None:
-        out = torch.empty((m, n), dtype=out_dtype or torch.float32, device=dev)
-        if out.dtype not in _TYPES:
+        if out_dtype is None:
+            out_dtype = torch.float32
+        elif out_dtype not in _TYPES:
             raise ValueError("out_dtype must be float32, bfloat16 or float16")
+        out = _empty((m, n), out_dtype, dev)
+        pitch = n
     else:
         _cuda("out", out, dev)
         if out.shape != (m, n) or out.dtype not in _TYPES or (out_dtype or out.dtype) != out.dtype:
             raise ValueError(f"out must be [{m}, {n}] of float32, bfloat16 or float16 and of out_dtype")
         if (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
             raise ValueError("out must have contiguous rows that do not overlap")
+        pitch = out.stride(0) if m > 1 else n
     if m == 0 or n == 0:
         return out
-    with _On(dev.index) as stream:
-        _lib.call("dh_gemm_i8_scaled", a.data_ptr(), a.stride(0), a_scale.data_ptr(), w.data_ptr(), w.stride(0),
-                  w_scale.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(),
-                  out.stride(0) if m > 1 else n, _TYPES[out.dtype], m, n, k, stream)
+    _call("dh_gemm_i8_scaled", dev, a.data_ptr(), a.stride(0), a_scale.data_ptr(), w.data_ptr(), w.stride(0),
+          w_scale.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), pitch, _TYPES[out.dtype],
+          m, n, k)
     return out
 
 
 def _targets(targets: Optional[torch.Tensor], rows: int, device: torch.device) -> tuple:
-    """(contiguous tensor or None, tokens per row)."""
+    """(contiguous tensor or None, tokens per row, bytes of an id)."""
     if targets is None:
-        return None, 0
+        return None, 0, 0
     _cuda("targets", targets, device)
-    if targets.dtype not in (torch.int32, torch.int64):
+    if targets.dtype is torch.int64:
+        size = 8
+    elif targets.dtype is torch.int32:
+        size = 4
+    else:
         raise ValueError("targets must be int32 or int64")
-    if targets.dim() not in (1, 2) or targets.shape[0] != rows:
+    shape = targets.shape
+    if len(shape) not in (1, 2) or shape[0] != rows:
         raise ValueError(f"targets must be [{rows}] or [{rows}, tokens]")
-    return (targets if targets.is_contiguous() else targets.contiguous()), \
-        1 if targets.dim() == 1 else targets.shape[1]
+    return (targets if targets.is_contiguous() else targets.contiguous()), 1 if len(shape) == 1 else shape[1], size
 
 
 def _excluded(mask_token_id: Optional[int], vocab: int) -> int:
@@ -153,11 +168,11 @@ def _outputs(targets: Optional[torch.Tensor], rows: int, top_k: int, device: tor
     if not 0 <= top_k <= MAX_TOP_K:
         raise ValueError(f"top_k must be in [0, {MAX_TOP_K}]")
     f32 = torch.float32
+    entropy = _empty((rows,), f32, device)
     return TokenScores(
-        None if targets is None else torch.empty(targets.shape, dtype=f32, device=device),
-        torch.empty(rows, dtype=f32, device=device), torch.empty(rows, dtype=f32, device=device),
-        torch.empty((rows, top_k), dtype=torch.int32, device=device) if top_k else None,
-        torch.empty((rows, top_k), dtype=f32, device=device) if top_k else None)
+        None if targets is None else torch.empty_like(targets, dtype=f32), entropy, torch.empty_like(entropy),
+        _empty((rows, top_k), torch.int32, device) if top_k else None,
+        _empty((rows, top_k), f32, device) if top_k else None)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -183,15 +198,13 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
         raise ValueError("the logits of a row must be contiguous")
     dev = logits.device
     mask = _excluded(mask_token_id, vocab)
-    targets, per_row = _targets(targets, rows, dev)
+    targets, per_row, id_bytes = _targets(targets, rows, dev)
     out = _outputs(targets, rows, top_k, dev)
     if rows == 0:
         return out
-    with _On(dev.index) as stream:
-        _lib.call("dh_token_logprobs", logits.data_ptr(), _TYPES[logits.dtype], logits.stride(0), rows, vocab, mask,
-                  _ptr(targets) if per_row else None, targets.element_size() if per_row else 0, per_row, top_k,
-                  _ptr(out.logprobs) if per_row else None, out.entropy.data_ptr(), out.logsumexp.data_ptr(),
-                  _ptr(out.top_ids), _ptr(out.top_logprobs), stream)
+    _call("dh_token_logprobs", dev, logits.data_ptr(), _TYPES[logits.dtype], logits.stride(0), rows, vocab, mask,
+          _ptr(targets) if per_row else None, id_bytes, per_row, top_k, _ptr(out.logprobs) if per_row else None,
+          out.entropy.data_ptr(), out.logsumexp.data_ptr(), _ptr(out.top_ids), _ptr(out.top_logprobs))
     return out
 
 
@@ -216,16 +229,23 @@ def head_logprobs(hidden: torch.Tensor, hidden_scale: torch.Tensor, weight: torc
     if bias is not None:
         bias = _vector("bias", bias, vocab, dev)
     mask = _excluded(mask_token_id, vocab)
-    targets, per_row = _targets(targets, rows, dev)
+    targets, per_row, id_bytes = _targets(targets, rows, dev)
     out = _outputs(targets, rows, top_k, dev)
     if rows == 0:
         return out
-    with _On(dev.index) as stream:
-        size_bytes = _lib.lib().dh_head_logprobs_workspace_size(rows, vocab, top_k)
-        ws = torch.empty(size_bytes, dtype=torch.uint8, device=dev)
-        _lib.call("dh_head_logprobs_i8", hidden.data_ptr(), hidden.stride(0), hidden_scale.data_ptr(),
-                  weight.data_ptr(), weight.stride(0), w_scale.data_ptr(), _ptr(bias), rows, size, vocab, mask,
-                  _ptr(targets) if per_row else None, targets.element_size() if per_row else 0, per_row, top_k,
-                  _ptr(out.logprobs) if per_row else None, out.entropy.data_ptr(), out.logsumexp.data_ptr(),
-                  _ptr(out.top_ids), _ptr(out.top_logprobs), ws.data_ptr(), size_bytes, stream)
+    # (the workspace goes back to the allocator's pool of the current stream,
+    # which the kernels that use it are on)
+    size_bytes = _workspace_bytes(rows, vocab, top_k > 0, dev.index)
+    ws = _empty((size_bytes,), torch.uint8, dev)
+    _call("dh_head_logprobs_i8", dev, hidden.data_ptr(), hidden.stride(0), hidden_scale.data_ptr(), weight.data_ptr(),
+          weight.stride(0), w_scale.data_ptr(), _ptr(bias), rows, size, vocab, mask,
+          _ptr(targets) if per_row else None, id_bytes, per_row, top_k, _ptr(out.logprobs) if per_row else None,
+          out.entropy.data_ptr(), out.logsumexp.data_ptr(), _ptr(out.top_ids), _ptr(out.top_logprobs), ws.data_ptr(),
+          size_bytes)
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(rows: int, vocab: int, top: bool, index: int) -> int:
+    with torch.cuda.device(index):
+        return int(_lib.lib().dh_head_logprobs_workspace_size(rows, vocab, 1 if top else 0))
