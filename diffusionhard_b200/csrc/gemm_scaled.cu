@@ -157,14 +157,13 @@ constexpr uint32_t kBigSmem = 1024 + kBigStages * (kABytes + kBBytes) + 1024 + k
 static_assert(kBigSmem <= 227 * 1024, "shared memory of a CTA");
 
 struct BigParams {
-    CUtensorMap out_map;  // with `tma`: out, box 32 rows x 128 bytes, 128-byte swizzle
+    CUtensorMap out_map;  // with Out::kTma: out, box 32 rows x 128 bytes, 128-byte swizzle
     const float* a_scale;
     const float* w_scale;
     const float* bias;
     void* out;
     uint64_t ldo;
     uint32_t m, n, k;
-    uint32_t align;       // of out and its row pitch: 16 (TMA stores) or less
 };
 
 // acc * combined + bias for positive normal `combined`, as ref_logit_bits.
@@ -180,33 +179,42 @@ DH_DEVINL float scaled_f32(uint32_t acc, float combined, double bias) {
 // 128-byte swizzle of the TMA stores.
 DH_DEVINL uint32_t swz128(uint32_t r, uint32_t c) { return r * 128 + ((c ^ (r & 7u)) << 4); }
 
-// One element a time of the warp's buffer, V bytes a lane, to rows of any pitch:
-// 32 rows x 128 bytes, the first `cols` elements of those below `rows`.
+// How outputs leave the warp's buffer: by TMA (start and row pitch multiples of
+// 16 bytes), or through the registers, 8, 4 or 2 bytes a lane.
+enum class Out { kTma, k8, k4, k2 };
+
+// The warp's buffer, 32 rows x 128 bytes, to rows of any pitch: the first `cols`
+// elements of the first `rows`, sizeof(V) bytes a lane.
 template <class T, class V>
 DH_DEVINL void store_rows(const uint8_t* buf, T* out, uint64_t ldo, uint32_t rows, uint32_t cols, uint32_t lane) {
     constexpr uint32_t kLanes = 128 / sizeof(V), kE = sizeof(V) / sizeof(T);  // lanes a row needs
-    constexpr uint32_t kAtOnce = kLanes < 32 ? 32 / kLanes : 1;
-#pragma unroll 8
-    for (uint32_t r0 = 0; r0 < 32; r0 += kAtOnce) {
-        const uint32_t r = r0 + (kLanes < 32 ? lane / kLanes : 0u);
+    constexpr uint32_t kRows = kLanes < 32 ? 32 / kLanes : 1;                 // rows an instruction covers
+    constexpr uint32_t kRounds = kLanes > 32 ? kLanes / 32 : 1;               // instructions a row needs
+    const uint32_t sub = lane / kLanes * (kLanes < 32), at = lane % kLanes;
+    out += sub * ldo + at * kE;
+    const uint32_t piece = at * sizeof(V) / 16, in = at * sizeof(V) % 16;
+    const bool whole = rows == 32 && cols * sizeof(T) == 128;
+#pragma unroll 4
+    for (uint32_t r0 = 0; r0 < 32; r0 += kRows) {
 #pragma unroll
-        for (uint32_t o = 0; o < (kLanes > 32 ? kLanes : 32u); o += 32) {
-            const uint32_t at = kLanes < 32 ? lane % kLanes : lane + o, e = at * kE;  // lane's first element
-            const V v = *reinterpret_cast<const V*>(buf + swz128(r, at * sizeof(V) / 16) + at * sizeof(V) % 16);
-            if (r < rows) {
-                if (e + kE <= cols) {
-                    *reinterpret_cast<V*>(out + r * ldo + e) = v;
-                } else if (kE > 1 && e < cols) {
+        for (uint32_t o = 0; o < kRounds; ++o) {
+            // piece c of row r lies at c ^ (r & 7)
+            const uint32_t c = piece + o * (32 * sizeof(V) / 16);
+            const V v = *reinterpret_cast<const V*>(buf + (r0 + sub) * 128 + ((c ^ sub ^ (r0 & 7u)) << 4) + in);
+            const uint32_t e = (at + 32 * o) * kE;
+            if (whole || (r0 + sub < rows && e + kE <= cols)) {
+                *reinterpret_cast<V*>(out + 32 * o * kE) = v;
+            } else if (kE > 1 && r0 + sub < rows) {
 #pragma unroll
-                    for (uint32_t i = 0; i < kE; ++i)
-                        if (e + i < cols) out[r * ldo + e + i] = reinterpret_cast<const T*>(&v)[i];
-                }
+                for (uint32_t i = 0; i < kE; ++i)
+                    if (e + i < cols) out[32 * o * kE + i] = reinterpret_cast<const T*>(&v)[i];
             }
         }
+        out += kRows * ldo;
     }
 }
 
-template <class T>
+template <class T, Out kOut>
 __global__ void __launch_bounds__(kBigThreads, 1)
 gemm_scaled_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                    const __grid_constant__ BigParams p) {
@@ -362,55 +370,62 @@ gemm_scaled_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
             const uint32_t taddr = tmem_base + ((quad * 32u) << 16) + acc * kBN + part * kPartCols;
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h) {  // 32 columns at a time
-                uint32_t v[2][16];
-                tc::tmem_ld_16x256b_x4(taddr + 32 * h, v[0]);
-                tc::tmem_ld_16x256b_x4(taddr + 32 * h + (16u << 16), v[1]);
                 float2 w[4], b[4];
 #pragma unroll
                 for (uint32_t j = 0; j < 4; ++j) {
                     w[j] = *reinterpret_cast<const float2*>(ws + 32 * h + 8 * j + 2 * quarter);
                     b[j] = *reinterpret_cast<const float2*>(bs + 32 * h + 8 * j + 2 * quarter);
                 }
-                if (p.align == 16 && (kF32 || h == 0)) {
+                if (kOut == Out::kTma && (kF32 || h == 0)) {
                     // the last store has read the buffer
                     if (lane == 0) tc::tma_store_wait_read<0>();
                     __syncwarp();
                 }
-                tc::tmem_ld_wait();
-                if (h == 1) {
-                    // the accumulators are read: their buffer may be filled again
-                    tc::tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(&acce_bar[acc]);
-                }
+                // 16 rows at a time (fp32's float64 temporaries leave no registers for
+                // both halves), or 32
+                constexpr uint32_t kHalves = kF32 ? 1 : 2;
 #pragma unroll
-                for (uint32_t r = 0; r < 4; ++r) {
-                    const uint32_t row = lane / 4 + 8 * r;
+                for (uint32_t q = 0; q < 2; q += kHalves) {
+                    uint32_t v[kHalves][16];
 #pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) {
-                        const uint32_t v0 = v[r / 2][4 * j + r % 2 * 2], v1 = v[r / 2][4 * j + r % 2 * 2 + 1];
-                        if constexpr (kF32) {
-                            float2 y;
-                            if (plain) {
-                                y.x = scaled_f32(v0, __fmul_rn(ab[r], w[j].x), static_cast<double>(b[j].x));
-                                y.y = scaled_f32(v1, __fmul_rn(ab[r], w[j].y), static_cast<double>(b[j].y));
+                    for (uint32_t i = 0; i < kHalves; ++i)
+                        tc::tmem_ld_16x256b_x4(taddr + 32 * h + ((16u * (q + i)) << 16), v[i]);
+                    tc::tmem_ld_wait();
+                    if (h == 1 && q + kHalves == 2) {
+                        // the accumulators are read: their buffer may be filled again
+                        tc::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(&acce_bar[acc]);
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < 2 * kHalves; ++i) {
+                        const uint32_t r = 2 * q + i, row = lane / 4 + 8 * r;
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; ++j) {
+                            const uint32_t v0 = v[i / 2][4 * j + i % 2 * 2], v1 = v[i / 2][4 * j + i % 2 * 2 + 1];
+                            if constexpr (kF32) {
+                                float2 y;
+                                if (plain) {
+                                    y.x = scaled_f32(v0, __fmul_rn(ab[r], w[j].x), static_cast<double>(b[j].x));
+                                    y.y = scaled_f32(v1, __fmul_rn(ab[r], w[j].y), static_cast<double>(b[j].y));
+                                } else {
+                                    y.x = ref_logit(static_cast<int32_t>(v0), ab[r], w[j].x, b[j].x);
+                                    y.y = ref_logit(static_cast<int32_t>(v1), ab[r], w[j].y, b[j].y);
+                                }
+                                *reinterpret_cast<float2*>(buf + swz128(row, 2 * j + quarter / 2) + quarter % 2 * 8) = y;
                             } else {
-                                y.x = ref_logit(static_cast<int32_t>(v0), ab[r], w[j].x, b[j].x);
-                                y.y = ref_logit(static_cast<int32_t>(v1), ab[r], w[j].y, b[j].y);
+                                const float2 y = __ffma2_rn(make_float2(static_cast<float>(static_cast<int32_t>(v0)),
+                                                                        static_cast<float>(static_cast<int32_t>(v1))),
+                                                            __fmul2_rn(make_float2(ab[r], ab[r]), w[j]), b[j]);
+                                *reinterpret_cast<uint32_t*>(buf + swz128(row, 4 * h + j) + quarter * 4) =
+                                    to_bits16(y.x, T()) | (static_cast<uint32_t>(to_bits16(y.y, T())) << 16);
                             }
-                            *reinterpret_cast<float2*>(buf + swz128(row, 2 * j + quarter / 2) + quarter % 2 * 8) = y;
-                        } else {
-                            const float2 y = __ffma2_rn(make_float2(static_cast<float>(static_cast<int32_t>(v0)),
-                                                                    static_cast<float>(static_cast<int32_t>(v1))),
-                                                        __fmul2_rn(make_float2(ab[r], ab[r]), w[j]), b[j]);
-                            *reinterpret_cast<uint32_t*>(buf + swz128(row, 4 * h + j) + quarter * 4) =
-                                to_bits16(y.x, T()) | (static_cast<uint32_t>(to_bits16(y.y, T())) << 16);
                         }
                     }
                 }
                 if (!kF32 && h == 0) continue;  // 64 columns of 2 bytes make a row of the buffer
                 const uint32_t col = col0 + (kF32 ? 32 * h : 0u);
-                if (p.align == 16) {
+                if (kOut == Out::kTma) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0 && col < p.n && row0 < p.m) {
@@ -422,8 +437,8 @@ gemm_scaled_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
                     if (col < p.n && row0 < p.m) {
                         T* out = static_cast<T*>(p.out) + row0 * p.ldo + col;
                         const uint32_t rows = min(32u, p.m - row0), cols = min(kSegCols, p.n - col);
-                        if (p.align == 8) store_rows<T, uint2>(buf, out, p.ldo, rows, cols, lane);
-                        else if (p.align == 4) store_rows<T, uint32_t>(buf, out, p.ldo, rows, cols, lane);
+                        if constexpr (kOut == Out::k8) store_rows<T, uint2>(buf, out, p.ldo, rows, cols, lane);
+                        else if constexpr (kOut == Out::k4) store_rows<T, uint32_t>(buf, out, p.ldo, rows, cols, lane);
                         else if constexpr (!kF32) store_rows<T, uint16_t>(buf, out, p.ldo, rows, cols, lane);
                     }
                     __syncwarp();
@@ -432,7 +447,7 @@ gemm_scaled_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
             acc ^= 1;
             phase ^= acc == 0;
         }
-        if (p.align == 16 && lane == 0) tc::tma_store_wait_all();
+        if (kOut == Out::kTma && lane == 0) tc::tma_store_wait_all();
     }
     tc::tc_fence_before();
     __syncthreads();
@@ -440,6 +455,16 @@ gemm_scaled_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
         tc::tc_fence_after();
         tc::tmem_dealloc(tmem_base, 2 * kBN);
     }
+}
+
+template <class T, Out kOut>
+cudaError_t launch_big(const CUtensorMap& ta, const CUtensorMap& tb, const BigParams& p, uint32_t tiles, cudaStream_t s) {
+    static std::atomic<uint64_t> configured{0};
+    const cudaError_t e = smem_optin_once(gemm_scaled_kernel<T, kOut>, kBigSmem, configured);
+    if (e != cudaSuccess) return e;
+    const uint32_t sms = device_sms();
+    gemm_scaled_kernel<T, kOut><<<tiles < sms ? tiles : sms, kBigThreads, kBigSmem, s>>>(ta, tb, p);
+    return cudaGetLastError();
 }
 
 template <class T>
@@ -455,18 +480,16 @@ cudaError_t launch_scaled(const CUtensorMap& ta, const CUtensorMap& tb, const Ge
     q.m = shape.M;
     q.n = shape.N;
     q.k = shape.K;
+    // (no map holds a pitch of 2^40 bytes)
+    if (p.vec && make_tmap_2d(&q.out_map, p.out,
+                              sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
+                              sizeof(T), shape.M, shape.N, p.ldo * sizeof(T), 32, 128 / sizeof(T)))
+        return launch_big<T, Out::kTma>(ta, tb, q, tiles, s);
     const uint64_t at = reinterpret_cast<uintptr_t>(p.out) | (p.ldo * sizeof(T));
-    q.align = at & 15u ? (at & 7u ? (at & 3u ? 2u : 4u) : 8u) : 16u;
-    if (q.align == 16 &&
-        !make_tmap_2d(&q.out_map, p.out, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
-                      sizeof(T), shape.M, shape.N, p.ldo * sizeof(T), 32, 128 / sizeof(T)))
-        q.align = 8;  // a pitch that no map holds (2^40 bytes)
-    static std::atomic<uint64_t> configured{0};
-    const cudaError_t e = smem_optin_once(gemm_scaled_kernel<T>, kBigSmem, configured);
-    if (e != cudaSuccess) return e;
-    const uint32_t sms = device_sms();
-    gemm_scaled_kernel<T><<<tiles < sms ? tiles : sms, kBigThreads, kBigSmem, s>>>(ta, tb, q);
-    return cudaGetLastError();
+    if (at % 8 == 0) return launch_big<T, Out::k8>(ta, tb, q, tiles, s);
+    if (at % 4 == 0) return launch_big<T, Out::k4>(ta, tb, q, tiles, s);
+    if constexpr (sizeof(T) == 2) return launch_big<T, Out::k2>(ta, tb, q, tiles, s);
+    return cudaErrorInvalidValue;
 }
 
 }  // namespace
