@@ -12,6 +12,8 @@ runs on the GPU and the ids come back on the input's device.
 ``run_conditioned_candidate_cache`` is the prefix-conditioned form
 (conditioned._run_conditioned_ddpm_candidate_cache, conditioned.py:132-242,
 with prefix K/V reuse under prefix isolation, prefix_drift.py:155-238).
+
+``score_tokens`` scores given tokens at the masked positions of a canvas.
 """
 
 from __future__ import annotations
@@ -156,3 +158,46 @@ def run_event_sampler(model: MDLMEngine, *, canvas_tokens: int = 64, prefix_toke
         "selected_output_rows": canvas_tokens,
         "prefix_tokens": len(prefix),
     }
+
+
+def score_tokens(model: MDLMEngine, input_ids: Any, target_ids: Any, *, mask_token_id: int, top_k: int = 0,
+                 every_position: bool = False) -> dict:
+    """How probable `target_ids` [B, L] are at the masked positions of the
+    canvas `input_ids` [B, L], by one forward and the fused head
+    (mdlm._mdlm_log_probabilities, mdlm.py:851-858, whose [B, L, V] array is
+    never made).  every_position: score the unmasked positions too.
+
+    Returns tensors on the device of `input_ids`: "scored" bool [B, L];
+    "logprobs" and "entropy" fp32 [B, L], 0 where nothing is scored;
+    "sequence_logprobs" [B], the sums of "logprobs"; and with top_k > 0
+    "top_ids" int32 and "top_logprobs" [B, L, top_k], -1 and -inf where
+    nothing is scored."""
+    import torch
+
+    if mask_token_id != model.cfg.mask_token_id:
+        raise ValueError("mask_token_id does not match the model")
+    shape = (model.B, model.L)
+    if tuple(input_ids.shape) != shape or tuple(target_ids.shape) != shape:
+        raise ValueError(f"input_ids and target_ids must be [{model.B}, {model.L}]")
+    src, dev = input_ids.device, model.device
+    ids = input_ids.to(dev, torch.int32).reshape(-1).contiguous()
+    targets = target_ids.to(dev, torch.int64).reshape(-1)
+    scored = torch.ones_like(ids, dtype=torch.bool) if every_position else ids == mask_token_id
+    rows = scored.nonzero().reshape(-1)
+    model.forward(ids)
+    r = model.score(targets[rows], rows=rows, top_k=top_k)
+
+    def spread(values: Any, fill: float) -> Any:
+        out = torch.full((model.M, *values.shape[1:]), fill, dtype=values.dtype, device=dev)
+        out[rows] = values
+        return out.view(*shape, *values.shape[1:]).to(src)
+
+    logprobs = spread(r.logprobs, 0.0)
+    out = {"scored": scored.view(shape).to(src), "logprobs": logprobs, "entropy": spread(r.entropy, 0.0),
+           "sequence_logprobs": logprobs.sum(1)}
+    if top_k:
+        out["top_ids"] = spread(r.top_ids, -1)
+        out["top_logprobs"] = spread(r.top_logprobs, float("-inf"))
+    with torch.cuda.device(dev):
+        _lib.check_device_error()
+    return out

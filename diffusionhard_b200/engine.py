@@ -28,6 +28,7 @@ import numpy as np
 from . import _lib
 from .model import QuantizedMDLM
 from .sampler import NOISE_EPSILON, MDLMStepMeasurement, hardware_candidate_cache_bytes, reveal_thresholds_q32
+from .scoring import TokenScores, head_logprobs, linear_i8
 
 
 class _DevLinear:
@@ -242,21 +243,47 @@ class MDLMEngine:
 
     @_on_device
     def logits(self) -> Any:
-        """fp32 logits [B, L, V] of the last forward: a debug / drift-analysis
-        path (the samplers never materialise logits).  int32 accumulators of
-        the int8 head from the tensor-core GEMM, then the reference dequant
-        out = fp32(acc * fp64(a_scale * w_scale) + bias)
+        """fp32 logits [B, L, V] of the last forward, for drift analysis and
+        debugging (the samplers and `score` never materialise logits): the
+        int8 head product with the reference dequant
+        out = fp32(acc * fp64(a_scale * w_scale) + bias) in its epilogue
         (fixed_mlp.quantized_linear, fixed_mlp.py:120-136)."""
-        torch = self.torch
         hq, hs = self.final_hidden_q()
         h = self.head
-        V = h.out_features
-        acc = torch.empty((self.M, V), dtype=torch.int32, device=self.device)
-        _lib.call("dh_gemm_i8_s32", self._p(hq), 768, self._p(h.w), 768, self._p(acc), V, self.M, V, 768,
-                  _lib.stream_handle())
-        combined = (hs[:, None] * h.w_scale[None, :]).double()
-        out = (acc.double() * combined + h.bias.double()[None, :]).float()
-        return out.view(self.B, self.L, V)
+        return linear_i8(hq, hs, h.w, h.w_scale, h.bias).view(self.B, self.L, h.out_features)
+
+    @_on_device
+    def score(self, targets: Any = None, *, rows: Any = None, top_k: int = 0) -> TokenScores:
+        """Scores of the last forward's distributions under the SUBS
+        parametrisation (mask token excluded; mdlm._mdlm_log_probabilities,
+        mdlm.py:851-858), the head's logits never stored: log probabilities of
+        `targets`, entropy, logsumexp and the `top_k` best tokens.
+
+        rows: int positions [n] of the flattened [B * L] canvas (default: all
+        of them, in order); targets: ids [n] or [n, tokens] for these rows,
+        a negative id for "no token"."""
+        torch = self.torch
+        h = self.head
+        if h.out_features != self.cfg.vocab_size:
+            raise ValueError("a vocabulary-sharded head holds no whole distribution")
+        if rows is None:
+            n = self.M
+            hq, hs = self.final_hidden_q()
+        else:
+            rows = rows.reshape(-1).to(device=self.device, dtype=torch.int32).contiguous()
+            n = rows.numel()
+            if n > self.M:
+                raise ValueError(f"at most {self.M} rows at a time")
+            if n and (int(rows.min()) < 0 or int(rows.max()) >= self.M):
+                raise ValueError("rows must lie inside the canvas")
+            if n:
+                hq, hs = self.final_hidden_q(rows, torch.tensor([n], dtype=torch.int32, device=self.device))
+            else:
+                hq, hs = self.head_q, self.head_scale
+        if targets is not None:
+            targets = targets.to(self.device)
+        return head_logprobs(hq[:n], hs[:n], h.w, h.w_scale, h.bias, targets, top_k=top_k,
+                             mask_token_id=self.cfg.mask_token_id)
 
     @_on_device
     def selected_logits(self, input_ids: Any, selected: Any) -> Any:
@@ -277,12 +304,7 @@ class MDLMEngine:
         cnt = torch.tensor([n], dtype=torch.int32, device=self.device)
         hq, hs = self.final_hidden_q(rows, cnt)
         h = self.head
-        V = h.out_features
-        acc = torch.empty((n, V), dtype=torch.int32, device=self.device)
-        _lib.call("dh_gemm_i8_s32", self._p(hq), 768, self._p(h.w), 768, self._p(acc), V, n, V, 768,
-                  _lib.stream_handle())
-        combined = (hs[:n, None] * h.w_scale[None, :]).double()
-        return (acc.double() * combined + h.bias.double()[None, :]).float()
+        return linear_i8(hq[:n], hs[:n], h.w, h.w_scale, h.bias)
 
     @_on_device
     def head_argmax(self, rows: int, mode: int, rows_count: Any = None, row_position: Any = None,
