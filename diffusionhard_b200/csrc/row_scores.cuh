@@ -149,18 +149,44 @@ DH_DEVINL float lanes_max(float v) {
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(v));
     return y;
 }
-// The k-th largest of the lanes' pairs a >= b (1 <= k <= 64, no NaN).  Whole warp.
+// One step of a bitonic sort across the lanes: partners `stride` apart, the
+// larger first where `desc`.
+DH_DEVINL float sort_step(float v, uint32_t stride, bool desc, uint32_t lane) {
+    const float o = __shfl_xor_sync(kFullMask, v, stride);
+    return ((lane & stride) != 0) != desc ? fmaxf(v, o) : fminf(v, o);
+}
+
+// The k-th largest of the lanes' pairs a >= b (1 <= k <= 64, no NaN): one maximum
+// after the other for a small k (~115 clocks each), else a sort of the 64.
+// Rolled up: code that runs once a row is fetched from afar each time, and
+// unrolled loops took longer to fetch than to run.  Whole warp.
 DH_DEVINL float kth_largest_of_pairs(float a, float b, uint32_t k, uint32_t lane) {
-    float y = 0.f;
+    if (k <= 8) {
+        float y = 0.f;
 #pragma unroll 1
-    for (uint32_t i = 0; i < k; ++i) {
-        y = lanes_max(a);
-        if (lane == __ffs(__ballot_sync(kFullMask, a == y)) - 1) {
-            a = b;
-            b = -CUDART_INF_F;
+        for (uint32_t i = 0; i < k; ++i) {
+            y = lanes_max(a);
+            if (lane == __ffs(__ballot_sync(kFullMask, a == y)) - 1) {
+                a = b;
+                b = -CUDART_INF_F;
+            }
+        }
+        return y;
+    }
+#pragma unroll 1
+    for (uint32_t size = 2; size <= 64; size <<= 1) {
+        if (size == 64) {
+            const float hi = fmaxf(a, b);
+            b = fminf(a, b);
+            a = hi;
+        }
+#pragma unroll 1
+        for (uint32_t stride = size == 64 ? 16 : size >> 1; stride > 0; stride >>= 1) {
+            a = sort_step(a, stride, size >= 32 || (lane & size) == 0, lane);
+            b = sort_step(b, stride, size == 64 || (size < 32 && (lane & size) == 0), lane);
         }
     }
-    return y;
+    return __shfl_sync(kFullMask, k <= 32 ? a : b, (k - 1) % 32);
 }
 // v joins the two largest of a set, a >= b.
 DH_DEVINL void two_largest(float& a, float& b, float v) {

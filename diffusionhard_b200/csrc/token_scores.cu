@@ -209,51 +209,37 @@ DH_DEVINL uint32_t batch_id(uint32_t stage, uint32_t thread) { return stage * kS
 template <class T>
 DH_DEVINL void collect(TopList& best, const RowView<T>& r, float bound, const uint32_t* batches, uint32_t n,
                        uint32_t lane) {
-    constexpr uint32_t VE = RowView<T>::VE, kUnroll = 4;
-    // all reads of 32 batches go out together: under the stream's load a round
-    // trip takes microseconds
+    constexpr uint32_t VE = RowView<T>::VE;
+    // (rolled up like all that runs once a row: see kth_largest_of_pairs)
 #pragma unroll 1
-    for (uint32_t i0 = 0; i0 < n * kScoreUnroll; i0 += 32 * kUnroll) {
-        uint4 raw[kUnroll];
-        uint32_t at[kUnroll];
+    for (uint32_t i0 = 0; i0 < n * kScoreUnroll; i0 += 32) {
+        const uint32_t i = i0 + lane;
+        uint32_t reach = 0, at = 0;  // which of the lane's logits reach the bound
+        float2 f[VE / 2];
+        if (i < n * kScoreUnroll) {
+            const uint32_t b = batches[i / kScoreUnroll];
+            at = r.v_lo + b / kScoreThreads * kStageVecs + b % kScoreThreads + i % kScoreUnroll * kScoreThreads;
+            if (at < r.v_hi) {
+                unpack(r.vector(at), f, T());
 #pragma unroll
-        for (uint32_t u = 0; u < kUnroll; ++u) {
-            const uint32_t i = i0 + 32 * u + lane;
-            at[u] = 0xFFFFFFFFu;
-            raw[u] = make_uint4(0u, 0u, 0u, 0u);
-            if (i < n * kScoreUnroll) {
-                const uint32_t b = batches[i / kScoreUnroll];
-                const uint32_t v = r.v_lo + b / kScoreThreads * kStageVecs + b % kScoreThreads + i % kScoreUnroll * kScoreThreads;
-                if (v < r.v_hi) {
-                    at[u] = v;
-                    raw[u] = r.vector(v);
+                for (uint32_t e = 0; e < VE; ++e) {
+                    const float y = e & 1 ? f[e / 2].y : f[e / 2].x;
+                    if (y >= bound && y > -CUDART_INF_F) reach |= 1u << e;
                 }
             }
         }
-#pragma unroll
-        for (uint32_t u = 0; u < kUnroll; ++u) {
-            float2 f[VE / 2];
-            unpack(raw[u], f, T());
-            uint32_t reach = 0;
-#pragma unroll
-            for (uint32_t e = 0; e < VE; ++e) {
-                const float y = e & 1 ? f[e / 2].y : f[e / 2].x;
-                if (y >= bound && y > -CUDART_INF_F) reach |= 1u << e;
-            }
-            if (at[u] == 0xFFFFFFFFu) reach = 0;
 #pragma unroll 1
-            while (__any_sync(kFullMask, reach != 0)) {
-                uint64_t key = 0;
-                if (reach) {
-                    const uint32_t e = __ffs(reach) - 1;
-                    reach &= reach - 1;
-                    float y = f[0].x;
+        while (__any_sync(kFullMask, reach != 0)) {
+            uint64_t key = 0;
+            if (reach) {
+                const uint32_t e = __ffs(reach) - 1;
+                reach &= reach - 1;
+                float y = f[0].x;
 #pragma unroll
-                    for (uint32_t j = 1; j < VE; ++j) y = j == e ? (j & 1 ? f[j / 2].y : f[j / 2].x) : y;
-                    key = token_key(y, at[u] * VE - r.off + e);
-                }
-                best.add(key);
+                for (uint32_t j = 1; j < VE; ++j) y = j == e ? (j & 1 ? f[j / 2].y : f[j / 2].x) : y;
+                key = token_key(y, at * VE - r.off + e);
             }
+            best.add(key);
         }
     }
 }
@@ -460,7 +446,7 @@ token_scores_kernel(const __grid_constant__ LogitRows p) {
 #pragma unroll 1
                 for (uint32_t j = 0; j < stages; ++j) {
                     n = 0;
-#pragma unroll
+#pragma unroll 2
                     for (uint32_t w = 0; w < kScoreWarps; ++w) {
                         const uint32_t i = w * 32 + lane;
                         gather(all ? sm.m[f][i] : sm.m_first[f][i], batch_id(j, i));
