@@ -62,6 +62,10 @@ static_assert(kSmemFixed + kStreamedStages * (kABytes + kBBytes) <= kSmemLimit, 
 constexpr uint32_t kExactK = 1024;
 constexpr uint64_t kMaxTiles = 1u << 30;
 
+// Logits up to this size take the epilogue's short way.  (Bases up to kSlipBase
+// carry a slip, at most 64 there; a logit is then 2e8 below any larger base.)
+constexpr float kPlainLogit = 8e8f, kSlipBase = 1e9f;
+
 // How a launch splits the work, shared by the two kernels: CTA c takes `each`
 // tiles, and one more if c < more, after those of the CTAs before it.
 struct HeadSplit {
@@ -103,7 +107,10 @@ DH_DEVINL float max3(float a, float b, float c) {
 }
 
 // A row's running statistics in this kernel: pairs of sums of e = 2^z and of
-// e z, z = (x - base) log2 e.
+// e z, z = (x - base) log2 e + slip.  slip is what rounding base log2 e to fp32
+// leaves off, so that z of a usual logit is one FMA, x log2 e - neg_base2, and
+// no error of base's size enters (dropping it: the log probabilities of logits
+// around 1e6 were off by 0.04, and past 1e9 it overflowed).
 struct PairStats {
     float base;  // -inf before the first logit above it
     float2 s, t;
@@ -111,19 +118,33 @@ struct PairStats {
         base = -CUDART_INF_F;
         s = t = make_float2(0.f, 0.f);
     }
-    // a new maximum (rare once a row has begun)
-    DH_DEVINL void raise(float m) {
-        const float z = base == -CUDART_INF_F ? 0.f : max_nan((base - m) * kLog2E, -1e30f), f = exp2_fast(z);
+    // -base log2 e as fp32; bounded, so that the z of a logit far below stays finite
+    DH_DEVINL static float neg_base2(float base) { return fmaxf(-__fmul_rn(base, kLog2E), -1e38f); }
+    // (a base past kSlipBase is met by usual logits from so far below that their
+    // e is 0 whatever the slip)
+    DH_DEVINL static float slip(float base) {
+        return fabsf(base) < kSlipBase ? __fmaf_rn(base, kLog2E, neg_base2(base)) : 0.f;
+    }
+    // z of the base in terms of another base
+    DH_DEVINL void shift(float z) {
+        const float f = exp2_fast(z);
         s = make_float2(s.x * f, s.y * f);
         t = make_float2(__fmaf_rn(s.x, z, f * t.x), __fmaf_rn(s.y, z, f * t.y));
+    }
+    // a new maximum (rare once a row has begun)
+    DH_DEVINL void raise(float m) {
+        shift(base == -CUDART_INF_F ? 0.f : max_nan(__fmaf_rn(base - m, kLog2E, slip(m) - slip(base)), -1e30f));
         base = m;
     }
-    DH_DEVINL RowStats sum() const { return RowStats{base, s.x + s.y, (t.x + t.y) * kLn2}; }
+    DH_DEVINL RowStats sum() {
+        shift(-slip(base));
+        return RowStats{base, s.x + s.y, (t.x + t.y) * kLn2};
+    }
 };
 
 // 32 columns of 4 rows (8 logits of each): accumulators to logits, to the rows'
-// statistics, and their maxima to g.  kClamp: some logit may be -inf (or NaN),
-// or so far below the others that a difference overflows.
+// statistics, and their maxima to g.  kClamp: some logit may be -inf or NaN, or
+// past kPlainLogit.
 template <bool kWide, bool kTop, bool kClamp>
 DH_DEVINL void add_block(PairStats (&st)[4], float (&g)[4], const uint32_t (&v)[2][16], const float (&ab)[4],
                          const float2 (&w)[4], const float2 (&b)[4]) {
@@ -157,13 +178,13 @@ DH_DEVINL void add_block(PairStats (&st)[4], float (&g)[4], const uint32_t (&v)[
             if (m[r] > st[r].base + kBaseSlack) st[r].raise(m[r]);
     }
     const float2 c2 = make_float2(kLog2E, kLog2E);
-    float2 nb[4];  // z is one FMA: the product of base and log2 e is rounded once for all logits
+    float2 nb[4], slip[4];
 #pragma unroll
     for (uint32_t r = 0; r < 4; ++r) {
-        float y = -st[r].base;
-        if (kClamp) y = st[r].base == -CUDART_INF_F ? 0.f : y;
-        else y = __fmul_rn(y, kLog2E);
+        const float base = st[r].base;
+        const float y = kClamp ? (base == -CUDART_INF_F ? 0.f : -base) : PairStats::neg_base2(base);
         nb[r] = make_float2(y, y);
+        if (kClamp) slip[r].x = slip[r].y = PairStats::slip(base);
     }
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
@@ -171,7 +192,7 @@ DH_DEVINL void add_block(PairStats (&st)[4], float (&g)[4], const uint32_t (&v)[
         for (uint32_t r = 0; r < 4; ++r) {
             float2 z;
             if (kClamp) {
-                z = __fmul2_rn(__fadd2_rn(x[r][j], nb[r]), c2);
+                z = __ffma2_rn(__fadd2_rn(x[r][j], nb[r]), c2, slip[r]);
                 z = make_float2(max_nan(z.x, -1e30f), max_nan(z.y, -1e30f));
             } else {
                 z = __ffma2_rn(x[r][j], c2, nb[r]);
@@ -368,29 +389,29 @@ head_stats_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                 }
             }
         };
-        bool odd_row = false;
+        float reach = 0.f;  // bounds |acc a_scale| of the warp's rows
         auto fetch_rows = [&](uint32_t m) {
-            odd_row = false;
+            float top = 0.f;
 #pragma unroll
             for (uint32_t r = 0; r < 4; ++r) {
                 const uint32_t row = m * kBM + row_in + 8 * r;
                 ab[r] = row < p.split.rows ? __ldg(p.a_scale + row) : 0.f;
-                odd_row = odd_row || !(fabsf(ab[r]) < 1e11f);
+                const float size = fabsf(ab[r]);
+                top = fmaxf(top, size < CUDART_INF_F ? size : CUDART_INF_F);  // (NaN: infinite)
             }
+            reach = lanes_max(top) * (16384.f * static_cast<float>(p.k));
         };
         fetch(nt);
         fetch_rows(mt);
         uint32_t acc = 0, phase = 0;
         for (uint32_t tile = tile0; tile < tile1; ++tile) {
             __syncwarp();
-            bool odd = odd_row;
+            bool odd = false;  // a logit may be past kPlainLogit, -inf or NaN
 #pragma unroll
             for (uint32_t i = 0; i < kPartCols / 32; ++i) {
                 bs[i * 32 + lane] = b_next[i];
                 ws[i * 32 + lane] = w_next[i];
-                // within these no logit overflows, so no difference of two is
-                // infinite or NaN
-                odd = odd || !(fabsf(b_next[i]) < 1e37f && fabsf(w_next[i]) < 1e18f);
+                odd = odd || !(fabsf(b_next[i]) < kPlainLogit / 2 && fabsf(w_next[i]) * reach < kPlainLogit / 2);
             }
             odd = __any_sync(kFullMask, odd);
             __syncwarp();

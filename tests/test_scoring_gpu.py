@@ -369,6 +369,42 @@ def test_head_logprobs_odd_rows(cuda):
     check_scores(got._replace(top_ids=None, top_logprobs=None), x, t[:2], 0)
 
 
+@pytest.mark.parametrize("size", [64, 1040])
+@pytest.mark.parametrize("shift", [0.0, 1e4, -1e6, 3e8, -5e8, 1e10, 1e30])
+def test_head_logprobs_far_from_zero(cuda, size, shift):
+    """Logits of any magnitude, about 0 or around a common value."""
+    (a, sa, w, sw, b), t = head_case(9, 3000, size, 7)
+    sa *= torch.tensor([1.0, 1e3, 1e6, 1e8, 1e9, 1e11, 1e14, 1e30, 0.0])
+    b += shift
+    b[2000:2100] -= abs(shift)  # one block of columns lies elsewhere
+    x = ref_linear(a, sa, w, sw, b)[1].float().double()
+    for k in (0, 5):
+        check_scores(scoring.head_logprobs(*cu((a, sa, w, sw, b)), t.cuda(), top_k=k), x, t, k)
+
+
+@pytest.mark.parametrize("size", [64, 1040])
+@pytest.mark.parametrize("shift, scale", [(1e4, 1.0), (-1e6, 1.0), (3e8, 1.0), (-1e10, 1.0), (0.0, 1e4), (0.0, 1e7),
+                                          (-1e5, 1e9), (0.0, 1e12)])
+def test_head_logprobs_same_magnitude(cuda, size, shift, scale):
+    """All rows' logits around the same large value, or as far apart."""
+    (a, sa, w, sw, b), t = head_case(9, 3000, size, 9)
+    b += shift
+    x = ref_linear(a, sa * scale, w, sw, b)[1].float().double()
+    for k in (0, 5):
+        check_scores(scoring.head_logprobs(*cu((a, sa * scale, w, sw, b)), t.cuda(), top_k=k), x, t, k)
+
+
+@pytest.mark.parametrize("at", [5, 600, 2999])
+def test_head_logprobs_lone_giants(cuda, at):
+    """One logit near the largest or the lowest number among usual ones."""
+    (a, sa, w, sw, b), t = head_case(5, 3000, 64, 8)
+    for value in (3e38, 2e38, 1.1e9, -3e38):
+        b[at] = value
+        x = ref_linear(a, sa, w, sw, b)[1].float().double()
+        for k in (0, 3):
+            check_scores(scoring.head_logprobs(*cu((a, sa, w, sw, b)), t.cuda(), top_k=k), x, t, k)
+
+
 def test_head_logprobs_padded_rows(cuda):
     (a, sa, w, sw, b), t = head_case(21, 333, 100, 2)
     x = ref_linear(a, sa, w, sw, b)[1].float().double()
