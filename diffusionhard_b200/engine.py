@@ -260,8 +260,8 @@ class MDLMEngine:
         `targets`, entropy, logsumexp and the `top_k` best tokens.
 
         rows: int positions [n] of the flattened [B * L] canvas (default: all
-        of them, in order); targets: ids [n] or [n, tokens] for these rows,
-        a negative id for "no token"."""
+        of them, in order; checked on the host, which waits for them); targets:
+        ids [n] or [n, tokens] for these rows, a negative id for "no token"."""
         torch = self.torch
         h = self.head
         if h.out_features != self.cfg.vocab_size:
@@ -270,12 +270,15 @@ class MDLMEngine:
             n = self.M
             hq, hs = self.final_hidden_q()
         else:
-            rows = rows.reshape(-1).to(device=self.device, dtype=torch.int32).contiguous()
+            if rows.dtype not in (torch.int32, torch.int64):
+                raise ValueError("rows must be int32 or int64")
+            rows = rows.reshape(-1)
             n = rows.numel()
             if n > self.M:
                 raise ValueError(f"at most {self.M} rows at a time")
             if n and (int(rows.min()) < 0 or int(rows.max()) >= self.M):
                 raise ValueError("rows must lie inside the canvas")
+            rows = rows.to(device=self.device, dtype=torch.int32).contiguous()
             if n:
                 hq, hs = self.final_hidden_q(rows, torch.tensor([n], dtype=torch.int32, device=self.device))
             else:

@@ -154,3 +154,12 @@ def test_refusals(engine):
     with pytest.raises(ValueError, match="sharded"):
         sharded.score()
     assert sharded.logits().shape == (1, 32, 500)
+
+
+def test_rows_of_other_types(engine):
+    """Rows are checked as they are given, not after they were narrowed."""
+    for bad in (torch.tensor([2 ** 32]), torch.tensor([-2 ** 32 + 1]), torch.tensor([0.5]), torch.tensor([True])):
+        with pytest.raises(ValueError, match="rows"):
+            engine.score(rows=bad)
+    a = engine.score(rows=torch.tensor([3, 5], dtype=torch.int32), top_k=2)
+    assert torch.equal(a.top_ids, engine.score(rows=torch.tensor([3, 5]).cuda(), top_k=2).top_ids)
