@@ -179,8 +179,8 @@ DH_DEVINL float scaled_f32(uint32_t acc, float combined, double bias) {
 // 128-byte swizzle of the TMA stores.
 DH_DEVINL uint32_t swz128(uint32_t r, uint32_t c) { return r * 128 + ((c ^ (r & 7u)) << 4); }
 
-// How outputs leave the warp's buffer: by TMA (start and row pitch multiples of
-// 16 bytes), or through the registers, 8, 4 or 2 bytes a lane.
+// How outputs leave the warp's buffer: by TMA (start, row pitch and the rows' own
+// bytes multiples of 16), or through the registers, 8, 4 or 2 bytes a lane.
 enum class Out { kTma, k8, k4, k2 };
 
 // The warp's buffer, 32 rows x 128 bytes, to rows of any pitch: the first `cols`
@@ -480,8 +480,9 @@ cudaError_t launch_scaled(const CUtensorMap& ta, const CUtensorMap& tb, const Ge
     q.m = shape.M;
     q.n = shape.N;
     q.k = shape.K;
-    // (no map holds a pitch of 2^40 bytes)
-    if (p.vec && make_tmap_2d(&q.out_map, p.out,
+    // (a store that ends inside 16 bytes writes all 16, beside the outputs; no map
+    // holds a pitch of 2^40 bytes)
+    if (p.vec && shape.N * sizeof(T) % 16 == 0 && make_tmap_2d(&q.out_map, p.out,
                               sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
                               sizeof(T), shape.M, shape.N, p.ldo * sizeof(T), 32, 128 / sizeof(T)))
         return launch_big<T, Out::kTma>(ta, tb, q, tiles, s);

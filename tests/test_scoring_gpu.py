@@ -204,8 +204,6 @@ def test_token_logprobs_far_rows(cuda):
     check_scores(scoring.token_logprobs(x, t.cuda(), top_k=3), src.double(), t, 3)
 
 
-# ------------------------------------------------------------ linear_i8
-
 def linear_case(m, n, k, seed, bias=True):
     g = torch.Generator().manual_seed(seed)
     a = torch.randint(-127, 128, (m, k), generator=g, dtype=torch.int32).to(torch.int8)
@@ -275,6 +273,32 @@ def test_linear_i8_out(cuda, dtype, pitch, start, m):
     ret = scoring.linear_i8(*dev, out=out)
     assert ret is out
     assert torch.equal(out, scoring.linear_i8(*dev, out_dtype=dtype))
+    out.fill_(7.0)
+    assert bool((buf == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, pitch, start", [
+    (5008, 5008, 0), (5008, 5024, 16), (5003, 5008, 0), (5002, 5002, 0), (5002, 5004, 2), (5001, 5001, 0),
+    (5001, 5010, 1), (5000, 5004, 4), (4900, 4902, 6),
+])
+def test_linear_i8_out_large(cuda, dtype, n, pitch, start):
+    """The large tiles: outputs of every alignment, ragged in rows and columns, and nothing beside them."""
+    m = 390
+    args = linear_case(m, n, 80, n + pitch)
+    dev = cu(args)
+    buf = torch.full((m + 2, pitch), 7.0, dtype=dtype, device="cuda")
+    flat = buf.view(-1)[start:start + m * pitch]
+    out = flat.as_strided((m, n), (pitch, 1), flat.storage_offset())
+    scoring.linear_i8(*dev, out=out)
+    y = ref_linear(*args)[1]
+    if dtype == torch.float32:
+        assert torch.equal(out.cpu(), y.float())
+    else:
+        prod = y - args[4].double()
+        lim = torch.finfo(dtype)
+        tol = U * (prod.abs() + y.abs()) * 1.01 + lim.eps / 2 * 1.01 * y.abs().clamp(min=lim.tiny)
+        assert bool(((out.cpu().double() - y).abs() <= tol).all())
     out.fill_(7.0)
     assert bool((buf == 7.0).all())
 
