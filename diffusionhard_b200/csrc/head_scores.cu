@@ -570,11 +570,23 @@ DH_DEVINL int2 group_sums(const int8_t* h, const int8_t* w, uint64_t ldw, uint32
 }
 
 constexpr uint32_t kRowWarps = 8;
-constexpr uint32_t kMaxStaged = 1280;  // words of shared memory a row: vocabularies up to 81,920
+constexpr uint32_t kMaxStaged = 1185;  // words of shared memory a row: vocabularies up to 75,776
 constexpr uint32_t kPicks = 96;  // groups kept for the k best (more, by ties: every group is looked at)
 // Rows below which each gets a CTA: 512 rows 46 / 50 us (1 / 8 alternatives)
 // against 44 / 64 with a warp each, 1001 rows 71 / 79 against 58 / 80.
 constexpr uint32_t kTeamRows = 768;
+
+template <uint32_t kTeam>
+struct RowsSmem {
+    static constexpr uint32_t kTeams = kRowWarps / kTeam;
+    float part_base[kRowWarps], part_s[kRowWarps], part_t[kRowWarps];
+    uint64_t keys[kRowWarps][32], lists[kTeam > 1 ? kRowWarps : 1][32];
+    uint32_t picks[kTeams][kPicks], pick_count[kTeams];
+    uint32_t parts[kRowWarps][160];
+    float pairs[kTeam > 1 ? kRowWarps : 1][2][32];
+};
+static_assert(sizeof(RowsSmem<1>) + kMaxStaged * kRowWarps * sizeof(float) <= 48 * 1024,
+              "shared memory of a launch without an opt-in");
 
 // kTeam warps a row: 1 when there are rows enough for every warp of the GPU,
 // all of a CTA's when there are few.
@@ -583,11 +595,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 4)
 head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged) {
     extern __shared__ float staged_max[];  // the part maxima of the CTA's rows, if `staged` holds them: [kTeams][staged]
     constexpr uint32_t kTeams = kRowWarps / kTeam;
-    __shared__ float part_base[kRowWarps], part_s[kRowWarps], part_t[kRowWarps];
-    __shared__ uint64_t keys[kRowWarps][32], lists[kRowWarps][32];
-    __shared__ uint32_t picks[kTeams][kPicks], pick_count[kTeams];
-    __shared__ uint32_t parts[kRowWarps][160];
-    __shared__ float pairs[kTeam > 1 ? kRowWarps : 1][2][32];
+    __shared__ RowsSmem<kTeam> sm;
 
     const uint32_t warp = warp_id(), lane = lane_id();
     const uint32_t team = warp / kTeam, member = warp % kTeam;
@@ -656,9 +664,9 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
     st.s = warp_sum_f32(st.s);
     st.t = warp_sum_f32(st.t);
     if (kTeam > 1 && lane == 0) {
-        part_base[warp] = top;
-        part_s[warp] = st.s;
-        part_t[warp] = st.t;
+        sm.part_base[warp] = top;
+        sm.part_s[warp] = st.s;
+        sm.part_t[warp] = st.t;
     }
 
     // the k-th largest of the lanes' maxima of parts (the two largest of each)
@@ -683,15 +691,15 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
 #pragma unroll
             for (uint32_t u = 0; u < 4; ++u) two_largest(a, b, v[u]);
         }
-        if (member == 0 && lane == 0) pick_count[team] = 0;
+        if (member == 0 && lane == 0) sm.pick_count[team] = 0;
         if (kTeam > 1) {
-            pairs[warp][0][lane] = a;
-            pairs[warp][1][lane] = b;
+            sm.pairs[warp][0][lane] = a;
+            sm.pairs[warp][1][lane] = b;
         }
     }
     team_sync();
     if (kTeam > 1) {
-        st = lane < kRowWarps ? RowStats{part_base[lane], part_s[lane], part_t[lane]} : RowStats{-CUDART_INF_F, 0.f, 0.f};
+        st = lane < kRowWarps ? RowStats{sm.part_base[lane], sm.part_s[lane], sm.part_t[lane]} : RowStats{-CUDART_INF_F, 0.f, 0.f};
         top = lanes_max(st.base);
         rebase(st, top);
         st.s = warp_sum_f32(st.s);
@@ -708,8 +716,8 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
         a = b = -CUDART_INF_F;
 #pragma unroll
         for (uint32_t w = 0; w < kRowWarps; ++w) {
-            two_largest(a, b, pairs[w][0][lane]);
-            two_largest(a, b, pairs[w][1][lane]);
+            two_largest(a, b, sm.pairs[w][0][lane]);
+            two_largest(a, b, sm.pairs[w][1][lane]);
         }
     }
     bound = kth_largest_of_pairs(a, b, k, lane);
@@ -725,7 +733,7 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
 #pragma unroll
             for (uint32_t u = 0; u < 4; ++u) {
                 const uint32_t who = __ballot_sync(kFullMask, v[u] >= bound && v[u] > -CUDART_INF_F);
-                if ((who >> lane) & 1u) parts[warp][n + __popc(who & ((1u << lane) - 1u))] = i0 + kStep * u + lane;
+                if ((who >> lane) & 1u) sm.parts[warp][n + __popc(who & ((1u << lane) - 1u))] = i0 + kStep * u + lane;
                 n += __popc(who);
             }
         }
@@ -734,15 +742,15 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
             // the 4 groups of 8 parts at a time
 #pragma unroll 1
             for (uint32_t j = lane / 4; j < n + lane / 4; j += 8) {
-                const uint32_t part = j < n ? parts[warp][j] : 0u;
+                const uint32_t part = j < n ? sm.parts[warp][j] : 0u;
                 const float y = j < n ? __ldg(p.group_max + p.split.slot(part, static_cast<uint32_t>(row)) * kGroupsPerPart +
                                               lane % 4)
                                       : -CUDART_INF_F;
                 const uint32_t in = __ballot_sync(kFullMask, y >= bound && y > -CUDART_INF_F);
                 uint32_t to = 0;
-                if (lane == 0 && in) to = atomicAdd(&pick_count[team], __popc(in));
+                if (lane == 0 && in) to = atomicAdd(&sm.pick_count[team], __popc(in));
                 to = __shfl_sync(kFullMask, to, 0) + __popc(in & ((1u << lane) - 1u));
-                if (((in >> lane) & 1u) && to < kPicks) picks[team][to] = part * kGroupsPerPart + lane % 4;
+                if (((in >> lane) & 1u) && to < kPicks) sm.picks[team][to] = part * kGroupsPerPart + lane % 4;
             }
             n = 0;
             __syncwarp();
@@ -750,12 +758,12 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
     }
     team_sync();
     // their logits
-    const bool all = pick_count[team] > kPicks;
-    const uint32_t n_pick = all ? p.split.n_tiles * kGroupsPerTile : pick_count[team];
-    TopList best(keys[warp], k, lane);
+    const bool all = sm.pick_count[team] > kPicks;
+    const uint32_t n_pick = all ? p.split.n_tiles * kGroupsPerTile : sm.pick_count[team];
+    TopList best(sm.keys[warp], k, lane);
 #pragma unroll 1
     for (uint32_t i = member; i < n_pick; i += kTeam) {
-        const uint32_t group = all ? i : picks[team][i];
+        const uint32_t group = all ? i : sm.picks[team][i];
         if (all && !(__ldg(p.group_max + p.split.slot(i / kGroupsPerPart, static_cast<uint32_t>(row)) * kGroupsPerPart +
                            i % kGroupsPerPart) >= bound))
             continue;
@@ -769,13 +777,13 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
     }
     best.flush();
     if (kTeam > 1) {
-        lists[warp][lane] = best.list;
+        sm.lists[warp][lane] = best.list;
         __syncthreads();
         if (member != 0) return;
         uint64_t least_of = 0;
-        for (uint32_t w = 0; w < kTeam; ++w) least_of = lists[w][k - 1] > least_of ? lists[w][k - 1] : least_of;
-        TopList all(keys[warp], k, lane);
-        for (uint32_t w = 0; w < kTeam; ++w) all.add(lists[w][lane] >= least_of ? lists[w][lane] : 0ull);
+        for (uint32_t w = 0; w < kTeam; ++w) least_of = sm.lists[w][k - 1] > least_of ? sm.lists[w][k - 1] : least_of;
+        TopList all(sm.keys[warp], k, lane);
+        for (uint32_t w = 0; w < kTeam; ++w) all.add(sm.lists[w][lane] >= least_of ? sm.lists[w][lane] : 0ull);
         all.flush();
         best.list = all.list;
     }

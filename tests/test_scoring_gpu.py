@@ -393,6 +393,17 @@ def test_head_logprobs_odd_rows(cuda):
     check_scores(got._replace(top_ids=None, top_logprobs=None), x, t[:2], 0)
 
 
+@pytest.mark.parametrize("vocab", [75776, 75777, 80000, 81665, 90001])
+def test_head_logprobs_large_vocabularies(cuda, vocab):
+    """As many rows as get a warp each, around the vocabularies whose maxima shared memory holds."""
+    (a, sa, w, sw, b), t = head_case(770, vocab, 16, vocab)
+    got = scoring.head_logprobs(*cu((a, sa, w, sw, b)), t.cuda(), top_k=8, mask_token_id=vocab - 1)
+    pick = torch.tensor([0, 1, 127, 128, 400, 767, 768, 769])
+    x = ref_linear(a[pick], sa[pick], w, sw, b)[1].float().double()
+    some = got._replace(**{f: v[pick.cuda()] for f, v in got._asdict().items()})
+    check_scores(some, x, t[pick], 8, vocab - 1)
+
+
 @pytest.mark.parametrize("size", [64, 1040])
 @pytest.mark.parametrize("shift", [0.0, 1e4, -1e6, 3e8, -5e8, 1e10, 1e30])
 def test_head_logprobs_far_from_zero(cuda, size, shift):
