@@ -204,6 +204,21 @@ def test_token_logprobs_far_rows(cuda):
     check_scores(scoring.token_logprobs(x, t.cuda(), top_k=3), src.double(), t, 3)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [20001, 50258])
+def test_token_logprobs_many_equal_or_ordered(cuda, dtype, vocab):
+    """Rows most of whose logits reach the bound of the k best: all equal, rising, falling, in steps."""
+    i = torch.arange(vocab, dtype=torch.float64)
+    x = torch.stack([torch.full_like(i, -2.5), i / 4000, -i / 4000, (i / 1000).floor(), -(i / 1000).floor(),
+                     i % 7, torch.where(i % 4096 == 5, 3.0, 1.0)]).to(dtype)
+    t = torch.tensor([[0, vocab - 1, 4096]] * x.shape[0])
+    for k in (1, 7, 9, 32):
+        check_scores(scoring.token_logprobs(x.cuda(), t.cuda(), top_k=k, mask_token_id=vocab - 2), x.double(), t, k,
+                     vocab - 2)
+
+
+# ------------------------------------------------------------ linear_i8
+
 def linear_case(m, n, k, seed, bias=True):
     g = torch.Generator().manual_seed(seed)
     a = torch.randint(-127, 128, (m, k), generator=g, dtype=torch.int32).to(torch.int8)
@@ -303,6 +318,19 @@ def test_linear_i8_out_large(cuda, dtype, n, pitch, start):
     assert bool((buf == 7.0).all())
 
 
+def test_linear_i8_odd_scales_large(cuda):
+    """Scales of 0, infinity, NaN, negative, tiny and huge, and odd biases, in the large tiles."""
+    a, sa, w, sw, b = linear_case(300, 5000, 64, 12)
+    sa[::7] = torch.tensor([0.0, math.inf, math.nan, -0.5, 1e-38, 1e30, 1e-45] * 7)[:sa[::7].numel()]
+    sw[::11] = torch.tensor([0.0, math.inf, math.nan, -0.5, 1e-38, 1e30, 1e-45] * 66)[:sw[::11].numel()]
+    b[::13] = torch.tensor([math.inf, -math.inf, math.nan, 3e38, 1e-45] * 78)[:b[::13].numel()]
+    for rows in (300, 100):  # and the small tiles'
+        y = ref_linear(a[:rows], sa[:rows], w, sw, b)[1].float()
+        got = scoring.linear_i8(*cu((a[:rows], sa[:rows], w, sw, b))).cpu()
+        assert torch.equal(torch.isnan(got), torch.isnan(y))
+        assert torch.equal(got.nan_to_num(0.5), y.nan_to_num(0.5))
+
+
 def test_linear_i8_far_out(cuda):
     args = linear_case(3, 100, 64, 4)
     dev = cu(args)
@@ -350,6 +378,45 @@ def test_head_logprobs(cuda, rows, vocab, size, top_k):
     mask = None if rows % 2 else vocab // 3
     got = scoring.head_logprobs(*cu(args), t.cuda(), top_k=top_k, mask_token_id=mask)
     check_scores(got, x, t, top_k, mask)
+
+
+@pytest.mark.parametrize("size", [784, 800, 1024])
+@pytest.mark.parametrize("rows, top_k", [(3, 8), (300, 0), (300, 5)])
+def test_head_logprobs_streamed(cuda, rows, top_k, size):
+    """Hidden sizes past those whose rows stay in shared memory."""
+    args, t = head_case(rows, 3001, size, size)
+    x = ref_linear(*args)[1].float().double()
+    check_scores(scoring.head_logprobs(*cu(args), t.cuda(), top_k=top_k), x, t, top_k)
+
+
+@pytest.mark.parametrize("rows", [3, 800])
+@pytest.mark.parametrize("size", [64, 1040])
+def test_head_logprobs_many_equal(cuda, rows, size):
+    """Rows whose every logit, or every bias of many, is equal: more groups reach the bound than are kept."""
+    (a, sa, w, sw, b), t = head_case(rows, 6001, size, rows, bias=True)
+    sa[::2] = 0.0
+    b[:] = 1.5
+    b[4000:] = 0.25
+    pick = torch.tensor([0, 1, 2] if rows == 3 else [0, 1, 2, 7, 128, 511, 798, 799])
+    x = ref_linear(a[pick], sa[pick], w, sw, b)[1].float().double()
+    for k in (1, 8, 32):
+        got = scoring.head_logprobs(*cu((a, sa, w, sw, b)), t.cuda(), top_k=k, mask_token_id=2)
+        some = got._replace(**{f: v[pick.cuda()] for f, v in got._asdict().items()})
+        check_scores(some, x, t[pick], k, 2)
+
+
+def test_head_logprobs_far_weights(cuda):
+    """Row offsets past 2^32 bytes in the weights and the hidden rows."""
+    (a, sa, w, sw, b), t = head_case(5, 40, 48, 6)
+    buf = torch.empty(2 ** 27 * 40 + 4096, dtype=torch.int8, device="cuda")
+    wv = buf.as_strided((40, 48), (2 ** 27 + 16, 1))
+    av = buf.as_strided((5, 48), (2 ** 30 + 64, 1), 1024)
+    wv.copy_(w)
+    av.copy_(a)
+    assert torch.equal(wv.cpu(), w)
+    x = ref_linear(a, sa, w, sw, b)[1].float().double()
+    check_scores(scoring.head_logprobs(av, sa.cuda(), wv, sw.cuda(), b.cuda(), t.cuda(), top_k=4), x, t, 4)
+    assert torch.equal(scoring.linear_i8(av, sa.cuda(), wv, sw.cuda(), b.cuda()).cpu(), x.float())
 
 
 def test_head_logprobs_matches_two_steps(cuda):
