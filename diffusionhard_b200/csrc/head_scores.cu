@@ -16,6 +16,8 @@
 //    computes the logits of the groups that reach the bound (about k) again (the
 //    same fp32 expression of the same integer sum, so the same bits), like the
 //    given tokens' logits.
+#include <cuda_fp16.h>
+
 #include "dequant.cuh"
 #include "row_scores.cuh"
 #include "tc_ptx.cuh"
@@ -88,8 +90,8 @@ struct HeadScoreParams {
     const float* w_scale;
     const float* bias;   // or null
     float4* partials;    // [grid][max_segs][kParts][128]: base, s, t of a row's part
-    float* group_max;    // [n_tiles * kParts][rows][4], or null: none asked for
-    float* part_max;     // [n_tiles * kParts][rows]; rows rounded up to row tiles
+    uint2* group_max;    // [n_tiles * kParts][rows]: 4 groups' (group_at), or null: none asked for
+    uint16_t* part_max;  // [n_tiles * kParts][rows]; rows rounded up to row tiles
 };
 
 // The logit of one accumulator.  kWide: k > kExactK, where float(acc) would
@@ -105,6 +107,29 @@ DH_DEVINL float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
+
+// Maxima are stored as half floats, rounded toward zero (past their range: the
+// largest finite one; -inf stays): rounding keeps the order, so that every group
+// with a logit of the k best still reaches the rounded bound.  Groups within a
+// rounding step of it are looked at for nothing, so 8 bits (bfloat16) are too few:
+// 241 us for the second kernel with 32768 x 50258 and 5 alternatives.
+DH_DEVINL uint32_t half_pair(float lo, float hi) {
+    uint32_t y;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+    return y;
+}
+DH_DEVINL float half_float(uint32_t h) { return __half2float(__ushort_as_half(static_cast<uint16_t>(h))); }
+constexpr uint32_t kNonePair = 0xFC00FC00u;  // -inf twice
+DH_DEVINL uint32_t max_pairs(uint32_t a, uint32_t b) {
+    const __half2 m = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+DH_DEVINL uint32_t min_pairs(uint32_t a, uint32_t b) {
+    const __half2 m = __hmin2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+// Where a quarter's group lies among the 4, and the other way round.
+DH_DEVINL uint32_t group_at(uint32_t q) { return (q & 1u) << 1 | q >> 1; }
 
 // A row's running statistics in this kernel: pairs of sums of e = 2^z and of
 // e z, z = (x - base) log2 e + slip.  slip is what rounding base log2 e to fp32
@@ -443,15 +468,19 @@ head_stats_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                 else add_block<kWide, kTop, false>(st, g, v, ab, w, b);
             }
             if (kTop) {
-#pragma unroll
-                for (uint32_t r = 0; r < 4; ++r) {
-                    // (rows past the last have room, and hold what nothing reads)
-                    const uint64_t at = p.split.slot(nt * kParts + part, mt * kBM + row_in + 8 * r);
-                    p.group_max[at * kGroupsPerPart + quarter] = g[r];
-                    g[r] = fmaxf(g[r], __shfl_xor_sync(kFullMask, g[r], 1));
-                    g[r] = fmaxf(g[r], __shfl_xor_sync(kFullMask, g[r], 2));
-                    if (quarter == 0) p.part_max[at] = g[r];
-                }
+                // the 4 threads of a row hold a group each of 4 rows: after two
+                // exchanges each has a row's 4 groups, of quarters 0, 2 and 1, 3
+                const uint32_t p01 = half_pair(g[0], g[1]), p23 = half_pair(g[2], g[3]);
+                const bool odd_q = quarter & 1u, upper_q = quarter & 2u;
+                const uint32_t other = __shfl_xor_sync(kFullMask, upper_q ? p01 : p23, 2);
+                const uint32_t q0 = upper_q ? other : p01, q2 = upper_q ? p23 : other;
+                const uint32_t keep = __byte_perm(q0, q2, odd_q ? 0x7632 : 0x5410);
+                const uint32_t got = __shfl_xor_sync(kFullMask, __byte_perm(q0, q2, odd_q ? 0x5410 : 0x7632), 1);
+                // (rows past the last have room, and hold what nothing reads)
+                const uint64_t at = p.split.slot(nt * kParts + part, mt * kBM + row_in + 8 * quarter);
+                p.group_max[at] = odd_q ? make_uint2(got, keep) : make_uint2(keep, got);
+                const uint32_t m = max_pairs(keep, got);
+                p.part_max[at] = static_cast<uint16_t>(max_pairs(m, m >> 16));
             }
             ++nt;
             if (last) {
@@ -487,8 +516,8 @@ struct HeadRowParams {
     const float* w_scale;
     const float* bias;
     const float4* partials;
-    const float* group_max;
-    const float* part_max;
+    const uint2* group_max;
+    const uint16_t* part_max;
     ScoreOutputs out;
 };
 
@@ -570,7 +599,7 @@ DH_DEVINL int2 group_sums(const int8_t* h, const int8_t* w, uint64_t ldw, uint32
 }
 
 constexpr uint32_t kRowWarps = 8;
-constexpr uint32_t kMaxStaged = 1185;  // words of shared memory a row: vocabularies up to 75,776
+constexpr uint32_t kMaxStaged = 1185;  // words of shared memory a row: vocabularies up to 151,552
 constexpr uint32_t kPicks = 96;  // groups kept for the k best (more, by ties: every group is looked at)
 // Rows below which each gets a CTA: 512 rows 46 / 50 us (1 / 8 alternatives)
 // against 44 / 64 with a warp each, 1001 rows 71 / 79 against 58 / 80.
@@ -593,7 +622,7 @@ static_assert(sizeof(RowsSmem<1>) + kMaxStaged * kRowWarps * sizeof(float) <= 48
 template <bool kWide, uint32_t kTeam>
 __global__ void __launch_bounds__(32 * kRowWarps, 4)
 head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged) {
-    extern __shared__ float staged_max[];  // the part maxima of the CTA's rows, if `staged` holds them: [kTeams][staged]
+    extern __shared__ uint32_t staged_max[];  // the part maxima of the CTA's rows, if `staged` holds them: [kTeams][staged]
     constexpr uint32_t kTeams = kRowWarps / kTeam;
     __shared__ RowsSmem<kTeam> sm;
 
@@ -605,19 +634,18 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
     };
     const uint64_t row = static_cast<uint64_t>(blockIdx.x) * kTeams + team;
     const uint32_t k = p.out.top_k, targets = p.out.targets_per_row;
-    const uint32_t n_part = p.split.n_tiles * kParts;
+    const uint32_t n_pair = p.split.n_tiles * kParts / 2;  // parts in pairs, a word each
     if (staged) {
-        // 8 consecutive rows of a part are one 32-byte sector
-        const float4* from = reinterpret_cast<const float4*>(p.part_max) + blockIdx.x * (kTeams / 4);
-        const uint32_t pitch = static_cast<uint32_t>(p.split.padded_rows() / 4), q = threadIdx.x % 2;
-#pragma unroll 4
-        for (uint32_t i = threadIdx.x / 2; i < n_part; i += 16 * kRowWarps) {
-            const float4 v = __ldg(from + static_cast<uint64_t>(i) * pitch + q);
-            float* to = staged_max + 4 * q * staged + i;
-            to[0] = v.x;
-            to[staged] = v.y;
-            to[2 * staged] = v.z;
-            to[3 * staged] = v.w;
+        // the CTA's 8 rows of a part are 16 bytes
+        const uint4* from = reinterpret_cast<const uint4*>(p.part_max) + blockIdx.x;
+        const uint64_t pitch = p.split.padded_rows() / 8;
+#pragma unroll 2
+        for (uint32_t j = threadIdx.x; j < n_pair; j += 32 * kRowWarps) {
+            const uint4 u = __ldg(from + 2 * j * pitch), v = __ldg(from + (2 * j + 1) * pitch);
+            const uint32_t lo[4] = {u.x, u.y, u.z, u.w}, hi[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (uint32_t r = 0; r < 8; ++r)
+                staged_max[r * staged + j] = __byte_perm(lo[r / 2], hi[r / 2], r % 2 ? 0x7632 : 0x5410);
         }
         __syncthreads();
     }
@@ -671,26 +699,34 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
 
     // the k-th largest of the lanes' maxima of parts (the two largest of each)
     // bounds the k-th best logit; the parts are dealt to the members
-    const float* maxima = staged ? staged_max + team * staged : p.part_max + row;
-    const uint64_t stride = staged ? 1u : p.split.padded_rows();
     constexpr uint32_t kStep = 32 * kTeam;
-    const float* mine = maxima + (member * 32 + lane) * stride;
-    const uint64_t hop = kStep * stride;
-    // 4 at a time, from `at` on, the i-th of all; -inf past the last
-    auto four = [&](const float* at, uint32_t i, float (&v)[4]) {
-#pragma unroll
-        for (uint32_t u = 0; u < 4; ++u) v[u] = i + kStep * u < n_part ? at[u * hop] : -CUDART_INF_F;
+    const uint32_t* words = staged_max + team * staged;
+    const uint16_t* column = p.part_max + row;
+    const uint64_t rows_of = p.split.padded_rows();
+    // parts 2 j and 2 j + 1; -inf past the last
+    auto pair_of = [&](uint32_t j) -> uint32_t {
+        if (j >= n_pair) return kNonePair;
+        if (staged) return words[j];
+        return __ldg(column + 2 * j * rows_of) | static_cast<uint32_t>(__ldg(column + (2 * j + 1) * rows_of)) << 16;
     };
     float a = -CUDART_INF_F, b = -CUDART_INF_F, bound = -CUDART_INF_F;
     if (k) {
-        const float* at = mine;
-#pragma unroll 2
-        for (uint32_t i = member * 32 + lane; i < n_part; i += 4 * kStep, at += 4 * hop) {
-            float v[4];
-            four(at, i, v);
+        uint32_t a2 = kNonePair, b2 = kNonePair;
+#pragma unroll 1
+        for (uint32_t j = member * 32 + lane; j < n_pair; j += 4 * kStep) {
+            uint32_t v[4];
 #pragma unroll
-            for (uint32_t u = 0; u < 4; ++u) two_largest(a, b, v[u]);
+            for (uint32_t u = 0; u < 4; ++u) v[u] = pair_of(j + u * kStep);
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u) {
+                b2 = max_pairs(b2, min_pairs(a2, v[u]));
+                a2 = max_pairs(a2, v[u]);
+            }
         }
+        a = half_float(a2);
+        b = half_float(b2);
+        two_largest(a, b, half_float(a2 >> 16));
+        two_largest(a, b, half_float(b2 >> 16));
         if (member == 0 && lane == 0) sm.pick_count[team] = 0;
         if (kTeam > 1) {
             sm.pairs[warp][0][lane] = a;
@@ -721,31 +757,37 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
         }
     }
     bound = kth_largest_of_pairs(a, b, k, lane);
+    // no logit below this rounds to it
+    const uint16_t bits = __half_as_ushort(__float2half_rz(bound));
+    const float least = bits >= 0x8000u && bits < 0xFC00u ? half_float(bits + 1u) : bound;
+    auto group_value = [&](uint32_t part, uint32_t quarter) {
+        const uint16_t* at = reinterpret_cast<const uint16_t*>(p.group_max + p.split.slot(part, static_cast<uint32_t>(row)));
+        return half_float(__ldg(at + group_at(quarter)));
+    };
     // the groups that reach it
     uint32_t n = 0;
-    const float* at = mine;
 #pragma unroll 1
-    for (uint32_t i0 = member * 32; i0 < n_part; i0 += 4 * kStep, at += 4 * hop) {
-        float v[4];
-        four(at, i0 + lane, v);
-        const float m = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+    for (uint32_t j0 = member * 32; j0 < n_pair; j0 += 2 * kStep) {
+        const uint32_t v[2] = {pair_of(j0 + lane), pair_of(j0 + kStep + lane)};
+        const uint32_t both = max_pairs(v[0], v[1]);
+        const float m = fmaxf(half_float(both), half_float(both >> 16));
         if (__any_sync(kFullMask, m >= bound && m > -CUDART_INF_F)) {
 #pragma unroll
             for (uint32_t u = 0; u < 4; ++u) {
-                const uint32_t who = __ballot_sync(kFullMask, v[u] >= bound && v[u] > -CUDART_INF_F);
-                if ((who >> lane) & 1u) sm.parts[warp][n + __popc(who & ((1u << lane) - 1u))] = i0 + kStep * u + lane;
+                const float y = half_float(v[u / 2] >> (u % 2 * 16));
+                const uint32_t who = __ballot_sync(kFullMask, y >= bound && y > -CUDART_INF_F);
+                if ((who >> lane) & 1u)
+                    sm.parts[warp][n + __popc(who & ((1u << lane) - 1u))] = 2 * (j0 + kStep * (u / 2) + lane) + u % 2;
                 n += __popc(who);
             }
         }
-        if (n > 32 || i0 + 4 * kStep >= n_part) {
+        if (n > 32 || j0 + 2 * kStep >= n_pair) {
             __syncwarp();
             // the 4 groups of 8 parts at a time
 #pragma unroll 1
             for (uint32_t j = lane / 4; j < n + lane / 4; j += 8) {
                 const uint32_t part = j < n ? sm.parts[warp][j] : 0u;
-                const float y = j < n ? __ldg(p.group_max + p.split.slot(part, static_cast<uint32_t>(row)) * kGroupsPerPart +
-                                              lane % 4)
-                                      : -CUDART_INF_F;
+                const float y = j < n ? group_value(part, lane % 4) : -CUDART_INF_F;
                 const uint32_t in = __ballot_sync(kFullMask, y >= bound && y > -CUDART_INF_F);
                 uint32_t to = 0;
                 if (lane == 0 && in) to = atomicAdd(&sm.pick_count[team], __popc(in));
@@ -764,16 +806,14 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
 #pragma unroll 1
     for (uint32_t i = member; i < n_pick; i += kTeam) {
         const uint32_t group = all ? i : sm.picks[team][i];
-        if (all && !(__ldg(p.group_max + p.split.slot(i / kGroupsPerPart, static_cast<uint32_t>(row)) * kGroupsPerPart +
-                           i % kGroupsPerPart) >= bound))
-            continue;
+        if (all && !(group_value(i / kGroupsPerPart, i % kGroupsPerPart) >= bound)) continue;
         // lanes with lane % 4 < 2 answer for token lane / 4 + 8 (lane % 4)
         const uint32_t c = group_token(group, lane / 4 + 8 * (lane % 4 & 1u));
         const bool in = lane % 4 < 2 && c < p.vocab && c != p.mask_id;
         const float w = in ? __ldg(p.w_scale + c) : 0.f, b = in && p.bias ? __ldg(p.bias + c) : 0.f;
         const int2 acc = group_sums(h, p.weights, p.ld_weights, group, p.vocab, p.k, lane);
         const float x = score_logit<kWide>(lane % 4 ? acc.y : acc.x, ab, w, b);
-        best.add(in && x >= bound && x > -CUDART_INF_F ? token_key(x, c) : 0ull);
+        best.add(in && x >= least && x > -CUDART_INF_F ? token_key(x, c) : 0ull);
     }
     best.flush();
     if (kTeam > 1) {
@@ -814,10 +854,10 @@ uint64_t partial_bytes(const HeadSplit& s) {
 }
 
 uint64_t group_bytes(const HeadSplit& s) {
-    return align256(s.padded_rows() * s.n_tiles * kGroupsPerTile * sizeof(float));
+    return align256(s.padded_rows() * s.n_tiles * kParts * sizeof(uint2));
 }
 uint64_t part_max_bytes(const HeadSplit& s) {
-    return align256(s.padded_rows() * s.n_tiles * kParts * sizeof(float));
+    return align256(s.padded_rows() * s.n_tiles * kParts * sizeof(uint16_t));
 }
 
 }  // namespace
@@ -874,8 +914,8 @@ extern "C" uint32_t dh_head_logprobs_i8(const int8_t* hidden, uint64_t ld_hidden
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     float4* partials = static_cast<float4*>(workspace);
     uint8_t* maxima = static_cast<uint8_t*>(workspace) + partial_bytes(split);
-    float* group_max = top_k ? reinterpret_cast<float*>(maxima) : nullptr;
-    float* part_max = top_k ? reinterpret_cast<float*>(maxima + group_bytes(split)) : nullptr;
+    uint2* group_max = top_k ? reinterpret_cast<uint2*>(maxima) : nullptr;
+    uint16_t* part_max = top_k ? reinterpret_cast<uint16_t*>(maxima + group_bytes(split)) : nullptr;
     const HeadScoreParams sp{split, vocabulary_size, mask_token_id, hidden_size, stages, a_scale, w_scale, bias,
                              partials, group_max, part_max};
     stats<<<split.grid, kHeadThreads, smem, s>>>(ta, tb, sp);
@@ -886,10 +926,10 @@ extern "C" uint32_t dh_head_logprobs_i8(const int8_t* hidden, uint64_t ld_hidden
     auto rows_kernel = wide ? (team ? head_rows_kernel<true, kRowWarps> : head_rows_kernel<true, 1>)
                             : (team ? head_rows_kernel<false, kRowWarps> : head_rows_kernel<false, 1>);
     // the part maxima of 8 rows, each row's 1 mod 2 words apart, where they fit
-    uint32_t staged = (split.n_tiles * kParts) | 1u;
+    uint32_t staged = (split.n_tiles * kParts / 2) | 1u;
     if (!top_k || team || staged > kMaxStaged) staged = 0;
     rows_kernel<<<team ? rows : (rows + kRowWarps - 1) / kRowWarps, 32 * kRowWarps,
-                  staged * kRowWarps * sizeof(float), s>>>(rp, staged);
+                  staged * kRowWarps * sizeof(uint32_t), s>>>(rp, staged);
     DH_LAUNCH_CHECK();
     return DH_OK;
 }
