@@ -40,8 +40,7 @@ constexpr uint32_t kEpiWarps = 16;                      // 4 for each lane quadr
 constexpr uint32_t kHeadThreads = 64 + 32 * kEpiWarps;
 constexpr uint32_t kParts = kEpiWarps / 4;              // of a tile's columns, one for each of those
 constexpr uint32_t kPartCols = kBN / kParts;
-constexpr uint32_t kGroup = 16;                         // logits per stored maximum: of a part's 64, every
-                                                        // 8 (i) the two at 2 (group % 4)
+constexpr uint32_t kGroup = 8;                          // logits per stored maximum (group_token)
 constexpr uint32_t kGroupsPerTile = kBN / kGroup;
 constexpr uint32_t kGroupsPerPart = kPartCols / kGroup;
 static_assert(kPartCols == 64, "two blocks of 32 columns");
@@ -90,7 +89,7 @@ struct HeadScoreParams {
     const float* w_scale;
     const float* bias;   // or null
     float4* partials;    // [grid][max_segs][kParts][128]: base, s, t of a row's part
-    uint2* group_max;    // [n_tiles * kParts][rows]: 4 groups' (group_at), or null: none asked for
+    uint2* group_max;    // [n_tiles * kParts][rows]: 8 groups' (group_at), or null: none asked for
     uint16_t* part_max;  // [n_tiles * kParts][rows]; rows rounded up to row tiles
 };
 
@@ -108,11 +107,12 @@ DH_DEVINL float max3(float a, float b, float c) {
     return y;
 }
 
-// Maxima are stored as half floats, rounded toward zero (past their range: the
-// largest finite one; -inf stays): rounding keeps the order, so that every group
-// with a logit of the k best still reaches the rounded bound.  Groups within a
-// rounding step of it are looked at for nothing, so 8 bits (bfloat16) are too few:
-// 241 us for the second kernel with 32768 x 50258 and 5 alternatives.
+// Maxima are stored as half floats rounded toward zero (past their range: the
+// largest finite one; -inf stays), those of groups as the upper byte of that:
+// rounding keeps the order, so that every part and group with a logit of the k best
+// still reaches the rounded bound.  Parts within a rounding step of it are looked
+// at for nothing, so 8 bits are too few for them (bfloat16: 8 us more of 233 for
+// 32768 x 50258 and 5 alternatives), but enough to tell the groups of a part apart.
 DH_DEVINL uint32_t half_pair(float lo, float hi) {
     uint32_t y;
     asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
@@ -128,8 +128,8 @@ DH_DEVINL uint32_t min_pairs(uint32_t a, uint32_t b) {
     const __half2 m = __hmin2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&m);
 }
-// Where a quarter's group lies among the 4, and the other way round.
-DH_DEVINL uint32_t group_at(uint32_t q) { return (q & 1u) << 1 | q >> 1; }
+// Which group of a part (group_token) is byte `b` of a row's 8.
+DH_DEVINL uint32_t group_at(uint32_t b, uint64_t row) { return b ^ (static_cast<uint32_t>(row) / 8 % 4 * 2); }
 
 // A row's running statistics in this kernel: pairs of sums of e = 2^z and of
 // e z, z = (x - base) log2 e + slip.  slip is what rounding base log2 e to fp32
@@ -167,8 +167,8 @@ struct PairStats {
     }
 };
 
-// 32 columns of 4 rows (8 logits of each): accumulators to logits, to the rows'
-// statistics, and their maxima to g.  kClamp: some logit may be -inf or NaN, or
+// 32 columns of 4 rows (8 logits of each, a group): accumulators to logits, to the
+// rows' statistics, and their maxima to g.  kClamp: some logit may be -inf or NaN, or
 // past kPlainLogit.
 template <bool kWide, bool kTop, bool kClamp>
 DH_DEVINL void add_block(PairStats (&st)[4], float (&g)[4], const uint32_t (&v)[2][16], const float (&ab)[4],
@@ -193,7 +193,7 @@ DH_DEVINL void add_block(PairStats (&st)[4], float (&g)[4], const uint32_t (&v)[
     for (uint32_t r = 0; r < 4; ++r) {
         m[r] = max3(fmaxf(x[r][0].x, x[r][0].y), x[r][1].x, x[r][1].y);
         m[r] = fmaxf(m[r], max3(fmaxf(x[r][2].x, x[r][2].y), x[r][3].x, x[r][3].y));
-        if (kTop) g[r] = fmaxf(g[r], m[r]);
+        if (kTop) g[r] = m[r];
         above = above || m[r] > st[r].base + kBaseSlack;
     }
     // (one branch for the four rows: what follows is one block of independent work)
@@ -445,7 +445,7 @@ head_stats_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             if (!tc::mbar_wait(&accf_bar[acc], phase, tc::kErrTimeoutAccFull)) break;
             tc::tc_fence_after();
             const uint32_t taddr = tmem_base + ((quad * 32u) << 16) + acc * kBN + part * kPartCols;
-            float g[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+            float g[2][4];
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h) {  // 32 columns at a time
                 uint32_t v[2][16];
@@ -464,22 +464,28 @@ head_stats_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&acce_bar[acc]);
                 }
-                if (odd) add_block<kWide, kTop, true>(st, g, v, ab, w, b);
-                else add_block<kWide, kTop, false>(st, g, v, ab, w, b);
+                if (odd) add_block<kWide, kTop, true>(st, g[h], v, ab, w, b);
+                else add_block<kWide, kTop, false>(st, g[h], v, ab, w, b);
             }
             if (kTop) {
-                // the 4 threads of a row hold a group each of 4 rows: after two
-                // exchanges each has a row's 4 groups, of quarters 0, 2 and 1, 3
-                const uint32_t p01 = half_pair(g[0], g[1]), p23 = half_pair(g[2], g[3]);
+                // the 4 threads of a row hold 2 groups each of 4 rows: after two
+                // exchanges each has a row's 8 groups
+                uint32_t own[4], got[2];
+#pragma unroll
+                for (uint32_t r = 0; r < 4; ++r) own[r] = half_pair(g[0][r], g[1][r]);
                 const bool odd_q = quarter & 1u, upper_q = quarter & 2u;
-                const uint32_t other = __shfl_xor_sync(kFullMask, upper_q ? p01 : p23, 2);
-                const uint32_t q0 = upper_q ? other : p01, q2 = upper_q ? p23 : other;
-                const uint32_t keep = __byte_perm(q0, q2, odd_q ? 0x7632 : 0x5410);
-                const uint32_t got = __shfl_xor_sync(kFullMask, __byte_perm(q0, q2, odd_q ? 0x5410 : 0x7632), 1);
+#pragma unroll
+                for (uint32_t e = 0; e < 2; ++e) {
+                    got[e] = __shfl_xor_sync(kFullMask, upper_q ? own[e] : own[2 + e], 2);
+                    own[e] = upper_q ? own[2 + e] : own[e];
+                }
+                const uint32_t q0 = odd_q ? own[1] : own[0], q2 = odd_q ? got[1] : got[0];
+                const uint32_t q1 = __shfl_xor_sync(kFullMask, odd_q ? own[0] : own[1], 1);
+                const uint32_t q3 = __shfl_xor_sync(kFullMask, odd_q ? got[0] : got[1], 1);
                 // (rows past the last have room, and hold what nothing reads)
                 const uint64_t at = p.split.slot(nt * kParts + part, mt * kBM + row_in + 8 * quarter);
-                p.group_max[at] = odd_q ? make_uint2(got, keep) : make_uint2(keep, got);
-                const uint32_t m = max_pairs(keep, got);
+                p.group_max[at] = make_uint2(__byte_perm(q0, q1, 0x7531), __byte_perm(q2, q3, 0x7531));
+                const uint32_t m = max_pairs(max_pairs(q0, q1), max_pairs(q2, q3));
                 p.part_max[at] = static_cast<uint16_t>(max_pairs(m, m >> 16));
             }
             ++nt;
@@ -544,22 +550,22 @@ DH_DEVINL void mma_s8(int32_t (&c)[4], int32_t a0, int32_t a1, int32_t a2, int32
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The j-th of a group's 16 tokens.
+// The j-th of a group's 8 tokens: of 32 columns of a part (group % 2), in every 8
+// the two of the quarter group / 2 % 4.
 DH_DEVINL uint32_t group_token(uint32_t group, uint32_t j) {
-    return group / kGroupsPerPart * kPartCols + j / 2 * 8 + group % kGroupsPerPart * 2 + j % 2;
+    return group / kGroupsPerPart * kPartCols + group % 2 * 32 + j / 2 * 8 + group / 2 % 4 * 2 + j % 2;
 }
 
-// Integer sums of the 16 tokens of a group with the hidden row, by a warp: a
+// Integer sums of the 8 tokens of two groups with the hidden row, by a warp: a
 // 16 x 8 x 32 MMA whose 16 rows are the tokens and whose 8 columns are all the
 // hidden row.  Any order of the k dimension serves as long as both operands
-// share it, so a lane loads 16 consecutive bytes of the tokens lane / 4 and
-// lane / 4 + 8, and feeds them to two MMAs.  Every lane receives the sums of
-// these two tokens (x and y).
-DH_DEVINL int2 group_sums(const int8_t* h, const int8_t* w, uint64_t ldw, uint32_t group, uint32_t vocab, uint32_t k,
-                          uint32_t lane) {
+// share it, so a lane loads 16 consecutive bytes of token lane / 4 of both, and
+// feeds them to two MMAs.  Every lane receives the sums of these two tokens.
+DH_DEVINL int2 group_sums(const int8_t* h, const int8_t* w, uint64_t ldw, uint32_t group_a, uint32_t group_b,
+                          uint32_t vocab, uint32_t k, uint32_t lane) {
     const uint32_t g = lane / 4, t = lane % 4;
-    const int8_t* wa = w + min(group_token(group, g), vocab - 1) * ldw;
-    const int8_t* wb = w + min(group_token(group, g + 8), vocab - 1) * ldw;
+    const int8_t* wa = w + min(group_token(group_a, g), vocab - 1) * ldw;
+    const int8_t* wb = w + min(group_token(group_b, g), vocab - 1) * ldw;
     const int4 *pa = reinterpret_cast<const int4*>(wa) + t, *pb = reinterpret_cast<const int4*>(wb) + t;
     const int4* px = reinterpret_cast<const int4*>(h) + t;
     int32_t c[4] = {0, 0, 0, 0};
@@ -599,8 +605,8 @@ DH_DEVINL int2 group_sums(const int8_t* h, const int8_t* w, uint64_t ldw, uint32
 }
 
 constexpr uint32_t kRowWarps = 8;
-constexpr uint32_t kMaxStaged = 1185;  // words of shared memory a row: vocabularies up to 151,552
-constexpr uint32_t kPicks = 96;  // groups kept for the k best (more, by ties: every group is looked at)
+constexpr uint32_t kMaxStaged = 1025;  // words of shared memory a row: vocabularies up to 131,072
+constexpr uint32_t kPicks = 256;  // groups kept for the k best (more, by ties: every group is looked at)
 // Rows below which each gets a CTA: 512 rows 46 / 50 us (1 / 8 alternatives)
 // against 44 / 64 with a warp each, 1001 rows 71 / 79 against 58 / 80.
 constexpr uint32_t kTeamRows = 768;
@@ -757,12 +763,14 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
         }
     }
     bound = kth_largest_of_pairs(a, b, k, lane);
-    // no logit below this rounds to it
+    // no logit below `least` rounds to it, no group's byte is below group_bound
     const uint16_t bits = __half_as_ushort(__float2half_rz(bound));
     const float least = bits >= 0x8000u && bits < 0xFC00u ? half_float(bits + 1u) : bound;
-    auto group_value = [&](uint32_t part, uint32_t quarter) {
-        const uint16_t* at = reinterpret_cast<const uint16_t*>(p.group_max + p.split.slot(part, static_cast<uint32_t>(row)));
-        return half_float(__ldg(at + group_at(quarter)));
+    const float group_bound = half_float(bits & 0xFF00u);
+    auto group_reaches = [&](uint32_t part, uint32_t b) {
+        const uint8_t* at = reinterpret_cast<const uint8_t*>(p.group_max + p.split.slot(part, static_cast<uint32_t>(row)));
+        const float y = half_float(static_cast<uint32_t>(__ldg(at + b)) << 8);
+        return y >= group_bound && y > -CUDART_INF_F;
     };
     // the groups that reach it
     uint32_t n = 0;
@@ -783,35 +791,41 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
         }
         if (n > 32 || j0 + 2 * kStep >= n_pair) {
             __syncwarp();
-            // the 4 groups of 8 parts at a time
+            // the 8 groups of 4 parts at a time
 #pragma unroll 1
-            for (uint32_t j = lane / 4; j < n + lane / 4; j += 8) {
+            for (uint32_t j = lane / 8; j < n + lane / 8; j += 4) {
                 const uint32_t part = j < n ? sm.parts[warp][j] : 0u;
-                const float y = j < n ? group_value(part, lane % 4) : -CUDART_INF_F;
-                const uint32_t in = __ballot_sync(kFullMask, y >= bound && y > -CUDART_INF_F);
+                const uint32_t in = __ballot_sync(kFullMask, j < n && group_reaches(part, lane % 8));
                 uint32_t to = 0;
                 if (lane == 0 && in) to = atomicAdd(&sm.pick_count[team], __popc(in));
                 to = __shfl_sync(kFullMask, to, 0) + __popc(in & ((1u << lane) - 1u));
-                if (((in >> lane) & 1u) && to < kPicks) sm.picks[team][to] = part * kGroupsPerPart + lane % 4;
+                if (((in >> lane) & 1u) && to < kPicks) sm.picks[team][to] = part * kGroupsPerPart + group_at(lane % 8, row);
             }
             n = 0;
             __syncwarp();
         }
     }
     team_sync();
-    // their logits
+    // their logits, two groups at a time
     const bool all = sm.pick_count[team] > kPicks;
     const uint32_t n_pick = all ? p.split.n_tiles * kGroupsPerTile : sm.pick_count[team];
     TopList best(sm.keys[warp], k, lane);
 #pragma unroll 1
-    for (uint32_t i = member; i < n_pick; i += kTeam) {
-        const uint32_t group = all ? i : sm.picks[team][i];
-        if (all && !(group_value(i / kGroupsPerPart, i % kGroupsPerPart) >= bound)) continue;
-        // lanes with lane % 4 < 2 answer for token lane / 4 + 8 (lane % 4)
-        const uint32_t c = group_token(group, lane / 4 + 8 * (lane % 4 & 1u));
-        const bool in = lane % 4 < 2 && c < p.vocab && c != p.mask_id;
+    for (uint32_t i = 2 * member; i < n_pick; i += 2 * kTeam) {
+        const bool two = i + 1 < n_pick;
+        const uint32_t ga = all ? i : sm.picks[team][i], gb = all ? i + 1 : sm.picks[team][two ? i + 1 : i];
+        if (all) {
+            const uint32_t part = i / kGroupsPerPart, pair = pair_of(part / 2);
+            if (!(half_float(part % 2 ? pair >> 16 : pair) >= bound) ||
+                !(group_reaches(part, group_at(ga % kGroupsPerPart, row)) ||
+                  group_reaches(part, group_at(gb % kGroupsPerPart, row))))
+                continue;
+        }
+        // lanes with lane % 4 < 2 answer for token lane / 4 of a group each
+        const uint32_t c = group_token(lane % 4 & 1u ? gb : ga, lane / 4);
+        const bool in = lane % 4 < (two ? 2u : 1u) && c < p.vocab && c != p.mask_id;
         const float w = in ? __ldg(p.w_scale + c) : 0.f, b = in && p.bias ? __ldg(p.bias + c) : 0.f;
-        const int2 acc = group_sums(h, p.weights, p.ld_weights, group, p.vocab, p.k, lane);
+        const int2 acc = group_sums(h, p.weights, p.ld_weights, ga, gb, p.vocab, p.k, lane);
         const float x = score_logit<kWide>(lane % 4 ? acc.y : acc.x, ab, w, b);
         best.add(in && x >= least && x > -CUDART_INF_F ? token_key(x, c) : 0ull);
     }
