@@ -503,6 +503,10 @@ head_stats_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     }
     tc::tc_fence_before();
     __syncthreads();
+    // The second kernel may be brought in; it waits for this one's end before it
+    // reads what this one writes.  (Earlier, its few CTAs would crowd on the SMs
+    // that are done first: 88 against 66 us for 1001 rows and 8 alternatives.)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 1) {
         tc::tc_fence_after();
         tc::tmem_dealloc(tmem_base, 2 * kBN);
@@ -607,8 +611,8 @@ DH_DEVINL int2 group_sums(const int8_t* h, const int8_t* w, uint64_t ldw, uint32
 constexpr uint32_t kRowWarps = 8;
 constexpr uint32_t kMaxStaged = 1025;  // words of shared memory a row: vocabularies up to 131,072
 constexpr uint32_t kPicks = 256;  // groups kept for the k best (more, by ties: every group is looked at)
-// Rows below which each gets a CTA: 512 rows 46 / 50 us (1 / 8 alternatives)
-// against 44 / 64 with a warp each, 1001 rows 71 / 79 against 58 / 80.
+// Rows below which each gets a CTA: 512 rows 43 / 43 us (1 / 8 alternatives)
+// against 41 / 51 with a warp each, 1001 rows 66 / 68 against 55 / 66.
 constexpr uint32_t kTeamRows = 768;
 
 template <uint32_t kTeam>
@@ -640,24 +644,9 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
     };
     const uint64_t row = static_cast<uint64_t>(blockIdx.x) * kTeams + team;
     const uint32_t k = p.out.top_k, targets = p.out.targets_per_row;
-    const uint32_t n_pair = p.split.n_tiles * kParts / 2;  // parts in pairs, a word each
-    if (staged) {
-        // the CTA's 8 rows of a part are 16 bytes
-        const uint4* from = reinterpret_cast<const uint4*>(p.part_max) + blockIdx.x;
-        const uint64_t pitch = p.split.padded_rows() / 8;
-#pragma unroll 2
-        for (uint32_t j = threadIdx.x; j < n_pair; j += 32 * kRowWarps) {
-            const uint4 u = __ldg(from + 2 * j * pitch), v = __ldg(from + (2 * j + 1) * pitch);
-            const uint32_t lo[4] = {u.x, u.y, u.z, u.w}, hi[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (uint32_t r = 0; r < 8; ++r)
-                staged_max[r * staged + j] = __byte_perm(lo[r / 2], hi[r / 2], r % 2 ? 0x7632 : 0x5410);
-        }
-        __syncthreads();
-    }
-    if (kTeam == 1 && row >= p.split.rows) return;  // (otherwise the grid is the rows)
+    const bool have = kTeam > 1 || row < p.split.rows;  // (with teams the grid is the rows)
     const int8_t* h = p.hidden + row * p.ld_hidden;
-    const float ab = __ldg(p.a_scale + row);
+    const float ab = have ? __ldg(p.a_scale + row) : 0.f;
 
     auto token_logit = [&](uint32_t c, int32_t acc) {
         if (c == p.mask_id) return -CUDART_INF_F;
@@ -674,7 +663,27 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
     const uint32_t first_target = kTeam - 1 - member;
     int64_t target = -1;
     float target_x = 0.f;
-    if (first_target < targets) target_x = target_logit(first_target, target);
+    if (have && first_target < targets) target_x = target_logit(first_target, target);
+
+    // so far the call's inputs alone: now the first kernel has to have ended (what
+    // it writes is read by plain loads, not through the read-only path)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t n_pair = p.split.n_tiles * kParts / 2;  // parts in pairs, a word each
+    if (staged) {
+        // the CTA's 8 rows of a part are 16 bytes
+        const uint4* from = reinterpret_cast<const uint4*>(p.part_max) + blockIdx.x;
+        const uint64_t pitch = p.split.padded_rows() / 8;
+#pragma unroll 2
+        for (uint32_t j = threadIdx.x; j < n_pair; j += 32 * kRowWarps) {
+            const uint4 u = from[2 * j * pitch], v = from[(2 * j + 1) * pitch];
+            const uint32_t lo[4] = {u.x, u.y, u.z, u.w}, hi[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (uint32_t r = 0; r < 8; ++r)
+                staged_max[r * staged + j] = __byte_perm(lo[r / 2], hi[r / 2], r % 2 ? 0x7632 : 0x5410);
+        }
+        __syncthreads();
+    }
+    if (!have) return;
 
     // the row's partial statistics
     const uint32_t mt = static_cast<uint32_t>(row / kBM), r_in = static_cast<uint32_t>(row % kBM);
@@ -685,7 +694,7 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
     for (uint32_t i = member * 32 + lane; i < (c_hi - c_lo + 1) * kParts; i += kTeam * 32) {
         const uint32_t c = c_lo + i / kParts;
         const uint32_t seg = mt - p.split.first_tile(c) / p.split.n_tiles;
-        const float4 q = __ldg(p.partials + ((static_cast<uint64_t>(c) * p.split.max_segs + seg) * kParts + i % kParts) * kBM + r_in);
+        const float4 q = p.partials[((static_cast<uint64_t>(c) * p.split.max_segs + seg) * kParts + i % kParts) * kBM + r_in];
         RowStats o{q.x, q.y, q.z};
         const float m = fmaxf(st.base, o.base);
         rebase(st, m);
@@ -713,7 +722,7 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
     auto pair_of = [&](uint32_t j) -> uint32_t {
         if (j >= n_pair) return kNonePair;
         if (staged) return words[j];
-        return __ldg(column + 2 * j * rows_of) | static_cast<uint32_t>(__ldg(column + (2 * j + 1) * rows_of)) << 16;
+        return column[2 * j * rows_of] | static_cast<uint32_t>(column[(2 * j + 1) * rows_of]) << 16;
     };
     float a = -CUDART_INF_F, b = -CUDART_INF_F, bound = -CUDART_INF_F;
     if (k) {
@@ -769,7 +778,7 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
     const float group_bound = half_float(bits & 0xFF00u);
     auto group_reaches = [&](uint32_t part, uint32_t b) {
         const uint8_t* at = reinterpret_cast<const uint8_t*>(p.group_max + p.split.slot(part, static_cast<uint32_t>(row)));
-        const float y = half_float(static_cast<uint32_t>(__ldg(at + b)) << 8);
+        const float y = half_float(static_cast<uint32_t>(at[b]) << 8);
         return y >= group_bound && y > -CUDART_INF_F;
     };
     // the groups that reach it
@@ -942,8 +951,17 @@ extern "C" uint32_t dh_head_logprobs_i8(const int8_t* hidden, uint64_t ld_hidden
     // the part maxima of 8 rows, each row's 1 mod 2 words apart, where they fit
     uint32_t staged = (split.n_tiles * kParts / 2) | 1u;
     if (!top_k || team || staged > kMaxStaged) staged = 0;
-    rows_kernel<<<team ? rows : (rows + kRowWarps - 1) / kRowWarps, 32 * kRowWarps,
-                  staged * kRowWarps * sizeof(uint32_t), s>>>(rp, staged);
-    DH_LAUNCH_CHECK();
-    return DH_OK;
+    // (its launch and its given tokens' logits overlap the first kernel's end: 32 rows
+    // 21.5 against 23.5 us, 1001 rows and 8 alternatives 64.5 against 66.6)
+    cudaLaunchAttribute overlap{};
+    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t launch{};
+    launch.gridDim = team ? rows : (rows + kRowWarps - 1) / kRowWarps;
+    launch.blockDim = 32 * kRowWarps;
+    launch.dynamicSmemBytes = staged * kRowWarps * sizeof(uint32_t);
+    launch.stream = s;
+    launch.attrs = &overlap;
+    launch.numAttrs = 1;
+    return cudaLaunchKernelEx(&launch, rows_kernel, rp, staged) == cudaSuccess ? DH_OK : DH_ERR_CUDA;
 }
