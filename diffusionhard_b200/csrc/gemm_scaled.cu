@@ -36,6 +36,7 @@ struct ScaledParams {
     uint64_t ldo;
     uint32_t n;
     bool vec;              // out and its row pitch are multiples of 16 bytes
+    bool tma;              // and so are its rows
 };
 
 constexpr uint32_t kFull = 0xFFFFFFFFu;
@@ -140,21 +141,33 @@ struct EpiScaled : EpiBase {
 
 // ------------------------------------------------------------ large products
 //
-// 128 x 256 tiles, the TMA ring, MMA thread and double-buffered accumulators of
-// gemm_tc.cuh, but an epilogue of 16 warps that all drain the same tile (none
-// idles while its accumulators are made) and whose threads hold 4 rows and 2 of
-// every 8 columns, so that a column's scale and bias are read from shared memory
-// once for 4 outputs.  Outputs leave through shared memory as whole row
-// segments: TMA stores where the row pitch allows them.
-constexpr uint32_t kBM = 128, kBN = 256, kBK = 128;
-constexpr uint32_t kBigStages = 3;
-constexpr uint32_t kABytes = kBM * kBK, kBBytes = kBN * kBK;
-constexpr uint32_t kEpiWarps = 16, kParts = kEpiWarps / 4, kPartCols = kBN / kParts;
-constexpr uint32_t kBigThreads = 64 + 32 * kEpiWarps;
-constexpr uint32_t kOutBytes = 4096;                     // a warp's outputs on their way
-constexpr uint32_t kColBytes = kPartCols * 8;            // and its columns' scales and biases
-constexpr uint32_t kBigSmem = 1024 + kBigStages * (kABytes + kBBytes) + 1024 + kEpiWarps * (kOutBytes + kColBytes);
-static_assert(kBigSmem <= 227 * 1024, "shared memory of a CTA");
+// Tiles of 128 x 192 or 256, the TMA ring, MMA thread and double-buffered
+// accumulators of gemm_tc.cuh, but an epilogue of 12 or 16 warps that all drain the
+// same tile (none idles while its accumulators are made) and whose threads hold 4
+// rows and 2 of every 8 columns, so that a column's scale and bias are read from
+// shared memory once for 4 outputs.  Outputs leave through shared memory as whole
+// row segments: TMA stores where the row pitch allows them (512 x 50264 x 768 to
+// bf16 35 us, 512 x 50257 through registers 44).
+//
+// What bounds it: with k = 768 the outputs' way to memory, at 3.0 to 3.3 TB/s for
+// plain stores (512 x 50260 x 768 to fp32 47 us, 2.2 TB/s; 32768 x 3072 x 768 to
+// bf16 80 us, 2.5 TB/s, 61 us without the stores); with k = 8192 the tensor cores
+// (8192^3 423 us, 2.6 Pop/s under the power cap).
+constexpr uint32_t kBM = 128, kBK = 128;
+constexpr uint32_t kABytes = kBM * kBK;
+constexpr uint32_t kPartCols = 64;             // columns of an epilogue warp
+constexpr uint32_t kOutBytes = 4096;           // its outputs on their way
+constexpr uint32_t kColBytes = kPartCols * 8;  // and its columns' scales and biases
+template <uint32_t kBN>
+struct BigTile {
+    static constexpr uint32_t kBBytes = kBN * kBK;
+    static constexpr uint32_t kEpiWarps = 4 * (kBN / kPartCols);
+    static constexpr uint32_t kThreads = 64 + 32 * kEpiWarps;
+    static constexpr uint32_t kFixed = 2048 + kEpiWarps * (kOutBytes + kColBytes);
+    static constexpr uint32_t kStages = (227 * 1024 - kFixed) / (kABytes + kBBytes);
+    static constexpr uint32_t kSmem = kFixed + kStages * (kABytes + kBBytes);
+    static_assert(kBN % kPartCols == 0 && kStages >= 3 && kSmem <= 227 * 1024, "shared memory of a CTA");
+};
 
 struct BigParams {
     CUtensorMap out_map;  // with Out::kTma: out, box 32 rows x 128 bytes, 128-byte swizzle
@@ -214,29 +227,32 @@ DH_DEVINL void store_rows(const uint8_t* buf, T* out, uint64_t ldo, uint32_t row
     }
 }
 
-template <class T, Out kOut>
-__global__ void __launch_bounds__(kBigThreads, 1)
+template <class T, Out kOut, uint32_t kBN>
+__global__ void __launch_bounds__(BigTile<kBN>::kThreads, 1)
 gemm_scaled_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                    const __grid_constant__ BigParams p) {
     constexpr bool kF32 = sizeof(T) == 4;
     constexpr uint32_t kSegCols = 128 / sizeof(T);  // columns of the buffer's 128-byte rows
+    constexpr uint32_t kStages = BigTile<kBN>::kStages, kBBytes = BigTile<kBN>::kBBytes;
+    constexpr uint32_t kEpiWarps = BigTile<kBN>::kEpiWarps;
+    constexpr uint32_t kTmemCols = 512;  // two accumulators, a power of two
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~static_cast<uintptr_t>(1023));
     uint8_t* a_smem = smem;
-    uint8_t* b_smem = smem + kBigStages * kABytes;
-    uint8_t* out_smem = b_smem + kBigStages * kBBytes;
+    uint8_t* b_smem = smem + kStages * kABytes;
+    uint8_t* out_smem = b_smem + kStages * kBBytes;
     uint8_t* col_smem = out_smem + kEpiWarps * kOutBytes;
     uint64_t* full_bar = reinterpret_cast<uint64_t*>(col_smem + kEpiWarps * kColBytes);
-    uint64_t* empty_bar = full_bar + kBigStages;
-    uint64_t* accf_bar = empty_bar + kBigStages;  // [2]
+    uint64_t* empty_bar = full_bar + kStages;
+    uint64_t* accf_bar = empty_bar + kStages;  // [2]
     uint64_t* acce_bar = accf_bar + 2;            // [2]
     uint64_t* drain_bar = acce_bar + 2;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain_bar + 1);
 
     const uint32_t warp = warp_id(), lane = lane_id();
     if (warp == 0 && lane == 0) {
-        for (uint32_t s = 0; s < kBigStages; ++s) {
+        for (uint32_t s = 0; s < kStages; ++s) {
             tc::mbar_init(&full_bar[s], 1);
             tc::mbar_init(&empty_bar[s], 1);
         }
@@ -249,7 +265,7 @@ gemm_scaled_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
         tc::prefetch_tmap(&tmap_a);
         tc::prefetch_tmap(&tmap_b);
     }
-    if (warp == 1) tc::tmem_alloc(tmem_holder, 2 * kBN);
+    if (warp == 1) tc::tmem_alloc(tmem_holder, kTmemCols);
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
@@ -277,14 +293,14 @@ gemm_scaled_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
                                     static_cast<int32_t>(kb * kBK), static_cast<int32_t>(n0));
                     issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
                     ++issued;
-                    if (++stage == kBigStages) {
+                    if (++stage == kStages) {
                         stage = 0;
                         phase ^= 1;
                     }
                 }
             }
             // Drain: every copy this CTA issued has landed before it may exit.
-            for (uint32_t s = 0; s < kBigStages && s < issued; ++s)
+            for (uint32_t s = 0; s < kStages && s < issued; ++s)
                 tc::mbar_wait(&full_bar[s], (issued_parity >> s) & 1u, tc::kErrTimeoutFull);
         }
     } else if (warp == 1) {
@@ -309,7 +325,7 @@ gemm_scaled_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
                         tc::mma_i8(tmem_base + acc * kBN, tc::desc_advance(a_desc, kk * 32),
                                    tc::desc_advance(b_desc, kk * 32), idesc, (kb | kk) != 0u);
                     tc::mma_commit(&empty_bar[stage]);
-                    if (++stage == kBigStages) {
+                    if (++stage == kStages) {
                         stage = 0;
                         phase ^= 1;
                     }
@@ -453,18 +469,25 @@ gemm_scaled_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
     __syncthreads();
     if (warp == 1) {
         tc::tc_fence_after();
-        tc::tmem_dealloc(tmem_base, 2 * kBN);
+        tc::tmem_dealloc(tmem_base, kTmemCols);
     }
 }
 
-template <class T, Out kOut>
+template <class T, Out kOut, uint32_t kBN>
 cudaError_t launch_big(const CUtensorMap& ta, const CUtensorMap& tb, const BigParams& p, uint32_t tiles, cudaStream_t s) {
+    using Tile = BigTile<kBN>;
     static std::atomic<uint64_t> configured{0};
-    const cudaError_t e = smem_optin_once(gemm_scaled_kernel<T, kOut>, kBigSmem, configured);
+    const cudaError_t e = smem_optin_once(gemm_scaled_kernel<T, kOut, kBN>, Tile::kSmem, configured);
     if (e != cudaSuccess) return e;
     const uint32_t sms = device_sms();
-    gemm_scaled_kernel<T, kOut><<<tiles < sms ? tiles : sms, kBigThreads, kBigSmem, s>>>(ta, tb, p);
+    gemm_scaled_kernel<T, kOut, kBN><<<tiles < sms ? tiles : sms, Tile::kThreads, Tile::kSmem, s>>>(ta, tb, p);
     return cudaGetLastError();
+}
+
+template <class T, Out kOut>
+cudaError_t launch_big(const CUtensorMap& ta, const CUtensorMap& tb, const BigParams& p, uint32_t bn, uint32_t tiles,
+                       cudaStream_t s) {
+    return bn == 192 ? launch_big<T, kOut, 192>(ta, tb, p, tiles, s) : launch_big<T, kOut, 256>(ta, tb, p, tiles, s);
 }
 
 template <class T>
@@ -480,16 +503,17 @@ cudaError_t launch_scaled(const CUtensorMap& ta, const CUtensorMap& tb, const Ge
     q.m = shape.M;
     q.n = shape.N;
     q.k = shape.K;
-    // (a store that ends inside 16 bytes writes all 16, beside the outputs; no map
-    // holds a pitch of 2^40 bytes)
-    if (p.vec && shape.N * sizeof(T) % 16 == 0 && make_tmap_2d(&q.out_map, p.out,
-                              sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
-                              sizeof(T), shape.M, shape.N, p.ldo * sizeof(T), 32, 128 / sizeof(T)))
-        return launch_big<T, Out::kTma>(ta, tb, q, tiles, s);
+    if (p.tma) {
+        if (!make_tmap_2d(&q.out_map, p.out,
+                          sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, sizeof(T),
+                          shape.M, shape.N, p.ldo * sizeof(T), 32, 128 / sizeof(T)))
+            return cudaErrorInvalidValue;
+        return launch_big<T, Out::kTma>(ta, tb, q, bn, tiles, s);
+    }
     const uint64_t at = reinterpret_cast<uintptr_t>(p.out) | (p.ldo * sizeof(T));
-    if (at % 8 == 0) return launch_big<T, Out::k8>(ta, tb, q, tiles, s);
-    if (at % 4 == 0) return launch_big<T, Out::k4>(ta, tb, q, tiles, s);
-    if constexpr (sizeof(T) == 2) return launch_big<T, Out::k2>(ta, tb, q, tiles, s);
+    if (at % 8 == 0) return launch_big<T, Out::k8>(ta, tb, q, bn, tiles, s);
+    if (at % 4 == 0) return launch_big<T, Out::k4>(ta, tb, q, bn, tiles, s);
+    if constexpr (sizeof(T) == 2) return launch_big<T, Out::k2>(ta, tb, q, bn, tiles, s);
     return cudaErrorInvalidValue;
 }
 
@@ -511,14 +535,27 @@ extern "C" uint32_t dh_gemm_i8_scaled(const int8_t* a, uint64_t lda, const float
                            reinterpret_cast<uintptr_t>(bias);
     if ((f32s & 3u) || (reinterpret_cast<uintptr_t>(out) & (es - 1))) return DH_ERR_ALIGNMENT;
     const uint32_t m_tiles = (m + 127) / 128;
-    const uint32_t bn = static_cast<uint64_t>(m_tiles) * ((n + 63) / 64) <= kNumSMs ? 64u : 256u;
+    const bool vec = ((reinterpret_cast<uintptr_t>(out) | (ldo * es)) & 15u) == 0;
+    // (a store that ends inside 16 bytes writes all 16, beside the outputs; no map
+    // holds a pitch of 2^40 bytes)
+    const bool tma = vec && n * static_cast<uint64_t>(es) % 16 == 0 && ldo < (1ull << 38);
+    const uint32_t sms = device_sms();
+    // Tiles of 64 columns where each gets an SM of its own; else of the width whose
+    // rounds over the SMs take fewer columns in all: 4096 x 4096 x 4096 to bf16
+    // (5 rounds of 192 or 4 of 256) 58 against 63 us, 1024 x 8192 x 8192 (3 or 2)
+    // 76 against 68, 512 x 50258 x 768 to fp32 (8 or 6: as many) 53 against 59.
+    auto columns = [&](uint32_t cols) {
+        const uint64_t t = static_cast<uint64_t>(m_tiles) * ((n + cols - 1) / cols);
+        return (t + sms - 1) / sms * cols;
+    };
+    const uint32_t bn = static_cast<uint64_t>(m_tiles) * ((n + 63) / 64) <= sms ? 64u
+                        : columns(192) <= columns(256) ? 192u : 256u;
     const uint64_t tiles = static_cast<uint64_t>(m_tiles) * ((n + bn - 1) / bn);
     if (tiles > 0x7FFFFFFFull || m > 0x7FFFFF00u || n > 0x7FFFFF00u) return DH_ERR_UNSUPPORTED_SHAPE;
     CUtensorMap ta, tb;
     const uint32_t st = make_i8_operand_maps(&ta, &tb, a, lda, w, ldw, m, n, k, bn);
     if (st != DH_OK) return st;
-    const bool vec = ((reinterpret_cast<uintptr_t>(out) | (ldo * es)) & 15u) == 0;
-    const ScaledParams p{a_scale, w_scale, bias, out, ldo, n, vec};
+    const ScaledParams p{a_scale, w_scale, bias, out, ldo, n, vec, tma};
     const GemmShape shape{m, n, k, nullptr};
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e;
