@@ -33,32 +33,34 @@ uint32_t make_i8_operand_maps(CUtensorMap* ta, CUtensorMap* tb, const int8_t* a,
 
 namespace {
 
-constexpr uint32_t kBM = 128, kBN = 256, kBK = 128;
+constexpr uint32_t kBM = 128, kBK = 128;
 constexpr uint32_t kMaxStages = 6;
-constexpr uint32_t kABytes = kBM * kBK, kBBytes = kBN * kBK;
-constexpr uint32_t kEpiWarps = 16;                      // 4 for each lane quadrant of TMEM
-constexpr uint32_t kHeadThreads = 64 + 32 * kEpiWarps;
-constexpr uint32_t kParts = kEpiWarps / 4;              // of a tile's columns, one for each of those
-constexpr uint32_t kPartCols = kBN / kParts;
+constexpr uint32_t kABytes = kBM * kBK;
+constexpr uint32_t kPartCols = 64;                      // a tile's columns are cut into parts of 64: two blocks of 32
 constexpr uint32_t kGroup = 8;                          // logits per stored maximum (group_token)
-constexpr uint32_t kGroupsPerTile = kBN / kGroup;
 constexpr uint32_t kGroupsPerPart = kPartCols / kGroup;
-static_assert(kPartCols == 64, "two blocks of 32 columns");
 constexpr uint32_t kBarBytes = 1024;
 constexpr uint32_t kStagePerWarp = kPartCols * 8;       // bias and w_scale of the warp's columns
 // Shared memory: with k <= kResidentK the row tile's A stays for all its column
 // tiles and the ring holds B alone (the copies into shared memory compete with
 // the MMA's and the epilogue's reads of it); otherwise a stage holds both.
 constexpr uint32_t kSmemLimit = 227 * 1024;
-constexpr uint32_t kSmemFixed = 1024 + kBarBytes + kEpiWarps * kStagePerWarp;
 constexpr uint32_t kResidentK = 768;
 constexpr uint32_t kStreamedStages = 4;
-constexpr uint32_t resident_stages(uint32_t k_blocks) {
-    const uint32_t n = (kSmemLimit - kSmemFixed - k_blocks * kABytes) / kBBytes;
-    return n < kMaxStages ? n : kMaxStages;
-}
-static_assert(resident_stages(kResidentK / kBK) >= 3, "room for a ring beside A");
-static_assert(kSmemFixed + kStreamedStages * (kABytes + kBBytes) <= kSmemLimit, "room for the streamed ring");
+template <uint32_t kBN>
+struct HeadTile {
+    static constexpr uint32_t kParts = kBN / kPartCols;
+    static constexpr uint32_t kEpiWarps = 4 * kParts;   // 4 for each part: the lane quadrants of TMEM
+    static constexpr uint32_t kThreads = 64 + 32 * kEpiWarps;
+    static constexpr uint32_t kBBytes = kBN * kBK;
+    static constexpr uint32_t kFixed = 1024 + kBarBytes + kEpiWarps * kStagePerWarp;
+    static constexpr uint32_t resident_stages(uint32_t k_blocks) {
+        const uint32_t n = (kSmemLimit - kFixed - k_blocks * kABytes) / kBBytes;
+        return n < kMaxStages ? n : kMaxStages;
+    }
+    static_assert(resident_stages(kResidentK / kBK) >= 3, "room for a ring beside A");
+    static_assert(kFixed + kStreamedStages * (kABytes + kBBytes) <= kSmemLimit, "room for the streamed ring");
+};
 // float(acc) is exact up to 2^24: k products of magnitude 127 * 127 (128 * 128)
 constexpr uint32_t kExactK = 1024;
 constexpr uint64_t kMaxTiles = 1u << 30;
@@ -70,7 +72,8 @@ constexpr float kPlainLogit = 8e8f, kSlipBase = 1e9f;
 // How a launch splits the work, shared by the two kernels: CTA c takes `each`
 // tiles, and one more if c < more, after those of the CTAs before it.
 struct HeadSplit {
-    uint32_t rows, n_tiles, grid, max_segs, each, more;
+    uint32_t rows, cols, n_tiles, parts, grid, max_segs, each, more;  // cols, parts: of a tile
+    __host__ __device__ uint32_t all_parts() const { return n_tiles * parts; }
     __host__ __device__ uint32_t first_tile(uint32_t cta) const { return cta * each + (cta < more ? cta : more); }
     // the CTA that holds tile t
     __host__ __device__ uint32_t cta_of(uint32_t t) const {
@@ -88,9 +91,9 @@ struct HeadScoreParams {
     const float* a_scale;
     const float* w_scale;
     const float* bias;   // or null
-    float4* partials;    // [grid][max_segs][kParts][128]: base, s, t of a row's part
-    uint2* group_max;    // [n_tiles * kParts][rows]: 8 groups' (group_at), or null: none asked for
-    uint16_t* part_max;  // [n_tiles * kParts][rows]; rows rounded up to row tiles
+    float4* partials;    // [grid][max_segs][parts][128]: base, s, t of a row's part
+    uint2* group_max;    // [n_tiles * parts][rows]: 8 groups' (group_at), or null: none asked for
+    uint16_t* part_max;  // [n_tiles * parts][rows]; rows rounded up to row tiles
 };
 
 // The logit of one accumulator.  kWide: k > kExactK, where float(acc) would
@@ -230,10 +233,12 @@ DH_DEVINL void add_block(PairStats (&st)[4], float (&g)[4], const uint32_t (&v)[
 }
 
 // kTop: some alternatives are asked for.
-template <bool kWide, bool kResident, bool kTop>
-__global__ void __launch_bounds__(kHeadThreads, 1)
+template <bool kWide, bool kResident, bool kTop, uint32_t kBN>
+__global__ void __launch_bounds__(HeadTile<kBN>::kThreads, 1)
 head_stats_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                   const __grid_constant__ HeadScoreParams p) {
+    constexpr uint32_t kBBytes = HeadTile<kBN>::kBBytes, kEpiWarps = HeadTile<kBN>::kEpiWarps;
+    constexpr uint32_t kParts = HeadTile<kBN>::kParts, kTmemCols = 512;  // two accumulators, a power of two
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~static_cast<uintptr_t>(1023));
@@ -268,7 +273,7 @@ head_stats_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         tc::prefetch_tmap(&tmap_a);
         tc::prefetch_tmap(&tmap_b);
     }
-    if (warp == 1) tc::tmem_alloc(tmem_holder, 2 * kBN);
+    if (warp == 1) tc::tmem_alloc(tmem_holder, kTmemCols);
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
@@ -509,7 +514,7 @@ head_stats_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 1) {
         tc::tc_fence_after();
-        tc::tmem_dealloc(tmem_base, 2 * kBN);
+        tc::tmem_dealloc(tmem_base, kTmemCols);
     }
 }
 
@@ -668,14 +673,15 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
     // so far the call's inputs alone: now the first kernel has to have ended (what
     // it writes is read by plain loads, not through the read-only path)
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const uint32_t n_pair = p.split.n_tiles * kParts / 2;  // parts in pairs, a word each
+    const uint32_t n_part = p.split.all_parts(), n_pair = (n_part + 1) / 2;  // parts in pairs, a word each
     if (staged) {
         // the CTA's 8 rows of a part are 16 bytes
         const uint4* from = reinterpret_cast<const uint4*>(p.part_max) + blockIdx.x;
         const uint64_t pitch = p.split.padded_rows() / 8;
 #pragma unroll 2
         for (uint32_t j = threadIdx.x; j < n_pair; j += 32 * kRowWarps) {
-            const uint4 u = from[2 * j * pitch], v = from[(2 * j + 1) * pitch];
+            const uint4 none = make_uint4(kNonePair, kNonePair, kNonePair, kNonePair);
+            const uint4 u = from[2 * j * pitch], v = 2 * j + 1 < n_part ? from[(2 * j + 1) * pitch] : none;
             const uint32_t lo[4] = {u.x, u.y, u.z, u.w}, hi[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (uint32_t r = 0; r < 8; ++r)
@@ -689,12 +695,13 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
     const uint32_t mt = static_cast<uint32_t>(row / kBM), r_in = static_cast<uint32_t>(row % kBM);
     const uint32_t t0 = mt * p.split.n_tiles;
     const uint32_t c_lo = p.split.cta_of(t0), c_hi = p.split.cta_of(t0 + p.split.n_tiles - 1);
+    const uint32_t parts = p.split.parts;
     RowStats st{-CUDART_INF_F, 0.f, 0.f};
 #pragma unroll 4
-    for (uint32_t i = member * 32 + lane; i < (c_hi - c_lo + 1) * kParts; i += kTeam * 32) {
-        const uint32_t c = c_lo + i / kParts;
+    for (uint32_t i = member * 32 + lane; i < (c_hi - c_lo + 1) * parts; i += kTeam * 32) {
+        const uint32_t c = c_lo + i / parts;
         const uint32_t seg = mt - p.split.first_tile(c) / p.split.n_tiles;
-        const float4 q = p.partials[((static_cast<uint64_t>(c) * p.split.max_segs + seg) * kParts + i % kParts) * kBM + r_in];
+        const float4 q = p.partials[((static_cast<uint64_t>(c) * p.split.max_segs + seg) * parts + i % parts) * kBM + r_in];
         RowStats o{q.x, q.y, q.z};
         const float m = fmaxf(st.base, o.base);
         rebase(st, m);
@@ -722,7 +729,8 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
     auto pair_of = [&](uint32_t j) -> uint32_t {
         if (j >= n_pair) return kNonePair;
         if (staged) return words[j];
-        return column[2 * j * rows_of] | static_cast<uint32_t>(column[(2 * j + 1) * rows_of]) << 16;
+        return column[2 * j * rows_of] |
+               (2 * j + 1 < n_part ? static_cast<uint32_t>(column[(2 * j + 1) * rows_of]) << 16 : kNonePair << 16);
     };
     float a = -CUDART_INF_F, b = -CUDART_INF_F, bound = -CUDART_INF_F;
     if (k) {
@@ -817,7 +825,7 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
     team_sync();
     // their logits, two groups at a time
     const bool all = sm.pick_count[team] > kPicks;
-    const uint32_t n_pick = all ? p.split.n_tiles * kGroupsPerTile : sm.pick_count[team];
+    const uint32_t n_pick = all ? n_part * kGroupsPerPart : sm.pick_count[team];
     TopList best(sm.keys[warp], k, lane);
 #pragma unroll 1
     for (uint32_t i = 2 * member; i < n_pick; i += 2 * kTeam) {
@@ -855,15 +863,21 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
 
 constexpr uint64_t align256(uint64_t v) { return (v + 255) / 256 * 256; }
 
-uint64_t tiles_of(uint32_t rows, uint32_t vocab) {
-    return static_cast<uint64_t>((rows + kBM - 1) / kBM) * ((vocab + kBN - 1) / kBN);
+uint64_t tiles_of(uint32_t rows, uint32_t vocab, uint32_t cols) {
+    return static_cast<uint64_t>((rows + kBM - 1) / kBM) * ((vocab + cols - 1) / cols);
 }
 
+// Tiles of 256 columns, or of 192 where the longest span of a CTA becomes shorter by
+// more than they cost: 32 x 50258 (2 of 192 or 2 of 256) 19.5 against 23.5 us, 32768
+// rows (454 or 341) 963 against 888.
 HeadSplit split_of(uint32_t rows, uint32_t vocab, uint32_t sms) {
+    auto columns = [&](uint32_t cols) { return (tiles_of(rows, vocab, cols) + sms - 1) / sms * cols; };
     HeadSplit s{};
     s.rows = rows;
-    s.n_tiles = (vocab + kBN - 1) / kBN;
-    const uint32_t total = static_cast<uint32_t>(tiles_of(rows, vocab));
+    s.cols = columns(192) * 10 < columns(256) * 9 ? 192 : 256;
+    s.n_tiles = (vocab + s.cols - 1) / s.cols;
+    s.parts = s.cols / kPartCols;
+    const uint32_t total = static_cast<uint32_t>(tiles_of(rows, vocab, s.cols));
     s.grid = total < sms ? total : sms;
     s.each = total / s.grid;
     s.more = total % s.grid;
@@ -873,14 +887,38 @@ HeadSplit split_of(uint32_t rows, uint32_t vocab, uint32_t sms) {
 }
 
 uint64_t partial_bytes(const HeadSplit& s) {
-    return align256(static_cast<uint64_t>(s.grid) * s.max_segs * kParts * kBM * sizeof(float4));
+    return align256(static_cast<uint64_t>(s.grid) * s.max_segs * s.parts * kBM * sizeof(float4));
 }
 
 uint64_t group_bytes(const HeadSplit& s) {
-    return align256(s.padded_rows() * s.n_tiles * kParts * sizeof(uint2));
+    return align256(s.padded_rows() * s.all_parts() * sizeof(uint2));
 }
 uint64_t part_max_bytes(const HeadSplit& s) {
-    return align256(s.padded_rows() * s.n_tiles * kParts * sizeof(uint16_t));
+    return align256(s.padded_rows() * s.all_parts() * sizeof(uint16_t));
+}
+
+template <uint32_t kBN, bool kWide, bool kResident, bool kTop>
+cudaError_t launch_stats(const CUtensorMap& ta, const CUtensorMap& tb, HeadScoreParams p, cudaStream_t s) {
+    using Tile = HeadTile<kBN>;
+    static std::atomic<uint64_t> configured{0};
+    auto kernel = head_stats_kernel<kWide, kResident, kTop, kBN>;
+    const cudaError_t e = smem_optin_once(kernel, kSmemLimit, configured);
+    if (e != cudaSuccess) return e;
+    const uint32_t k_blocks = (p.k + kBK - 1) / kBK;
+    p.stages = kResident ? Tile::resident_stages(k_blocks) : kStreamedStages;
+    const uint32_t smem = Tile::kFixed + (kResident ? k_blocks : p.stages) * kABytes + p.stages * Tile::kBBytes;
+    kernel<<<p.split.grid, Tile::kThreads, smem, s>>>(ta, tb, p);
+    return cudaGetLastError();
+}
+
+template <uint32_t kBN>
+cudaError_t launch_stats(const CUtensorMap& ta, const CUtensorMap& tb, const HeadScoreParams& p, bool wide, cudaStream_t s) {
+    if (wide) return p.group_max ? launch_stats<kBN, true, false, true>(ta, tb, p, s)
+                                 : launch_stats<kBN, true, false, false>(ta, tb, p, s);
+    if (p.k <= kResidentK) return p.group_max ? launch_stats<kBN, false, true, true>(ta, tb, p, s)
+                                              : launch_stats<kBN, false, true, false>(ta, tb, p, s);
+    return p.group_max ? launch_stats<kBN, false, false, true>(ta, tb, p, s)
+                       : launch_stats<kBN, false, false, false>(ta, tb, p, s);
 }
 
 }  // namespace
@@ -889,7 +927,7 @@ uint64_t part_max_bytes(const HeadSplit& s) {
 using namespace dh;
 
 extern "C" size_t dh_head_logprobs_workspace_size(uint32_t rows, uint32_t vocabulary_size, uint32_t top_k) {
-    if (rows == 0 || vocabulary_size == 0 || tiles_of(rows, vocabulary_size) > kMaxTiles) return 0;
+    if (rows == 0 || vocabulary_size == 0 || tiles_of(rows, vocabulary_size, 192) > kMaxTiles) return 0;
     const HeadSplit s = split_of(rows, vocabulary_size, device_sms());
     return partial_bytes(s) + (top_k ? group_bytes(s) + part_max_bytes(s) : 0u);
 }
@@ -913,7 +951,7 @@ extern "C" uint32_t dh_head_logprobs_i8(const int8_t* hidden, uint64_t ld_hidden
     if (st != DH_OK) return st;
     if (top_k > kMaxTopK || hidden_size > 131071 || rows > (1u << 24) || vocabulary_size > (1u << 24))
         return DH_ERR_UNSUPPORTED_SHAPE;
-    if (tiles_of(rows, vocabulary_size) > kMaxTiles) return DH_ERR_UNSUPPORTED_SHAPE;
+    if (tiles_of(rows, vocabulary_size, 192) > kMaxTiles) return DH_ERR_UNSUPPORTED_SHAPE;
     const HeadSplit split = split_of(rows, vocabulary_size, device_sms());
     if (((reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(w_scale) |
           reinterpret_cast<uintptr_t>(bias)) & 3u) || (reinterpret_cast<uintptr_t>(workspace) & 255u))
@@ -921,35 +959,25 @@ extern "C" uint32_t dh_head_logprobs_i8(const int8_t* hidden, uint64_t ld_hidden
     if (workspace_bytes < dh_head_logprobs_workspace_size(rows, vocabulary_size, top_k)) return DH_ERR_WORKSPACE;
     CUtensorMap ta, tb;
     st = make_i8_operand_maps(&ta, &tb, hidden, ld_hidden, weights, ld_weights, rows, vocabulary_size,
-                              hidden_size, kBN);
+                              hidden_size, split.cols);
     if (st != DH_OK) return st;
     const bool wide = hidden_size > kExactK;
-    const bool resident = hidden_size <= kResidentK;
-    auto stats = top_k ? (wide ? head_stats_kernel<true, false, true>
-                               : (resident ? head_stats_kernel<false, true, true> : head_stats_kernel<false, false, true>))
-                       : (wide ? head_stats_kernel<true, false, false>
-                               : (resident ? head_stats_kernel<false, true, false> : head_stats_kernel<false, false, false>));
-    const uint32_t k_blocks = (hidden_size + kBK - 1) / kBK;
-    const uint32_t stages = resident ? resident_stages(k_blocks) : kStreamedStages;
-    const uint32_t smem = kSmemFixed + (resident ? k_blocks * kABytes + stages * kBBytes : stages * (kABytes + kBBytes));
-    static std::atomic<uint64_t> configured[2][3];
-    if (smem_optin_once(stats, kSmemLimit, configured[top_k ? 1 : 0][wide ? 2 : (resident ? 1 : 0)]) != cudaSuccess) return DH_ERR_CUDA;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     float4* partials = static_cast<float4*>(workspace);
     uint8_t* maxima = static_cast<uint8_t*>(workspace) + partial_bytes(split);
     uint2* group_max = top_k ? reinterpret_cast<uint2*>(maxima) : nullptr;
     uint16_t* part_max = top_k ? reinterpret_cast<uint16_t*>(maxima + group_bytes(split)) : nullptr;
-    const HeadScoreParams sp{split, vocabulary_size, mask_token_id, hidden_size, stages, a_scale, w_scale, bias,
+    const HeadScoreParams sp{split, vocabulary_size, mask_token_id, hidden_size, 0, a_scale, w_scale, bias,
                              partials, group_max, part_max};
-    stats<<<split.grid, kHeadThreads, smem, s>>>(ta, tb, sp);
-    DH_LAUNCH_CHECK();
+    const cudaError_t e = split.cols == 192 ? launch_stats<192>(ta, tb, sp, wide, s) : launch_stats<256>(ta, tb, sp, wide, s);
+    if (e != cudaSuccess) return DH_ERR_CUDA;
     const HeadRowParams rp{split, vocabulary_size, mask_token_id, hidden_size, hidden, ld_hidden, weights,
                            ld_weights, a_scale, w_scale, bias, partials, group_max, part_max, out};
     const bool team = rows < kTeamRows;
     auto rows_kernel = wide ? (team ? head_rows_kernel<true, kRowWarps> : head_rows_kernel<true, 1>)
                             : (team ? head_rows_kernel<false, kRowWarps> : head_rows_kernel<false, 1>);
     // the part maxima of 8 rows, each row's 1 mod 2 words apart, where they fit
-    uint32_t staged = (split.n_tiles * kParts / 2) | 1u;
+    uint32_t staged = ((split.all_parts() + 1) / 2) | 1u;
     if (!top_k || team || staged > kMaxStaged) staged = 0;
     // (its launch and its given tokens' logits overlap the first kernel's end: 32 rows
     // 21.5 against 23.5 us, 1001 rows and 8 alternatives 64.5 against 66.6)

@@ -389,6 +389,18 @@ def test_head_logprobs_streamed(cuda, rows, top_k, size):
     check_scores(scoring.head_logprobs(*cu(args), t.cuda(), top_k=top_k), x, t, top_k)
 
 
+@pytest.mark.parametrize("size", [64, 800, 1040])
+@pytest.mark.parametrize("rows, vocab, top_k", [(300, 20000, 0), (300, 20000, 9), (900, 9001, 32), (128, 37888, 4)])
+def test_head_logprobs_many_tiles(cuda, rows, vocab, top_k, size):
+    """Enough tiles for several to a multiprocessor, of either width."""
+    (a, sa, w, sw, b), t = head_case(rows, vocab, size, size + top_k)
+    got = scoring.head_logprobs(*cu((a, sa, w, sw, b)), t.cuda(), top_k=top_k, mask_token_id=7)
+    pick = torch.tensor([0, 1, 8, 17, 63, 64, 126, 127] + ([128, 255, 256, 299] if rows > 128 else []))
+    x = ref_linear(a[pick], sa[pick], w, sw, b)[1].float().double()
+    some = got._replace(**{f: v[pick.cuda()] for f, v in got._asdict().items() if v is not None})
+    check_scores(some, x, t[pick], top_k, 7)
+
+
 @pytest.mark.parametrize("rows", [3, 800])
 @pytest.mark.parametrize("size", [64, 1040])
 def test_head_logprobs_many_equal(cuda, rows, size):
