@@ -13,8 +13,9 @@
 //
 // The k best tokens: the k-th largest of any maxima of disjoint sets of logits
 // is at most the k-th best logit.  The threads leave their maxima so far in
-// shared memory after the first and the third stage of a row; each warp takes a
-// bound from what it finds there and from then on notes each batch of a thread
+// shared memory after the first and the third stage of a row (for more than 8
+// alternatives also after the 7th, 15th and so on); each warp takes a bound from what
+// it finds there and from then on notes each batch of a thread
 // whose maximum, which the softmax needs anyway, reaches it.  At the end of the
 // row the bound from all threads' maxima leaves about k batches of 64 bytes,
 // which the finisher reads again, from L2.  Which batches are noted depends on
@@ -24,10 +25,11 @@
 //
 // What bounds it: memory, with rows enough to fill the GPU (16384 x 50258 fp32
 // logits without alternatives 486 us, 6.8 TB/s; 8880 x 50258 fp32 with 8
-// alternatives 311 us, 5.7 TB/s); the end of the last rows with few (512 x 50258
+// alternatives 309 us, 5.8 TB/s); the end of the last rows with few (512 x 50258
 // fp32 27 us, 35 with 5 alternatives, one row 12 and 18), which is latency of
-// shared memory, shuffles and code that runs once a row.  Large k adds notes
-// (8880 x 50258 fp32 with 32 alternatives 645 us).
+// shared memory, shuffles and code that runs once a row.  A large k adds notes
+// (8880 x 50258 fp32 with 32 alternatives 430 us; 645 with two bounds a row and room
+// for 256 notes, where rows lost some and were read again).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -264,15 +266,15 @@ constexpr uint32_t kFinishers = 2;
 constexpr uint32_t kThreads = kScoreThreads + 32 + 32 * kFinishers;
 constexpr uint32_t kRingStages = 3;
 constexpr uint32_t kCtasPerSM = 3;
-constexpr uint32_t kNotes = 256;    // batches a row may note (more: its threads' whole shares are read again)
+constexpr uint32_t kNotes = 448;    // batches a row may note (more: its threads' whole shares are read again)
 constexpr uint32_t kBatches = kScoreThreads + kNotes;
 
 struct StreamSmem {
     uint4 ring[kRingStages][kStageVecs];
     // what a row's threads end with, and what a finisher needs for it
     float m[kFinishers][kScoreThreads], s[kFinishers][kScoreThreads], t[kFinishers][kScoreThreads];
-    // the threads' maxima after these stages of the row, -inf before
-    float m_first[kFinishers][kScoreThreads], m_third[kFinishers][kScoreThreads];
+    // the threads' maxima after the first stage of the row and a later one, -inf before
+    float m_first[kFinishers][kScoreThreads], m_later[kFinishers][kScoreThreads];
     uint2 notes[kFinishers][kNotes];   // maximum and batch
     uint32_t note_count[kFinishers];
     uint32_t batches[kFinishers][kBatches];
@@ -282,6 +284,7 @@ struct StreamSmem {
     uint64_t taken[kFinishers];   // and were read
 };
 constexpr uint32_t kStreamSmem = sizeof(StreamSmem) + 128;
+static_assert(kCtasPerSM * (kStreamSmem + 1024) <= 228 * 1024, "shared memory of an SM");
 
 template <class T, bool kTop>
 __global__ void __launch_bounds__(kThreads, kCtasPerSM)
@@ -304,7 +307,7 @@ token_scores_kernel(const __grid_constant__ LogitRows p) {
         tc::fence_barrier_init();
     }
     for (uint32_t i = tid; i < kFinishers * kScoreThreads; i += kThreads)
-        (&sm.m_first[0][0])[i] = (&sm.m_third[0][0])[i] = -CUDART_INF_F;
+        (&sm.m_first[0][0])[i] = (&sm.m_later[0][0])[i] = -CUDART_INF_F;
     __syncthreads();
 
     if (warp < kScoreWarps) {
@@ -318,7 +321,7 @@ token_scores_kernel(const __grid_constant__ LogitRows p) {
             if (tid < x.edges) add_one(st, m, x.element(x.edge_id(tid)));
             // this row's results go where the finisher's last row's were
             if (!tc::mbar_wait(&sm.taken[f], f_phase ^ 1, tc::kErrTimeoutEmpty)) break;
-            uint32_t j = 0;  // the row's stage
+            uint32_t j = 0, take = 1;  // the row's stage, and the one that takes the next bound
             for (uint32_t v = x.v_lo; v < x.v_hi; v += kStageVecs, ++j) {
                 if (!tc::mbar_wait(&sm.full[stage], phase, tc::kErrTimeoutFull)) {
                     ok = false;
@@ -347,17 +350,19 @@ token_scores_kernel(const __grid_constant__ LogitRows p) {
                     phase ^= 1;
                 }
                 if (kTop) {
-                    if (j == 1 || j == 3) {
-                        const volatile float* held = j == 1 ? sm.m_first[f] : sm.m_third[f];
+                    if (j == take) {
+                        const volatile float* held = j == 1 ? sm.m_first[f] : sm.m_later[f];
                         float a = -CUDART_INF_F, b = -CUDART_INF_F;
 #pragma unroll
                         for (uint32_t w = 0; w < kScoreWarps; ++w) two_largest(a, b, held[w * 32 + lane]);
                         bound = kth_largest_of_pairs(a, b, p.out.top_k, lane);
+                        // (a larger k's bound is lower, and worth taking again as it rises)
+                        take = j == 1 || p.out.top_k > 8 ? 2 * j + 1 : 0xFFFFFFFFu;
                     }
                     if (j == 0) {
                         sm.m_first[f][tid] = m;
                     } else {
-                        if (j == 2) sm.m_third[f][tid] = m;
+                        if (j + 1 == take) sm.m_later[f][tid] = m;
                         const bool note = h >= bound && h > -CUDART_INF_F;
                         const uint32_t who = __ballot_sync(kFullMask, note);
                         if (who) {
@@ -469,7 +474,7 @@ token_scores_kernel(const __grid_constant__ LogitRows p) {
                         // everything of this row was read
 #pragma unroll
                         for (uint32_t w = 0; w < kScoreWarps; ++w)
-                            sm.m_first[f][w * 32 + lane] = sm.m_third[f][w * 32 + lane] = -CUDART_INF_F;
+                            sm.m_first[f][w * 32 + lane] = sm.m_later[f][w * 32 + lane] = -CUDART_INF_F;
                         if (lane == 0) sm.note_count[f] = 0;
                         __syncwarp();
                         if (lane == 0) tc::mbar_arrive(&sm.taken[f]);
