@@ -205,6 +205,23 @@ def test_token_logprobs_far_rows(cuda):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shift, scale", [(1e4, 1.0), (-1e6, 1.0), (3e8, 1.0), (-1e10, 1.0), (3e38, 1.0), (0.0, 1e3),
+                                          (0.0, 1e7), (-1e5, 1e9), (0.0, 1e12), (0.0, 1e37)])
+def test_token_logprobs_magnitudes(cuda, dtype, shift, scale):
+    """Logits around any value, and as far apart, with giants among usual ones."""
+    x, t = logits_case(8, 30011, torch.float32, 17, scale=scale)
+    x += shift
+    x[3] = logits_case(1, 30011, torch.float32, 18)[0][0]
+    x[4] = x[3]
+    x[5] = x[3]
+    x[3, 7000], x[4, 29000], x[5, 3] = 3e38, -3e38, 1.1e9
+    lim = torch.finfo(dtype).max
+    x = x.clamp(-lim, lim).to(dtype)
+    for k in (0, 5):
+        check_scores(scoring.token_logprobs(x.cuda(), t.cuda(), top_k=k), x.double(), t, k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("vocab", [20001, 50258])
 def test_token_logprobs_many_equal_or_ordered(cuda, dtype, vocab):
     """Rows most of whose logits reach the bound of the k best: all equal, rising, falling, in steps."""
