@@ -576,6 +576,8 @@ DH_DEVINL uint32_t group_token(uint32_t group, uint32_t j) {
 // hidden row.  Any order of the k dimension serves as long as both operands
 // share it, so a lane loads 16 consecutive bytes of token lane / 4 of both, and
 // feeds them to two MMAs.  Every lane receives the sums of these two tokens.
+// kUnroll: how many 64 bytes of each row are in flight.
+template <uint32_t kUnroll>
 DH_DEVINL int2 group_sums(const int8_t* h, const int8_t* w, uint64_t ldw, uint32_t group_a, uint32_t group_b,
                           uint32_t vocab, uint32_t k, uint32_t lane) {
     const uint32_t g = lane / 4, t = lane % 4;
@@ -585,7 +587,6 @@ DH_DEVINL int2 group_sums(const int8_t* h, const int8_t* w, uint64_t ldw, uint32
     const int4* px = reinterpret_cast<const int4*>(h) + t;
     int32_t c[4] = {0, 0, 0, 0};
     const uint32_t vecs = k / 16;
-    constexpr uint32_t kUnroll = 3;  // of 64 bytes a row: 6 loads a lane in flight
     uint32_t at = 0;
 #pragma unroll 1
     for (; at + 4 * kUnroll <= vecs; at += 4 * kUnroll, pa += 4 * kUnroll, pb += 4 * kUnroll, px += 4 * kUnroll) {
@@ -639,9 +640,11 @@ static_assert(sizeof(RowsSmem<1>) + kMaxStaged * kRowWarps * sizeof(float) <= 48
               "shared memory of a launch without an opt-in");
 
 // kTeam warps a row: 1 when there are rows enough for every warp of the GPU,
-// all of a CTA's when there are few.
-template <bool kWide, uint32_t kTeam>
-__global__ void __launch_bounds__(32 * kRowWarps, 4)
+// all of a CTA's when there are few.  kPerSM: CTAs an SM holds, 4, or 2 with the
+// registers for more loads in flight (32 rows and 8 alternatives 25.6 against 27.6
+// us, 256 rows 31.8 against 33.8; 512 rows, in two turns, 48 against 42).
+template <bool kWide, uint32_t kTeam, uint32_t kPerSM>
+__global__ void __launch_bounds__(32 * kRowWarps, kPerSM)
 head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged) {
     extern __shared__ uint32_t staged_max[];  // the part maxima of the CTA's rows, if `staged` holds them: [kTeams][staged]
     constexpr uint32_t kTeams = kRowWarps / kTeam;
@@ -848,7 +851,7 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
         const uint32_t c = group_token(lane % 4 & 1u ? gb : ga, lane / 4);
         const bool in = lane % 4 < (two ? 2u : 1u) && c < p.vocab && c != p.mask_id;
         const float w = in ? __ldg(p.w_scale + c) : 0.f, b = in && p.bias ? __ldg(p.bias + c) : 0.f;
-        const int2 acc = group_sums(h, p.weights, p.ld_weights, ga, gb, p.vocab, p.k, lane);
+        const int2 acc = group_sums<kPerSM == 2 ? 6 : 3>(h, p.weights, p.ld_weights, ga, gb, p.vocab, p.k, lane);
         const float x = score_logit<kWide>(lane % 4 ? acc.y : acc.x, ab, w, b);
         best.add(in && x >= least && x > -CUDART_INF_F ? token_key(x, c) : 0ull);
     }
@@ -980,8 +983,12 @@ extern "C" uint32_t dh_head_logprobs_i8(const int8_t* hidden, uint64_t ld_hidden
     const HeadRowParams rp{split, vocabulary_size, mask_token_id, hidden_size, hidden, ld_hidden, weights,
                            ld_weights, a_scale, w_scale, bias, partials, group_max, part_max, out};
     const bool team = rows < kTeamRows;
-    auto rows_kernel = wide ? (team ? head_rows_kernel<true, kRowWarps> : head_rows_kernel<true, 1>)
-                            : (team ? head_rows_kernel<false, kRowWarps> : head_rows_kernel<false, 1>);
+    const bool deep = rows <= 2 * device_sms();
+    auto rows_kernel =
+        wide ? (team ? (deep ? head_rows_kernel<true, kRowWarps, 2> : head_rows_kernel<true, kRowWarps, 4>)
+                     : head_rows_kernel<true, 1, 4>)
+             : (team ? (deep ? head_rows_kernel<false, kRowWarps, 2> : head_rows_kernel<false, kRowWarps, 4>)
+                     : head_rows_kernel<false, 1, 4>);
     // the part maxima of 8 rows, each row's 1 mod 2 words apart, where they fit
     uint32_t staged = ((split.all_parts() + 1) / 2) | 1u;
     if (!top_k || team || staged > kMaxStaged) staged = 0;

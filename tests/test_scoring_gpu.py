@@ -489,7 +489,7 @@ def test_head_logprobs_odd_rows(cuda):
     check_scores(got._replace(top_ids=None, top_logprobs=None), x, t[:2], 0)
 
 
-@pytest.mark.parametrize("vocab", [75776, 75777, 80000, 81665, 90001])
+@pytest.mark.parametrize("vocab", [75776, 75777, 80000, 81665, 90001, 131072, 131073])
 def test_head_logprobs_large_vocabularies(cuda, vocab):
     """As many rows as get a warp each, around the vocabularies whose maxima shared memory holds."""
     (a, sa, w, sw, b), t = head_case(770, vocab, 16, vocab)
