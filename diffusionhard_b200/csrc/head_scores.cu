@@ -21,7 +21,7 @@
 // (32768 x 50258, hidden 768: 880 us, of which 785 remain with an epilogue that
 // reads nothing, 2.9 Pop/s; with maxima 965); the second, reads of weight rows from
 // L2 (5 alternatives 175 us, 32 of 4096 rows 127 us, about 10 TB/s; none 30 us).
-// With few rows both are latency: 32 rows 19.5 us, 28 with 8 alternatives.
+// With few rows both are latency: 32 rows 19.5 us, 25.6 with 8 alternatives.
 #include <cuda_fp16.h>
 
 #include "dequant.cuh"

@@ -13,9 +13,8 @@
 //
 // The k best tokens: the k-th largest of any maxima of disjoint sets of logits
 // is at most the k-th best logit.  The threads leave their maxima so far in
-// shared memory after the first and the third stage of a row (for more than 8
-// alternatives also after the 7th, 15th and so on); each warp takes a bound from what
-// it finds there and from then on notes each batch of a thread
+// shared memory after the first, third, 7th, 15th and so on stage of a row; each warp
+// takes a bound from what it finds there and from then on notes each batch of a thread
 // whose maximum, which the softmax needs anyway, reaches it.  At the end of the
 // row the bound from all threads' maxima leaves about k batches of 64 bytes,
 // which the finisher reads again, from L2.  Which batches are noted depends on
@@ -25,7 +24,7 @@
 //
 // What bounds it: memory, with rows enough to fill the GPU (16384 x 50258 fp32
 // logits without alternatives 486 us, 6.8 TB/s; 8880 x 50258 fp32 with 8
-// alternatives 309 us, 5.8 TB/s); the end of the last rows with few (512 x 50258
+// alternatives 301 us, 5.9 TB/s); the end of the last rows with few (512 x 50258
 // fp32 27 us, 35 with 5 alternatives, one row 12 and 18), which is latency of
 // shared memory, shuffles and code that runs once a row.  A large k adds notes
 // (8880 x 50258 fp32 with 32 alternatives 430 us; 645 with two bounds a row and room
@@ -211,6 +210,17 @@ DH_DEVINL void add_one(RowStats& st, float& m, float x) {
     st.t = __fmaf_rn(e, d, st.t);
 }
 
+// At most the k-th largest of the lanes' values (k <= 16, no NaN): the least maximum
+// of k or more groups of lanes.  Lower than kth_largest_of_pairs, so that more is
+// noted, but without its k steps one after the other, which every warp takes several
+// times a row: 4096 x 50258 bf16 logits with 8 alternatives 116 against 123 us, 16000
+// x 8000 fp32 174 against 187.  For more than 8 it would be too low.  Whole warp.
+DH_DEVINL float least_of_groups(float v, uint32_t k) {
+#pragma unroll 1
+    for (uint32_t d = 1; d * k <= 16; d <<= 1) v = fmaxf(v, __shfl_xor_sync(kFullMask, v, d));
+    return -lanes_max(-v);
+}
+
 // A batch: the kScoreUnroll vectors of one stage that one thread adds.
 DH_DEVINL uint32_t batch_id(uint32_t stage, uint32_t thread) { return stage * kScoreThreads + thread; }
 
@@ -355,9 +365,9 @@ token_scores_kernel(const __grid_constant__ LogitRows p) {
                         float a = -CUDART_INF_F, b = -CUDART_INF_F;
 #pragma unroll
                         for (uint32_t w = 0; w < kScoreWarps; ++w) two_largest(a, b, held[w * 32 + lane]);
-                        bound = kth_largest_of_pairs(a, b, p.out.top_k, lane);
-                        // (a larger k's bound is lower, and worth taking again as it rises)
-                        take = j == 1 || p.out.top_k > 8 ? 2 * j + 1 : 0xFFFFFFFFu;
+                        bound = p.out.top_k > 2 && p.out.top_k <= 8 ? least_of_groups(a, p.out.top_k)
+                                                                    : kth_largest_of_pairs(a, b, p.out.top_k, lane);
+                        take = 2 * j + 1;
                     }
                     if (j == 0) {
                         sm.m_first[f][tid] = m;
