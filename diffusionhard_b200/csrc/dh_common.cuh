@@ -48,12 +48,20 @@ inline cudaError_t smem_optin_once(Kernel kernel, uint32_t bytes, std::atomic<ui
     return e;
 }
 
-// Host: streaming multiprocessors of the current device.
+// Host: streaming multiprocessors of the current device, asked once for each.
 inline uint32_t device_sms() {
+    static std::atomic<uint32_t> known[64];
     int dev = 0, v = 0;
-    if (cudaGetDevice(&dev) == cudaSuccess &&
-        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0)
+    if (cudaGetDevice(&dev) != cudaSuccess) return kNumSMs;
+    const bool keep = dev >= 0 && dev < 64;
+    if (keep) {
+        const uint32_t n = known[dev].load(std::memory_order_relaxed);
+        if (n) return n;
+    }
+    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0) {
+        if (keep) known[dev].store(static_cast<uint32_t>(v), std::memory_order_relaxed);
         return static_cast<uint32_t>(v);
+    }
     return kNumSMs;
 }
 
