@@ -49,7 +49,8 @@ constexpr uint32_t kBarBytes = 1024;
 constexpr uint32_t kStagePerWarp = kPartCols * 8;       // bias and w_scale of the warp's columns
 // Shared memory: with k <= kResidentK the row tile's A stays for all its column
 // tiles and the ring holds B alone (the copies into shared memory compete with
-// the MMA's and the epilogue's reads of it); otherwise a stage holds both.
+// the MMA's and the epilogue's reads of it: 32768 x 50258, hidden 768, 871 against
+// 915 us); otherwise a stage holds both.
 constexpr uint32_t kSmemLimit = 227 * 1024;
 constexpr uint32_t kResidentK = 768;
 constexpr uint32_t kStreamedStages = 4;
