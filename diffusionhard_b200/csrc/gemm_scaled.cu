@@ -44,9 +44,9 @@ constexpr uint32_t kFull = 0xFFFFFFFFu;
 DH_DEVINL uint16_t to_bits16(float v, __nv_bfloat16) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
 DH_DEVINL uint16_t to_bits16(float v, __half) { return __half_as_ushort(__float2half_rn(v)); }
 
-// ------------------------------------------------------------ small products
+// ---------------------------------------------------- small and tall products
 //
-// 128 x 64 tiles on the kernel of gemm_tc.cuh: at most one a CTA.  Latency of the
+// 128 x 64 tiles on the kernel of gemm_tc.cuh, mostly one a CTA.  Latency of the
 // k-blocks bounds it: 1 x 2304 x 768 4.7 us from a graph, 32 x 768 x 3072 7.3.
 template <class T>
 struct EpiScaled : EpiBase {
@@ -541,18 +541,19 @@ extern "C" uint32_t dh_gemm_i8_scaled(const int8_t* a, uint64_t lda, const float
     // holds a pitch of 2^40 bytes)
     const bool tma = vec && n * static_cast<uint64_t>(es) % 16 == 0 && ldo < (1ull << 38);
     const uint32_t sms = device_sms();
-    // Tiles of 64 columns where each gets an SM of its own (launched from a graph, 256 x
-    // 4736 x 768 to bf16 4.9 against 6.7 us in wide tiles; in two rounds of them 512 x
-    // 3600 x 4096 took 15.8 against 14.5); else of the width whose rounds over the SMs
-    // take fewer columns in all: 4096 x 4096 x 4096 to bf16
-    // (5 rounds of 192 or 4 of 256) 58 against 63 us, 1024 x 8192 x 8192 (3 or 2)
-    // 76 against 68, 512 x 50258 x 768 to fp32 (8 or 6: as many) 53 against 59.
+    // Wide tiles of the width whose rounds over the SMs take fewer columns in all: 4096
+    // x 4096 x 4096 to bf16 (5 rounds of 192 or 4 of 256) 58 against 63 us, 1024 x 8192 x
+    // 8192 (3 or 2) 76 against 68, 512 x 50258 x 768 to fp32 (8 or 6: as many) 53 against
+    // 59.  Tiles of 64 columns where each gets an SM of its own (launched from a graph,
+    // 256 x 4736 x 768 to bf16 4.9 against 6.7 us), or where they take fewer columns at
+    // one and a half times the price: 32768 x 64 x 768 to bf16 7.5 against 12.0 us, 32768
+    // x 128 x 4096 (4 rounds or 2 of 192) 32.9 against 31.2.
     auto columns = [&](uint32_t cols) {
         const uint64_t t = static_cast<uint64_t>(m_tiles) * ((n + cols - 1) / cols);
         return (t + sms - 1) / sms * cols;
     };
-    const uint32_t bn = static_cast<uint64_t>(m_tiles) * ((n + 63) / 64) <= sms ? 64u
-                        : columns(192) <= columns(256) ? 192u : 256u;
+    const uint32_t wide = columns(192) <= columns(256) ? 192u : 256u;
+    const uint32_t bn = columns(64) == 64 || columns(64) * 3 < columns(wide) * 2 ? 64u : wide;
     const uint64_t tiles = static_cast<uint64_t>(m_tiles) * ((n + bn - 1) / bn);
     if (tiles > 0x7FFFFFFFull || m > 0x7FFFFF00u || n > 0x7FFFFF00u) return DH_ERR_UNSUPPORTED_SHAPE;
     CUtensorMap ta, tb;

@@ -335,6 +335,26 @@ def test_linear_i8_out_large(cuda, dtype, n, pitch, start):
     assert bool((buf == 7.0).all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m, n, k, pitch", [(19001, 64, 96, 64), (32768, 50, 64, 53), (38000, 1, 128, 1), (20000, 61, 144, 64)])
+def test_linear_i8_tall(cuda, dtype, m, n, k, pitch):
+    """Many rows and few columns: several narrow tiles to a multiprocessor."""
+    args = linear_case(m, n, k, m + n)
+    buf = torch.full((m + 1, pitch), 7.0, dtype=dtype, device="cuda")
+    out = buf[:m, :n]
+    scoring.linear_i8(*cu(args), out=out)
+    y = ref_linear(*args)[1]
+    if dtype == torch.float32:
+        assert torch.equal(out.cpu(), y.float())
+    else:
+        prod = y - args[4].double()
+        lim = torch.finfo(dtype)
+        tol = U * (prod.abs() + y.abs()) * 1.01 + lim.eps / 2 * 1.01 * y.abs().clamp(min=lim.tiny)
+        assert bool(((out.cpu().double() - y).abs() <= tol).all())
+    out.fill_(7.0)
+    assert bool((buf == 7.0).all())
+
+
 def test_linear_i8_odd_scales_large(cuda):
     """Scales of 0, infinity, NaN, negative, tiny and huge, and odd biases, in the large tiles."""
     a, sa, w, sw, b = linear_case(300, 5000, 64, 12)
