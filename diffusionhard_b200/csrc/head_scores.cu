@@ -790,8 +790,10 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
         }
     }
     bound = kth_largest_of_pairs(a, b, k, lane);
-    // no logit below `least` rounds to it, no group's byte is below group_bound
-    const uint16_t bits = __half_as_ushort(__float2half_rz(bound));
+    // no logit below `least` rounds to it, no group's byte is below group_bound.  (A
+    // bound of zero counts as -0, what logits just below zero round to: the zeros
+    // compare equal, so that its sign may be that of another maximum.)
+    const uint16_t bits = bound == 0.f ? 0x8000u : __half_as_ushort(__float2half_rz(bound));
     const float least = bits >= 0x8000u && bits < 0xFC00u ? half_float(bits + 1u) : bound;
     const float group_bound = half_float(bits & 0xFF00u);
     auto group_reaches = [&](uint32_t part, uint32_t b) {

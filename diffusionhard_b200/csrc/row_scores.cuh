@@ -156,8 +156,9 @@ DH_DEVINL float sort_step(float v, uint32_t stride, bool desc, uint32_t lane) {
     return ((lane & stride) != 0) != desc ? fmaxf(v, o) : fminf(v, o);
 }
 
-// The k-th largest of the lanes' pairs a >= b (1 <= k <= 64, no NaN): one maximum
-// after the other for a small k (~115 clocks each), else a sort of the 64.
+// The k-th largest of the lanes' pairs a >= b (1 <= k <= 64, no NaN; of a zero the
+// sign may be either): one maximum after the other for a small k (~115 clocks each),
+// else a sort of the 64.
 // Rolled up: code that runs once a row is fetched from afar each time, and
 // unrolled loops took longer to fetch than to run.  Whole warp.
 DH_DEVINL float kth_largest_of_pairs(float a, float b, uint32_t k, uint32_t lane) {

@@ -567,6 +567,30 @@ def test_head_logprobs_padded_rows(cuda):
         check_scores(got, x, t, 7)
 
 
+@pytest.mark.parametrize("size", [64, 1040])
+@pytest.mark.parametrize("rows", [5, 800])
+@pytest.mark.parametrize("kind", ["one zero", "few above", "both signs", "subnormal"])
+def test_head_logprobs_near_zero(cuda, kind, rows, size):
+    """Logits next to zero on either side, far below what a half float tells from it."""
+    (a, sa, w, sw, b), t = head_case(rows, 1000, size, 11)
+    g = torch.Generator().manual_seed(12)
+    b[:] = -1e-8
+    if kind == "one zero":
+        b[200] = 0.0
+    elif kind == "few above":
+        b[[40, 200, 777]] = torch.tensor([1e-9, 3e-8, 5e-8])
+    else:
+        b[:] = torch.randn(1000, generator=g) * (1e-8 if kind == "both signs" else 1e-40)
+    sa[:] = 0.0  # every logit its bias
+    sa[1::2] = 1e-9 if kind != "subnormal" else 1e-39
+    pick = torch.tensor([0, 1, 2, 3, 4] if rows == 5 else [0, 1, 127, 128, 513, 798, 799])
+    x = ref_linear(a[pick], sa[pick], w, sw, b)[1].float().double()
+    for k in (1, 2, 3, 5, 8, 9, 32):
+        got = scoring.head_logprobs(*cu((a, sa, w, sw, b)), t.cuda(), top_k=k, mask_token_id=3)
+        some = got._replace(**{f: v[pick.cuda()] for f, v in got._asdict().items()})
+        check_scores(some, x, t[pick], k, 3)
+
+
 # ------------------------------------------------------- use of the calls
 
 def _calls():
