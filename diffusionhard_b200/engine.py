@@ -151,6 +151,7 @@ class MDLMEngine:
         self._compact_bufs: Optional[tuple] = None  # seq_list, per-row head input and scale
         self._graphs: Dict[Any, Any] = {}
         self._events = (torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True))
+        self._whole_forward = False  # self.x is a forward of the whole canvas, and no generation came after it
         self.launches_per_forward = 1 + 9 * len(self.blocks)
 
     def shard_head(self, v0: int, v1: int, group: Any = None, reduce: Any = None) -> None:
@@ -192,6 +193,7 @@ class MDLMEngine:
         are the packed positions of the listed sequences.  hook(i) runs after
         block i."""
         s = _lib.stream_handle()
+        self._whole_forward = False
         tok = self.tokens if tokens is None else tokens
         rr = self._p(run_rows) if run_rows is not None else None
         if seq_list is not None:
@@ -204,6 +206,7 @@ class MDLMEngine:
             self._forward_block(i, blk, rr, s)
             if hook is not None:
                 hook(i)
+        self._whole_forward = run_rows is None and seq_list is None
 
     def _forward_block(self, i: int, blk: dict, rr: Any, s: Any) -> None:
         M, L = self.M, self.L
@@ -247,17 +250,21 @@ class MDLMEngine:
         debugging (the samplers and `score` never materialise logits): the
         int8 head product with the reference dequant
         out = fp32(acc * fp64(a_scale * w_scale) + bias) in its epilogue
-        (fixed_mlp.quantized_linear, fixed_mlp.py:120-136)."""
+        (fixed_mlp.quantized_linear, fixed_mlp.py:120-136).  The forward is
+        :meth:`forward` of the whole canvas: a generation keeps its residual
+        stream elsewhere, or leaves that of an earlier canvas or of packed rows."""
         hq, hs = self.final_hidden_q()
         h = self.head
         return linear_i8(hq, hs, h.w, h.w_scale, h.bias).view(self.B, self.L, h.out_features)
 
     @_on_device
     def score(self, targets: Any = None, *, rows: Any = None, top_k: int = 0) -> TokenScores:
-        """Scores of the last forward's distributions under the SUBS
+        """Scores of the distributions of the last :meth:`forward` under the SUBS
         parametrisation (mask token excluded; mdlm._mdlm_log_probabilities,
         mdlm.py:851-858), the head's logits never stored: log probabilities of
-        `targets`, entropy, logsumexp and the `top_k` best tokens.
+        `targets`, entropy, logsumexp and the `top_k` best tokens.  That forward
+        was of the whole canvas, with no generation after it (RuntimeError): to
+        score what was generated, call ``forward()`` first (api.score_tokens does).
 
         rows: int positions [n] of the flattened [B * L] canvas (default: all
         of them, in order; checked on the host, which waits for them); targets:
@@ -266,6 +273,8 @@ class MDLMEngine:
         h = self.head
         if h.out_features != self.cfg.vocab_size:
             raise ValueError("a vocabulary-sharded head holds no whole distribution")
+        if not self._whole_forward:
+            raise RuntimeError("score() needs a forward() of the whole canvas, with no generation after it")
         if rows is None:
             n = self.M
             hq, hs = self.final_hidden_q()
@@ -497,6 +506,7 @@ class MDLMEngine:
 
             def enqueue() -> None:
                 self._enqueue_generation(steps, seed, thresholds)
+        self._whole_forward = False
         if graph:
             key = (native, self._compact_now, steps, seed, sampling_epsilon, self.seq_offset)
             g = self._graphs.get(key)
@@ -595,6 +605,7 @@ class MDLMEngine:
             self._events[0].record()
             self._enqueue_event_generation(sched, seed, counts)
             self._events[1].record()
+        self._whole_forward = False
         return self.tokens.view(self.B, self.L)
 
     def generation_ms(self) -> float:

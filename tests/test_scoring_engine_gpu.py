@@ -163,3 +163,54 @@ def test_rows_of_other_types(engine):
             engine.score(rows=bad)
     a = engine.score(rows=torch.tensor([3, 5], dtype=torch.int32), top_k=2)
     assert torch.equal(a.top_ids, engine.score(rows=torch.tensor([3, 5]).cuda(), top_k=2).top_ids)
+
+
+def test_score_wants_a_whole_forward(cuda):
+    """Nothing is scored from a residual stream that no forward of the whole canvas left."""
+    eng = MDLMEngine(build_quantized(MDLMConfig(vocab_size=VOCAB, mask_token_id=MASK, blocks=2), seed=0), 2, 32, "cuda")
+    ids = torch.full((2, 32), MASK)
+    tokens = ids.view(-1).to("cuda", torch.int32)
+    t = torch.arange(64, device="cuda")
+
+    def refused():
+        for rows in (None, torch.tensor([1])):
+            with pytest.raises(RuntimeError, match="forward"):
+                eng.score(rows=rows)
+
+    refused()
+    eng.forward(tokens)
+    want = eng.score(t, top_k=3)
+
+    def generations():
+        for native in (True, False):
+            for compact in (True, False):
+                for graph in (False, True):
+                    eng.compact = compact
+                    yield lambda: eng.generate(ids, steps=4, native=native, graph=graph)
+        for graph in (False, True, True):
+            yield lambda: api.run_event_driven_candidate_sampler(eng, ids, mask_token_id=MASK, steps=4, reveal_seed=1,
+                                                                 graph=graph)
+        yield lambda: eng.forward(tokens, run_rows=eng.fwd_rows.fill_(32))
+
+    for generation in generations():
+        generation()
+        refused()
+        eng.forward(tokens)
+        assert all(torch.equal(p, q) for p, q in zip(want, eng.score(t, top_k=3)))
+    eng.generate(ids, steps=4)
+    generated = eng.tokens.view(2, 32).long()
+    r = api.score_tokens(eng, generated, generated, mask_token_id=MASK, every_position=True)
+    eng.forward(generated.view(-1).to(torch.int32))
+    _, lp = reference_of(eng)
+    assert close(r["logprobs"].view(-1), lp.gather(1, generated.view(-1, 1))[:, 0])
+    with pytest.raises(ValueError, match="input_ids"):
+        eng.generate(ids[:1], steps=4)
+    eng.score(t)  # the refused generation ran nothing
+    _lib.check_device_error()
+
+
+def reference_of(eng):
+    logits = eng.logits().view(-1, VOCAB)
+    x = logits.double()
+    x[:, MASK] = -math.inf
+    return logits, torch.log_softmax(x, 1)
