@@ -412,7 +412,8 @@ head_stats_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         uint32_t mt = mt0, nt = tile0 % n_tiles;  // this tile
         // the next tile's scales and biases, fetched while one is added: columns
         // that are excluded (past the vocabulary, the masked token) get a logit
-        // of -inf from a scale of 0 and that bias
+        // of -inf from a scale of 0 and that bias (NaN in rows whose own scale is
+        // infinite or NaN: settle_row answers these)
         float w_next[kPartCols / 32], b_next[kPartCols / 32], ab[4];
         auto fetch = [&](uint32_t n) {
 #pragma unroll
@@ -621,6 +622,34 @@ DH_DEVINL int2 group_sums(const int8_t* h, const int8_t* w, uint64_t ldw, uint32
     return sums;
 }
 
+// A row whose scale is infinite or NaN, from end to end.  All of its logits are
+// infinite or NaN, so it is empty (each -inf) or has no answer, and mostly the first
+// tokens tell.  (The first kernel's statistics of such a row are NaN either way, from
+// columns that are no token; setting these to -inf there cost every call 1 to 3%.)
+// Out of line, and the row ends with it: hardly a row needs it.  Whole warp.
+template <bool kWide>
+static __device__ __noinline__ void settle_row(const HeadRowParams& p, uint64_t row) {
+    const uint32_t lane = lane_id();
+    const int8_t* h = p.hidden + row * p.ld_hidden;
+    const float ab = __ldg(p.a_scale + row);
+    bool bad = false;
+#pragma unroll 1
+    for (uint32_t c = lane; c - lane < p.vocab && !bad; c += 32) {
+        bool other = false;
+        if (c < p.vocab && c != p.mask_id) {
+            const int32_t acc = dot_share(h, p.weights + c * p.ld_weights, p.k, 0, 1);
+            const float x = score_logit<kWide>(acc, ab, __ldg(p.w_scale + c), p.bias ? __ldg(p.bias + c) : 0.f);
+            other = !(x == -CUDART_INF_F);
+        }
+        bad = __any_sync(kFullMask, other);
+    }
+    const RowResult r = row_result(-CUDART_INF_F, bad ? CUDART_NAN_F : 0.f, 0.f);
+    if (lane == 0) store_row(p.out, row, r);
+    store_top(p.out, row, r, 0, lane);
+    for (uint32_t i = lane; i < p.out.targets_per_row; i += 32)
+        p.out.logprobs[row * p.out.targets_per_row + i] = given_logprob(r, target_of(p.out, row, i), p.vocab, 0.f);
+}
+
 constexpr uint32_t kRowWarps = 8;
 constexpr uint32_t kMaxStaged = 1025;  // words of shared memory a row: vocabularies up to 131,072
 constexpr uint32_t kPicks = 256;  // groups kept for the k best (more, by ties: every group is looked at)
@@ -700,6 +729,10 @@ head_rows_kernel(const __grid_constant__ HeadRowParams p, const uint32_t staged)
         __syncthreads();
     }
     if (!have) return;
+    if (!(fabsf(ab) < CUDART_INF_F)) {  // the whole team's row
+        if (member == 0) settle_row<kWide>(p, row);
+        return;
+    }
 
     // the row's partial statistics
     const uint32_t mt = static_cast<uint32_t>(row / kBM), r_in = static_cast<uint32_t>(row % kBM);

@@ -591,6 +591,56 @@ def test_head_logprobs_near_zero(cuda, kind, rows, size):
         check_scores(some, x, t[pick], k, 3)
 
 
+@pytest.mark.parametrize("size", [64, 784, 1040])
+@pytest.mark.parametrize("rows, vocab", [(6, 1000), (6, 1536), (6, 50), (800, 1536), (800, 1111)])
+def test_head_logprobs_infinite_scales(cuda, rows, vocab, size):
+    """Columns that are no token, or the excluded one, make no row NaN whose own logits are all -inf."""
+    (a, sa, w, sw, b), _ = head_case(rows, vocab, size, 13)
+    a = a.abs().clamp(min=1)
+    w = -w.abs().clamp(min=1)
+    a[5] = -a[5]
+    sa[0] = math.inf    # every logit -inf
+    sa[1] = 3e38        # the products finite, or past the largest float
+    sa[2] = math.nan
+    sa[4] = -math.inf   # every logit +inf
+    sa[5] = -math.inf   # -inf again
+    sw[7::50] = 1e30
+    t = torch.tensor([[0, 8, -1, vocab - 1, vocab]] * rows)
+    pick = torch.tensor([0, 1, 2, 3, 4, 5] + ([127, 128, 799] if rows > 6 else []))
+    for mask in (None, 8):
+        # an excluded logit is taken out before NaN or infinity can come of it
+        x = ref_linear(a[pick], sa[pick], w, sw, b)[1].float().double()
+        for k in (0, 5, 32):
+            got = scoring.head_logprobs(*cu((a, sa, w, sw, b)), t.cuda(), top_k=k, mask_token_id=mask)
+            some = got._replace(**{f: v[pick.cuda()] for f, v in got._asdict().items() if v is not None})
+            check_scores(some, x, t[pick], k, mask)
+
+
+@pytest.mark.parametrize("size", [64, 1040])
+def test_head_logprobs_nothing_left(cuda, size):
+    """The only token excluded: a row is empty, whatever its scale."""
+    (a, sa, w, sw, b), _ = head_case(5, 1, size, 14)
+    sa[:] = torch.tensor([1.0, 0.0, math.inf, -math.inf, math.nan])
+    t = torch.zeros((5, 1), dtype=torch.int64)
+    x = ref_linear(a, sa, w, sw, b)[1].float().double()
+    got = scoring.head_logprobs(*cu((a, sa, w, sw, b)), t.cuda(), top_k=2, mask_token_id=0)
+    check_scores(got, x, t, 2, 0)
+
+
+@pytest.mark.parametrize("bits", [-1, 0x7FFFFFFF, 0x7FC00000, -0x400000, 0x7F800001])
+@pytest.mark.parametrize("size", [64, 1040])
+def test_head_logprobs_nan_bias(cuda, size, bits):
+    """A token's NaN bias makes every row NaN, whatever its bits; the excluded token's none."""
+    (a, sa, w, sw, b), t = head_case(5, 700, size, 15)
+    b[33] = torch.tensor([bits], dtype=torch.int32).view(torch.float32)[0]
+    x = ref_linear(a, sa, w, sw, b)[1].float().double()
+    assert bool(torch.isnan(x[:, 33]).all())
+    dev = cu((a, sa, w, sw, b))
+    dev[4].view(torch.int32)[33] = bits  # as given, not as the host rounds it
+    for mask in (None, 32, 33):
+        check_scores(scoring.head_logprobs(*dev, t.cuda(), top_k=3, mask_token_id=mask), x, t, 3, mask)
+
+
 # ------------------------------------------------------- use of the calls
 
 def _calls():
