@@ -21,14 +21,16 @@ from __future__ import annotations
 
 import ctypes
 import functools
-from typing import Any, Dict, List, Optional
+from typing import TYPE_CHECKING, Any, Dict, List, Optional
 
 import numpy as np
 
 from . import _lib
 from .model import QuantizedMDLM
 from .sampler import NOISE_EPSILON, MDLMStepMeasurement, hardware_candidate_cache_bytes, reveal_thresholds_q32
-from .scoring import TokenScores, head_logprobs, linear_i8
+
+if TYPE_CHECKING:
+    from .scoring import TokenScores  # (imports torch, which this module leaves to the engine)
 
 
 class _DevLinear:
@@ -253,6 +255,8 @@ class MDLMEngine:
         (fixed_mlp.quantized_linear, fixed_mlp.py:120-136).  The forward is
         :meth:`forward` of the whole canvas: a generation keeps its residual
         stream elsewhere, or leaves that of an earlier canvas or of packed rows."""
+        from .scoring import linear_i8
+
         hq, hs = self.final_hidden_q()
         h = self.head
         return linear_i8(hq, hs, h.w, h.w_scale, h.bias).view(self.B, self.L, h.out_features)
@@ -269,6 +273,8 @@ class MDLMEngine:
         rows: int positions [n] of the flattened [B * L] canvas (default: all
         of them, in order; checked on the host, which waits for them); targets:
         ids [n] or [n, tokens] for these rows, a negative id for "no token"."""
+        from .scoring import head_logprobs
+
         torch = self.torch
         h = self.head
         if h.out_features != self.cfg.vocab_size:
@@ -304,6 +310,8 @@ class MDLMEngine:
         forward over the whole canvas, then the final LayerNorm, quantisation
         and head GEMM of the selected rows only, dequantised as
         fixed_mlp.quantized_linear (fixed_mlp.py:120-136)."""
+        from .scoring import linear_i8
+
         torch = self.torch
         if self.B != 1 or input_ids.numel() != self.L:
             raise ValueError("selected_logits takes one sequence of the engine's length")

@@ -35,3 +35,16 @@ def test_pinned_method_enters_the_engine_device():
     assert launch(fake, 41) == 42
     assert seen == [("enter", "cuda:1"), ("body", 41), ("exit", "cuda:1")]
 
+
+def test_importing_the_engine_does_not_import_torch():
+    """Commands that end before they need an engine do not wait for torch."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = ("import sys\n"
+            "import diffusionhard_b200.api, diffusionhard_b200.session, diffusionhard_b200.prefix\n"
+            "import diffusionhard_b200.conditioned, diffusionhard_b200.event\n"
+            "sys.exit('torch' in sys.modules)")
+    root = Path(engine_mod.__file__).resolve().parents[1]
+    assert subprocess.run([sys.executable, "-c", code], cwd=root).returncode == 0
