@@ -165,7 +165,9 @@ def score_tokens(model: MDLMEngine, input_ids: Any, target_ids: Any, *, mask_tok
     """How probable `target_ids` [B, L] are at the masked positions of the
     canvas `input_ids` [B, L], by one forward and the fused head
     (mdlm._mdlm_log_probabilities, mdlm.py:851-858, whose [B, L, V] array is
-    never made).  every_position: score the unmasked positions too.
+    never made).  every_position: score the unmasked positions too.  Both are
+    integer tensors; as in a generation, an input id outside the vocabulary is
+    embedded as the last token.
 
     Returns tensors on the device of `input_ids`: "scored" bool [B, L];
     "logprobs" and "entropy" fp32 [B, L], 0 where nothing is scored;
@@ -179,10 +181,15 @@ def score_tokens(model: MDLMEngine, input_ids: Any, target_ids: Any, *, mask_tok
     shape = (model.B, model.L)
     if tuple(input_ids.shape) != shape or tuple(target_ids.shape) != shape:
         raise ValueError(f"input_ids and target_ids must be [{model.B}, {model.L}]")
+    for name, t in (("input_ids", input_ids), ("target_ids", target_ids)):
+        if t.dtype not in (torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64):
+            raise ValueError(f"{name} must be integers")
     src, dev = input_ids.device, model.device
-    ids = input_ids.to(dev, torch.int32).reshape(-1).contiguous()
+    ids = input_ids.to(dev, torch.int64).reshape(-1)
     targets = target_ids.to(dev, torch.int64).reshape(-1)
     scored = torch.ones_like(ids, dtype=torch.bool) if every_position else ids == mask_token_id
+    # (compared first, and held to ids that 32 bits keep apart from the vocabulary's)
+    ids = ids.clamp(-1, model.cfg.vocab_size).to(torch.int32)
     rows = scored.nonzero().reshape(-1)
     model.forward(ids)
     r = model.score(targets[rows], rows=rows, top_k=top_k)

@@ -1,9 +1,11 @@
 """Argument checks of the scoring entry points and functions (no device work)."""
 
+import types
+
 import pytest
 import torch
 
-from diffusionhard_b200 import _lib, scoring
+from diffusionhard_b200 import _lib, api, scoring
 
 P = 4096  # a non-null, 256-byte aligned address that no refused call touches
 NULL, ALIGN, WORKSPACE, SHAPE, ARG = 100, 101, 102, 103, 105
@@ -85,3 +87,13 @@ def test_functions_refuse_host_tensors():
         scoring.token_logprobs(torch.zeros(2, 10))
     with pytest.raises(ValueError, match="CUDA"):
         scoring.head_logprobs(i8, f, i8, f)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bool, torch.complex64])
+def test_score_tokens_wants_integers(dtype):
+    model = types.SimpleNamespace(cfg=types.SimpleNamespace(mask_token_id=9, vocab_size=10), B=1, L=4, device="cuda:0")
+    ids, other = torch.zeros((1, 4), dtype=torch.int64), torch.zeros((1, 4), dtype=dtype)
+    with pytest.raises(ValueError, match="input_ids must be integers"):
+        api.score_tokens(model, other, ids, mask_token_id=9)
+    with pytest.raises(ValueError, match="target_ids must be integers"):
+        api.score_tokens(model, ids, other, mask_token_id=9)

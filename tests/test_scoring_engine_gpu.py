@@ -214,3 +214,27 @@ def reference_of(eng):
     x = logits.double()
     x[:, MASK] = -math.inf
     return logits, torch.log_softmax(x, 1)
+
+
+def test_score_tokens_far_ids(engine):
+    """Ids past 32 bits are not taken for the tokens that their low bits spell."""
+    targets = torch.randint(0, MASK, (3, 64), generator=torch.Generator().manual_seed(6))
+    ids = engine.ids.clone()
+    ids[0, :4] = torch.tensor([2 ** 32 + MASK, 2 ** 32 + 5, -2 ** 32 + 7, -1])
+    r = api.score_tokens(engine, ids, targets, mask_token_id=MASK, top_k=1)
+    assert torch.equal(r["scored"], ids == MASK)
+    last = ids.clone()
+    last[0, :4] = VOCAB - 1  # what an id outside the vocabulary is embedded as
+    full = api.score_tokens(engine, ids, targets, mask_token_id=MASK, every_position=True)
+    want = api.score_tokens(engine, last, targets, mask_token_id=MASK, every_position=True)
+    assert torch.equal(full["logprobs"], want["logprobs"])
+    far = targets.clone()
+    far[0, 0], far[1, 1] = 2 ** 40, -2 ** 40
+    r = api.score_tokens(engine, ids, far, mask_token_id=MASK, every_position=True)
+    assert bool(torch.isnan(r["logprobs"][0, 0])) and float(r["logprobs"][1, 1]) == 0.0
+    for dtype in (torch.uint8, torch.int16, torch.int32):
+        small = engine.ids.clamp(max=200 if dtype == torch.uint8 else MASK)
+        a = api.score_tokens(engine, small.to(dtype), targets, mask_token_id=MASK, every_position=True)
+        b = api.score_tokens(engine, small, targets, mask_token_id=MASK, every_position=True)
+        assert torch.equal(a["logprobs"], b["logprobs"])
+    engine.forward(engine.ids.view(-1).to("cuda", torch.int32))
