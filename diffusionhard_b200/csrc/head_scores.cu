@@ -989,14 +989,15 @@ extern "C" uint32_t dh_head_logprobs_i8(const int8_t* hidden, uint64_t ld_hidden
     if (hidden_size == 0) return DH_HEAD_INVALID_HIDDEN_SIZE;
     if (vocabulary_size == 0) return DH_HEAD_INVALID_VOCABULARY_SIZE;
     if (mask_token_id != DH_NO_TOKEN && mask_token_id >= vocabulary_size) return DH_HEAD_INVALID_MASK_TOKEN;
+    // (first of these, as the workspace query has no size for such shapes)
+    if (top_k > kMaxTopK || hidden_size > 131071 || rows > (1u << 24) || vocabulary_size > (1u << 24) ||
+        tiles_of(rows, vocabulary_size, 192) > kMaxTiles)
+        return DH_ERR_UNSUPPORTED_SHAPE;
     if (!hidden || !a_scale || !weights || !w_scale || !workspace) return DH_ERR_NULL_POINTER;
     const ScoreOutputs out{logprobs, entropy, logsumexp, top_ids, top_logprobs, targets,
                            targets_per_row, target_bytes, top_k};
     uint32_t st = check_score_outputs(out);
     if (st != DH_OK) return st;
-    if (top_k > kMaxTopK || hidden_size > 131071 || rows > (1u << 24) || vocabulary_size > (1u << 24))
-        return DH_ERR_UNSUPPORTED_SHAPE;
-    if (tiles_of(rows, vocabulary_size, 192) > kMaxTiles) return DH_ERR_UNSUPPORTED_SHAPE;
     const HeadSplit split = split_of(rows, vocabulary_size, device_sms());
     if (((reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(w_scale) |
           reinterpret_cast<uintptr_t>(bias)) & 3u) || (reinterpret_cast<uintptr_t>(workspace) & 255u))

@@ -579,8 +579,10 @@ uint32_t dh_token_logprobs(const void* logits, uint32_t logits_type, uint64_t ro
  * hidden_size] int8 as in dh_gemm_i8_scaled, bias NULL or [vocabulary_size];
  * the rest as in dh_token_logprobs.  workspace: 256-byte aligned device
  * memory of the size the query returns for these rows and this top_k on the
- * current device; calls that may overlap need one each.  Status: head family
- * codes, then DH_ERR_*. */
+ * current device (0: refused, DH_ERR_UNSUPPORTED_SHAPE); calls that may overlap
+ * need one each.  rows and vocabulary_size up to 2^24 and 2^30 tiles of 128 x
+ * 192 of them, hidden_size up to 131,071.  Status: head family codes, then
+ * DH_ERR_*. */
 size_t dh_head_logprobs_workspace_size(uint32_t rows, uint32_t vocabulary_size, uint32_t top_k);
 uint32_t dh_head_logprobs_i8(const int8_t* hidden, uint64_t ld_hidden, const float* a_scale, const int8_t* weights,
                              uint64_t ld_weights, const float* w_scale, const float* bias, uint32_t rows,

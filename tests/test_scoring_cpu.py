@@ -97,3 +97,11 @@ def test_score_tokens_wants_integers(dtype):
         api.score_tokens(model, other, ids, mask_token_id=9)
     with pytest.raises(ValueError, match="target_ids must be integers"):
         api.score_tokens(model, ids, other, mask_token_id=9)
+
+
+def test_head_shapes_without_a_workspace():
+    """Where the query has no size, the call says that it is for the shape."""
+    f = _lib.lib().dh_head_logprobs_workspace_size
+    assert f(1 << 24, 1 << 24, 1) == 0
+    assert _head(rows=1 << 24, vocab=1 << 24, ws=None, ws_bytes=0) == SHAPE
+    assert _head(rows=(1 << 24) + 1, ws=None, ws_bytes=0) == SHAPE
