@@ -1,8 +1,9 @@
 // dequant.cuh -- the W8A8 output of one int32 accumulator,
 //   y = fp32(acc * fp32(a_scale * w_scale) + bias)
 // evaluated in float64 and rounded once to fp32: exactly the reference's
-// fixed_mlp.quantized_linear (fixed_mlp.py:98-106).  Shared by the fused
-// heads and the scaled matrix product, so that their logits are the same bits.
+// fixed_mlp.quantized_linear (fixed_mlp.py:98-106).  Shared by the fused argmax
+// head, the fp32 outputs of the scaled matrix product and the scoring head above
+// its fp32 sizes, so that their logits are the same bits.
 #pragma once
 
 #include "dh_common.cuh"

@@ -150,10 +150,11 @@ struct EpiScaled : EpiBase {
 // row segments: TMA stores where the row pitch allows them (512 x 50264 x 768 to
 // bf16 35 us, 512 x 50257 through registers 44).
 //
-// What bounds it: with k = 768 the outputs' way to memory, at 3.0 to 3.3 TB/s for
-// plain stores (512 x 50260 x 768 to fp32 47 us, 2.2 TB/s; 32768 x 3072 x 768 to
-// bf16 80 us, 2.5 TB/s, 61 us without the stores); with k = 8192 the tensor cores
-// (8192^3 423 us, 2.6 Pop/s under the power cap).
+// What bounds it: with k = 768 the outputs' way to memory beside the MMAs (512 x 50260
+// x 768 to fp32 47 us, where a kernel that only stores, in the same tiles, takes 27;
+// 50258 columns 54 and 31; 32768 x 3072 x 768 to bf16 80 us, 61 without the stores,
+// which alone take 37); with k = 8192 the tensor cores (8192^3 423 us, 2.6 Pop/s under
+// the power cap).
 constexpr uint32_t kBM = 128, kBK = 128;
 constexpr uint32_t kABytes = kBM * kBK;
 constexpr uint32_t kPartCols = 64;             // columns of an epilogue warp

@@ -50,7 +50,11 @@ constexpr uint32_t kStagePerWarp = kPartCols * 8;       // bias and w_scale of t
 // Shared memory: with k <= kResidentK the row tile's A stays for all its column
 // tiles and the ring holds B alone (the copies into shared memory compete with
 // the MMA's and the epilogue's reads of it: 32768 x 50258, hidden 768, 871 against
-// 915 us); otherwise a stage holds both.
+// 915 us); otherwise a stage holds both.  Above 768 the ring beside A shrinks to 3 stages
+// (hidden 832: resident 55.1 against 52.2 us at 1001 rows, 87.0 against 82.9 at 2048;
+// 896: 54.5 against 52.2, 273 against 271 at 8192, but 337 against 351 with 5
+// alternatives), and past 896 to 2.  Rows at an odd multiple of 16 bytes are the
+// exception: streaming them costs more (784: resident 308 against 416 us at 8192 rows).
 constexpr uint32_t kSmemLimit = 227 * 1024;
 constexpr uint32_t kResidentK = 768;
 constexpr uint32_t kStreamedStages = 4;
@@ -68,7 +72,8 @@ struct HeadTile {
     static_assert(resident_stages(kResidentK / kBK) >= 3, "room for a ring beside A");
     static_assert(kFixed + kStreamedStages * (kABytes + kBBytes) <= kSmemLimit, "room for the streamed ring");
 };
-// float(acc) is exact up to 2^24: k products of magnitude 127 * 127 (128 * 128)
+// float(acc) is exact up to 2^24: k products of magnitude 127 * 127 (128 * 128).
+// (float64 there instead: 8192 x 50258, hidden 1024, 716 against 298 us)
 constexpr uint32_t kExactK = 1024;
 constexpr uint64_t kMaxTiles = 1u << 30;
 
@@ -103,8 +108,11 @@ struct HeadScoreParams {
     uint16_t* part_max;  // [n_tiles * parts][rows]; rows rounded up to row tiles
 };
 
-// The logit of one accumulator.  kWide: k > kExactK, where float(acc) would
-// round and the expression is evaluated in float64.
+// The logit of one accumulator, by an FMA whose only rounding is the logit's.  kWide:
+// k > kExactK, where float(acc) would round and the expression is evaluated in float64
+// and rounded again.  (The scaled product always does the latter: where the float64
+// value is halfway between two fp32 ones and the exact one is not, about one logit in
+// 2^29, the last bits differ.)
 template <bool kWide>
 DH_DEVINL float score_logit(int32_t acc, float ab, float w, float b) {
     if (kWide) return ref_logit(acc, ab, w, b);
@@ -380,7 +388,8 @@ head_stats_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         // quadrant's) and a quarter of its part's columns (2 of every 8), so that
         // it reads a column's scale and bias once for 4 logits: with a row a
         // thread, these reads from shared memory were what set the pace (1000
-        // against 860 us without them).  A group is the thread's 16 columns.
+        // against 860 us without them).  A group is 8 of the thread's 16 columns, those of
+        // one 32.
         const uint32_t ew = warp - 2, quad = warp & 3u, part = ew >> 2;
         float* bs = reinterpret_cast<float*>(staging + ew * kStagePerWarp);
         float* ws = bs + kPartCols;

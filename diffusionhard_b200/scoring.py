@@ -216,11 +216,14 @@ def head_logprobs(hidden: torch.Tensor, hidden_scale: torch.Tensor, weight: torc
     """:func:`token_logprobs` of ``linear_i8(hidden, hidden_scale, weight,
     w_scale, bias)`` without its logits ever reaching memory
     (dh_head_logprobs_i8): int8 ``hidden`` [rows, hidden_size] with a scale per
-    row, int8 ``weight`` [vocab, hidden_size] with a scale per token.
+    row, int8 ``weight`` [vocab, hidden_size] with a scale per token.  The logits
+    are those of ``linear_i8`` up to the rounding of a last bit.
 
     With ``top_k`` a call takes 10 bytes of workspace for each row and 64 tokens
-    of the vocabulary (257 MB for 32768 x 50258); alternatives cost more time
-    when a row's best logits differ by less than 2^-10 of their size."""
+    of the vocabulary (257 MB for 32768 x 50258).  Alternatives cost more time
+    where many parts of 64 logits come close to a row's k-th best: within 2^-10 of
+    its size where that lies between 6e-5 and 65504, within 6e-8 below, and at any
+    distance above."""
     hidden = _rows_i8("hidden", hidden)
     dev = hidden.device
     weight = _rows_i8("weight", weight, dev)

@@ -575,7 +575,8 @@ uint32_t dh_token_logprobs(const void* logits, uint32_t logits_type, uint64_t ro
 /* The scores of dh_token_logprobs for the logits of an int8 output head,
  *   x[r, v] = fp32(acc[r, v] * fp32(a_scale[r] * w_scale[v]) + bias[v]),
  * which never reach memory (mlx_mdlm._FinalLayer, mlx_mdlm.py:456-498, then
- * mdlm.py:851-858).  hidden [rows, hidden_size] and weights [vocabulary_size,
+ * mdlm.py:851-858).  Up to hidden_size 1024 they are rounded once, above as those
+ * of dh_gemm_i8_scaled (float64, then fp32); the two may differ in a last bit.  hidden [rows, hidden_size] and weights [vocabulary_size,
  * hidden_size] int8 as in dh_gemm_i8_scaled, bias NULL or [vocabulary_size];
  * the rest as in dh_token_logprobs.  workspace: 256-byte aligned device
  * memory of the size the query returns for these rows and this top_k on the

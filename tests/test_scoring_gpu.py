@@ -641,6 +641,32 @@ def test_head_logprobs_nan_bias(cuda, size, bits):
         check_scores(scoring.head_logprobs(*dev, t.cuda(), top_k=3, mask_token_id=mask), x, t, 3, mask)
 
 
+@pytest.mark.parametrize("size", [752, 768, 769, 896, 1023])
+@pytest.mark.parametrize("rows, vocab, top_k", [(3, 3001, 8), (300, 20000, 5), (128, 37888, 0)])
+def test_head_logprobs_around_residency(cuda, rows, vocab, top_k, size):
+    """Hidden sizes on both sides of the largest whose rows stay in shared memory, in tiles of either width."""
+    (a, sa, w, sw, b), t = head_case(rows, vocab, size, size + rows)
+    got = scoring.head_logprobs(*cu((a, sa, w, sw, b)), t.cuda(), top_k=top_k, mask_token_id=9)
+    pick = torch.tensor([0, 1, 2] if rows == 3 else [0, 1, 63, 64, 127] + ([128, 299] if rows > 128 else []))
+    x = ref_linear(a[pick], sa[pick], w, sw, b)[1].float().double()
+    some = got._replace(**{f: v[pick.cuda()] for f, v in got._asdict().items() if v is not None})
+    check_scores(some, x, t[pick], top_k, 9)
+
+
+def test_head_logprobs_rounds_once(cuda):
+    """Up to hidden 1024 a logit is its exact value rounded once, where float64 would be halfway."""
+    # 13325 * 80581 = 2^30 + 1, so that token 1's logit is 1 + 2^-24 + 2^-54
+    a, w = torch.zeros((1, 128), dtype=torch.int8), torch.zeros((2, 128), dtype=torch.int8)
+    a[0, :104], a[0, 104] = 127, 117
+    w[1, :105] = 1
+    assert int(a[0].long() @ w[1].long()) == 13325
+    sa, sw, b = torch.tensor([80581 * 2.0 ** -54]), torch.ones(2), torch.ones(2)
+    dev = cu((a, sa, w, sw, b))
+    got = scoring.head_logprobs(*dev, top_k=2)
+    assert got.top_ids.tolist() == [[1, 0]]
+    assert scoring.linear_i8(*dev).tolist() == [[1.0, 1.0]]  # as the reference rounds it
+
+
 # ------------------------------------------------------- use of the calls
 
 def _calls():
