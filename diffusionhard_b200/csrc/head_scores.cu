@@ -111,8 +111,8 @@ struct HeadScoreParams {
 // The logit of one accumulator, by an FMA whose only rounding is the logit's.  kWide:
 // k > kExactK, where float(acc) would round and the expression is evaluated in float64
 // and rounded again.  (The scaled product always does the latter: where the float64
-// value is halfway between two fp32 ones and the exact one is not, about one logit in
-// 2^29, the last bits differ.)
+// value is halfway between two fp32 ones and the exact one is not, as with a bias that
+// float64 drops beside a product of few bits, the last bits differ.)
 template <bool kWide>
 DH_DEVINL float score_logit(int32_t acc, float ab, float w, float b) {
     if (kWide) return ref_logit(acc, ab, w, b);
