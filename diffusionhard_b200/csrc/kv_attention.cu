@@ -1,0 +1,1058 @@
+// kv_attention.cu -- attention over K/V caches: softmax(scale Q K^T) V where a
+// sequence's keys are [the prefix of its group ; its own rows], either part in
+// 16 bits or as int8 codes with a scale for each (head, position), every
+// sequence with its own number of keys, several query heads for each K/V head,
+// any number of queries from one up.
+//
+// For a query i: s_j = scale (q_i . k_j), m = max_j s_j, p_j = e^(s_j - m),
+// out = sum_j p_j v_j / sum_j p_j, lse = m + log sum_j p_j; without keys out = 0
+// and lse = -inf.
+//
+// Work items.  A row is a (query, query head of the K/V head) pair; 128 rows
+// make a tile of the tensor core.  An item is (row tile, K/V head, a range of
+// key tiles of 64).  Rows of one sequence walk its prefix and its own keys.  With
+// few rows a sequence, the rows of all sequences of a group are stacked over the
+// prefix, which is then read once for all of them, and the sequences' own keys
+// are items of their own.  Where keys of a row fall to several items, each
+// leaves its unnormalised sums and maximum in the workspace and a second kernel
+// joins them in a fixed order.
+//
+// One persistent kernel, two CTAs per SM, 8 warps:
+//   warp 0    loads: TMA tiles of K and V (16 bits), or the contiguous codes and
+//             scales of 64 keys (int8)
+//   warp 1    tcgen05 MMAs: S = Q K^T, Q from TMEM; [O | l] += P [V | 1], P from
+//             TMEM, where a column of ones beside V sums P
+//   warps 2-3 int8: codes to f16 tiles, see convert_rows.  16 bits: zeros over
+//             the rows of V behind the last key (0 * NaN must not reach O)
+//   warps 4-7 softmax, a thread a row: P = 2^(s c - m) over S in TMEM; O in TMEM
+//             is rescaled only when the maximum grew by more than 2^8
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "tc_ptx.cuh"
+#include "tmap.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace dh {
+namespace {
+
+constexpr uint32_t kDh = 64;
+constexpr uint32_t kRows = 128;                  // rows per item
+constexpr uint32_t kKT = 64;                     // keys per tile
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kTileBytes = kKT * kDh * 2;   // 8 KB: a 16-bit K or V tile
+constexpr uint32_t kOnesBytes = 2048;            // 16 rows of 128 bytes
+constexpr uint32_t kVPitch = kTileBytes + kOnesBytes;
+constexpr uint32_t kRawBytes = 2 * kKT * kDh + 2 * kKT * 4;  // codes and scales of 64 keys
+constexpr uint32_t kTmemCols = 256;
+constexpr uint32_t kOCol = 128;                  // S/P buffers at 0 and 64, O at 128, l at 192
+constexpr uint32_t kQCol = 224;
+constexpr uint32_t kPvN = kDh + 16;
+// Factors of scores stay above zero: keys behind the last one score -inf, and
+// -inf * 0 would be NaN.
+constexpr float kLeastFactor = 1.17549435e-38f;
+constexpr uint32_t kExpRing = 8;                 // tiles whose exponents are kept
+
+enum Kind : int { kV16 = 0, kVBf16 = 1, kInt8 = 2 };
+
+template <int KIND>
+struct Cfg {
+    static constexpr bool int8 = KIND == kInt8;
+    static constexpr uint32_t raw_stages = int8 ? 4 : 0;
+    static constexpr uint32_t k_stages = int8 ? 2 : 4;
+    static constexpr uint32_t v_stages = int8 ? 2 : 3;
+    static constexpr uint32_t q_at = 0;
+    static constexpr uint32_t k_at = kRows * 128;
+    static constexpr uint32_t v_at = k_at + k_stages * kTileBytes;
+    static constexpr uint32_t ones_at = v_at + v_stages * kVPitch;
+    static constexpr uint32_t raw_at = ones_at + kOnesBytes;
+    static constexpr uint32_t bars_at = raw_at + raw_stages * kRawBytes;
+    static constexpr uint32_t bytes = 1024 + bars_at + 512;
+};
+
+// Rows and keys of one class of items.
+struct Class {
+    uint32_t groups, seqs, row_tiles, splits, items, slot;
+    uint32_t with_prefix, with_own;
+};
+
+struct Segment {
+    const int8_t* k;
+    const int8_t* v;
+    const float* k_scale;
+    const float* v_scale;
+    const int32_t* lengths;
+    uint32_t length, capacity;
+};
+
+struct Args {
+    Class cls[2];
+    Segment prefix, own;
+    const uint8_t* q;                        // 16-bit elements
+    uint64_t q_seq, q_head, q_row;           // strides in bytes
+    uint32_t q_bf16;
+    uint32_t sequences, queries, heads, kv_heads, ratio, per_prefix;
+    uint32_t v_transposed, idesc_s, idesc_o;
+    float c;                                 // scale * log2(e)
+    uint8_t* out;                            // [sequences, queries, heads, 64], of q's type
+    float* lse;                              // [sequences, queries, heads], or null
+    float2* part_ml;                         // [slots][rows], or null: one slot
+    float* part_o;                           // [slots][rows][64]
+    uint64_t total_rows;
+    const uint32_t* run_rows;
+};
+
+enum Bar : uint32_t {
+    kRawFull = 0, kRawEmpty = kRawFull + 4, kKFull = kRawEmpty + 4, kKEmpty = kKFull + 4, kVFull = kKEmpty + 4,
+    kVEmpty = kVFull + 4, kSFull = kVEmpty + 4, kPFull = kSFull + 2, kSPFree = kPFull + 2, kOFull = kSPFree + 2,
+    kOFree, kQReady, kVPart, kDrain = kVPart + 4, kNumBars
+};
+static_assert(kNumBars * 8 + 8 + 2 * kExpRing * 4 <= 512, "barrier area");
+
+DH_DEVINL void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+DH_DEVINL float ex2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// maxima that are NaN if an operand is
+DH_DEVINL float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+DH_DEVINL float max_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+DH_DEVINL uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+DH_DEVINL uint32_t pack_bf16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// 2^n, -126 <= n <= 127
+DH_DEVINL float pow2(int32_t n) { return __uint_as_float(static_cast<uint32_t>(n + 127) << 23); }
+// e with 2^(e - 1) <= x < 2^e for the normal fp32 with these bits
+DH_DEVINL int32_t exponent_of(uint32_t bits) { return static_cast<int32_t>((bits >> 23) & 0xFFu) - 126; }
+
+// 2^x of two values on the FMA pipe (x <= 8): x = n + f with n = rint(x) by the
+// 1.5 * 2^23 shifter, 2^f on [-0.5, 0.5] by a cubic (largest relative error
+// 7.8e-5, a third of an f16 half step), 2^n into the exponent field.  Takes a
+// quarter of the exponentials off the MUFU.
+constexpr float kExp2C0 = 0.99992895f, kExp2C1 = 0.69327623f, kExp2C2 = 0.24260406f, kExp2C3 = 0.05508874f;
+DH_DEVINL float2 exp2_poly2(float2 x) {
+    x = make_float2(fmaxf(x.x, -120.f), fmaxf(x.y, -120.f));
+    const float2 t = __fadd2_rn(x, make_float2(12582912.f, 12582912.f));
+    const float2 n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
+    const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+    float2 p = __ffma2_rn(make_float2(kExp2C3, kExp2C3), f, make_float2(kExp2C2, kExp2C2));
+    p = __ffma2_rn(p, f, make_float2(kExp2C1, kExp2C1));
+    p = __ffma2_rn(p, f, make_float2(kExp2C0, kExp2C0));
+    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+constexpr uint32_t kPolyPairMask = 0x11u;  // pairs e with bit e % 8 set
+
+struct Item {
+    uint32_t seq0, kv_head, row0, rows, slot;  // rows: live rows of the tile (may be 0)
+    uint32_t prefix, own;                      // cache entries
+    uint32_t len0, len1, n0, t0, t1;           // keys and tiles of the two parts, tile range
+};
+
+DH_DEVINL uint32_t length_of(const Segment& s, uint32_t entry) {
+    const int32_t n = s.lengths ? __ldg(s.lengths + entry) : static_cast<int32_t>(s.length);
+    return static_cast<uint32_t>(min(max(n, 0), static_cast<int32_t>(s.capacity)));
+}
+
+DH_DEVINL Item item_of(const Args& a, uint32_t w, uint32_t live) {
+    Item it;
+    const Class& c = w < a.cls[0].items ? a.cls[0] : a.cls[1];
+    if (w >= a.cls[0].items) w -= a.cls[0].items;
+    const uint32_t split = w % c.splits;
+    w /= c.splits;
+    const uint32_t tile = w % c.row_tiles;
+    w /= c.row_tiles;
+    it.kv_head = w % a.kv_heads;
+    const uint32_t group = w / a.kv_heads;
+    it.seq0 = group * c.seqs;
+    it.slot = c.slot + split;
+    it.row0 = tile * kRows;
+    const uint32_t seqs = live > it.seq0 ? min(live - it.seq0, c.seqs) : 0u;
+    const uint32_t rows = seqs * a.queries * a.ratio;
+    it.rows = rows > it.row0 ? min(rows - it.row0, kRows) : 0u;
+    it.own = it.seq0;
+    it.prefix = it.seq0 / a.per_prefix;
+    it.len0 = c.with_prefix ? length_of(a.prefix, it.prefix) : 0u;
+    it.len1 = c.with_own ? length_of(a.own, it.own) : 0u;
+    it.n0 = (it.len0 + kKT - 1) / kKT;
+    const uint32_t n = it.n0 + (it.len1 + kKT - 1) / kKT;
+    it.t0 = static_cast<uint32_t>(static_cast<uint64_t>(n) * split / c.splits);
+    it.t1 = static_cast<uint32_t>(static_cast<uint64_t>(n) * (split + 1) / c.splits);
+    if (it.rows == 0) it.t1 = it.t0;
+    return it;
+}
+// keys left from tile j on in its part (a full tile: 64 or more)
+DH_DEVINL uint32_t keys_left(const Item& it, uint32_t j) {
+    return j < it.n0 ? it.len0 - j * kKT : it.len1 - (j - it.n0) * kKT;
+}
+
+// Row r of an item: its query, as an index of [sequences, queries, heads].
+DH_DEVINL uint64_t row_index(const Args& a, const Item& it, uint32_t r, const uint8_t** q) {
+    const uint32_t row = it.row0 + r;
+    const uint32_t token = row / a.ratio;
+    const uint32_t head = it.kv_head * a.ratio + row % a.ratio;
+    const uint32_t seq = it.seq0 + token / a.queries, s = token % a.queries;
+    if (q) *q = a.q + seq * a.q_seq + head * a.q_head + s * a.q_row;
+    return (static_cast<uint64_t>(seq) * a.queries + s) * a.heads + head;
+}
+
+// 16 codes -> 16 f16 of code * ratio * 2^-9, where f = f16(ratio * 2^15): a code
+// plus 128 as the bits of a subnormal f16 is (code + 128) 2^-24, so one FMA with
+// f and -f 2^-17 (exact, a power of two) takes the 128 off and scales, with one
+// rounding.
+DH_DEVINL void convert16(const uint4& codes, __half2 f, __half2 off, uint4& lo, uint4& hi) {
+    const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+    uint32_t o[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t u = w[i] ^ 0x80808080u;
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+            uint32_t p = __byte_perm(u, 0u, h ? 0x4342u : 0x4140u);
+            __half2 x = __hfma2(*reinterpret_cast<__half2*>(&p), f, off);
+            o[2 * i + h] = *reinterpret_cast<uint32_t*>(&x);
+        }
+    }
+    lo = make_uint4(o[0], o[1], o[2], o[3]);
+    hi = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+// Half of a tile's 64 rows of codes (those of this warp) into a 128-byte
+// swizzled f16 tile; `scale` holds the lane's two rows' f16 factors.
+DH_DEVINL void convert_rows(const uint8_t* raw, uint8_t* tile, uint32_t warp_half, uint32_t lane, __half f0, __half f1) {
+    const uint32_t c = lane & 3u;
+    uint4 codes[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t row = warp_half * 32 + i * 8 + (lane >> 2);
+        codes[i] = *reinterpret_cast<const uint4*>(raw + row * kDh + c * 16);
+    }
+    const uint32_t mine = __half_as_ushort(warp_half ? f1 : f0);
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t row = warp_half * 32 + i * 8 + (lane >> 2);
+        const __half f = __ushort_as_half(static_cast<uint16_t>(__shfl_sync(0xFFFFFFFFu, mine, i * 8 + (lane >> 2))));
+        const __half2 f2 = __half2half2(f);
+        const __half2 off = __hmul2(f2, __half2half2(__ushort_as_half(0x8080)));  // -2^-17
+        uint4 lo, hi;
+        convert16(codes[i], f2, off, lo, hi);
+        uint8_t* dst = tile + row * 128;
+        *reinterpret_cast<uint4*>(dst + (((2 * c) ^ (row & 7u)) * 16)) = lo;
+        *reinterpret_cast<uint4*>(dst + (((2 * c + 1) ^ (row & 7u)) * 16)) = hi;
+    }
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(kThreads, 2)
+kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ CUtensorMap tpv,
+                    const __grid_constant__ CUtensorMap tok, const __grid_constant__ CUtensorMap tov,
+                    const __grid_constant__ Args a) {
+    using C = Cfg<KIND>;
+    const uint32_t live = a.run_rows ? min(a.sequences, *a.run_rows / a.queries) : a.sequences;
+    if (live == 0) return;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                               ~static_cast<uintptr_t>(1023));
+    uint8_t* q_s = smem + C::q_at;
+    uint8_t* k_ring = smem + C::k_at;
+    uint8_t* v_ring = smem + C::v_at;
+    uint8_t* ones = smem + C::ones_at;
+    uint8_t* raw_ring = smem + C::raw_at;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::bars_at);
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + kNumBars);
+    int32_t* exps = reinterpret_cast<int32_t*>(tmem_holder + 2);  // [kExpRing][2]: K, V of a tile
+
+    const uint32_t warp = warp_id(), lane = lane_id();
+    const uint32_t total = a.cls[0].items + a.cls[1].items;
+
+    if (warp == 0 && lane == 0) {
+        for (uint32_t i = 0; i < kNumBars; ++i) {
+            uint32_t count = 1;
+            if ((i >= kPFull && i < kPFull + 2) || i == kOFree || i == kQReady) count = 128;
+            if (C::int8 && ((i >= kRawEmpty && i < kRawEmpty + 4) || (i >= kKFull && i < kKFull + 4) ||
+                            (i >= kVFull && i < kVFull + 4)))
+                count = 2;
+            tc::mbar_init(&bars[i], count);
+        }
+        tc::fence_barrier_init();
+        if (!C::int8) {
+            tc::prefetch_tmap(&tok);
+            tc::prefetch_tmap(&tov);
+            if (a.cls[0].with_prefix | a.cls[1].with_prefix) {
+                tc::prefetch_tmap(&tpk);
+                tc::prefetch_tmap(&tpv);
+            }
+        }
+    }
+    // The column of ones.  V as it is stored ([key][64]): 16 rows (keys) whose
+    // first element is 1, the same for every 16 keys.  Transposed V ([64][key]): 16
+    // further rows under every tile, the first of them ones.
+    const uint32_t one2 = KIND == kVBf16 ? 0x3F803F80u : 0x3C003C00u;
+    if (a.v_transposed) {
+        for (uint32_t i = threadIdx.x; i < C::v_stages * 512; i += kThreads) {
+            const uint32_t st = i / 512, w = i % 512;
+            reinterpret_cast<uint32_t*>(v_ring + st * kVPitch + kTileBytes)[w] = w < 32 ? one2 : 0u;
+        }
+    } else {
+        for (uint32_t i = threadIdx.x; i < 512; i += kThreads) {
+            const uint32_t r = i / 32, w = i % 32;
+            reinterpret_cast<uint32_t*>(ones)[i] = w == (r & 7u) * 4 ? (one2 & 0xFFFFu) : 0u;
+        }
+    }
+    fence_proxy_async_smem();
+    if (warp == 1) tc::tmem_alloc(tmem_holder, kTmemCols);
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = *tmem_holder;
+
+    if (warp == 0) {
+        // ---------------------------------------------------------- loads
+        if (tc::elect_one()) {
+            uint32_t g = 0;
+            bool ok = true;
+            for (uint32_t w = blockIdx.x; w < total && ok; w += gridDim.x) {
+                const Item it = item_of(a, w, live);
+                for (uint32_t j = it.t0; j < it.t1; ++j, ++g) {
+                    const bool own = j >= it.n0;
+                    const uint32_t key = (own ? j - it.n0 : j) * kKT;
+                    const uint32_t entry = own ? it.own : it.prefix;
+                    if constexpr (C::int8) {
+                        const uint32_t rs = g % C::raw_stages;
+                        if (!tc::mbar_wait_suspend(&bars[kRawEmpty + rs], ((g / C::raw_stages) & 1u) ^ 1u,
+                                                   tc::kErrTimeoutEmpty)) {
+                            ok = false;
+                            break;
+                        }
+                        const Segment& s = own ? a.own : a.prefix;
+                        const uint64_t at = (static_cast<uint64_t>(entry) * a.kv_heads + it.kv_head) * s.capacity + key;
+                        uint8_t* dst = raw_ring + rs * kRawBytes;
+                        uint64_t* bar = &bars[kRawFull + rs];
+                        tc::mbar_arrive_expect_tx(bar, kRawBytes);
+                        tc::bulk_load(dst, s.k + at * kDh, kKT * kDh, bar);
+                        tc::bulk_load(dst + 2 * kKT * kDh, s.k_scale + at, kKT * 4, bar);
+                        tc::bulk_load(dst + kKT * kDh, s.v + at * kDh, kKT * kDh, bar);
+                        tc::bulk_load(dst + 2 * kKT * kDh + kKT * 4, s.v_scale + at, kKT * 4, bar);
+                    } else {
+                        const uint32_t ks = g % C::k_stages, vs = g % C::v_stages;
+                        if (!tc::mbar_wait_suspend(&bars[kKEmpty + ks], ((g / C::k_stages) & 1u) ^ 1u,
+                                                   tc::kErrTimeoutEmpty)) {
+                            ok = false;
+                            break;
+                        }
+                        tc::mbar_arrive_expect_tx(&bars[kKFull + ks], kTileBytes);
+                        tc::tma_load_4d(k_ring + ks * kTileBytes, own ? &tok : &tpk, &bars[kKFull + ks], 0, key,
+                                        it.kv_head, entry);
+                        if (!tc::mbar_wait_suspend(&bars[kVEmpty + vs], ((g / C::v_stages) & 1u) ^ 1u,
+                                                   tc::kErrTimeoutEmpty)) {
+                            ++g;  // (the K tile is on its way)
+                            ok = false;
+                            break;
+                        }
+                        // (a tile with rows behind the last key goes to warp 2 first)
+                        uint64_t* bar = &bars[(keys_left(it, j) < kKT ? kVPart : kVFull) + vs];
+                        tc::mbar_arrive_expect_tx(bar, kTileBytes);
+                        tc::tma_load_4d(v_ring + vs * kVPitch, own ? &tov : &tpv, bar, a.v_transposed ? key : 0,
+                                        a.v_transposed ? 0 : key, it.kv_head, entry);
+                    }
+                }
+            }
+            // every copy this CTA issued has landed before it may exit
+            if constexpr (C::int8) {
+                for (uint32_t x = g > C::raw_stages ? g - C::raw_stages : 0; x < g; ++x)
+                    tc::mbar_wait_suspend(&bars[kRawFull + x % C::raw_stages], (x / C::raw_stages) & 1u,
+                                          tc::kErrTimeoutFull);
+            } else {
+                for (uint32_t x = g > C::k_stages ? g - C::k_stages : 0; x < g; ++x)
+                    tc::mbar_wait_suspend(&bars[kKFull + x % C::k_stages], (x / C::k_stages) & 1u,
+                                          tc::kErrTimeoutFull);
+                for (uint32_t x = g > C::v_stages ? g - C::v_stages : 0; x < g; ++x)
+                    tc::mbar_wait_suspend(&bars[kVFull + x % C::v_stages], (x / C::v_stages) & 1u,
+                                          tc::kErrTimeoutFull);
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA
+        if (tc::elect_one()) {
+            const uint32_t o_tmem = tmem + kOCol;
+            auto issue_s = [&](uint32_t g) -> bool {
+                const uint32_t ks = g % C::k_stages, sb = g & 1u;
+                if (!tc::mbar_wait_suspend(&bars[kKFull + ks], (g / C::k_stages) & 1u, tc::kErrTimeoutFull) ||
+                    !tc::mbar_wait_suspend(&bars[kSPFree + sb], ((g >> 1) & 1u) ^ 1u, tc::kErrTimeoutAccEmpty))
+                    return false;
+                tc::tc_fence_after();
+                const uint64_t k_desc = tc::smem_desc_sw128(k_ring + ks * kTileBytes);
+#pragma unroll
+                for (uint32_t kk = 0; kk < kDh / 16; ++kk)
+                    tc::mma_f16_ts(tmem + sb * kKT, tmem + kQCol + kk * 8, tc::desc_advance(k_desc, kk * 32),
+                                   a.idesc_s, kk != 0);
+                tc::mma_commit(&bars[kSFull + sb]);
+                tc::mma_commit(&bars[kKEmpty + ks]);
+                return true;
+            };
+            uint32_t g = 0, n_items = 0;
+            bool ok = true;
+            for (uint32_t w = blockIdx.x; w < total && ok; w += gridDim.x) {
+                const Item it = item_of(a, w, live);
+                if (it.t0 == it.t1) continue;
+                if (!tc::mbar_wait_suspend(&bars[kQReady], n_items & 1u, tc::kErrTimeoutFull)) break;
+                tc::tc_fence_after();
+                if (!issue_s(g)) break;
+                for (uint32_t j = it.t0; j < it.t1; ++j, ++g) {
+                    if (j + 1 < it.t1 && !issue_s(g + 1)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t vs = g % C::v_stages, sb = g & 1u;
+                    ok = tc::mbar_wait_suspend(&bars[kPFull + sb], (g >> 1) & 1u, tc::kErrTimeoutFull) &&
+                         tc::mbar_wait_suspend(&bars[kVFull + vs], (g / C::v_stages) & 1u, tc::kErrTimeoutFull) &&
+                         (j != it.t0 ||
+                          tc::mbar_wait_suspend(&bars[kOFree], (n_items & 1u) ^ 1u, tc::kErrTimeoutAccEmpty));
+                    if (!ok) break;
+                    tc::tc_fence_after();
+                    const uint8_t* v_tile = v_ring + vs * kVPitch;
+                    if (a.v_transposed) {
+                        const uint64_t v_desc = tc::smem_desc_sw128(v_tile);
+#pragma unroll
+                        for (uint32_t kk = 0; kk < kKT / 16; ++kk)
+                            tc::mma_f16_ts(o_tmem, tmem + sb * kKT + kk * 8, tc::desc_advance(v_desc, kk * 32),
+                                           a.idesc_o, kk != 0 || j != it.t0);
+                    } else {
+#pragma unroll
+                        for (uint32_t kk = 0; kk < kKT / 16; ++kk) {
+                            const uint8_t* at = v_tile + kk * 2048;
+                            tc::mma_f16_ts(o_tmem, tmem + sb * kKT + kk * 8,
+                                           tc::smem_desc_mn_sw128(at, static_cast<uint32_t>(ones - at)), a.idesc_o,
+                                           kk != 0 || j != it.t0);
+                        }
+                    }
+                    tc::mma_commit(&bars[kVEmpty + vs]);
+                    tc::mma_commit(&bars[kSPFree + sb]);
+                    if (j + 1 == it.t1) tc::mma_commit(&bars[kOFull]);
+                }
+                ++n_items;
+            }
+            tc::mma_commit(&bars[kDrain]);
+            tc::mbar_wait_suspend(&bars[kDrain], 0, tc::kErrTimeoutAccFull);
+        }
+    } else if (warp < 4) {
+        uint32_t g = 0;
+        bool ok = true;
+        if constexpr (C::int8) {
+            // ---------------------------------------------------- conversion
+            const uint32_t half = warp - 2;
+            for (uint32_t w = blockIdx.x; w < total && ok; w += gridDim.x) {
+                const Item it = item_of(a, w, live);
+                int32_t ev = -1000;
+                for (uint32_t j = it.t0; j < it.t1; ++j, ++g) {
+                    const uint32_t rs = g % C::raw_stages, ks = g % C::k_stages, vs = g % C::v_stages;
+                    if (!tc::mbar_wait_suspend(&bars[kRawFull + rs], (g / C::raw_stages) & 1u, tc::kErrTimeoutFull)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint8_t* raw = raw_ring + rs * kRawBytes;
+                    const float* scales = reinterpret_cast<const float*>(raw + 2 * kKT * kDh);
+                    const uint32_t left = keys_left(it, j);
+                    // scales of rows lane and lane + 32, 0 behind the last key (what lies
+                    // there is anything); the tile's exponents, from the finite ones
+                    float sc[2][2];
+                    int32_t e[2];
+#pragma unroll
+                    for (uint32_t side = 0; side < 2; ++side) {
+                        uint32_t peak = 0;
+#pragma unroll
+                        for (uint32_t h = 0; h < 2; ++h) {
+                            const uint32_t row = lane + 32 * h;
+                            const float f = row < left ? scales[side * kKT + row] : 0.f;
+                            sc[side][h] = f;
+                            const uint32_t bits = __float_as_uint(f) & 0x7FFFFFFFu;
+                            if (bits < 0x7F800000u) peak = max(peak, bits);
+                        }
+                        e[side] = max(exponent_of(__reduce_max_sync(0xFFFFFFFFu, peak)), -100);
+                    }
+                    // O keeps one exponent of V for all tiles of an item: it only grows,
+                    // by two more than it has to, and O is rescaled when it does
+                    ev = e[1] > ev ? min(e[1] + (j == it.t0 ? 0 : 2), 126) : ev;
+                    const float fk = pow2(15 - min(e[0], 126)), fv = pow2(15 - ev);
+                    if (!tc::mbar_wait_suspend(&bars[kKEmpty + ks], ((g / C::k_stages) & 1u) ^ 1u,
+                                               tc::kErrTimeoutEmpty)) {
+                        ok = false;
+                        break;
+                    }
+                    if (half == 0 && lane == 0) {
+                        exps[(g % kExpRing) * 2] = min(e[0], 126) + 9;
+                        exps[(g % kExpRing) * 2 + 1] = ev + 9;
+                    }
+                    convert_rows(raw, k_ring + ks * kTileBytes, half, lane, __float2half_rn(sc[0][0] * fk),
+                                 __float2half_rn(sc[0][1] * fk));
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&bars[kKFull + ks]);
+                    if (!tc::mbar_wait_suspend(&bars[kVEmpty + vs], ((g / C::v_stages) & 1u) ^ 1u,
+                                               tc::kErrTimeoutEmpty)) {
+                        ok = false;
+                        break;
+                    }
+                    convert_rows(raw + kKT * kDh, v_ring + vs * kVPitch, half, lane, __float2half_rn(sc[1][0] * fv),
+                                 __float2half_rn(sc[1][1] * fv));
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tc::mbar_arrive(&bars[kVFull + vs]);
+                        tc::mbar_arrive(&bars[kRawEmpty + rs]);
+                    }
+                }
+            }
+        } else if (warp == 2) {
+            // ------------------------------------------- rows behind the last key
+            // Such tiles of V arrive on kVPart, and this warp's arrival on kVFull hands
+            // them on: a stage is loaded again only after that, so no phase is missed.
+            uint32_t phases = 0;  // a bit for each stage
+            for (uint32_t w = blockIdx.x; w < total && ok; w += gridDim.x) {
+                const Item it = item_of(a, w, live);
+                for (uint32_t j = it.t0; j < it.t1; ++j, ++g) {
+                    const uint32_t left = keys_left(it, j), vs = g % C::v_stages;
+                    if (left >= kKT) continue;
+                    if (!tc::mbar_wait_suspend(&bars[kVPart + vs], (phases >> vs) & 1u, tc::kErrTimeoutFull)) {
+                        ok = false;
+                        break;
+                    }
+                    phases ^= 1u << vs;
+                    uint8_t* tile = v_ring + vs * kVPitch;
+                    if (a.v_transposed) {
+                        for (uint32_t i = lane; i < kDh * kKT; i += 32) {
+                            const uint32_t d = i / kKT, key = i % kKT;
+                            if (key >= left)
+                                *reinterpret_cast<uint16_t*>(tile + d * 128 + (((key >> 3) ^ (d & 7u)) * 16) +
+                                                             (key & 7u) * 2) = 0;
+                        }
+                    } else {
+                        for (uint32_t i = left * 8 + lane; i < kKT * 8; i += 32)
+                            *reinterpret_cast<uint4*>(tile + i * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&bars[kVFull + vs]);
+                }
+            }
+        }
+    } else {
+        // ----------------------------------------------------------- softmax
+        const uint32_t quad = warp & 3u;
+        const uint32_t r = quad * 32 + lane;
+        const uint32_t lane_base = (quad * 32u) << 16;
+        uint8_t* my_q = q_s + r * 128;
+
+        auto write_row = [&](const Item& it, float m, float l, float f, const uint32_t (&v0)[32],
+                             const uint32_t (&v1)[32]) {
+            const uint64_t row = row_index(a, it, r, nullptr);
+            if (a.part_ml) {
+                const uint64_t at = it.slot * a.total_rows + row;
+                a.part_ml[at] = make_float2(m, l);
+                if (l == 0.f) return;
+                float4* dst = reinterpret_cast<float4*>(a.part_o + at * kDh);
+#pragma unroll
+                for (uint32_t d = 0; d < 32; d += 4) {
+                    dst[d / 4] = make_float4(__uint_as_float(v0[d]) * f, __uint_as_float(v0[d + 1]) * f,
+                                             __uint_as_float(v0[d + 2]) * f, __uint_as_float(v0[d + 3]) * f);
+                    dst[8 + d / 4] = make_float4(__uint_as_float(v1[d]) * f, __uint_as_float(v1[d + 1]) * f,
+                                                 __uint_as_float(v1[d + 2]) * f, __uint_as_float(v1[d + 3]) * f);
+                }
+                return;
+            }
+            const float inv = l == 0.f ? 0.f : f / l;
+            uint4* dst = reinterpret_cast<uint4*>(a.out + row * (kDh * 2));
+#pragma unroll
+            for (uint32_t d = 0; d < 64; d += 8) {
+                uint32_t o[4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint32_t e = d + 2 * i;
+                    const float x = __uint_as_float(e < 32 ? v0[e & 31] : v1[e & 31]) * inv;
+                    const float y = __uint_as_float(e < 32 ? v0[(e + 1) & 31] : v1[(e + 1) & 31]) * inv;
+                    o[i] = a.q_bf16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
+                }
+                dst[d / 8] = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+            if (a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+        };
+        // From item w on: rows of items without keys are answered at once; the
+        // first item with keys (w >= total: none), its query row on its way to
+        // shared memory.
+        auto next_item = [&](uint32_t& w, Item& it) {
+            for (; w < total; w += gridDim.x) {
+                it = item_of(a, w, live);
+                if (it.t0 != it.t1) break;
+                if (r < it.rows) {
+                    const uint32_t zero[32] = {};
+                    write_row(it, 0.f, 0.f, 1.f, zero, zero);
+                }
+            }
+            if (w < total && r < it.rows) {
+                const uint8_t* q;
+                row_index(a, it, r, &q);
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                                     smem_u32(my_q + ((i ^ (r & 7u)) * 16))),
+                                 "l"(__cvta_generic_to_global(q + i * 16)));
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        // This thread's query row from shared memory into TMEM.  Returns the
+        // factor of its scores.  int8: the row as f16 between 1/2 and 1 in
+        // magnitude, its exponent in the factor.
+        auto copy_q = [&]() -> float {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            uint32_t qv[32];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                const uint4 v = *reinterpret_cast<const uint4*>(my_q + ((i ^ (r & 7u)) * 16));
+                qv[4 * i] = v.x, qv[4 * i + 1] = v.y, qv[4 * i + 2] = v.z, qv[4 * i + 3] = v.w;
+            }
+            float c = a.c;
+            if constexpr (C::int8) {
+                uint32_t peak = 0;
+                if (a.q_bf16) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; ++i)
+                        peak = max(peak, max((qv[i] << 16) & 0x7FFF0000u, qv[i] & 0x7FFF0000u));
+                } else {
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; ++i) {
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qv[i]));
+                        peak = max(peak, max(__float_as_uint(f.x) & 0x7FFFFFFFu, __float_as_uint(f.y) & 0x7FFFFFFFu));
+                    }
+                }
+                const int32_t e = min(max(exponent_of(peak), -100), 126);
+                const float f = pow2(-e);
+#pragma unroll
+                for (uint32_t i = 0; i < 32; ++i) {
+                    float2 x;
+                    if (a.q_bf16)
+                        x = make_float2(__uint_as_float(qv[i] << 16), __uint_as_float(qv[i] & 0xFFFF0000u));
+                    else
+                        x = __half22float2(*reinterpret_cast<const __half2*>(&qv[i]));
+                    qv[i] = pack_f16x2(x.x * f, x.y * f);
+                }
+                c *= pow2(e);
+            }
+            tc::tmem_st_32x32b_x32(tmem + lane_base + kQCol, qv);
+            tc::tmem_st_wait();
+            tc::tc_fence_before();
+            tc::mbar_arrive(&bars[kQReady]);
+            return c;
+        };
+
+        uint32_t g = 0, n_items = 0;
+        bool ok = true;
+        Item it;
+        uint32_t w = blockIdx.x;
+        next_item(w, it);
+        float c = 0.f;
+        if (w < total) c = copy_q();
+        while (w < total && ok) {
+            Item next;
+            uint32_t next_w = w + gridDim.x;
+            next_item(next_w, next);
+            const bool active = quad * 32 < it.rows;  // the warp has rows
+            float m = 0.f;
+            int32_t ev = 0;  // exponent of O (int8)
+            for (uint32_t j = it.t0; j < it.t1; ++j, ++g) {
+                const uint32_t sb = g & 1u;
+                if (!tc::mbar_wait_suspend(&bars[kSFull + sb], (g >> 1) & 1u, tc::kErrTimeoutAccFull)) {
+                    ok = false;
+                    break;
+                }
+                tc::tc_fence_after();
+                if (active) {
+                    uint32_t sv[64];
+                    tc::tmem_ld_32x32b_x32(tmem + lane_base + sb * kKT, *reinterpret_cast<uint32_t(*)[32]>(&sv[0]));
+                    tc::tmem_ld_32x32b_x32(tmem + lane_base + sb * kKT + 32,
+                                           *reinterpret_cast<uint32_t(*)[32]>(&sv[32]));
+                    float ct = c;
+                    int32_t et = 0;
+                    if constexpr (C::int8) {
+                        ct = fmaxf(c * pow2(min(exps[(g % kExpRing) * 2], 127)), kLeastFactor);
+                        et = exps[(g % kExpRing) * 2 + 1];
+                    }
+                    const uint32_t left = keys_left(it, j);
+                    tc::tmem_ld_wait();
+                    if (left < kKT) {
+#pragma unroll
+                        for (uint32_t e = 0; e < 64; ++e)
+                            if (e >= left) sv[e] = 0xFF800000u;
+                    }
+                    float pm[8];
+#pragma unroll
+                    for (uint32_t q = 0; q < 8; ++q) pm[q] = __uint_as_float(sv[q]);
+#pragma unroll
+                    for (uint32_t e = 8; e < 56; e += 16) {
+#pragma unroll
+                        for (uint32_t q = 0; q < 8; ++q)
+                            pm[q] = max_nan(pm[q], __uint_as_float(sv[e + q]), __uint_as_float(sv[e + 8 + q]));
+                    }
+#pragma unroll
+                    for (uint32_t q = 0; q < 8; ++q) pm[q] = max_nan(pm[q], __uint_as_float(sv[56 + q]));
+                    const float tmax = max_nan(max_nan(max_nan(pm[0], pm[1]), pm[2], pm[3]),
+                                               max_nan(max_nan(pm[4], pm[5]), pm[6], pm[7]));
+                    // finite (a row of -inf would give inf - inf), or NaN for an infinite
+                    // score, as for one that is NaN: the row is NaN
+                    float mt = max_nan(tmax * ct, -3.0e38f);
+                    mt = __fmaf_rn(mt, -0.f, mt);
+                    float alpha = 1.f, alpha_o = 1.f;
+                    bool need = false;
+                    if (j == it.t0) {
+                        m = mt;
+                        ev = et;
+                    } else {
+                        if (!(mt <= m + 8.0f)) {
+                            need = true;
+                            alpha = ex2_approx(m - mt);
+                            m = mt;
+                        }
+                        alpha_o = alpha;
+                        if (C::int8 && et > ev) {
+                            need = true;
+                            alpha_o = alpha * pow2(max(ev - et, -126));
+                            ev = et;
+                        }
+                    }
+                    const float2 c2 = make_float2(ct, ct);
+                    const float2 nm2 = make_float2(-m, -m);
+                    uint32_t pk[32];
+#pragma unroll
+                    for (uint32_t e = 0; e < 32; ++e) {
+                        const float2 s2 = make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1]));
+                        const float2 x = __ffma2_rn(s2, c2, nm2);
+                        float2 y;
+                        if ((kPolyPairMask >> (e & 7u)) & 1u)
+                            y = exp2_poly2(x);
+                        else
+                            y = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                        pk[e] = KIND == kVBf16 ? pack_bf16x2(y.x, y.y) : pack_f16x2(y.x, y.y);
+                    }
+                    tc::tmem_st_32x32b_x32(tmem + lane_base + sb * kKT, pk);
+                    if (__any_sync(0xFFFFFFFFu, need)) {
+                        // PV of the tile before (the only one that may still run) finished
+                        if (!tc::mbar_wait_suspend(&bars[kSPFree + (sb ^ 1u)], ((g - 1) >> 1) & 1u,
+                                                   tc::kErrTimeoutEmpty)) {
+                            ok = false;
+                            break;
+                        }
+                        tc::tc_fence_after();
+#pragma unroll
+                        for (uint32_t h2 = 0; h2 < 2; ++h2) {
+                            uint32_t ov[32];
+                            tc::tmem_ld_32x32b_x32(tmem + lane_base + kOCol + 32 * h2, ov);
+                            tc::tmem_ld_wait();
+#pragma unroll
+                            for (uint32_t d = 0; d < 32; ++d)
+                                ov[d] = __float_as_uint(__uint_as_float(ov[d]) * alpha_o);
+                            tc::tmem_st_32x32b_x32(tmem + lane_base + kOCol + 32 * h2, ov);
+                        }
+                        const uint32_t lv = tc::tmem_ld_32x32b_x1(tmem + lane_base + kOCol + kDh);
+                        tc::tmem_ld_wait();
+                        tc::tmem_st_32x32b_x1(tmem + lane_base + kOCol + kDh,
+                                              __float_as_uint(__uint_as_float(lv) * alpha));
+                    }
+                    tc::tmem_st_wait();
+                    tc::tc_fence_before();
+                }
+                tc::mbar_arrive(&bars[kPFull + sb]);
+            }
+            if (!ok) break;
+            // the next item's Q before this item's result, so that its S can start
+            float next_c = 0.f;
+            if (next_w < total) next_c = copy_q();
+            if (!tc::mbar_wait_suspend(&bars[kOFull], n_items & 1u, tc::kErrTimeoutAccFull)) break;
+            tc::tc_fence_after();
+            uint32_t v0[32], v1[32];
+            tc::tmem_ld_32x32b_x32(tmem + lane_base + kOCol, v0);
+            tc::tmem_ld_32x32b_x32(tmem + lane_base + kOCol + 32, v1);
+            const uint32_t l_bits = tc::tmem_ld_32x32b_x1(tmem + lane_base + kOCol + kDh);
+            tc::tmem_ld_wait();
+            tc::tc_fence_before();
+            tc::mbar_arrive(&bars[kOFree]);
+            if (r < it.rows)
+                write_row(it, m, __uint_as_float(l_bits), C::int8 ? pow2(min(ev, 127)) : 1.f, v0, v1);
+            ++n_items;
+            w = next_w;
+            it = next;
+            c = next_c;
+        }
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc::tc_fence_after();
+        tc::tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+// Joins the parts of a row, a warp a row: with M = max m, w_s = 2^(m_s - M),
+// out = sum w_s O_s / sum w_s l_s over the slots in their order.
+__global__ void __launch_bounds__(128) kv_join_kernel(const float2* ml, const float* part, uint32_t slots,
+                                                      uint64_t rows, uint32_t queries, uint32_t heads, uint32_t bf16,
+                                                      uint8_t* out, float* lse, const uint32_t* run_rows) {
+    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * 4 + warp_id();
+    const uint32_t lane = lane_id();
+    if (row >= rows) return;
+    if (run_rows) {
+        const uint64_t live = *run_rows / queries * static_cast<uint64_t>(queries) * heads;
+        if (row >= live) return;
+    }
+    float top = -INFINITY;
+    for (uint32_t s = lane; s < slots; s += 32) {
+        const float2 x = ml[s * rows + row];
+        if (x.y != 0.f) top = max_nan(top, x.x);
+    }
+#pragma unroll
+    for (uint32_t o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    float l = 0.f;
+    float2 sum = make_float2(0.f, 0.f);
+    for (uint32_t s = 0; s < slots; ++s) {
+        const float2 x = ml[s * rows + row];
+        if (x.y == 0.f) continue;
+        const float f = exp2f(x.x - top);
+        const float2 o = reinterpret_cast<const float2*>(part + (s * rows + row) * kDh)[lane];
+        l = __fmaf_rn(f, x.y, l);
+        sum = make_float2(__fmaf_rn(f, o.x, sum.x), __fmaf_rn(f, o.y, sum.y));
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    reinterpret_cast<uint32_t*>(out)[row * (kDh / 2) + lane] =
+        bf16 ? pack_bf16x2(sum.x * inv, sum.y * inv) : pack_f16x2(sum.x * inv, sum.y * inv);
+    if (lse && lane == 0) lse[row] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+}
+
+// ------------------------------------------------------------------ plan
+
+// Rows a sequence must have before its items walk the prefix by themselves.
+constexpr uint32_t kStackBelow = 128;
+constexpr uint32_t kMaxSplits = 64;
+
+struct Plan {
+    Class cls[2];
+    uint32_t slots;
+};
+
+uint32_t ceil_div(uint64_t a, uint64_t b) { return static_cast<uint32_t>((a + b - 1) / b); }
+
+// The split of the keys into 1 to 64 parts: the one with the shortest estimated
+// time, in tiles: full rounds of items on `ctas` CTAs, two tiles of start and end
+// for each item, three for a join.
+Plan plan_of(uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t prefixes, uint32_t prefix_keys,
+             uint32_t own_keys, uint32_t ctas) {
+    Plan p{};
+    const uint32_t per = prefixes ? sequences / prefixes : sequences;
+    const bool stacked = prefixes && per > 1 && rows < kStackBelow;
+    const uint32_t t0 = ceil_div(prefix_keys, kKT), t1 = ceil_div(own_keys, kKT);
+    uint32_t tiles[2] = {0, 0};
+    if (stacked) {
+        p.cls[0] = Class{prefixes, per, ceil_div(static_cast<uint64_t>(per) * rows, kRows), 1, 0, 0, 1, 0};
+        tiles[0] = t0;
+    }
+    p.cls[1] = Class{sequences, 1, ceil_div(rows, kRows), 1, 0, 0, prefixes && !stacked, 1};
+    tiles[1] = t1 + (stacked || !prefixes ? 0 : t0);
+    uint64_t items[2];
+    for (int i = 0; i < 2; ++i)
+        items[i] = static_cast<uint64_t>(p.cls[i].groups) * kv_heads * p.cls[i].row_tiles;
+    uint64_t best = ~0ull;
+    uint32_t best_splits[2] = {1, 1};
+    const uint32_t most = std::max(std::max(tiles[0], tiles[1]), 1u);
+    for (uint32_t n = 1; n <= kMaxSplits; ++n) {
+        const uint32_t chunk = ceil_div(most, n);
+        uint64_t work = 0, longest = 0;
+        uint32_t splits[2];
+        for (int i = 0; i < 2; ++i) {
+            splits[i] = std::min(std::max(ceil_div(tiles[i], chunk), 1u), kMaxSplits);
+            const uint64_t each = ceil_div(tiles[i], splits[i]) + 2;
+            if (!items[i]) continue;
+            work += items[i] * splits[i] * each;
+            longest = std::max(longest, each);
+        }
+        const uint64_t count = items[0] * splits[0] + items[1] * splits[1];
+        uint64_t time = std::max<uint64_t>(ceil_div(count, ctas) * longest, ceil_div(work, ctas));
+        if (stacked || splits[1] > 1) time += 3;
+        if (time < best) {
+            best = time;
+            best_splits[0] = splits[0];
+            best_splits[1] = splits[1];
+        }
+        if (chunk == 1) break;
+    }
+    for (int i = 0; i < 2; ++i) {
+        if (!items[i]) continue;
+        p.cls[i].splits = best_splits[i];
+        p.cls[i].items = static_cast<uint32_t>(std::min<uint64_t>(items[i] * best_splits[i], 0xFFFFFFFFull));
+        p.cls[i].slot = p.slots;
+        p.slots += best_splits[i];
+    }
+    return p;
+}
+
+bool fits(uint32_t sequences, uint32_t queries, uint32_t heads, uint32_t kv_heads, uint32_t prefixes) {
+    // items and rows stay below 2^31: at most 64 splits of 128-row tiles
+    const uint64_t rows = static_cast<uint64_t>(sequences) * queries;
+    if (rows > (1ull << 31)) return false;
+    const uint64_t per_seq = ceil_div(static_cast<uint64_t>(queries) * (heads / kv_heads), kRows);
+    return rows * heads <= (1ull << 31) && per_seq * sequences * kv_heads <= (1ull << 24) && prefixes <= sequences;
+}
+
+bool misaligned(const void* p, uint32_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
+
+size_t workspace_of(uint32_t slots, uint64_t rows) {
+    return slots < 2 ? 0 : static_cast<size_t>(slots) * rows * (sizeof(float2) + kDh * sizeof(float));
+}
+
+uint32_t check_view(const dh_kv_view& v) {
+    if (!v.k || !v.v) return DH_ERR_NULL_POINTER;
+    if (v.capacity == 0 || v.capacity > 0x7FFFFFFFu || (!v.lengths && v.length > v.capacity))
+        return DH_ERR_INVALID_ARGUMENT;
+    if (v.k_type == DH_TYPE_I8 && v.v_type == DH_TYPE_I8) {
+        if (!v.k_scale || !v.v_scale) return DH_ERR_NULL_POINTER;
+        if (v.capacity % kKT) return DH_ERR_UNSUPPORTED_SHAPE;
+        if (misaligned(v.k, 16) || misaligned(v.v, 16) || misaligned(v.k_scale, 16) || misaligned(v.v_scale, 16) ||
+            misaligned(v.lengths, 4))
+            return DH_ERR_ALIGNMENT;
+        return DH_OK;
+    }
+    if ((v.k_type != DH_TYPE_BF16 && v.k_type != DH_TYPE_F16) || (v.v_type != DH_TYPE_BF16 && v.v_type != DH_TYPE_F16))
+        return DH_ERR_INVALID_ARGUMENT;
+    const bool rows = v.v_strides[3] == 1, turned = v.v_strides[2] == 1;
+    if (v.k_strides[3] != 1 || (!rows && !turned)) return DH_ERR_UNSUPPORTED_SHAPE;
+    const uint64_t all = v.k_strides[0] | v.k_strides[1] | v.k_strides[2] | v.v_strides[0] | v.v_strides[1] |
+                         v.v_strides[rows ? 2 : 3];
+    if (misaligned(v.k, 16) || misaligned(v.v, 16) || all % 8 || misaligned(v.lengths, 4)) return DH_ERR_ALIGNMENT;
+    if (all >> 38) return DH_ERR_UNSUPPORTED_SHAPE;  // (a tensor map's strides lie below 2^40 bytes)
+    return DH_OK;
+}
+
+bool view_maps(CUtensorMap* k, CUtensorMap* v, const dh_kv_view& s, uint32_t entries, uint32_t heads) {
+    const auto type = [](uint32_t t) {
+        return t == DH_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    };
+    const bool rows = s.v_strides[3] == 1;
+    return make_tmap_4d(k, s.k, type(s.k_type), kDh, s.capacity, heads, entries, s.k_strides[2] * 2,
+                        s.k_strides[1] * 2, s.k_strides[0] * 2, kKT) &&
+           make_tmap_4d(v, s.v, type(s.v_type), rows ? kDh : s.capacity, rows ? s.capacity : kDh, heads, entries,
+                        s.v_strides[rows ? 2 : 3] * 2, s.v_strides[1] * 2, s.v_strides[0] * 2, kKT);
+}
+
+template <int KIND>
+uint32_t launch(const CUtensorMap (&maps)[4], const Args& a, uint32_t grid, cudaStream_t st) {
+    static std::atomic<uint64_t> configured{0};
+    if (smem_optin_once(kv_attention_kernel<KIND>, Cfg<KIND>::bytes, configured) != cudaSuccess) return DH_ERR_CUDA;
+    kv_attention_kernel<KIND><<<grid, kThreads, Cfg<KIND>::bytes, st>>>(maps[0], maps[1], maps[2], maps[3], a);
+    DH_LAUNCH_CHECK();
+    return DH_OK;
+}
+
+}  // namespace
+}  // namespace dh
+
+using namespace dh;
+
+extern "C" size_t dh_kv_attention_workspace_size(uint32_t sequences, uint32_t queries, uint32_t heads,
+                                                 uint32_t kv_heads, uint32_t prefixes, uint32_t prefix_capacity,
+                                                 uint32_t own_capacity) {
+    if (!sequences || !queries || !heads || !kv_heads || heads % kv_heads || (prefixes && sequences % prefixes) ||
+        !fits(sequences, queries, heads, kv_heads, prefixes))
+        return 0;
+    const Plan p = plan_of(sequences, queries * (heads / kv_heads), kv_heads, prefixes, prefix_capacity, own_capacity,
+                           2 * device_sms());
+    return workspace_of(p.slots, static_cast<uint64_t>(sequences) * queries * heads);
+}
+
+extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64_t* q_strides, uint32_t sequences,
+                                    uint32_t queries, uint32_t heads, uint32_t kv_heads, const dh_kv_view* own,
+                                    const dh_kv_view* prefix, uint32_t prefixes, float scale, void* out, float* lse,
+                                    const uint32_t* run_rows, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!q || !q_strides || !own || !out || (prefixes && !prefix)) return DH_ERR_NULL_POINTER;
+    if ((q_type != DH_TYPE_BF16 && q_type != DH_TYPE_F16) || !sequences || !queries || !heads || !kv_heads ||
+        heads % kv_heads || (prefixes && sequences % prefixes) || !(scale > 0.f) || !std::isfinite(scale))
+        return DH_ERR_INVALID_ARGUMENT;
+    if (!fits(sequences, queries, heads, kv_heads, prefixes)) return DH_ERR_UNSUPPORTED_SHAPE;
+    if (uint32_t st = check_view(*own)) return st;
+    const bool int8 = own->k_type == DH_TYPE_I8;
+    if (!int8 && own->k_type != q_type) return DH_ERR_INVALID_ARGUMENT;
+    if (prefixes) {
+        if (uint32_t st = check_view(*prefix)) return st;
+        if (prefix->k_type != own->k_type || prefix->v_type != own->v_type) return DH_ERR_INVALID_ARGUMENT;
+        if (!int8 && (prefix->v_strides[3] == 1) != (own->v_strides[3] == 1)) return DH_ERR_INVALID_ARGUMENT;
+    }
+    if (misaligned(q, 16) || (q_strides[0] | q_strides[1] | q_strides[2]) % 8 || misaligned(out, 16) ||
+        misaligned(lse, 4) || misaligned(run_rows, 4))
+        return DH_ERR_ALIGNMENT;
+    const uint32_t ratio = heads / kv_heads;
+    const uint64_t rows = static_cast<uint64_t>(sequences) * queries * heads;
+    const uint32_t ctas = 2 * device_sms();
+    const Plan p = plan_of(sequences, queries * ratio, kv_heads, prefixes, prefixes ? prefix->capacity : 0,
+                           own->capacity, ctas);
+    const size_t need = workspace_of(p.slots, rows);
+    if (need && !workspace) return DH_ERR_NULL_POINTER;
+    if (need > workspace_bytes) return DH_ERR_WORKSPACE;
+    if (misaligned(workspace, 256)) return DH_ERR_ALIGNMENT;
+
+    Args a{};
+    a.cls[0] = p.cls[0], a.cls[1] = p.cls[1];
+    const auto segment = [](const dh_kv_view& v) {
+        return Segment{static_cast<const int8_t*>(v.k), static_cast<const int8_t*>(v.v), v.k_scale, v.v_scale,
+                       v.lengths, v.length, v.capacity};
+    };
+    a.own = segment(*own);
+    if (prefixes) a.prefix = segment(*prefix);
+    a.q = static_cast<const uint8_t*>(q);
+    a.q_seq = q_strides[0] * 2, a.q_head = q_strides[1] * 2, a.q_row = q_strides[2] * 2;
+    a.q_bf16 = q_type == DH_TYPE_BF16;
+    a.sequences = sequences, a.queries = queries, a.heads = heads, a.kv_heads = kv_heads, a.ratio = ratio;
+    a.per_prefix = prefixes ? sequences / prefixes : sequences;
+    a.v_transposed = !int8 && own->v_strides[3] != 1;
+    a.idesc_s = int8 || q_type == DH_TYPE_F16 ? tc::idesc_f16_f32<kRows, kKT>() : tc::idesc_bf16_f32<kRows, kKT>();
+    const bool v_bf16 = own->v_type == DH_TYPE_BF16;
+    a.idesc_o = (v_bf16 ? tc::idesc_bf16_f32<kRows, kPvN>() : tc::idesc_f16_f32<kRows, kPvN>()) |
+                (a.v_transposed ? 0u : tc::kIdescBMnMajor);
+    a.c = std::max(scale * 1.4426950408889634f, kLeastFactor);
+    a.out = static_cast<uint8_t*>(out);
+    a.lse = lse;
+    a.total_rows = rows;
+    a.run_rows = run_rows;
+    if (p.slots > 1) {
+        a.part_o = static_cast<float*>(workspace);
+        a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<size_t>(p.slots) * rows * kDh);
+    }
+    CUtensorMap maps[4] = {};
+    if (!int8) {
+        if (!view_maps(&maps[2], &maps[3], *own, sequences, kv_heads)) return DH_ERR_CUDA;
+        if (prefixes && !view_maps(&maps[0], &maps[1], *prefix, prefixes, kv_heads)) return DH_ERR_CUDA;
+    }
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(a.cls[0].items) + a.cls[1].items, ctas));
+    const uint32_t status = int8 ? launch<kInt8>(maps, a, grid, st)
+                                 : (v_bf16 ? launch<kVBf16>(maps, a, grid, st) : launch<kV16>(maps, a, grid, st));
+    if (status || p.slots < 2) return status;
+    kv_join_kernel<<<ceil_div(rows, 4), 128, 0, st>>>(a.part_ml, a.part_o, p.slots, rows, queries, heads, a.q_bf16,
+                                                      a.out, lse, run_rows);
+    DH_LAUNCH_CHECK();
+    return DH_OK;
+}

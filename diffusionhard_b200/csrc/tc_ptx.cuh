@@ -164,6 +164,24 @@ DH_DEVINL void tma_load_3d(void* smem_dst, const void* tmap, uint64_t* bar, int3
         : "memory");
 }
 
+DH_DEVINL void tma_load_4d(void* smem_dst, const void* tmap, uint64_t* bar, int32_t x, int32_t y,
+                           int32_t z, int32_t w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Contiguous copy global -> shared: both addresses and `bytes` multiples of 16.
+DH_DEVINL void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+            smem_u32(smem_dst)),
+        "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(smem_u32(bar))
+        : "memory");
+}
+
 DH_DEVINL void prefetch_tmap(const void* tmap) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tmap)) : "memory");
 }
@@ -247,6 +265,10 @@ DH_DEVINL void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
         : "memory");
 }
 
+DH_DEVINL void tmem_st_32x32b_x1(uint32_t taddr, uint32_t r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(r) : "memory");
+}
+
 DH_DEVINL void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // ------------------------------------------------------------ descriptors
@@ -263,6 +285,20 @@ DH_DEVINL uint64_t smem_desc_sw128(const void* smem_ptr) {
     d |= static_cast<uint64_t>(1024u >> 4) << 32;     // SBO
     d |= static_cast<uint64_t>(1u) << 46;             // descriptor version (sm100)
     d |= static_cast<uint64_t>(2u) << 61;             // SWIZZLE_128B
+    return d;
+}
+
+// Shared-memory matrix descriptor of an MN-major operand of 16-bit elements
+// with 128-byte swizzle: one 128-byte row of 64 M/N elements for each k, 8-row
+// groups 1024 bytes apart (SBO), the next 64 M/N elements `lbo` bytes on.
+DH_DEVINL uint64_t smem_desc_mn_sw128(const void* smem_ptr, uint32_t lbo) {
+    const uint32_t addr = smem_u32(smem_ptr);
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((addr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16;
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= static_cast<uint64_t>(1u) << 46;
+    d |= static_cast<uint64_t>(2u) << 61;
     return d;
 }
 
@@ -288,6 +324,9 @@ template <uint32_t M, uint32_t N>
 __host__ __device__ constexpr uint32_t idesc_f16_f32() {
     return (1u << 4) | ((N >> 3) << 17) | ((M >> 4) << 24);
 }
+
+// B operand MN-major (its rows run along k) in an instruction descriptor.
+constexpr uint32_t kIdescBMnMajor = 1u << 16;
 
 // D[tmem] (+)= A[smem] * B[smem]^T, one instruction (M x N x 32 for i8,
 // M x N x 16 for bf16).  Issued by a single thread.

@@ -1,0 +1,318 @@
+"""K/V caches in 8 bits, and attention over cached keys.
+
+Three operators over the C ABI (include/dh_b200.h):
+
+* :func:`write_kv` -- K and V rows into an int8 cache as they are produced, a
+  scale for each position and head (:class:`KVCacheI8`).
+* :func:`read_kv` -- positions of such a cache back in floating point.
+* :func:`attend` -- attention over the keys of a cache (int8, or 16-bit tensors)
+  with a number of keys for each sequence, and behind a prefix that a batch
+  shares and that is held and read once (prefix_drift._cached_suffix_forward,
+  prefix_drift.py:155-238, keeps one for each sequence).
+
+Every call runs on the current stream of its tensors' device, returns without
+waiting for it, and can be captured in a CUDA graph.  Arguments are checked
+before anything is launched; starts, counts and lengths that lie on the device
+are not, but are kept inside the cache.  Results carry no gradients, and an
+`out` tensor must not overlap the inputs.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+from typing import Any, NamedTuple, Optional, Tuple, Union
+
+import torch
+
+from . import _lib
+from .scoring import _call, _cuda, _ptr, _TYPES
+
+HEAD_DIM = 64
+CAPACITY_STEP = 64
+_TYPE_I8 = 3
+_U64x4 = ctypes.c_uint64 * 4
+
+Lengths = Union[int, torch.Tensor, None]
+
+
+class KVCacheI8(NamedTuple):
+    """Int8 K and V of ``entries`` sequences: position p of a head holds the row
+    ``codes[p] * scale[p]``.  Build one with :meth:`empty`, or from tensors of
+    these shapes, contiguous, with a capacity that is a multiple of 64."""
+
+    k: torch.Tensor        # int8 [entries, heads, capacity, 64]
+    k_scale: torch.Tensor  # fp32 [entries, heads, capacity]
+    v: torch.Tensor
+    v_scale: torch.Tensor
+
+    @classmethod
+    def empty(cls, entries: int, heads: int, capacity: int, device: Any = "cuda") -> "KVCacheI8":
+        """Room for `capacity` positions (rounded up to a multiple of 64); what
+        it holds is undefined until it is written."""
+        if entries <= 0 or heads <= 0 or capacity <= 0:
+            raise ValueError("entries, heads and capacity must be positive")
+        capacity = -(-capacity // CAPACITY_STEP) * CAPACITY_STEP
+        codes = [torch.empty((entries, heads, capacity, HEAD_DIM), dtype=torch.int8, device=device) for _ in range(2)]
+        scales = [torch.empty((entries, heads, capacity), dtype=torch.float32, device=device) for _ in range(2)]
+        return cls(codes[0], scales[0], codes[1], scales[1])
+
+    @property
+    def capacity(self) -> int:
+        return self.k.shape[2]
+
+    def nbytes(self, positions: Optional[int] = None) -> int:
+        """Bytes that `positions` positions of every entry take (default: all)."""
+        n, h, c, d = self.k.shape
+        return n * h * (c if positions is None else positions) * 2 * (d + 4)
+
+
+def _check_cache(name: str, c: KVCacheI8, device: Optional[torch.device] = None) -> KVCacheI8:
+    k = _cuda(name, c.k, device)
+    shape = k.shape
+    if len(shape) != 4 or shape[3] != HEAD_DIM or shape[2] == 0 or shape[2] % CAPACITY_STEP:
+        raise ValueError(f"{name} must hold int8 codes [entries, heads, capacity, 64], its capacity a multiple of 64")
+    if c.v.shape != shape or c.k_scale.shape != shape[:3] or c.v_scale.shape != shape[:3]:
+        raise ValueError(f"the codes and scales of {name} must have one shape")
+    f32 = torch.float32
+    if not (k.dtype is c.v.dtype is torch.int8) or not (c.k_scale.dtype is c.v_scale.dtype is f32):
+        raise ValueError(f"{name} must hold int8 codes and float32 scales")
+    dev = k.device
+    for t in c:
+        if t.device != dev:
+            raise ValueError(f"all of {name} must be on {dev}")
+        if not t.is_contiguous():
+            raise ValueError(f"the tensors of {name} must be contiguous")
+        if t.data_ptr() & 15:
+            raise ValueError(f"the tensors of {name} must start at 16-byte boundaries")
+    return c
+
+
+def _ints(name: str, t: torch.Tensor, n: int, device: torch.device) -> torch.Tensor:
+    _cuda(name, t, device)
+    if t.dtype is not torch.int32 or t.shape != (n,):
+        raise ValueError(f"{name} must be an int32 vector of {n}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _strides(t: torch.Tensor) -> Tuple[int, ...]:
+    """Element strides; 64 where a dimension holds one element and any will do."""
+    return tuple(s if n > 1 else HEAD_DIM for s, n in zip(t.stride()[:3], t.shape)) + (t.stride(3),)
+
+
+def _run_rows(run_rows: Optional[torch.Tensor], device: torch.device) -> Optional[int]:
+    if run_rows is None:
+        return None
+    _cuda("run_rows", run_rows, device)
+    if run_rows.dtype not in (torch.int32, torch.uint32) or run_rows.numel() != 1:
+        raise ValueError("run_rows must be one int32 word")
+    return run_rows.data_ptr()
+
+
+def write_kv(cache: KVCacheI8, k: torch.Tensor, v: torch.Tensor, start: Union[int, torch.Tensor] = 0,
+             counts: Optional[torch.Tensor] = None, *, run_rows: Optional[torch.Tensor] = None) -> None:
+    """Quantise rows ``k`` and ``v`` [entries, heads, n, 64] (fp32, bf16 or f16,
+    each its own, any strides: a transposed V as the QKV product leaves it is
+    ``vt.transpose(2, 3)``) into positions ``start``, ``start`` + 1, ... of
+    `cache` (dh_kv_write_i8).
+
+    ``start``: an int, or int32 [entries] on the device; ``counts``: int32
+    [entries] on the device, the rows of each sequence to write (default: all,
+    which must fit behind an int ``start``).  Positions that lie outside the
+    cache by a device ``start`` are not written, and all others stay as they
+    were.  The scale of a row is its largest magnitude / 127; a row below 2^-100
+    counts as zero, one with an infinity or NaN gets the scale NaN."""
+    _check_cache("cache", cache)
+    dev = cache.k.device
+    entries, heads, capacity, _ = cache.k.shape
+    if k.dim() != 4 or k.shape[0] != entries or k.shape[1] != heads or k.shape[3] != HEAD_DIM or v.shape != k.shape:
+        raise ValueError(f"k and v must be [{entries}, {heads}, n, {HEAD_DIM}]")
+    _cuda("k", k, dev)
+    _cuda("v", v, dev)
+    if k.dtype not in _TYPES or v.dtype not in _TYPES:
+        raise ValueError("k and v must be float32, bfloat16 or float16")
+    rows = k.shape[2]
+    starts = None
+    if isinstance(start, torch.Tensor):
+        starts, start = _ints("start", start, entries, dev), 0
+    elif start < 0 or start > capacity or (counts is None and start + rows > capacity):
+        raise ValueError(f"{rows} rows from {start} on do not fit the capacity of {capacity}")
+    if counts is not None:
+        counts = _ints("counts", counts, entries, dev)
+    run = _run_rows(run_rows, dev)
+    if rows == 0 or entries == 0 or heads == 0:
+        return
+    _call("dh_kv_write_i8", dev, k.data_ptr(), _TYPES[k.dtype], _U64x4(*k.stride()), v.data_ptr(), _TYPES[v.dtype],
+          _U64x4(*v.stride()), entries, heads, rows, _ptr(starts), start, _ptr(counts), cache.k.data_ptr(),
+          cache.k_scale.data_ptr(), cache.v.data_ptr(), cache.v_scale.data_ptr(), capacity, run)
+
+
+def read_kv(cache: KVCacheI8, start: int = 0, rows: Optional[int] = None, *,
+            dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """K and V [entries, heads, rows, 64] of positions [start, start + rows)
+    (default: to the end of the capacity) of every entry: codes * scales, rounded
+    to `dtype` (fp32, bf16 or f16; dh_kv_read_i8)."""
+    _check_cache("cache", cache)
+    entries, heads, capacity, _ = cache.k.shape
+    rows = capacity - start if rows is None else rows
+    if start < 0 or rows < 0 or start + rows > capacity:
+        raise ValueError(f"positions [{start}, {start + rows}) lie outside the capacity of {capacity}")
+    if dtype not in _TYPES:
+        raise ValueError("dtype must be float32, bfloat16 or float16")
+    dev = cache.k.device
+    k = torch.empty((entries, heads, rows, HEAD_DIM), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    if k.numel():
+        _call("dh_kv_read_i8", dev, cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(),
+              cache.v_scale.data_ptr(), entries, heads, capacity, start, rows, k.data_ptr(), v.data_ptr(),
+              _TYPES[dtype])
+    return k, v
+
+
+class _View(ctypes.Structure):
+    """dh_kv_view of include/dh_b200.h."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("k_strides", _U64x4),
+                ("v_strides", _U64x4), ("k_type", ctypes.c_uint32), ("v_type", ctypes.c_uint32),
+                ("capacity", ctypes.c_uint32), ("length", ctypes.c_uint32)]
+
+
+_NO_STRIDES = _U64x4()
+
+
+def _view(name: str, kv: Any, lengths: Lengths, q: torch.Tensor) -> tuple:
+    """(dh_kv_view, entries, heads, tensors it points into)."""
+    dev = q.device
+    if isinstance(kv, KVCacheI8):
+        _check_cache(name, kv, dev)
+        entries, heads, capacity, _ = kv.k.shape
+        kt = vt = _TYPE_I8
+        ks = vs = _NO_STRIDES
+        k, v, k_scale, v_scale = kv.k, kv.v, kv.k_scale.data_ptr(), kv.v_scale.data_ptr()
+    else:
+        k, v = kv
+        _cuda(name, k, dev)
+        _cuda(name, v, dev)
+        if k.dim() != 4 or k.shape[3] != HEAD_DIM or v.shape != k.shape or k.shape[2] == 0:
+            raise ValueError(f"k and v of {name} must be [entries, heads, n, {HEAD_DIM}] with n > 0")
+        if k.dtype is not q.dtype or v.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"k of {name} must be of q's type, v bfloat16 or float16")
+        entries, heads, capacity, _ = k.shape
+        kt, vt = _TYPES[k.dtype], _TYPES[v.dtype]
+        ks, vs = _strides(k), _strides(v)
+        if vs[3] == 1:
+            aligned = vs[0] | vs[1] | vs[2]
+        elif capacity == 1 or vs[2] == 1:  # its columns are contiguous
+            vs = (vs[0], vs[1], 1, vs[3])
+            aligned = vs[0] | vs[1] | vs[3]
+        else:
+            raise ValueError(f"v of {name} must have contiguous rows or contiguous columns")
+        if ks[3] != 1:
+            raise ValueError(f"k of {name} must have contiguous rows")
+        if (aligned | ks[0] | ks[1] | ks[2]) % 8 or (k.data_ptr() | v.data_ptr()) & 15:
+            raise ValueError(f"k and v of {name} must start at 16-byte boundaries, as must their rows and heads")
+        ks, vs = _U64x4(*ks), _U64x4(*vs)
+        k_scale = v_scale = None
+    held = None
+    length = capacity
+    if isinstance(lengths, torch.Tensor):
+        held = _ints(f"lengths of {name}", lengths, entries, dev)
+    elif lengths is not None:
+        length = int(lengths)
+        if not 0 <= length <= capacity:
+            raise ValueError(f"{length} keys of {name} do not lie within its capacity of {capacity}")
+    view = _View(k.data_ptr(), v.data_ptr(), k_scale, v_scale, _ptr(held), ks, vs, kt, vt, capacity, length)
+    return view, entries, heads, held
+
+
+def attend(q: torch.Tensor, kv: Any, lengths: Lengths = None, *, prefix: Any = None, prefix_lengths: Lengths = None,
+           scale: Optional[float] = None, return_lse: bool = False, out: Optional[torch.Tensor] = None,
+           run_rows: Optional[torch.Tensor] = None) -> Any:
+    """``softmax(scale q k^T) v`` of queries ``q`` [batch, heads, n, 64] (bf16 or
+    f16) over cached keys (dh_kv_attention).  Returns [batch, n, heads, 64] of
+    q's type: rows of a token together, as the attention-out product reads them.
+
+    ``kv``: a :class:`KVCacheI8` with an entry for each sequence, or a pair of
+    16-bit tensors k, v [batch, kv_heads, capacity, 64]: k of q's type, v bf16 or
+    f16, its rows or its columns contiguous (``vt.transpose(2, 3)``), rows and
+    heads at 16-byte boundaries.  ``heads`` is a multiple of ``kv_heads``; query
+    head h reads K/V head ``h * kv_heads // heads``.
+    ``lengths``: how many of the keys each sequence has, an int or int32 [batch]
+    on the device (default: all); what lies behind them is not used, whatever it
+    holds.
+
+    ``prefix``: keys before those, of the same kind and layout as `kv`, with an
+    entry for each group of consecutive sequences (their number divides the
+    batch: 1 for a prefix of the whole batch), ``prefix_lengths`` as `lengths`
+    for them.
+
+    ``scale`` defaults to 1/8.  A query without keys gives 0.  With
+    ``return_lse`` also the log of the sum of exponentials, fp32 [batch, n, heads]
+    (-inf without keys), to join results over disjoint keys.  Scores and sums are
+    fp32; the weights enter the product with V rounded to 16 bits (f16; bf16 for
+    V in bf16), int8 rows rounded to f16.  ``run_rows``: one device word, only the
+    sequences within its first rows of [batch * n] are computed.
+
+    Calls that split the keys take up to 264 bytes of workspace for each query,
+    head and part."""
+    _cuda("q", q)
+    if q.dim() != 4 or q.shape[3] != HEAD_DIM or q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"q must be [batch, heads, n, {HEAD_DIM}] of bfloat16 or float16")
+    dev = q.device
+    batch, heads, n, _ = q.shape
+    qs = _strides(q)
+    if qs[3] != 1 or (qs[0] | qs[1] | qs[2]) % 8 or q.data_ptr() & 15:
+        q = q.contiguous()
+        qs = q.stride()
+    view, entries, kv_heads, _own = _view("kv", kv, lengths, q)
+    if entries != batch:
+        raise ValueError(f"kv has {entries} entries for {batch} sequences")
+    if kv_heads == 0 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads are no multiple of {kv_heads} K/V heads")
+    prefixes, prefix_capacity, pview, _pre = 0, 0, None, None
+    if prefix is not None:
+        if isinstance(prefix, KVCacheI8) != isinstance(kv, KVCacheI8):
+            raise ValueError("prefix must be of the same kind as kv")
+        pview, prefixes, prefix_heads, _pre = _view("prefix", prefix, prefix_lengths, q)
+        if prefix_heads != kv_heads:
+            raise ValueError(f"prefix has {prefix_heads} heads and kv {kv_heads}")
+        if prefixes == 0 or batch % prefixes:
+            raise ValueError(f"{prefixes} prefixes do not divide {batch} sequences")
+        if pview.v_type != view.v_type or (pview.k_type != _TYPE_I8
+                                           and (pview.v_strides[3] == 1) != (view.v_strides[3] == 1)):
+            raise ValueError("v of prefix must have the type and layout of v of kv")
+        prefix_capacity = pview.capacity
+    elif prefix_lengths is not None:
+        raise ValueError("prefix_lengths without a prefix")
+    scale = 0.125 if scale is None else float(scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError("scale must be positive and finite")
+    if out is None:
+        out = torch.empty((batch, n, heads, HEAD_DIM), dtype=q.dtype, device=dev)
+    else:
+        _cuda("out", out, dev)
+        if out.numel() != batch * n * heads * HEAD_DIM or out.dtype is not q.dtype or not out.is_contiguous() \
+                or out.data_ptr() & 15:
+            raise ValueError(f"out must hold [{batch}, {n}, {heads}, {HEAD_DIM}] of q's type, contiguous and 16-byte "
+                             "aligned")
+    lse = torch.empty((batch, n, heads), dtype=torch.float32, device=dev) if return_lse else None
+    run = _run_rows(run_rows, dev)
+    if out.numel():
+        size = _workspace_bytes(batch, n, heads, kv_heads, prefixes, prefix_capacity, view.capacity, dev.index)
+        # (goes back to the allocator's pool of the current stream, which the
+        # kernels that use it are on)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+        _call("dh_kv_attention", dev, q.data_ptr(), _TYPES[q.dtype], _U64x4(*qs), batch, n, heads, kv_heads,
+              ctypes.addressof(view), None if pview is None else ctypes.addressof(pview), prefixes, scale,
+              out.data_ptr(), _ptr(lse), run, _ptr(ws), size)
+    return (out, lse) if return_lse else out
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(batch: int, n: int, heads: int, kv_heads: int, prefixes: int, prefix_capacity: int,
+                     capacity: int, index: int) -> int:
+    with torch.cuda.device(index):
+        return int(_lib.lib().dh_kv_attention_workspace_size(batch, n, heads, kv_heads, prefixes, prefix_capacity,
+                                                             capacity))

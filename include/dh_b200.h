@@ -51,6 +51,7 @@ extern "C" {
 #define DH_TYPE_F32 0u
 #define DH_TYPE_BF16 1u
 #define DH_TYPE_F16 2u
+#define DH_TYPE_I8 3u /* codes with a scale for each row: K/V caches alone */
 
 /* No token (mask_token_id of the scoring entry points). */
 #define DH_NO_TOKEN 0xFFFFFFFFu
@@ -715,6 +716,86 @@ uint32_t dh_sample_loop(const dh_mdlm_weights* weights, const int32_t* input_ids
  * tie rule of ordered_noisy_argmax_reducer.sv:106-133.  DH_ERR_NCCL when
  * NCCL is not loaded or the call fails. */
 uint32_t dh_vocab_shard_reduce(void* nccl_comm, uint64_t* packed, uint64_t count, void* stream);
+
+/* -------------------------------------------------------------- K/V caches */
+
+/* K and V rows into an int8 cache as they are produced (what
+ * prefix_drift._materialize_cached_block, prefix_drift.py:241-264, keeps in
+ * floating point).  The cache: codes [entries, heads, capacity, 64] int8 (8-byte
+ * aligned) and scales [entries, heads, capacity] fp32, of K and of V.  With amax =
+ * max |x| of a row of 64,
+ *   scale = fp32(amax / 127), code = rint(fp32(x / scale)) within +-127
+ * (fixed_mlp._quantize_symmetric, fixed_mlp.py:11-35); amax < 2^-100: scale 0 and
+ * codes 0; a value that is not finite: scale NaN and codes 0.
+ *   k, v        rows of k_type / v_type (DH_TYPE_F32, _BF16, _F16), element (b, h,
+ *               i, d) at b s[0] + h s[1] + i s[2] + d s[3] of k_strides / v_strides
+ *               (host arrays of 4, in elements), aligned to their elements
+ *   starts      device [sequences]: row i of sequence b goes to position starts[b]
+ *               + i; NULL: start + i.  Positions outside the cache are not written
+ *   counts      device [sequences]: rows of each sequence that are written (NULL:
+ *               all of them, which then have to fit)
+ *   run_rows    device word, or NULL: only the sequences of the first *run_rows
+ *               rows (sequence b's rows end at (b + 1) rows) are written
+ * All other positions stay as they were.  Sequence b is entry b.  Status: DH_ERR_*. */
+uint32_t dh_kv_write_i8(const void* k, uint32_t k_type, const uint64_t* k_strides, const void* v, uint32_t v_type,
+                        const uint64_t* v_strides, uint32_t sequences, uint32_t heads, uint32_t rows,
+                        const int32_t* starts, uint32_t start, const int32_t* counts, int8_t* k_codes, float* k_scale,
+                        int8_t* v_codes, float* v_scale, uint32_t capacity, const uint32_t* run_rows, void* stream);
+
+/* Positions [start, start + rows) of every entry of such a cache back as code *
+ * scale, rounded to out_type (DH_TYPE_F32, _BF16, _F16): k and v [entries, heads,
+ * rows, 64], 16-byte aligned.  Status: DH_ERR_*. */
+uint32_t dh_kv_read_i8(const int8_t* k_codes, const float* k_scale, const int8_t* v_codes, const float* v_scale,
+                       uint32_t entries, uint32_t heads, uint32_t capacity, uint32_t start, uint32_t rows, void* k,
+                       void* v, uint32_t out_type, void* stream);
+
+/* Keys and values of dh_kv_attention: entries x kv_heads x capacity rows of 64.
+ *   DH_TYPE_I8 (k and v): a cache of dh_kv_write_i8, contiguous, 16-byte aligned,
+ *               capacity a multiple of 64
+ *   16 bits     k of the queries' type, v DH_TYPE_BF16 or _F16, strides (entry,
+ *               head, row, element) in elements; k's rows contiguous, v's rows or
+ *               v's columns (a transposed V); starts and all other strides at
+ *               multiples of 16 bytes
+ * length: the keys of every entry (the first ones of its capacity), or lengths:
+ * device [entries], clamped to [0, capacity].  What lies behind them is not used,
+ * whatever it holds. */
+typedef struct dh_kv_view {
+    const void* k;
+    const void* v;
+    const float* k_scale;
+    const float* v_scale;
+    const int32_t* lengths;
+    uint64_t k_strides[4];
+    uint64_t v_strides[4];
+    uint32_t k_type, v_type;
+    uint32_t capacity, length;
+} dh_kv_view;
+
+/* Attention over cached keys, each sequence's being those of its group's prefix
+ * and then its own (prefix_drift._cached_suffix_forward, prefix_drift.py:213-223,
+ * where every sequence holds its prefix):
+ *   s_j = scale (q . k_j), out = sum_j e^(s_j) v_j / sum_j e^(s_j),
+ *   lse = log sum_j e^(s_j);
+ * without keys out = 0 and lse = -inf.
+ *   q           [sequences, heads, queries] rows of 64 of q_type (DH_TYPE_BF16,
+ *               _F16), strides (sequence, head, query) in elements, 16-byte aligned
+ *   own         keys of each sequence (an entry each), heads / kv_heads query heads
+ *               for each K/V head
+ *   prefix      NULL (prefixes 0), or `prefixes` entries: of consecutive sequences,
+ *               each sequences / prefixes share one.  Types and layout of V as in own
+ *   out         [sequences, queries, heads, 64] of q_type; lse the same without the
+ *               64, or NULL
+ *   run_rows    as in dh_kv_write_i8, with queries rows a sequence
+ *   workspace   256-byte aligned, of the size the query returns for the current
+ *               device (0: none); calls that may overlap need one each
+ * Results do not depend on timing: the same call gives the same bits.
+ * Status: DH_ERR_*. */
+size_t dh_kv_attention_workspace_size(uint32_t sequences, uint32_t queries, uint32_t heads, uint32_t kv_heads,
+                                      uint32_t prefixes, uint32_t prefix_capacity, uint32_t own_capacity);
+uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64_t* q_strides, uint32_t sequences,
+                         uint32_t queries, uint32_t heads, uint32_t kv_heads, const dh_kv_view* own,
+                         const dh_kv_view* prefix, uint32_t prefixes, float scale, void* out, float* lse,
+                         const uint32_t* run_rows, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------- diagnostics */
 
