@@ -27,10 +27,8 @@
 //   warps 4-7 softmax, a thread a row: P = 2^(s c - m) over S in TMEM; O in TMEM
 //             is rescaled only when the maximum grew by more than 2^8
 #include <cuda.h>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 
-#include "tc_ptx.cuh"
+#include "kv_few.h"
 #include "tmap.h"
 
 #include <algorithm>
@@ -39,21 +37,16 @@
 namespace dh {
 namespace {
 
-constexpr uint32_t kDh = 64;
+using namespace kv;
+
 constexpr uint32_t kRows = 128;                  // rows per item
-constexpr uint32_t kKT = 64;                     // keys per tile
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kTileBytes = kKT * kDh * 2;   // 8 KB: a 16-bit K or V tile
 constexpr uint32_t kOnesBytes = 2048;            // 16 rows of 128 bytes
 constexpr uint32_t kVPitch = kTileBytes + kOnesBytes;
-constexpr uint32_t kRawBytes = 2 * kKT * kDh + 2 * kKT * 4;  // codes and scales of 64 keys
 constexpr uint32_t kTmemCols = 256;
 constexpr uint32_t kOCol = 128;                  // S/P buffers at 0 and 64, O at 128, l at 192
 constexpr uint32_t kQCol = 224;
 constexpr uint32_t kPvN = kDh + 16;
-// Factors of scores stay above zero: keys behind the last one score -inf, and
-// -inf * 0 would be NaN.
-constexpr float kLeastFactor = 1.17549435e-38f;
 constexpr uint32_t kExpRing = 8;                 // tiles whose exponents are kept
 
 enum Kind : int { kV16 = 0, kVBf16 = 1, kInt8 = 2 };
@@ -73,38 +66,6 @@ struct Cfg {
     static constexpr uint32_t bytes = 1024 + bars_at + 512;
 };
 
-// Rows and keys of one class of items.
-struct Class {
-    uint32_t groups, seqs, row_tiles, splits, items, slot;
-    uint32_t with_prefix, with_own;
-};
-
-struct Segment {
-    const int8_t* k;
-    const int8_t* v;
-    const float* k_scale;
-    const float* v_scale;
-    const int32_t* lengths;
-    uint32_t length, capacity;
-};
-
-struct Args {
-    Class cls[2];
-    Segment prefix, own;
-    const uint8_t* q;                        // 16-bit elements
-    uint64_t q_seq, q_head, q_row;           // strides in bytes
-    uint32_t q_bf16;
-    uint32_t sequences, queries, heads, kv_heads, ratio, per_prefix;
-    uint32_t v_transposed, idesc_s, idesc_o;
-    float c;                                 // scale * log2(e)
-    uint8_t* out;                            // [sequences, queries, heads, 64], of q's type
-    float* lse;                              // [sequences, queries, heads], or null
-    float2* part_ml;                         // [slots][rows], or null: one slot
-    float* part_o;                           // [slots][rows][64]
-    uint64_t total_rows;
-    const uint32_t* run_rows;
-};
-
 enum Bar : uint32_t {
     kRawFull = 0, kRawEmpty = kRawFull + 4, kKFull = kRawEmpty + 4, kKEmpty = kKFull + 4, kVFull = kKEmpty + 4,
     kVEmpty = kVFull + 4, kSFull = kVEmpty + 4, kPFull = kSFull + 2, kSPFree = kPFull + 2, kOFull = kSPFree + 2,
@@ -113,37 +74,6 @@ enum Bar : uint32_t {
 static_assert(kNumBars * 8 + 8 + 2 * kExpRing * 4 <= 512, "barrier area");
 
 DH_DEVINL void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-DH_DEVINL float ex2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// maxima that are NaN if an operand is
-DH_DEVINL float max_nan(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-DH_DEVINL float max_nan(float a, float b, float c) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-DH_DEVINL uint32_t pack_f16x2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-DH_DEVINL uint32_t pack_bf16x2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-// 2^n, -126 <= n <= 127
-DH_DEVINL float pow2(int32_t n) { return __uint_as_float(static_cast<uint32_t>(n + 127) << 23); }
-// e with 2^(e - 1) <= x < 2^e for the normal fp32 with these bits
-DH_DEVINL int32_t exponent_of(uint32_t bits) { return static_cast<int32_t>((bits >> 23) & 0xFFu) - 126; }
 
 // 2^x of two values on the FMA pipe (x <= 8): x = n + f with n = rint(x) by the
 // 1.5 * 2^23 shifter, 2^f on [-0.5, 0.5] by a cubic (largest relative error
@@ -162,59 +92,6 @@ DH_DEVINL float2 exp2_poly2(float2 x) {
                        __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 constexpr uint32_t kPolyPairMask = 0x11u;  // pairs e with bit e % 8 set
-
-struct Item {
-    uint32_t seq0, kv_head, row0, rows, slot;  // rows: live rows of the tile (may be 0)
-    uint32_t prefix, own;                      // cache entries
-    uint32_t len0, len1, n0, t0, t1;           // keys and tiles of the two parts, tile range
-};
-
-DH_DEVINL uint32_t length_of(const Segment& s, uint32_t entry) {
-    const int32_t n = s.lengths ? __ldg(s.lengths + entry) : static_cast<int32_t>(s.length);
-    return static_cast<uint32_t>(min(max(n, 0), static_cast<int32_t>(s.capacity)));
-}
-
-DH_DEVINL Item item_of(const Args& a, uint32_t w, uint32_t live) {
-    Item it;
-    const Class& c = w < a.cls[0].items ? a.cls[0] : a.cls[1];
-    if (w >= a.cls[0].items) w -= a.cls[0].items;
-    const uint32_t split = w % c.splits;
-    w /= c.splits;
-    const uint32_t tile = w % c.row_tiles;
-    w /= c.row_tiles;
-    it.kv_head = w % a.kv_heads;
-    const uint32_t group = w / a.kv_heads;
-    it.seq0 = group * c.seqs;
-    it.slot = c.slot + split;
-    it.row0 = tile * kRows;
-    const uint32_t seqs = live > it.seq0 ? min(live - it.seq0, c.seqs) : 0u;
-    const uint32_t rows = seqs * a.queries * a.ratio;
-    it.rows = rows > it.row0 ? min(rows - it.row0, kRows) : 0u;
-    it.own = it.seq0;
-    it.prefix = it.seq0 / a.per_prefix;
-    it.len0 = c.with_prefix ? length_of(a.prefix, it.prefix) : 0u;
-    it.len1 = c.with_own ? length_of(a.own, it.own) : 0u;
-    it.n0 = (it.len0 + kKT - 1) / kKT;
-    const uint32_t n = it.n0 + (it.len1 + kKT - 1) / kKT;
-    it.t0 = static_cast<uint32_t>(static_cast<uint64_t>(n) * split / c.splits);
-    it.t1 = static_cast<uint32_t>(static_cast<uint64_t>(n) * (split + 1) / c.splits);
-    if (it.rows == 0) it.t1 = it.t0;
-    return it;
-}
-// keys left from tile j on in its part (a full tile: 64 or more)
-DH_DEVINL uint32_t keys_left(const Item& it, uint32_t j) {
-    return j < it.n0 ? it.len0 - j * kKT : it.len1 - (j - it.n0) * kKT;
-}
-
-// Row r of an item: its query, as an index of [sequences, queries, heads].
-DH_DEVINL uint64_t row_index(const Args& a, const Item& it, uint32_t r, const uint8_t** q) {
-    const uint32_t row = it.row0 + r;
-    const uint32_t token = row / a.ratio;
-    const uint32_t head = it.kv_head * a.ratio + row % a.ratio;
-    const uint32_t seq = it.seq0 + token / a.queries, s = token % a.queries;
-    if (q) *q = a.q + seq * a.q_seq + head * a.q_head + s * a.q_row;
-    return (static_cast<uint64_t>(seq) * a.queries + s) * a.heads + head;
-}
 
 // 16 codes -> 16 f16 of code * ratio * 2^-9, where f = f16(ratio * 2^15): a code
 // plus 128 as the bits of a subnormal f16 is (code + 128) 2^-24, so one FMA with
@@ -262,13 +139,19 @@ DH_DEVINL void convert_rows(const uint8_t* raw, uint8_t* tile, uint32_t warp_hal
     }
 }
 
+// Item w of both classes, `first` the number of the first class's (0: they are not
+// this kernel's).
+DH_DEVINL Item item_at(const Args& a, uint32_t first, uint32_t w, uint32_t live) {
+    return w < first ? item_of(a, a.cls[0], w, live) : item_of(a, a.cls[1], w - first, live);
+}
+
 template <int KIND>
 __global__ void __launch_bounds__(kThreads, 2)
 kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ CUtensorMap tpv,
                     const __grid_constant__ CUtensorMap tok, const __grid_constant__ CUtensorMap tov,
-                    const __grid_constant__ Args a) {
+                    const __grid_constant__ Args a, const uint32_t first, const uint32_t total) {
     using C = Cfg<KIND>;
-    const uint32_t live = a.run_rows ? min(a.sequences, *a.run_rows / a.queries) : a.sequences;
+    const uint32_t live = a.run_rows ? min(a.sequences, a.queries.of(min(*a.run_rows, 0x7FFFFFFFu))) : a.sequences;
     if (live == 0) return;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -283,7 +166,6 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
     int32_t* exps = reinterpret_cast<int32_t*>(tmem_holder + 2);  // [kExpRing][2]: K, V of a tile
 
     const uint32_t warp = warp_id(), lane = lane_id();
-    const uint32_t total = a.cls[0].items + a.cls[1].items;
 
     if (warp == 0 && lane == 0) {
         for (uint32_t i = 0; i < kNumBars; ++i) {
@@ -332,7 +214,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
             uint32_t g = 0;
             bool ok = true;
             for (uint32_t w = blockIdx.x; w < total && ok; w += gridDim.x) {
-                const Item it = item_of(a, w, live);
+                const Item it = item_at(a, first, w, live);
                 for (uint32_t j = it.t0; j < it.t1; ++j, ++g) {
                     const bool own = j >= it.n0;
                     const uint32_t key = (own ? j - it.n0 : j) * kKT;
@@ -345,7 +227,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                             break;
                         }
                         const Segment& s = own ? a.own : a.prefix;
-                        const uint64_t at = (static_cast<uint64_t>(entry) * a.kv_heads + it.kv_head) * s.capacity + key;
+                        const uint64_t at = (static_cast<uint64_t>(entry) * a.kv_heads.d + it.kv_head) * s.capacity + key;
                         uint8_t* dst = raw_ring + rs * kRawBytes;
                         uint64_t* bar = &bars[kRawFull + rs];
                         tc::mbar_arrive_expect_tx(bar, kRawBytes);
@@ -413,7 +295,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
             uint32_t g = 0, n_items = 0;
             bool ok = true;
             for (uint32_t w = blockIdx.x; w < total && ok; w += gridDim.x) {
-                const Item it = item_of(a, w, live);
+                const Item it = item_at(a, first, w, live);
                 if (it.t0 == it.t1) continue;
                 if (!tc::mbar_wait_suspend(&bars[kQReady], n_items & 1u, tc::kErrTimeoutFull)) break;
                 tc::tc_fence_after();
@@ -462,7 +344,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
             // ---------------------------------------------------- conversion
             const uint32_t half = warp - 2;
             for (uint32_t w = blockIdx.x; w < total && ok; w += gridDim.x) {
-                const Item it = item_of(a, w, live);
+                const Item it = item_at(a, first, w, live);
                 int32_t ev = -1000;
                 for (uint32_t j = it.t0; j < it.t1; ++j, ++g) {
                     const uint32_t rs = g % C::raw_stages, ks = g % C::k_stages, vs = g % C::v_stages;
@@ -529,7 +411,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
             // them on: a stage is loaded again only after that, so no phase is missed.
             uint32_t phases = 0;  // a bit for each stage
             for (uint32_t w = blockIdx.x; w < total && ok; w += gridDim.x) {
-                const Item it = item_of(a, w, live);
+                const Item it = item_at(a, first, w, live);
                 for (uint32_t j = it.t0; j < it.t1; ++j, ++g) {
                     const uint32_t left = keys_left(it, j), vs = g % C::v_stages;
                     if (left >= kKT) continue;
@@ -601,7 +483,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
         // shared memory.
         auto next_item = [&](uint32_t& w, Item& it) {
             for (; w < total; w += gridDim.x) {
-                it = item_of(a, w, live);
+                it = item_at(a, first, w, live);
                 if (it.t0 != it.t1) break;
                 if (r < it.rows) {
                     const uint32_t zero[32] = {};
@@ -753,7 +635,8 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                         pk[e] = KIND == kVBf16 ? pack_bf16x2(y.x, y.y) : pack_f16x2(y.x, y.y);
                     }
                     tc::tmem_st_32x32b_x32(tmem + lane_base + sb * kKT, pk);
-                    if (__any_sync(0xFFFFFFFFu, need)) {
+                    // (rows behind the last hold anything: they ask for nothing)
+                    if (__any_sync(0xFFFFFFFFu, need && r < it.rows)) {
                         // PV of the tile before (the only one that may still run) finished
                         if (!tc::mbar_wait_suspend(&bars[kSPFree + (sb ^ 1u)], ((g - 1) >> 1) & 1u,
                                                    tc::kErrTimeoutEmpty)) {
@@ -852,34 +735,38 @@ constexpr uint32_t kStackBelow = 128;
 constexpr uint32_t kMaxSplits = 64;
 
 struct Plan {
-    Class cls[2];
+    Class cls[2];         // prefix of stacked rows, and each sequence's own keys
+    bool few[2];          // items of the kernel for few rows, on `cluster` CTAs each
+    uint32_t cluster[2];
     uint32_t slots;
 };
 
 uint32_t ceil_div(uint64_t a, uint64_t b) { return static_cast<uint32_t>((a + b - 1) / b); }
 
-// The split of the keys into 1 to 64 parts: the one with the shortest estimated
-// time, in tiles: full rounds of items on `ctas` CTAs, two tiles of start and end
-// for each item, three for a join.
-Plan plan_of(uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t prefixes, uint32_t prefix_keys,
-             uint32_t own_keys, uint32_t ctas) {
-    Plan p{};
-    const uint32_t per = prefixes ? sequences / prefixes : sequences;
-    const bool stacked = prefixes && per > 1 && rows < kStackBelow;
-    const uint32_t t0 = ceil_div(prefix_keys, kKT), t1 = ceil_div(own_keys, kKT);
-    uint32_t tiles[2] = {0, 0};
-    if (stacked) {
-        p.cls[0] = Class{prefixes, per, ceil_div(static_cast<uint64_t>(per) * rows, kRows), 1, 0, 0, 1, 0};
-        tiles[0] = t0;
+// Few rows: a warp an item where there are items enough with few tiles.  Else parts
+// of at least a tile a warp, up to eight in a cluster until the GPU has four CTAs
+// an SM, then as many clusters as that still takes.
+void split_few(Class& c, uint32_t& cluster, uint64_t items, uint32_t tiles, uint32_t sms) {
+    if (items >= 8ull * sms && tiles <= 32) {
+        cluster = 0;
+        return;
     }
-    p.cls[1] = Class{sequences, 1, ceil_div(rows, kRows), 1, 0, 0, prefixes && !stacked, 1};
-    tiles[1] = t1 + (stacked || !prefixes ? 0 : t0);
-    uint64_t items[2];
-    for (int i = 0; i < 2; ++i)
-        items[i] = static_cast<uint64_t>(p.cls[i].groups) * kv_heads * p.cls[i].row_tiles;
+    cluster = 1;
+    while (cluster < kMaxCluster && cluster * 8 <= tiles && items * cluster < 4ull * sms) cluster *= 2;
+    const uint64_t ctas = items * cluster;
+    if (ctas < 2ull * sms)
+        c.splits = FastDiv(static_cast<uint32_t>(
+            std::min<uint64_t>({kMaxSplits, std::max<uint64_t>(tiles / (cluster * 8), 1),
+                                std::max<uint64_t>(3ull * sms / ctas, 1)})));
+}
+
+// Tensor-core tiles: 1 to 64 parts of the keys, by the shortest estimated time, in
+// tiles: full rounds of items on `ctas` CTAs, two tiles of start and end for each
+// item, three for a join.
+void split_many(Class* cls, const uint64_t* items, const uint32_t* tiles, uint32_t ctas, bool joined) {
     uint64_t best = ~0ull;
     uint32_t best_splits[2] = {1, 1};
-    const uint32_t most = std::max(std::max(tiles[0], tiles[1]), 1u);
+    const uint32_t most = std::max(std::max(items[0] ? tiles[0] : 0, items[1] ? tiles[1] : 0), 1u);
     for (uint32_t n = 1; n <= kMaxSplits; ++n) {
         const uint32_t chunk = ceil_div(most, n);
         uint64_t work = 0, longest = 0;
@@ -893,7 +780,7 @@ Plan plan_of(uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t pref
         }
         const uint64_t count = items[0] * splits[0] + items[1] * splits[1];
         uint64_t time = std::max<uint64_t>(ceil_div(count, ctas) * longest, ceil_div(work, ctas));
-        if (stacked || splits[1] > 1) time += 3;
+        if (joined || splits[1] > 1) time += 3;
         if (time < best) {
             best = time;
             best_splits[0] = splits[0];
@@ -901,12 +788,42 @@ Plan plan_of(uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t pref
         }
         if (chunk == 1) break;
     }
+    for (int i = 0; i < 2; ++i)
+        if (items[i]) cls[i].splits = FastDiv(best_splits[i]);
+}
+
+Plan plan_of(uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t prefixes, uint32_t prefix_keys,
+             uint32_t own_keys, uint32_t sms) {
+    Plan p{};
+    const uint32_t per = prefixes ? sequences / prefixes : sequences;
+    const bool stacked = prefixes && per > 1 && rows < kStackBelow;
+    const uint32_t t0 = ceil_div(prefix_keys, kKT), t1 = ceil_div(own_keys, kKT);
+    const uint32_t tiles[2] = {stacked ? t0 : 0, t1 + (stacked || !prefixes ? 0 : t0)};
+    uint64_t items[2] = {0, 0}, many[2] = {0, 0};
+    for (int i = stacked ? 0 : 1; i < 2; ++i) {
+        Class& c = p.cls[i];
+        c.groups = i ? sequences : prefixes;
+        c.seqs = i ? 1 : per;
+        c.with_prefix = prefixes && (!i || !stacked);
+        c.with_own = i;
+        const uint64_t all = static_cast<uint64_t>(c.seqs) * rows;
+        const bool few = all <= kFewRows;
+        c.tile_rows = few ? (all > 16 ? 32 : (all > 8 ? 16 : 8)) : kRows;
+        c.row_tiles = FastDiv(ceil_div(all, c.tile_rows));
+        items[i] = static_cast<uint64_t>(c.groups) * kv_heads * c.row_tiles.d;
+        p.few[i] = few;
+        if (few)
+            split_few(c, p.cluster[i], items[i], tiles[i], sms);
+        else
+            many[i] = items[i];
+    }
+    if (many[0] || many[1]) split_many(p.cls, many, tiles, 2 * sms, stacked);
     for (int i = 0; i < 2; ++i) {
         if (!items[i]) continue;
-        p.cls[i].splits = best_splits[i];
-        p.cls[i].items = static_cast<uint32_t>(std::min<uint64_t>(items[i] * best_splits[i], 0xFFFFFFFFull));
-        p.cls[i].slot = p.slots;
-        p.slots += best_splits[i];
+        Class& c = p.cls[i];
+        c.items = static_cast<uint32_t>(items[i] * c.splits.d);
+        c.slot = p.slots;
+        p.slots += c.splits.d;
     }
     return p;
 }
@@ -960,10 +877,12 @@ bool view_maps(CUtensorMap* k, CUtensorMap* v, const dh_kv_view& s, uint32_t ent
 }
 
 template <int KIND>
-uint32_t launch(const CUtensorMap (&maps)[4], const Args& a, uint32_t grid, cudaStream_t st) {
+uint32_t launch(const CUtensorMap (&maps)[4], const Args& a, uint32_t first, uint32_t total, cudaStream_t st) {
     static std::atomic<uint64_t> configured{0};
     if (smem_optin_once(kv_attention_kernel<KIND>, Cfg<KIND>::bytes, configured) != cudaSuccess) return DH_ERR_CUDA;
-    kv_attention_kernel<KIND><<<grid, kThreads, Cfg<KIND>::bytes, st>>>(maps[0], maps[1], maps[2], maps[3], a);
+    const uint32_t grid = std::min(total, 2 * device_sms());
+    kv_attention_kernel<KIND><<<grid, kThreads, Cfg<KIND>::bytes, st>>>(maps[0], maps[1], maps[2], maps[3], a, first,
+                                                                       total);
     DH_LAUNCH_CHECK();
     return DH_OK;
 }
@@ -980,7 +899,7 @@ extern "C" size_t dh_kv_attention_workspace_size(uint32_t sequences, uint32_t qu
         !fits(sequences, queries, heads, kv_heads, prefixes))
         return 0;
     const Plan p = plan_of(sequences, queries * (heads / kv_heads), kv_heads, prefixes, prefix_capacity, own_capacity,
-                           2 * device_sms());
+                           device_sms());
     return workspace_of(p.slots, static_cast<uint64_t>(sequences) * queries * heads);
 }
 
@@ -1006,9 +925,8 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
         return DH_ERR_ALIGNMENT;
     const uint32_t ratio = heads / kv_heads;
     const uint64_t rows = static_cast<uint64_t>(sequences) * queries * heads;
-    const uint32_t ctas = 2 * device_sms();
     const Plan p = plan_of(sequences, queries * ratio, kv_heads, prefixes, prefixes ? prefix->capacity : 0,
-                           own->capacity, ctas);
+                           own->capacity, device_sms());
     const size_t need = workspace_of(p.slots, rows);
     if (need && !workspace) return DH_ERR_NULL_POINTER;
     if (need > workspace_bytes) return DH_ERR_WORKSPACE;
@@ -1025,8 +943,9 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
     a.q = static_cast<const uint8_t*>(q);
     a.q_seq = q_strides[0] * 2, a.q_head = q_strides[1] * 2, a.q_row = q_strides[2] * 2;
     a.q_bf16 = q_type == DH_TYPE_BF16;
-    a.sequences = sequences, a.queries = queries, a.heads = heads, a.kv_heads = kv_heads, a.ratio = ratio;
-    a.per_prefix = prefixes ? sequences / prefixes : sequences;
+    a.sequences = sequences, a.heads = heads;
+    a.queries = FastDiv(queries), a.kv_heads = FastDiv(kv_heads), a.ratio = FastDiv(ratio);
+    a.per_prefix = FastDiv(prefixes ? sequences / prefixes : sequences);
     a.v_transposed = !int8 && own->v_strides[3] != 1;
     a.idesc_s = int8 || q_type == DH_TYPE_F16 ? tc::idesc_f16_f32<kRows, kKT>() : tc::idesc_bf16_f32<kRows, kKT>();
     const bool v_bf16 = own->v_type == DH_TYPE_BF16;
@@ -1047,9 +966,16 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
         if (prefixes && !view_maps(&maps[0], &maps[1], *prefix, prefixes, kv_heads)) return DH_ERR_CUDA;
     }
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(a.cls[0].items) + a.cls[1].items, ctas));
-    const uint32_t status = int8 ? launch<kInt8>(maps, a, grid, st)
-                                 : (v_bf16 ? launch<kVBf16>(maps, a, grid, st) : launch<kV16>(maps, a, grid, st));
+    uint32_t status = DH_OK, first = 0, total = 0;
+    for (uint32_t i = 0; i < 2 && !status; ++i) {
+        if (p.few[i])
+            status = launch_few(maps, a, i, p.cluster[i], int8, v_bf16, st);
+        else
+            total += a.cls[i].items, first += i ? 0 : a.cls[0].items;
+    }
+    if (total && !status)
+        status = int8 ? launch<kInt8>(maps, a, first, total, st)
+                      : (v_bf16 ? launch<kVBf16>(maps, a, first, total, st) : launch<kV16>(maps, a, first, total, st));
     if (status || p.slots < 2) return status;
     kv_join_kernel<<<ceil_div(rows, 4), 128, 0, st>>>(a.part_ml, a.part_o, p.slots, rows, queries, heads, a.q_bf16,
                                                       a.out, lse, run_rows);

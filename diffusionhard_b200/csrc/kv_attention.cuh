@@ -1,0 +1,147 @@
+// kv_attention.cuh -- what the kernels of attention over K/V caches share: the
+// arguments, which rows and keys a work item has, and small arithmetic.  The
+// operator is described in kv_attention.cu.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "fast_div.cuh"
+#include "tc_ptx.cuh"
+
+namespace dh {
+namespace kv {
+
+constexpr uint32_t kDh = 64;
+constexpr uint32_t kKT = 64;                                 // keys per tile
+constexpr uint32_t kTileBytes = kKT * kDh * 2;               // 8 KB: a 16-bit K or V tile
+constexpr uint32_t kRawBytes = 2 * kKT * kDh + 2 * kKT * 4;  // codes and scales of 64 keys
+// Factors of scores stay above zero: keys behind the last one score -inf, and
+// -inf * 0 would be NaN.
+constexpr float kLeastFactor = 1.17549435e-38f;
+
+// Rows and keys of one class of items.
+struct Class {
+    uint32_t groups, seqs;               // groups of consecutive sequences whose rows are stacked
+    uint32_t tile_rows, items, slot;     // rows of an item; all items; the first part's slot
+    FastDiv row_tiles, splits;           // items a group and K/V head; parts of the keys
+    uint32_t with_prefix, with_own;
+};
+
+struct Segment {
+    const int8_t* k;
+    const int8_t* v;
+    const float* k_scale;
+    const float* v_scale;
+    const int32_t* lengths;
+    uint32_t length, capacity;
+};
+
+struct Args {
+    Class cls[2];
+    Segment prefix, own;
+    const uint8_t* q;                        // 16-bit elements
+    uint64_t q_seq, q_head, q_row;           // strides in bytes
+    uint32_t q_bf16;
+    uint32_t sequences, heads;
+    FastDiv queries, kv_heads, ratio, per_prefix;  // ratio: query heads of a K/V head
+    uint32_t v_transposed, idesc_s, idesc_o;
+    float c;                                 // scale * log2(e)
+    uint8_t* out;                            // [sequences, queries, heads, 64], of q's type
+    float* lse;                              // [sequences, queries, heads], or null
+    float2* part_ml;                         // [slots][rows], or null: one slot
+    float* part_o;                           // [slots][rows][64]
+    uint64_t total_rows;
+    const uint32_t* run_rows;
+};
+
+DH_DEVINL float ex2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// maxima that are NaN if an operand is
+DH_DEVINL float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+DH_DEVINL float max_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+DH_DEVINL uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+DH_DEVINL uint32_t pack_bf16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// 2^n, -126 <= n <= 127
+DH_DEVINL float pow2(int32_t n) { return __uint_as_float(static_cast<uint32_t>(n + 127) << 23); }
+// e with 2^(e - 1) <= x < 2^e for the normal fp32 with these bits
+DH_DEVINL int32_t exponent_of(uint32_t bits) { return static_cast<int32_t>((bits >> 23) & 0xFFu) - 126; }
+
+struct Item {
+    uint32_t seq0, kv_head, row0, rows, slot;  // rows: live rows of the tile (may be 0)
+    uint32_t prefix, own;                      // cache entries
+    uint32_t len0, len1, n0, t0, t1;           // keys and tiles of the two parts, tile range
+};
+
+DH_DEVINL uint32_t length_of(const Segment& s, uint32_t entry) {
+    const int32_t n = s.lengths ? __ldg(s.lengths + entry) : static_cast<int32_t>(s.length);
+    return static_cast<uint32_t>(min(max(n, 0), static_cast<int32_t>(s.capacity)));
+}
+
+// Item w of a class, of the first `live` sequences.
+DH_DEVINL Item item_of(const Args& a, const Class& c, uint32_t w, uint32_t live) {
+    Item it;
+    uint32_t split = w, tile, head;
+    tile = c.splits.split(split);
+    head = c.row_tiles.split(tile);
+    const uint32_t group = a.kv_heads.split(head);
+    it.kv_head = head;
+    it.seq0 = group * c.seqs;
+    it.slot = c.slot + split;
+    it.row0 = tile * c.tile_rows;
+    const uint32_t seqs = live > it.seq0 ? min(live - it.seq0, c.seqs) : 0u;
+    const uint32_t rows = seqs * a.queries.d * a.ratio.d;
+    it.rows = rows > it.row0 ? min(rows - it.row0, c.tile_rows) : 0u;
+    it.own = it.seq0;
+    it.prefix = a.per_prefix.of(it.seq0);
+    it.len0 = c.with_prefix ? length_of(a.prefix, it.prefix) : 0u;
+    it.len1 = c.with_own ? length_of(a.own, it.own) : 0u;
+    it.n0 = (it.len0 + kKT - 1) / kKT;
+    const uint32_t n = it.n0 + (it.len1 + kKT - 1) / kKT;
+    if (c.splits.d == 1) {
+        it.t0 = 0, it.t1 = n;
+    } else {
+        uint32_t more = n;  // `more` parts have a tile more than the others
+        const uint32_t each = c.splits.split(more);
+        it.t0 = each * split + c.splits.of(more * split);
+        it.t1 = each * (split + 1) + c.splits.of(more * (split + 1));
+    }
+    if (it.rows == 0) it.t1 = it.t0;
+    return it;
+}
+// keys left from tile j on in its part (a full tile: 64 or more)
+DH_DEVINL uint32_t keys_left(const Item& it, uint32_t j) {
+    return j < it.n0 ? it.len0 - j * kKT : it.len1 - (j - it.n0) * kKT;
+}
+
+// Row r of an item: its query, as an index of [sequences, queries, heads].
+DH_DEVINL uint64_t row_index(const Args& a, const Item& it, uint32_t r, const uint8_t** q) {
+    uint32_t in_kv = it.row0 + r;
+    uint32_t s = a.ratio.split(in_kv);  // the token among the group's, then in its sequence
+    const uint32_t head = it.kv_head * a.ratio.d + in_kv;
+    const uint32_t seq = it.seq0 + a.queries.split(s);
+    if (q) *q = a.q + seq * a.q_seq + head * a.q_head + s * a.q_row;
+    return (static_cast<uint64_t>(seq) * a.queries.d + s) * a.heads + head;
+}
+
+}  // namespace kv
+}  // namespace dh
