@@ -49,6 +49,8 @@ constexpr uint32_t kQCol = 224;
 constexpr uint32_t kPvN = kDh + 16;
 constexpr uint32_t kExpRing = 8;                 // tiles whose exponents are kept
 
+constexpr uint32_t kMaxSplits = 64;              // parts of an item's keys
+
 enum Kind : int { kV16 = 0, kVBf16 = 1, kInt8 = 2 };
 
 template <int KIND>
@@ -166,6 +168,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
     int32_t* exps = reinterpret_cast<int32_t*>(tmem_holder + 2);  // [kExpRing][2]: K, V of a tile
 
     const uint32_t warp = warp_id(), lane = lane_id();
+    grid_launch_dependents();
 
     if (warp == 0 && lane == 0) {
         for (uint32_t i = 0; i < kNumBars; ++i) {
@@ -445,38 +448,16 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
         const uint32_t lane_base = (quad * 32u) << 16;
         uint8_t* my_q = q_s + r * 128;
 
-        auto write_row = [&](const Item& it, float m, float l, float f, const uint32_t (&v0)[32],
-                             const uint32_t (&v1)[32]) {
-            const uint64_t row = row_index(a, it, r, nullptr);
+        // Row `row` of slot `slot` has no keys.
+        auto write_empty = [&](uint64_t row, uint32_t slot) {
             if (a.part_ml) {
-                const uint64_t at = it.slot * a.total_rows + row;
-                a.part_ml[at] = make_float2(m, l);
-                if (l == 0.f) return;
-                float4* dst = reinterpret_cast<float4*>(a.part_o + at * kDh);
-#pragma unroll
-                for (uint32_t d = 0; d < 32; d += 4) {
-                    dst[d / 4] = make_float4(__uint_as_float(v0[d]) * f, __uint_as_float(v0[d + 1]) * f,
-                                             __uint_as_float(v0[d + 2]) * f, __uint_as_float(v0[d + 3]) * f);
-                    dst[8 + d / 4] = make_float4(__uint_as_float(v1[d]) * f, __uint_as_float(v1[d + 1]) * f,
-                                                 __uint_as_float(v1[d + 2]) * f, __uint_as_float(v1[d + 3]) * f);
-                }
+                a.part_ml[slot * a.total_rows + row] = make_float2(0.f, 0.f);
                 return;
             }
-            const float inv = l == 0.f ? 0.f : f / l;
             uint4* dst = reinterpret_cast<uint4*>(a.out + row * (kDh * 2));
 #pragma unroll
-            for (uint32_t d = 0; d < 64; d += 8) {
-                uint32_t o[4];
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    const uint32_t e = d + 2 * i;
-                    const float x = __uint_as_float(e < 32 ? v0[e & 31] : v1[e & 31]) * inv;
-                    const float y = __uint_as_float(e < 32 ? v0[(e + 1) & 31] : v1[(e + 1) & 31]) * inv;
-                    o[i] = a.q_bf16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
-                }
-                dst[d / 8] = make_uint4(o[0], o[1], o[2], o[3]);
-            }
-            if (a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+            for (uint32_t i = 0; i < 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
+            if (a.lse) a.lse[row] = -INFINITY;
         };
         // From item w on: rows of items without keys are answered at once; the
         // first item with keys (w >= total: none), its query row on its way to
@@ -485,10 +466,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
             for (; w < total; w += gridDim.x) {
                 it = item_at(a, first, w, live);
                 if (it.t0 != it.t1) break;
-                if (r < it.rows) {
-                    const uint32_t zero[32] = {};
-                    write_row(it, 0.f, 0.f, 1.f, zero, zero);
-                }
+                if (r < it.rows) write_empty(row_index(a, it, r, nullptr), it.slot);
             }
             if (w < total && r < it.rows) {
                 const uint8_t* q;
@@ -670,15 +648,48 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
             if (next_w < total) next_c = copy_q();
             if (!tc::mbar_wait_suspend(&bars[kOFull], n_items & 1u, tc::kErrTimeoutAccFull)) break;
             tc::tc_fence_after();
-            uint32_t v0[32], v1[32];
-            tc::tmem_ld_32x32b_x32(tmem + lane_base + kOCol, v0);
-            tc::tmem_ld_32x32b_x32(tmem + lane_base + kOCol + 32, v1);
-            const uint32_t l_bits = tc::tmem_ld_32x32b_x1(tmem + lane_base + kOCol + kDh);
+            const float l = __uint_as_float(tc::tmem_ld_32x32b_x1(tmem + lane_base + kOCol + kDh));
+            const uint64_t row = row_index(a, it, r, nullptr);
+            const bool mine = r < it.rows;
             tc::tmem_ld_wait();
+            float f = C::int8 ? pow2(min(ev, 127)) : 1.f;
+            float4* part = nullptr;
+            if (a.part_ml) {
+                const uint64_t at = it.slot * a.total_rows + row;
+                if (mine) a.part_ml[at] = make_float2(m, l);
+                part = reinterpret_cast<float4*>(a.part_o + at * kDh);
+            } else {
+                f = l == 0.f ? 0.f : f / l;
+                if (mine && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+            }
+            uint4* dst = reinterpret_cast<uint4*>(a.out + row * (kDh * 2));
+            // (a loop: code that runs once an item is mostly time to fetch it)
+#pragma unroll 1
+            for (uint32_t h = 0; h < 4; ++h) {
+                uint32_t v[16];
+                tc::tmem_ld_32x32b_x16(tmem + lane_base + kOCol + 16 * h, v);
+                tc::tmem_ld_wait();
+                if (!mine) continue;
+                float x[16];
+#pragma unroll
+                for (uint32_t i = 0; i < 16; ++i) x[i] = __uint_as_float(v[i]) * f;
+                if (part) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i)
+                        part[4 * h + i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+                } else {
+#pragma unroll
+                    for (uint32_t i = 0; i < 2; ++i) {
+                        const float* y = x + 8 * i;
+                        dst[2 * h + i] = a.q_bf16 ? make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]),
+                                                               pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]))
+                                                  : make_uint4(pack_f16x2(y[0], y[1]), pack_f16x2(y[2], y[3]),
+                                                               pack_f16x2(y[4], y[5]), pack_f16x2(y[6], y[7]));
+                    }
+                }
+            }
             tc::tc_fence_before();
             tc::mbar_arrive(&bars[kOFree]);
-            if (r < it.rows)
-                write_row(it, m, __uint_as_float(l_bits), C::int8 ? pow2(min(ev, 127)) : 1.f, v0, v1);
             ++n_items;
             w = next_w;
             it = next;
@@ -693,46 +704,73 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
     }
 }
 
-// Joins the parts of a row, a warp a row: with M = max m, w_s = 2^(m_s - M),
-// out = sum w_s O_s / sum w_s l_s over the slots in their order.
-__global__ void __launch_bounds__(128) kv_join_kernel(const float2* ml, const float* part, uint32_t slots,
-                                                      uint64_t rows, uint32_t queries, uint32_t heads, uint32_t bf16,
-                                                      uint8_t* out, float* lse, const uint32_t* run_rows) {
-    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * 4 + warp_id();
-    const uint32_t lane = lane_id();
-    if (row >= rows) return;
-    if (run_rows) {
-        const uint64_t live = *run_rows / queries * static_cast<uint64_t>(queries) * heads;
-        if (row >= live) return;
-    }
+// Joins the parts of a row, 8 lanes a row: with M = max m, w_s = 2^(m_s - M),
+// out = sum w_s O_s / sum w_s l_s over the slots in their order.  A lane holds the
+// weights of every 8th slot and 8 values of the row.
+constexpr uint32_t kJoinThreads = 256;
+__global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const float2* ml, const float* part, uint32_t slots,
+                                                               uint64_t rows, FastDiv queries, uint32_t heads,
+                                                               uint32_t bf16, uint8_t* out, float* lse,
+                                                               const uint32_t* run_rows) {
+    grid_wait();  // (the parts are other kernels')
+    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * (kJoinThreads / 8) + threadIdx.x / 8;
+    const uint32_t c = threadIdx.x & 7u;
+    uint64_t live = rows;
+    if (run_rows)
+        live = min(rows, static_cast<uint64_t>(queries.of(min(*run_rows, 0x7FFFFFFFu))) * queries.d * heads);
+    const bool mine = row < live;  // (lanes of other rows stay for the exchanges)
     float top = -INFINITY;
-    for (uint32_t s = lane; s < slots; s += 32) {
-        const float2 x = ml[s * rows + row];
+    for (uint32_t s = c; s < slots; s += 8) {
+        const float2 x = mine ? ml[s * rows + row] : make_float2(0.f, 0.f);
         if (x.y != 0.f) top = max_nan(top, x.x);
     }
 #pragma unroll
-    for (uint32_t o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    for (uint32_t o = 1; o < 8; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     float l = 0.f;
-    float2 sum = make_float2(0.f, 0.f);
-    for (uint32_t s = 0; s < slots; ++s) {
-        const float2 x = ml[s * rows + row];
-        if (x.y == 0.f) continue;
-        const float f = exp2f(x.x - top);
-        const float2 o = reinterpret_cast<const float2*>(part + (s * rows + row) * kDh)[lane];
-        l = __fmaf_rn(f, x.y, l);
-        sum = make_float2(__fmaf_rn(f, o.x, sum.x), __fmaf_rn(f, o.y, sum.y));
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    const float4* from = reinterpret_cast<const float4*>(part + row * kDh) + c;
+    for (uint32_t s0 = 0; s0 < slots; s0 += 8) {
+        float w = 0.f;
+        if (mine && s0 + c < slots) {
+            const float2 x = ml[(s0 + c) * rows + row];
+            w = x.y != 0.f ? ex2_approx(x.x - top) : 0.f;
+            l = __fmaf_rn(w, x.y, l);
+        }
+        // (all loads before their use: what an empty part holds is dropped, not added)
+        float4 xs[8], ys[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) {
+            xs[k] = ys[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (mine && s0 + k < slots) {
+                const float4* at = from + (s0 + k) * rows * (kDh / 4);
+                xs[k] = at[0], ys[k] = at[8];
+            }
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) {
+            const float f = __shfl_sync(0xFFFFFFFFu, w, (threadIdx.x & 24u) + k);
+            if (f == 0.f) continue;
+            const float4 x = xs[k], y = ys[k];
+            a = make_float4(__fmaf_rn(f, x.x, a.x), __fmaf_rn(f, x.y, a.y), __fmaf_rn(f, x.z, a.z), __fmaf_rn(f, x.w, a.w));
+            b = make_float4(__fmaf_rn(f, y.x, b.x), __fmaf_rn(f, y.y, b.y), __fmaf_rn(f, y.z, b.z), __fmaf_rn(f, y.w, b.w));
+        }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    reinterpret_cast<uint32_t*>(out)[row * (kDh / 2) + lane] =
-        bf16 ? pack_bf16x2(sum.x * inv, sum.y * inv) : pack_f16x2(sum.x * inv, sum.y * inv);
-    if (lse && lane == 0) lse[row] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+#pragma unroll
+    for (uint32_t o = 1; o < 8; o <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
+    if (!mine) return;
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    uint2* dst = reinterpret_cast<uint2*>(out) + row * (kDh / 4) + c;
+    dst[0] = bf16 ? make_uint2(pack_bf16x2(a.x * f, a.y * f), pack_bf16x2(a.z * f, a.w * f))
+                  : make_uint2(pack_f16x2(a.x * f, a.y * f), pack_f16x2(a.z * f, a.w * f));
+    dst[8] = bf16 ? make_uint2(pack_bf16x2(b.x * f, b.y * f), pack_bf16x2(b.z * f, b.w * f))
+                  : make_uint2(pack_f16x2(b.x * f, b.y * f), pack_f16x2(b.z * f, b.w * f));
+    if (lse && c == 0) lse[row] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
 }
 
 // ------------------------------------------------------------------ plan
 
 // Rows a sequence must have before its items walk the prefix by themselves.
 constexpr uint32_t kStackBelow = 128;
-constexpr uint32_t kMaxSplits = 64;
 
 struct Plan {
     Class cls[2];         // prefix of stacked rows, and each sequence's own keys
@@ -808,7 +846,7 @@ Plan plan_of(uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t pref
         c.with_own = i;
         const uint64_t all = static_cast<uint64_t>(c.seqs) * rows;
         const bool few = all <= kFewRows;
-        c.tile_rows = few ? (all > 16 ? 32 : (all > 8 ? 16 : 8)) : kRows;
+        c.tile_rows = few ? (all > 8 ? 16 : 8) : kRows;
         c.row_tiles = FastDiv(ceil_div(all, c.tile_rows));
         items[i] = static_cast<uint64_t>(c.groups) * kv_heads * c.row_tiles.d;
         p.few[i] = few;
@@ -817,7 +855,8 @@ Plan plan_of(uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t pref
         else
             many[i] = items[i];
     }
-    if (many[0] || many[1]) split_many(p.cls, many, tiles, 2 * sms, stacked);
+    // (beside the kernel for few rows one CTA fits an SM)
+    if (many[0] || many[1]) split_many(p.cls, many, tiles, p.few[1] ? sms : 2 * sms, stacked);
     for (int i = 0; i < 2; ++i) {
         if (!items[i]) continue;
         Class& c = p.cls[i];
@@ -876,15 +915,35 @@ bool view_maps(CUtensorMap* k, CUtensorMap* v, const dh_kv_view& s, uint32_t ent
                         s.v_strides[rows ? 2 : 3] * 2, s.v_strides[1] * 2, s.v_strides[0] * 2, kKT);
 }
 
+// Launch that may begin while the kernel before it in the stream still runs
+// (`beside`; that one lets it, and the kernel itself waits before it needs or ends).
+template <class Kernel, class... A>
+uint32_t launch_beside(Kernel kernel, uint32_t grid, uint32_t threads, uint32_t smem, bool beside, cudaStream_t st,
+                       const A&... args) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = smem;
+    config.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attr;
+    config.numAttrs = beside ? 1 : 0;
+    if (cudaLaunchKernelEx(&config, kernel, args...) != cudaSuccess) {
+        cudaGetLastError();
+        return DH_ERR_CUDA;
+    }
+    return DH_OK;
+}
+
 template <int KIND>
 uint32_t launch(const CUtensorMap (&maps)[4], const Args& a, uint32_t first, uint32_t total, cudaStream_t st) {
     static std::atomic<uint64_t> configured{0};
-    if (smem_optin_once(kv_attention_kernel<KIND>, Cfg<KIND>::bytes, configured) != cudaSuccess) return DH_ERR_CUDA;
+    if (all_shared_once(kv_attention_kernel<KIND>, Cfg<KIND>::bytes, configured) != cudaSuccess) return DH_ERR_CUDA;
     const uint32_t grid = std::min(total, 2 * device_sms());
-    kv_attention_kernel<KIND><<<grid, kThreads, Cfg<KIND>::bytes, st>>>(maps[0], maps[1], maps[2], maps[3], a, first,
-                                                                       total);
-    DH_LAUNCH_CHECK();
-    return DH_OK;
+    return launch_beside(kv_attention_kernel<KIND>, grid, kThreads, Cfg<KIND>::bytes, false, st, maps[0], maps[1],
+                         maps[2], maps[3], a, first, total);
 }
 
 }  // namespace
@@ -966,19 +1025,21 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
         if (prefixes && !view_maps(&maps[0], &maps[1], *prefix, prefixes, kv_heads)) return DH_ERR_CUDA;
     }
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    // Tensor-core tiles first: their few CTAs take long, and the others run beside them.
     uint32_t status = DH_OK, first = 0, total = 0;
-    for (uint32_t i = 0; i < 2 && !status; ++i) {
-        if (p.few[i])
-            status = launch_few(maps, a, i, p.cluster[i], int8, v_bf16, st);
-        else
-            total += a.cls[i].items, first += i ? 0 : a.cls[0].items;
-    }
-    if (total && !status)
+    for (uint32_t i = 0; i < 2; ++i)
+        if (!p.few[i]) total += a.cls[i].items, first += i ? 0 : a.cls[0].items;
+    if (total)
         status = int8 ? launch<kInt8>(maps, a, first, total, st)
                       : (v_bf16 ? launch<kVBf16>(maps, a, first, total, st) : launch<kV16>(maps, a, first, total, st));
+    bool beside = total;
+    for (uint32_t i = 0; i < 2 && !status; ++i) {
+        if (!p.few[i]) continue;
+        status = launch_few(maps, a, i, p.cluster[i], int8, v_bf16, beside, st);
+        beside = true;
+    }
     if (status || p.slots < 2) return status;
-    kv_join_kernel<<<ceil_div(rows, 4), 128, 0, st>>>(a.part_ml, a.part_o, p.slots, rows, queries, heads, a.q_bf16,
-                                                      a.out, lse, run_rows);
-    DH_LAUNCH_CHECK();
-    return DH_OK;
+    return launch_beside(kv_join_kernel, ceil_div(rows, kJoinThreads / 8), kJoinThreads, 0, true, st,
+                         static_cast<const float2*>(a.part_ml), static_cast<const float*>(a.part_o), p.slots, rows,
+                         a.queries, heads, a.q_bf16, a.out, lse, run_rows);
 }

@@ -55,6 +55,11 @@ struct Args {
     const uint32_t* run_rows;
 };
 
+// Programmatic dependent launch: the next kernel may begin; all before this one have
+// ended and their writes are seen.
+DH_DEVINL void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
+DH_DEVINL void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 DH_DEVINL float ex2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -1,8 +1,8 @@
 // kv_few.cu -- attention over K/V caches for few rows (queries times query heads of
 // a K/V head): single tokens and short blocks.  The operator is described in
-// kv_attention.cu; this kernel has the items with at most 32 rows.
+// kv_attention.cu; this kernel has the items with at most 16 rows.
 //
-// With 1 to 32 rows a key costs at most 8,192 FLOP for its 136 (int8) or 256
+// With 1 to 16 rows a key costs at most 4,096 FLOP for its 136 (int8) or 256
 // (16-bit) bytes, so the cache's bytes bound it, and the kernel is built around
 // their flow: every warp streams tiles of 64 keys of its own through two buffers
 // in shared memory (one bulk copy for each array of codes and scales, or a TMA
@@ -18,10 +18,10 @@
 // instructions for the softmax and the products.)  P^T gets from the layout of a
 // result to that of an operand by movmatrix.
 //
-// int8: scores are (q . codes) * scale of the key, the codes exact as f16, the
-// query as f16 with its exponent taken out.  The weights enter the second product
-// as f16(p * v_scale 2^-E), E an exponent that only grows (one for a warp), the
-// codes of V exact again.
+// int8: scores are (q . codes) * scale of the key, by the integer instruction on the
+// codes as they are, with the query in two int8 parts (15 bits of its row's largest
+// value).  The weights enter the second product as f16(p * v_scale 2^-E), E an
+// exponent that only grows (one for a warp), the codes of V exact as f16.
 //
 // An item's keys are shared by the four warps of a CTA and the CTAs of a cluster, which
 // join their sums through shared memory in a fixed order.  Where there are items
@@ -30,6 +30,7 @@
 #include <cuda.h>
 
 #include "kv_few.h"
+#include "row_quant.cuh"
 
 #include <algorithm>
 
@@ -40,6 +41,7 @@ namespace {
 constexpr uint32_t kWarps = 4;
 constexpr uint32_t kThreads = 32 * kWarps;
 constexpr uint32_t kStages = 2;
+constexpr int32_t kShift = 0x4B400000;  // 1.5 * 2^23 as fp32
 constexpr float kNoMax = -3.0e38f;  // below every maximum, and finite
 
 enum Kind : int { kV16 = 0, kVBf16 = 1, kInt8 = 2 };
@@ -61,6 +63,14 @@ DH_DEVINL void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uin
                      "{%0, %1, %2, %3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// int8, 32 deep
+DH_DEVINL void mma_16832(int32_t (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 DH_DEVINL void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -129,7 +139,7 @@ DH_DEVINL uint32_t key_of(uint32_t n) { return n ^ ((n >> 1) & 1u); }
 
 // NT: groups of 8 rows.
 template <int KIND, bool QBF16, int NT>
-__global__ void __launch_bounds__(kThreads, NT < 4 ? 3 : 2)
+__global__ void __launch_bounds__(kThreads, 3)
 kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ CUtensorMap tpv,
               const __grid_constant__ CUtensorMap tok, const __grid_constant__ CUtensorMap tov,
               const __grid_constant__ Args a, const uint32_t cls, const uint32_t cluster) {
@@ -142,6 +152,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
     uint64_t* all_bars = reinterpret_cast<uint64_t*>(smem + kWarps * kStages * kStageBytes<KIND>);
     const uint32_t warp = warp_id(), lane = lane_id(), g = lane >> 2, c = lane & 3u;
     const Class& cl = a.cls[cls];
+    grid_launch_dependents();
     const bool solo = cluster == 0;
     const uint32_t rank = cluster > 1 ? cluster_rank() : 0u;
 
@@ -182,25 +193,28 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
             ahead_j = ahead.t0;
         }
         if (ahead_w >= cl.items) return;
-        if (lane == 0) {
-            const bool own = ahead_j >= ahead.n0;
-            const uint32_t key = (own ? ahead_j - ahead.n0 : ahead_j) * kKT;
-            const uint32_t entry = own ? ahead.own : ahead.prefix;
-            uint8_t* dst = ring + st * kStageBytes<KIND>;
-            uint64_t* bar = &bars[st];
-            tc::mbar_arrive_expect_tx(bar, kStageBytes<KIND>);
-            if constexpr (kI8) {
+        const bool own = ahead_j >= ahead.n0;
+        const uint32_t key = (own ? ahead_j - ahead.n0 : ahead_j) * kKT;
+        const uint32_t entry = own ? ahead.own : ahead.prefix;
+        uint8_t* dst = ring + st * kStageBytes<KIND>;
+        uint64_t* bar = &bars[st];
+        if (lane == 0) tc::mbar_arrive_expect_tx(bar, kStageBytes<KIND>);
+        __syncwarp();
+        // a lane a copy, in one instruction
+        if constexpr (kI8) {
+            if (lane < 4) {
                 const Segment& s = own ? a.own : a.prefix;
                 const uint64_t at = (static_cast<uint64_t>(entry) * a.kv_heads.d + ahead.kv_head) * s.capacity + key;
-                tc::bulk_load(dst, s.k + at * kDh, kKT * kDh, bar);
-                tc::bulk_load(dst + 2 * kKT * kDh, s.k_scale + at, kKT * 4, bar);
-                tc::bulk_load(dst + kKT * kDh, s.v + at * kDh, kKT * kDh, bar);
-                tc::bulk_load(dst + 2 * kKT * kDh + kKT * 4, s.v_scale + at, kKT * 4, bar);
-            } else {
-                tc::tma_load_4d(dst, own ? &tok : &tpk, bar, 0, key, ahead.kv_head, entry);
-                tc::tma_load_4d(dst + kTileBytes, own ? &tov : &tpv, bar, a.v_transposed ? key : 0,
-                                a.v_transposed ? 0 : key, ahead.kv_head, entry);
+                const bool is_v = lane & 1u, is_scale = lane & 2u;
+                const void* codes = (is_v ? s.v : s.k) + at * kDh;
+                const void* scales = (is_v ? s.v_scale : s.k_scale) + at;
+                tc::bulk_load(dst + (is_scale ? 2 * kKT * kDh : 0) + (is_v ? (is_scale ? kKT * 4 : kKT * kDh) : 0),
+                              is_scale ? scales : codes, is_scale ? kKT * 4 : kKT * kDh, bar);
             }
+        } else if (lane < 2) {
+            const bool turned = lane && a.v_transposed;
+            const CUtensorMap* map = lane ? (own ? &tov : &tpv) : (own ? &tok : &tpk);
+            tc::tma_load_4d(dst + lane * kTileBytes, map, bar, turned ? key : 0, turned ? 0 : key, ahead.kv_head, entry);
         }
         ++issued;
         ahead_j += step;
@@ -245,14 +259,23 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
             }
             peak = max(peak, __shfl_xor_sync(0xFFFFFFFFu, peak, 1));
             peak = max(peak, __shfl_xor_sync(0xFFFFFFFFu, peak, 2));
-            const int32_t e = min(max(exponent_of(peak), -100), 126);
-            const float by = pow2(-e), factor = fmaxf(a.c * pow2(e), kLeastFactor);
+            // a value is (128 hi + lo) amax / 16256, hi and lo int8
+            const bool live = peak >= 0x0D800000u;  // 2^-100
+            const float amax = __uint_as_float(peak);
+            const float by = live ? __fdiv_rn(16256.0f, amax) : 0.f;
+            const float factor = peak >= 0x7F800000u ? __uint_as_float(0x7FC00000u)
+                                                     : fmaxf(a.c * (live ? amax * (1.0f / 16256.0f) : 0.f), kLeastFactor);
             cr[t][0] = __shfl_sync(0xFFFFFFFFu, factor, 8 * c);
             cr[t][1] = __shfl_sync(0xFFFFFFFFu, factor, 8 * c + 4);
 #pragma unroll
-            for (uint32_t s = 0; s < 4; ++s) {
-                qb[t][s][0] = pack_f16x2(f[2 * s].x * by, f[2 * s].y * by);
-                qb[t][s][1] = pack_f16x2(f[2 * s + 1].x * by, f[2 * s + 1].y * by);
+            for (uint32_t k = 0; k < 4; ++k) {  // four values
+                int32_t v[4], hi[4];
+                v[0] = __float2int_rn(f[2 * k].x * by), v[1] = __float2int_rn(f[2 * k].y * by);
+                v[2] = __float2int_rn(f[2 * k + 1].x * by), v[3] = __float2int_rn(f[2 * k + 1].y * by);
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) hi[i] = (v[i] + 64) >> 7, v[i] -= hi[i] * 128;
+                qb[t][k][0] = pack4_i8(hi[0], hi[1], hi[2], hi[3]);
+                qb[t][k][1] = pack4_i8(v[0], v[1], v[2], v[3]);
             }
         } else {
             cr[t][0] = cr[t][1] = a.c;
@@ -289,18 +312,27 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
                 const uint8_t* row = tile + (16 * i + key_of(g)) * kDh + 16 * c;
                 const uint4 w0 = *reinterpret_cast<const uint4*>(row);
                 const uint4 w1 = *reinterpret_cast<const uint4*>(row + 8 * kDh);
-                const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-                for (uint32_t k = 0; k < 4; ++k) {
-                    const uint32_t u0 = x0[k] ^ 0x80808080u, u1 = x1[k] ^ 0x80808080u;
-                    const uint32_t ka[4] = {codes_f16<false>(u0), codes_f16<false>(u1), codes_f16<true>(u0),
-                                            codes_f16<true>(u1)};
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) mma_16816<false>(s[t][i], ka, qb[t][k][0], qb[t][k][1]);
-                }
+                const uint32_t ka[2][4] = {{w0.x, w1.x, w0.y, w1.y}, {w0.z, w1.z, w0.w, w1.w}};
                 const float k0 = scales[16 * i + key_of(g)], k1 = scales[16 * i + 8 + key_of(g)];
 #pragma unroll
-                for (int t = 0; t < NT; ++t) s[t][i][0] *= k0, s[t][i][1] *= k0, s[t][i][2] *= k1, s[t][i][3] *= k1;
+                for (int t = 0; t < NT; ++t) {
+                    // integers below 2^22 on top of 1.5 2^23: the sums' bits are floats
+                    int32_t hi[4] = {kShift, kShift, kShift, kShift}, lo[4] = {kShift, kShift, kShift, kShift};
+#pragma unroll
+                    for (uint32_t k = 0; k < 2; ++k) {
+                        mma_16832(hi, ka[k], qb[t][2 * k][0], qb[t][2 * k + 1][0]);
+                        mma_16832(lo, ka[k], qb[t][2 * k][1], qb[t][2 * k + 1][1]);
+                    }
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; ++h) {
+                        const float2 m2 = make_float2(-__int_as_float(kShift), -__int_as_float(kShift));
+                        const float2 a2 = __fadd2_rn(make_float2(__int_as_float(hi[2 * h]), __int_as_float(hi[2 * h + 1])), m2);
+                        const float2 b2 = __fadd2_rn(make_float2(__int_as_float(lo[2 * h]), __int_as_float(lo[2 * h + 1])), m2);
+                        const float ks = h ? k1 : k0;
+                        const float2 x = __fmul2_rn(__ffma2_rn(a2, make_float2(128.f, 128.f), b2), make_float2(ks, ks));
+                        s[t][i][2 * h] = x.x, s[t][i][2 * h + 1] = x.y;
+                    }
+                }
             } else {
                 const uint32_t key = 16 * i + ((lane >> 3) & 1u) * 8 + (lane & 7u);
                 const uint32_t row = smem_u32(tile) + key * 128;
@@ -316,17 +348,22 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
         float vs[4][2];  // v_scale 2^-E of this thread's keys
         float fe = 1.f;
         if constexpr (kI8) {
-            uint32_t peak = 0;
+            float peak = 0.f;  // (of the numbers among them)
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i)
 #pragma unroll
-                for (uint32_t h = 0; h < 2; ++h) {
-                    const uint32_t key = 16 * i + 8 * h + key_of(g);
-                    vs[i][h] = key < left ? scales[kKT + key] : 0.f;
-                    const uint32_t bits = __float_as_uint(vs[i][h]) & 0x7FFFFFFFu;
-                    if (bits < 0x7F800000u) peak = max(peak, bits);
-                }
-            const int32_t et = max(ev, min(exponent_of(__reduce_max_sync(0xFFFFFFFFu, peak)), 126));
+                for (uint32_t h = 0; h < 2; ++h) vs[i][h] = scales[kKT + 16 * i + 8 * h + key_of(g)];
+            if (left < kKT) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i)
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; ++h)
+                        if (16 * i + 8 * h + key_of(g) >= left) vs[i][h] = 0.f;
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) peak = fmaxf(peak, fmaxf(fabsf(vs[i][0]), fabsf(vs[i][1])));
+            const int32_t et =
+                max(ev, min(exponent_of(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(peak))), 126));
             const float by = pow2(-et);
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) vs[i][0] *= by, vs[i][1] *= by;
@@ -361,6 +398,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
         // weights, in place
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
+            float next[2], alpha[2];
 #pragma unroll
             for (uint32_t e = 0; e < 2; ++e) {
                 float top = max_nan(max_nan(s[t][0][e], s[t][0][e + 2], s[t][1][e]), s[t][1][e + 2],
@@ -369,23 +407,33 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
                 top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
                 top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
                 // finite, or NaN for a score that is infinite or NaN: the row is NaN
-                float next = max_nan(max_nan(top * cr[t][e], kNoMax), m[t][e]);
-                next = __fmaf_rn(next, -0.f, next);
-                const float alpha = ex2_approx(m[t][e] - next), ao = alpha * fe;
-                m[t][e] = next;
-                float sum = 0.f;
+                next[e] = max_nan(max_nan(top * cr[t][e], kNoMax), m[t][e]);
+                next[e] = __fmaf_rn(next[e], -0.f, next[e]);
+                alpha[e] = ex2_approx(m[t][e] - next[e]);
+                m[t][e] = next[e];
+                l[t][e] *= alpha[e];
+                alpha[e] *= fe;
+            }
+            const float2 cr2 = make_float2(cr[t][0], cr[t][1]), nm2 = make_float2(-next[0], -next[1]);
+            float2 sum = make_float2(l[t][0], l[t][1]);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    const float2 x = __ffma2_rn(make_float2(s[t][i][2 * h], s[t][i][2 * h + 1]), cr2, nm2);
+                    float2 p = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                    sum = __fadd2_rn(sum, p);
+                    if constexpr (kI8) p = __fmul2_rn(p, make_float2(vs[i][h], vs[i][h]));
+                    s[t][i][2 * h] = p.x, s[t][i][2 * h + 1] = p.y;
+                }
+            }
+            l[t][0] = sum.x, l[t][1] = sum.y;
+            if (__any_sync(0xFFFFFFFFu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) {
-#pragma unroll
-                    for (uint32_t h = 0; h < 2; ++h) {
-                        float& x = s[t][i][2 * h + e];
-                        x = ex2_approx(__fmaf_rn(x, cr[t][e], -next));
-                        sum += x;
-                        if constexpr (kI8) x *= vs[i][h];
-                    }
-                    o[t][i][e] *= ao, o[t][i][e + 2] *= ao;
+                    o[t][i][0] *= alpha[0], o[t][i][2] *= alpha[0];
+                    o[t][i][1] *= alpha[1], o[t][i][3] *= alpha[1];
                 }
-                l[t][e] = __fmaf_rn(l[t][e], alpha, sum);
             }
         }
         // O^T += V^T P^T, 16 keys at a time
@@ -591,13 +639,15 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
     }
     cluster_sync();  // (no CTA leaves while its sums are read)
     }
+    grid_wait();  // (what waits for this kernel waits for one that it may run beside, too)
 }
 
 template <int KIND, bool QBF16, int NT>
-uint32_t launch(const CUtensorMap (&maps)[4], const Args& a, uint32_t cls, uint32_t cluster, cudaStream_t st) {
+uint32_t launch(const CUtensorMap (&maps)[4], const Args& a, uint32_t cls, uint32_t cluster, bool beside,
+                cudaStream_t st) {
     const auto kernel = kv_few_kernel<KIND, QBF16, NT>;
     static std::atomic<uint64_t> configured{0};
-    if (smem_optin_once(kernel, kSmem<KIND>, configured) != cudaSuccess) return DH_ERR_CUDA;
+    if (all_shared_once(kernel, kSmem<KIND>, configured) != cudaSuccess) return DH_ERR_CUDA;
     cudaLaunchConfig_t config{};
     // solo: as many CTAs as fit, their warps walk the items
     const uint32_t fit = device_sms() * (227u * 1024u / (kSmem<KIND> + 1024u));
@@ -606,11 +656,18 @@ uint32_t launch(const CUtensorMap (&maps)[4], const Args& a, uint32_t cls, uint3
     config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = kSmem<KIND>;
     config.stream = st;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = cluster, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
-    config.attrs = &attr;
-    config.numAttrs = cluster > 1 ? 1 : 0;
+    cudaLaunchAttribute attrs[2] = {};
+    config.attrs = attrs;
+    if (cluster > 1) {
+        attrs[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attrs[config.numAttrs].val.clusterDim.x = cluster;
+        attrs[config.numAttrs].val.clusterDim.y = attrs[config.numAttrs].val.clusterDim.z = 1;
+        ++config.numAttrs;
+    }
+    if (beside) {
+        attrs[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attrs[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
     if (cudaLaunchKernelEx(&config, kernel, maps[0], maps[1], maps[2], maps[3], a, cls, cluster) != cudaSuccess) {
         cudaGetLastError();
         return DH_ERR_CUDA;
@@ -619,25 +676,25 @@ uint32_t launch(const CUtensorMap (&maps)[4], const Args& a, uint32_t cls, uint3
 }
 
 template <int KIND, bool QBF16>
-uint32_t launch_rows(const CUtensorMap (&maps)[4], const Args& a, uint32_t cls, uint32_t cluster, cudaStream_t st) {
-    const uint32_t rows = a.cls[cls].tile_rows;
-    return rows <= 8 ? launch<KIND, QBF16, 1>(maps, a, cls, cluster, st)
-                     : (rows <= 16 ? launch<KIND, QBF16, 2>(maps, a, cls, cluster, st)
-                                   : launch<KIND, QBF16, 4>(maps, a, cls, cluster, st));
+uint32_t launch_rows(const CUtensorMap (&maps)[4], const Args& a, uint32_t cls, uint32_t cluster, bool beside,
+                cudaStream_t st) {
+    return a.cls[cls].tile_rows <= 8 ? launch<KIND, QBF16, 1>(maps, a, cls, cluster, beside, st)
+                                     : launch<KIND, QBF16, 2>(maps, a, cls, cluster, beside, st);
 }
 
 template <int KIND>
-uint32_t launch_type(const CUtensorMap (&maps)[4], const Args& a, uint32_t cls, uint32_t cluster, cudaStream_t st) {
-    return a.q_bf16 ? launch_rows<KIND, true>(maps, a, cls, cluster, st)
-                    : launch_rows<KIND, false>(maps, a, cls, cluster, st);
+uint32_t launch_type(const CUtensorMap (&maps)[4], const Args& a, uint32_t cls, uint32_t cluster, bool beside,
+                cudaStream_t st) {
+    return a.q_bf16 ? launch_rows<KIND, true>(maps, a, cls, cluster, beside, st)
+                    : launch_rows<KIND, false>(maps, a, cls, cluster, beside, st);
 }
 
 }  // namespace
 
 uint32_t launch_few(const CUtensorMap (&maps)[4], const Args& a, uint32_t cls, uint32_t cluster, bool int8, bool v_bf16,
-                    cudaStream_t st) {
-    return int8 ? launch_type<kInt8>(maps, a, cls, cluster, st)
-                : (v_bf16 ? launch_type<kVBf16>(maps, a, cls, cluster, st) : launch_type<kV16>(maps, a, cls, cluster, st));
+                    bool beside, cudaStream_t st) {
+    return int8 ? launch_type<kInt8>(maps, a, cls, cluster, beside, st)
+                : (v_bf16 ? launch_type<kVBf16>(maps, a, cls, cluster, beside, st) : launch_type<kV16>(maps, a, cls, cluster, beside, st));
 }
 
 }  // namespace kv

@@ -8,13 +8,25 @@
 namespace dh {
 namespace kv {
 
-constexpr uint32_t kFewRows = 32;     // rows of an item at most
+constexpr uint32_t kFewRows = 16;     // rows of an item at most
 constexpr uint32_t kMaxCluster = 8;   // CTAs that share an item's keys
 
+// smem_optin_once, with an SM's whole carve-out as shared memory: two kernels that
+// run beside each other on an SM need the same one.
+template <class Kernel>
+inline cudaError_t all_shared_once(Kernel kernel, uint32_t bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64 && (done.load(std::memory_order_acquire) >> dev & 1u)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    return e == cudaSuccess ? smem_optin_once(kernel, bytes, done) : e;
+}
+
 // Class `cls` of a's items on clusters of `cluster` CTAs (0: a warp an item).  maps: prefix K, V, own K,
-// V (16 bits).
+// V (16 bits).  beside: may begin while the kernel before it in the stream runs.
 uint32_t launch_few(const CUtensorMap (&maps)[4], const Args& a, uint32_t cls, uint32_t cluster, bool int8, bool v_bf16,
-                    cudaStream_t st);
+                    bool beside, cudaStream_t st);
 
 }  // namespace kv
 }  // namespace dh
