@@ -19,20 +19,19 @@ are not, but are kept inside the cache.  Results carry no gradients, and an
 
 from __future__ import annotations
 
-import ctypes
 import functools
 import math
+import struct
 from typing import Any, NamedTuple, Optional, Tuple, Union
 
 import torch
 
 from . import _lib
-from .scoring import _call, _cuda, _ptr, _TYPES
+from .scoring import _TYPES, _current_device, _ptr, _raw_stream
 
 HEAD_DIM = 64
 CAPACITY_STEP = 64
 _TYPE_I8 = 3
-_U64x4 = ctypes.c_uint64 * 4
 
 Lengths = Union[int, torch.Tensor, None]
 
@@ -68,29 +67,42 @@ class KVCacheI8(NamedTuple):
         return n * h * (c if positions is None else positions) * 2 * (d + 4)
 
 
-def _check_cache(name: str, c: KVCacheI8, device: Optional[torch.device] = None) -> KVCacheI8:
-    k = _cuda(name, c.k, device)
+# Calls take a few microseconds of the host and the smallest of them little more of
+# the GPU: a call that is as it should be passes few checks, and what it passes to C
+# is packed in one go.
+_pack4 = struct.Struct("=4Q").pack
+_pack_view = struct.Struct("=5Q8Q4I").pack  # dh_kv_view of include/dh_b200.h
+
+
+def _check_cache(name: str, c: KVCacheI8, index: int) -> tuple:
+    """Shape of the codes of a cache that is all on GPU `index` (-1: the host)."""
+    k, k_scale, v, v_scale = c
     shape = k.shape
+    if index < 0 or not (k.get_device() == v.get_device() == k_scale.get_device() == v_scale.get_device() == index):
+        if k.is_cuda:
+            raise ValueError(f"all of {name} and the other tensors must be on one device")
+        raise ValueError(f"{name} must hold CUDA tensors")
     if len(shape) != 4 or shape[3] != HEAD_DIM or shape[2] == 0 or shape[2] % CAPACITY_STEP:
         raise ValueError(f"{name} must hold int8 codes [entries, heads, capacity, 64], its capacity a multiple of 64")
-    if c.v.shape != shape or c.k_scale.shape != shape[:3] or c.v_scale.shape != shape[:3]:
+    if not (v.shape == shape and k_scale.shape == v_scale.shape == shape[:3]):
         raise ValueError(f"the codes and scales of {name} must have one shape")
-    f32 = torch.float32
-    if not (k.dtype is c.v.dtype is torch.int8) or not (c.k_scale.dtype is c.v_scale.dtype is f32):
+    if not (k.dtype is v.dtype is torch.int8 and k_scale.dtype is v_scale.dtype is torch.float32):
         raise ValueError(f"{name} must hold int8 codes and float32 scales")
-    dev = k.device
-    for t in c:
-        if t.device != dev:
-            raise ValueError(f"all of {name} must be on {dev}")
-        if not t.is_contiguous():
-            raise ValueError(f"the tensors of {name} must be contiguous")
-        if t.data_ptr() & 15:
-            raise ValueError(f"the tensors of {name} must start at 16-byte boundaries")
-    return c
+    if not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
+        raise ValueError(f"the tensors of {name} must be contiguous")
+    if (k.data_ptr() | v.data_ptr() | k_scale.data_ptr() | v_scale.data_ptr()) & 15:
+        raise ValueError(f"the tensors of {name} must start at 16-byte boundaries")
+    return shape
 
 
-def _ints(name: str, t: torch.Tensor, n: int, device: torch.device) -> torch.Tensor:
-    _cuda(name, t, device)
+def _on(name: str, t: torch.Tensor, index: int) -> torch.Tensor:
+    if t.get_device() != index:
+        raise ValueError(f"{name} must be a CUDA tensor on the device of the others")
+    return t
+
+
+def _ints(name: str, t: torch.Tensor, n: int, index: int) -> torch.Tensor:
+    _on(name, t, index)
     if t.dtype is not torch.int32 or t.shape != (n,):
         raise ValueError(f"{name} must be an int32 vector of {n}")
     return t if t.is_contiguous() else t.contiguous()
@@ -98,16 +110,29 @@ def _ints(name: str, t: torch.Tensor, n: int, device: torch.device) -> torch.Ten
 
 def _strides(t: torch.Tensor) -> Tuple[int, ...]:
     """Element strides; 64 where a dimension holds one element and any will do."""
-    return tuple(s if n > 1 else HEAD_DIM for s, n in zip(t.stride()[:3], t.shape)) + (t.stride(3),)
+    a, b, c, d = t.stride()
+    n, h, rows, _ = t.shape
+    return (a if n > 1 else HEAD_DIM, b if h > 1 else HEAD_DIM, c if rows > 1 else HEAD_DIM, d)
 
 
-def _run_rows(run_rows: Optional[torch.Tensor], device: torch.device) -> Optional[int]:
+def _run_rows(run_rows: Optional[torch.Tensor], index: int) -> Optional[int]:
     if run_rows is None:
         return None
-    _cuda("run_rows", run_rows, device)
+    _on("run_rows", run_rows, index)
     if run_rows.dtype not in (torch.int32, torch.uint32) or run_rows.numel() != 1:
         raise ValueError("run_rows must be one int32 word")
     return run_rows.data_ptr()
+
+
+def _call_on(name: str, index: int, *args: Any) -> None:
+    """An entry point on the current stream of GPU `index`, its last argument."""
+    if _current_device() == index:
+        status = getattr(_lib.lib(), name)(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = getattr(_lib.lib(), name)(*args, _raw_stream(index))
+    if status:
+        raise _lib.DHStatusError(name, int(status))
 
 
 def write_kv(cache: KVCacheI8, k: torch.Tensor, v: torch.Tensor, start: Union[int, torch.Tensor] = 0,
@@ -122,30 +147,33 @@ def write_kv(cache: KVCacheI8, k: torch.Tensor, v: torch.Tensor, start: Union[in
     which must fit behind an int ``start``).  Positions that lie outside the
     cache by a device ``start`` are not written, and all others stay as they
     were.  The scale of a row is its largest magnitude / 127; a row below 2^-100
-    counts as zero, one with an infinity or NaN gets the scale NaN."""
-    _check_cache("cache", cache)
-    dev = cache.k.device
-    entries, heads, capacity, _ = cache.k.shape
-    if k.dim() != 4 or k.shape[0] != entries or k.shape[1] != heads or k.shape[3] != HEAD_DIM or v.shape != k.shape:
+    counts as zero, one with an infinity or NaN gets the scale NaN.
+    ``run_rows``: one device word, only the sequences within its first rows of
+    [entries * n] are written."""
+    index = cache.k.get_device()
+    shape = _check_cache("cache", cache, index)
+    entries, heads, capacity, _ = shape
+    rows = k.shape[2] if k.dim() == 4 else -1
+    if k.shape != (entries, heads, rows, HEAD_DIM) or v.shape != k.shape:
         raise ValueError(f"k and v must be [{entries}, {heads}, n, {HEAD_DIM}]")
-    _cuda("k", k, dev)
-    _cuda("v", v, dev)
-    if k.dtype not in _TYPES or v.dtype not in _TYPES:
+    k_type, v_type = _TYPES.get(k.dtype), _TYPES.get(v.dtype)
+    if k_type is None or v_type is None:
         raise ValueError("k and v must be float32, bfloat16 or float16")
-    rows = k.shape[2]
+    if not k.get_device() == v.get_device() == index:
+        raise ValueError("k and v must be CUDA tensors on the device of the cache")
     starts = None
     if isinstance(start, torch.Tensor):
-        starts, start = _ints("start", start, entries, dev), 0
+        starts, start = _ints("start", start, entries, index), 0
     elif start < 0 or start > capacity or (counts is None and start + rows > capacity):
         raise ValueError(f"{rows} rows from {start} on do not fit the capacity of {capacity}")
     if counts is not None:
-        counts = _ints("counts", counts, entries, dev)
-    run = _run_rows(run_rows, dev)
+        counts = _ints("counts", counts, entries, index)
+    run = _run_rows(run_rows, index)
     if rows == 0 or entries == 0 or heads == 0:
         return
-    _call("dh_kv_write_i8", dev, k.data_ptr(), _TYPES[k.dtype], _U64x4(*k.stride()), v.data_ptr(), _TYPES[v.dtype],
-          _U64x4(*v.stride()), entries, heads, rows, _ptr(starts), start, _ptr(counts), cache.k.data_ptr(),
-          cache.k_scale.data_ptr(), cache.v.data_ptr(), cache.v_scale.data_ptr(), capacity, run)
+    _call_on("dh_kv_write_i8", index, k.data_ptr(), k_type, _pack4(*k.stride()), v.data_ptr(), v_type,
+             _pack4(*v.stride()), entries, heads, rows, _ptr(starts), start, _ptr(counts), cache.k.data_ptr(),
+             cache.k_scale.data_ptr(), cache.v.data_ptr(), cache.v_scale.data_ptr(), capacity, run)
 
 
 def read_kv(cache: KVCacheI8, start: int = 0, rows: Optional[int] = None, *,
@@ -153,51 +181,47 @@ def read_kv(cache: KVCacheI8, start: int = 0, rows: Optional[int] = None, *,
     """K and V [entries, heads, rows, 64] of positions [start, start + rows)
     (default: to the end of the capacity) of every entry: codes * scales, rounded
     to `dtype` (fp32, bf16 or f16; dh_kv_read_i8)."""
-    _check_cache("cache", cache)
-    entries, heads, capacity, _ = cache.k.shape
+    index = cache.k.get_device()
+    entries, heads, capacity, _ = _check_cache("cache", cache, index)
     rows = capacity - start if rows is None else rows
     if start < 0 or rows < 0 or start + rows > capacity:
         raise ValueError(f"positions [{start}, {start + rows}) lie outside the capacity of {capacity}")
-    if dtype not in _TYPES:
+    out_type = _TYPES.get(dtype)
+    if out_type is None:
         raise ValueError("dtype must be float32, bfloat16 or float16")
-    dev = cache.k.device
-    k = torch.empty((entries, heads, rows, HEAD_DIM), dtype=dtype, device=dev)
+    k = cache.k.new_empty((entries, heads, rows, HEAD_DIM), dtype=dtype)
     v = torch.empty_like(k)
-    if k.numel():
-        _call("dh_kv_read_i8", dev, cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(),
-              cache.v_scale.data_ptr(), entries, heads, capacity, start, rows, k.data_ptr(), v.data_ptr(),
-              _TYPES[dtype])
+    if rows and entries and heads:
+        _call_on("dh_kv_read_i8", index, cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(),
+                 cache.v_scale.data_ptr(), entries, heads, capacity, start, rows, k.data_ptr(), v.data_ptr(), out_type)
     return k, v
 
 
-class _View(ctypes.Structure):
-    """dh_kv_view of include/dh_b200.h."""
-
-    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
-                ("v_scale", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("k_strides", _U64x4),
-                ("v_strides", _U64x4), ("k_type", ctypes.c_uint32), ("v_type", ctypes.c_uint32),
-                ("capacity", ctypes.c_uint32), ("length", ctypes.c_uint32)]
-
-
-_NO_STRIDES = _U64x4()
+class _Keys(NamedTuple):
+    view: bytes          # dh_kv_view
+    entries: int
+    heads: int
+    capacity: int
+    v_type: int          # with `turned`: what a prefix must have alike
+    turned: bool         # V's columns are contiguous
+    held: Any            # a tensor the view points into
 
 
-def _view(name: str, kv: Any, lengths: Lengths, q: torch.Tensor) -> tuple:
-    """(dh_kv_view, entries, heads, tensors it points into)."""
-    dev = q.device
+def _view(name: str, kv: Any, lengths: Lengths, q: torch.Tensor, index: int) -> _Keys:
+    turned = False
     if isinstance(kv, KVCacheI8):
-        _check_cache(name, kv, dev)
-        entries, heads, capacity, _ = kv.k.shape
+        k, k_scale, v, v_scale = kv
+        entries, heads, capacity, _ = _check_cache(name, kv, index)
         kt = vt = _TYPE_I8
-        ks = vs = _NO_STRIDES
-        k, v, k_scale, v_scale = kv.k, kv.v, kv.k_scale.data_ptr(), kv.v_scale.data_ptr()
+        ks = vs = (0, 0, 0, 0)
+        pointers = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
     else:
         k, v = kv
-        _cuda(name, k, dev)
-        _cuda(name, v, dev)
+        if not k.get_device() == v.get_device() == index:
+            raise ValueError(f"{name} must be CUDA tensors on the device of the others")
         if k.dim() != 4 or k.shape[3] != HEAD_DIM or v.shape != k.shape or k.shape[2] == 0:
             raise ValueError(f"k and v of {name} must be [entries, heads, n, {HEAD_DIM}] with n > 0")
-        if k.dtype is not q.dtype or v.dtype not in (torch.bfloat16, torch.float16):
+        if k.dtype is not q.dtype or (v.dtype is not torch.bfloat16 and v.dtype is not torch.float16):
             raise ValueError(f"k of {name} must be of q's type, v bfloat16 or float16")
         entries, heads, capacity, _ = k.shape
         kt, vt = _TYPES[k.dtype], _TYPES[v.dtype]
@@ -205,26 +229,28 @@ def _view(name: str, kv: Any, lengths: Lengths, q: torch.Tensor) -> tuple:
         if vs[3] == 1:
             aligned = vs[0] | vs[1] | vs[2]
         elif capacity == 1 or vs[2] == 1:  # its columns are contiguous
+            turned = True
             vs = (vs[0], vs[1], 1, vs[3])
             aligned = vs[0] | vs[1] | vs[3]
         else:
             raise ValueError(f"v of {name} must have contiguous rows or contiguous columns")
         if ks[3] != 1:
             raise ValueError(f"k of {name} must have contiguous rows")
-        if (aligned | ks[0] | ks[1] | ks[2]) % 8 or (k.data_ptr() | v.data_ptr()) & 15:
+        pointers = (k.data_ptr(), v.data_ptr(), 0, 0)
+        if (aligned | ks[0] | ks[1] | ks[2]) % 8 or (pointers[0] | pointers[1]) & 15:
             raise ValueError(f"k and v of {name} must start at 16-byte boundaries, as must their rows and heads")
-        ks, vs = _U64x4(*ks), _U64x4(*vs)
-        k_scale = v_scale = None
     held = None
     length = capacity
-    if isinstance(lengths, torch.Tensor):
-        held = _ints(f"lengths of {name}", lengths, entries, dev)
-    elif lengths is not None:
+    if lengths is None:
+        pass
+    elif isinstance(lengths, torch.Tensor):
+        held = _ints(f"lengths of {name}", lengths, entries, index)
+    else:
         length = int(lengths)
         if not 0 <= length <= capacity:
             raise ValueError(f"{length} keys of {name} do not lie within its capacity of {capacity}")
-    view = _View(k.data_ptr(), v.data_ptr(), k_scale, v_scale, _ptr(held), ks, vs, kt, vt, capacity, length)
-    return view, entries, heads, held
+    view = _pack_view(*pointers, 0 if held is None else held.data_ptr(), *ks, *vs, kt, vt, capacity, length)
+    return _Keys(view, entries, heads, capacity, vt, turned, held)
 
 
 def attend(q: torch.Tensor, kv: Any, lengths: Lengths = None, *, prefix: Any = None, prefix_lengths: Lengths = None,
@@ -257,56 +283,56 @@ def attend(q: torch.Tensor, kv: Any, lengths: Lengths = None, *, prefix: Any = N
 
     Calls that split the keys take up to 264 bytes of workspace for each query,
     head and part."""
-    _cuda("q", q)
-    if q.dim() != 4 or q.shape[3] != HEAD_DIM or q.dtype not in (torch.bfloat16, torch.float16):
+    index = q.get_device()
+    q_type = _TYPES.get(q.dtype)
+    if index < 0:
+        raise ValueError("q must be a CUDA tensor")
+    if q.dim() != 4 or q.shape[3] != HEAD_DIM or not q_type:
         raise ValueError(f"q must be [batch, heads, n, {HEAD_DIM}] of bfloat16 or float16")
-    dev = q.device
     batch, heads, n, _ = q.shape
     qs = _strides(q)
     if qs[3] != 1 or (qs[0] | qs[1] | qs[2]) % 8 or q.data_ptr() & 15:
         q = q.contiguous()
-        qs = q.stride()
-    view, entries, kv_heads, _own = _view("kv", kv, lengths, q)
-    if entries != batch:
-        raise ValueError(f"kv has {entries} entries for {batch} sequences")
+        qs = _strides(q)
+    keys = _view("kv", kv, lengths, q, index)
+    kv_heads = keys.heads
+    if keys.entries != batch:
+        raise ValueError(f"kv has {keys.entries} entries for {batch} sequences")
     if kv_heads == 0 or heads % kv_heads:
         raise ValueError(f"{heads} query heads are no multiple of {kv_heads} K/V heads")
-    prefixes, prefix_capacity, pview, _pre = 0, 0, None, None
+    prefixes, prefix_capacity, prefix_view = 0, 0, None
     if prefix is not None:
         if isinstance(prefix, KVCacheI8) != isinstance(kv, KVCacheI8):
             raise ValueError("prefix must be of the same kind as kv")
-        pview, prefixes, prefix_heads, _pre = _view("prefix", prefix, prefix_lengths, q)
-        if prefix_heads != kv_heads:
-            raise ValueError(f"prefix has {prefix_heads} heads and kv {kv_heads}")
+        before = _view("prefix", prefix, prefix_lengths, q, index)
+        prefixes = before.entries
+        if before.heads != kv_heads:
+            raise ValueError(f"prefix has {before.heads} heads and kv {kv_heads}")
         if prefixes == 0 or batch % prefixes:
             raise ValueError(f"{prefixes} prefixes do not divide {batch} sequences")
-        if pview.v_type != view.v_type or (pview.k_type != _TYPE_I8
-                                           and (pview.v_strides[3] == 1) != (view.v_strides[3] == 1)):
+        if before.v_type != keys.v_type or before.turned != keys.turned:
             raise ValueError("v of prefix must have the type and layout of v of kv")
-        prefix_capacity = pview.capacity
+        prefix_capacity, prefix_view = before.capacity, before.view
     elif prefix_lengths is not None:
         raise ValueError("prefix_lengths without a prefix")
-    scale = 0.125 if scale is None else float(scale)
-    if not (scale > 0 and math.isfinite(scale)):
+    if scale is None:
+        scale = 0.125
+    elif not (scale > 0 and math.isfinite(scale)):
         raise ValueError("scale must be positive and finite")
     if out is None:
-        out = torch.empty((batch, n, heads, HEAD_DIM), dtype=q.dtype, device=dev)
-    else:
-        _cuda("out", out, dev)
-        if out.numel() != batch * n * heads * HEAD_DIM or out.dtype is not q.dtype or not out.is_contiguous() \
-                or out.data_ptr() & 15:
-            raise ValueError(f"out must hold [{batch}, {n}, {heads}, {HEAD_DIM}] of q's type, contiguous and 16-byte "
-                             "aligned")
-    lse = torch.empty((batch, n, heads), dtype=torch.float32, device=dev) if return_lse else None
-    run = _run_rows(run_rows, dev)
-    if out.numel():
-        size = _workspace_bytes(batch, n, heads, kv_heads, prefixes, prefix_capacity, view.capacity, dev.index)
+        out = q.new_empty((batch, n, heads, HEAD_DIM))
+    elif _on("out", out, index).numel() != batch * n * heads * HEAD_DIM or out.dtype is not q.dtype \
+            or not out.is_contiguous() or out.data_ptr() & 15:
+        raise ValueError(f"out must hold [{batch}, {n}, {heads}, {HEAD_DIM}] of q's type, contiguous and 16-byte aligned")
+    lse = q.new_empty((batch, n, heads), dtype=torch.float32) if return_lse else None
+    run = _run_rows(run_rows, index)
+    if batch and n and heads:
+        size = _workspace_bytes(batch, n, heads, kv_heads, prefixes, prefix_capacity, keys.capacity, index)
         # (goes back to the allocator's pool of the current stream, which the
         # kernels that use it are on)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-        _call("dh_kv_attention", dev, q.data_ptr(), _TYPES[q.dtype], _U64x4(*qs), batch, n, heads, kv_heads,
-              ctypes.addressof(view), None if pview is None else ctypes.addressof(pview), prefixes, scale,
-              out.data_ptr(), _ptr(lse), run, _ptr(ws), size)
+        ws = q.new_empty((size,), dtype=torch.uint8) if size else None
+        _call_on("dh_kv_attention", index, q.data_ptr(), q_type, _pack4(*qs), batch, n, heads, kv_heads, keys.view,
+                 prefix_view, prefixes, scale, out.data_ptr(), _ptr(lse), run, _ptr(ws), size)
     return (out, lse) if return_lse else out
 
 

@@ -55,13 +55,13 @@ def _view(**kw):
     a = dict(k=P, v=P, k_scale=P, v_scale=P, lengths=None, k_strides=U64x4(65536, 4096, 64, 1),
              v_strides=U64x4(65536, 4096, 64, 1), k_type=1, v_type=1, capacity=64, length=64)
     a.update(kw)
-    return kvcache._View(*a.values())
+    return kvcache._pack_view(*(a[n] or 0 for n in ("k", "v", "k_scale", "v_scale", "lengths")), *a["k_strides"],
+                              *a["v_strides"], a["k_type"], a["v_type"], a["capacity"], a["length"])
 
 
 def _attend(own=None, prefix=None, **kw):
     own = _view() if own is None else own
-    a = dict(q=P, qt=1, qs=U64x4(4096, 1024, 64), n=2, queries=16, heads=4, kv_heads=4, own=ctypes.addressof(own),
-             prefix=None if prefix is None else ctypes.addressof(prefix), prefixes=0 if prefix is None else 1,
+    a = dict(q=P, qt=1, qs=U64x4(4096, 1024, 64), n=2, queries=16, heads=4, kv_heads=4, own=own, prefix=prefix, prefixes=0 if prefix is None else 1,
              scale=0.125, out=P, lse=None, run=None, ws=P, size=1 << 30)
     a.update(kw)
     return _lib.raw("dh_kv_attention", *a.values(), None)
