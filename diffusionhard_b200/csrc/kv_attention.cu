@@ -17,14 +17,13 @@
 // leaves its unnormalised sums and maximum in the workspace and a second kernel
 // joins them in a fixed order.
 //
-// One persistent kernel, two CTAs per SM, 8 warps:
+// One persistent kernel, two CTAs per SM, 6 warps (int8: 8):
 //   warp 0    loads: TMA tiles of K and V (16 bits), or the contiguous codes and
 //             scales of 64 keys (int8)
 //   warp 1    tcgen05 MMAs: S = Q K^T, Q from TMEM; [O | l] += P [V | 1], P from
 //             TMEM, where a column of ones beside V sums P
-//   warps 2-3 int8: codes to f16 tiles, see convert_rows.  16 bits: zeros over
-//             the rows of V behind the last key (0 * NaN must not reach O)
-//   warps 4-7 softmax, a thread a row: P = 2^(s c - m) over S in TMEM; O in TMEM
+//   warps 2-3 int8 alone: codes to f16 tiles, see convert_rows
+//   four more softmax, a thread a row: P = 2^(s c - m) over S in TMEM; O in TMEM
 //             is rescaled only when the maximum grew by more than 2^8
 #include <cuda.h>
 
@@ -40,7 +39,6 @@ namespace {
 using namespace kv;
 
 constexpr uint32_t kRows = 128;                  // rows per item
-constexpr uint32_t kThreads = 256;
 constexpr uint32_t kOnesBytes = 2048;            // 16 rows of 128 bytes
 constexpr uint32_t kVPitch = kTileBytes + kOnesBytes;
 constexpr uint32_t kTmemCols = 256;
@@ -56,6 +54,7 @@ enum Kind : int { kV16 = 0, kVBf16 = 1, kInt8 = 2 };
 template <int KIND>
 struct Cfg {
     static constexpr bool int8 = KIND == kInt8;
+    static constexpr uint32_t threads = int8 ? 256 : 192;
     static constexpr uint32_t raw_stages = int8 ? 4 : 0;
     static constexpr uint32_t k_stages = int8 ? 2 : 4;
     static constexpr uint32_t v_stages = int8 ? 2 : 3;
@@ -71,7 +70,7 @@ struct Cfg {
 enum Bar : uint32_t {
     kRawFull = 0, kRawEmpty = kRawFull + 4, kKFull = kRawEmpty + 4, kKEmpty = kKFull + 4, kVFull = kKEmpty + 4,
     kVEmpty = kVFull + 4, kSFull = kVEmpty + 4, kPFull = kSFull + 2, kSPFree = kPFull + 2, kOFull = kSPFree + 2,
-    kOFree, kQReady, kVPart, kDrain = kVPart + 4, kNumBars
+    kOFree, kQReady, kDrain, kNumBars
 };
 static_assert(kNumBars * 8 + 8 + 2 * kExpRing * 4 <= 512, "barrier area");
 
@@ -141,6 +140,20 @@ DH_DEVINL void convert_rows(const uint8_t* raw, uint8_t* tile, uint32_t warp_hal
     }
 }
 
+// Zeros over the rows of a V tile from `left` on, by the 128 softmax threads.
+DH_DEVINL void zero_rows(uint8_t* tile, uint32_t left, uint32_t transposed, uint32_t thread) {
+    if (transposed) {
+        for (uint32_t i = thread; i < kDh * kKT; i += 128) {
+            const uint32_t d = i / kKT, key = i % kKT;
+            if (key >= left)
+                *reinterpret_cast<uint16_t*>(tile + d * 128 + (((key >> 3) ^ (d & 7u)) * 16) + (key & 7u) * 2) = 0;
+        }
+    } else {
+        for (uint32_t i = left * 8 + thread; i < kKT * 8; i += 128)
+            *reinterpret_cast<uint4*>(tile + i * 16) = make_uint4(0, 0, 0, 0);
+    }
+}
+
 // Item w of both classes, `first` the number of the first class's (0: they are not
 // this kernel's).
 DH_DEVINL Item item_at(const Args& a, uint32_t first, uint32_t w, uint32_t live) {
@@ -148,7 +161,7 @@ DH_DEVINL Item item_at(const Args& a, uint32_t first, uint32_t w, uint32_t live)
 }
 
 template <int KIND>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(Cfg<KIND>::threads, 2)
 kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ CUtensorMap tpv,
                     const __grid_constant__ CUtensorMap tok, const __grid_constant__ CUtensorMap tov,
                     const __grid_constant__ Args a, const uint32_t first, const uint32_t total) {
@@ -194,12 +207,12 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
     // further rows under every tile, the first of them ones.
     const uint32_t one2 = KIND == kVBf16 ? 0x3F803F80u : 0x3C003C00u;
     if (a.v_transposed) {
-        for (uint32_t i = threadIdx.x; i < C::v_stages * 512; i += kThreads) {
+        for (uint32_t i = threadIdx.x; i < C::v_stages * 512; i += C::threads) {
             const uint32_t st = i / 512, w = i % 512;
             reinterpret_cast<uint32_t*>(v_ring + st * kVPitch + kTileBytes)[w] = w < 32 ? one2 : 0u;
         }
     } else {
-        for (uint32_t i = threadIdx.x; i < 512; i += kThreads) {
+        for (uint32_t i = threadIdx.x; i < 512; i += C::threads) {
             const uint32_t r = i / 32, w = i % 32;
             reinterpret_cast<uint32_t*>(ones)[i] = w == (r & 7u) * 4 ? (one2 & 0xFFFFu) : 0u;
         }
@@ -254,11 +267,9 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                             ok = false;
                             break;
                         }
-                        // (a tile with rows behind the last key goes to warp 2 first)
-                        uint64_t* bar = &bars[(keys_left(it, j) < kKT ? kVPart : kVFull) + vs];
-                        tc::mbar_arrive_expect_tx(bar, kTileBytes);
-                        tc::tma_load_4d(v_ring + vs * kVPitch, own ? &tov : &tpv, bar, a.v_transposed ? key : 0,
-                                        a.v_transposed ? 0 : key, it.kv_head, entry);
+                        tc::mbar_arrive_expect_tx(&bars[kVFull + vs], kTileBytes);
+                        tc::tma_load_4d(v_ring + vs * kVPitch, own ? &tov : &tpv, &bars[kVFull + vs],
+                                        a.v_transposed ? key : 0, a.v_transposed ? 0 : key, it.kv_head, entry);
                     }
                 }
             }
@@ -340,7 +351,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
             tc::mma_commit(&bars[kDrain]);
             tc::mbar_wait_suspend(&bars[kDrain], 0, tc::kErrTimeoutAccFull);
         }
-    } else if (warp < 4) {
+    } else if (C::int8 && warp < 4) {
         uint32_t g = 0;
         bool ok = true;
         if constexpr (C::int8) {
@@ -406,38 +417,6 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                         tc::mbar_arrive(&bars[kVFull + vs]);
                         tc::mbar_arrive(&bars[kRawEmpty + rs]);
                     }
-                }
-            }
-        } else if (warp == 2) {
-            // ------------------------------------------- rows behind the last key
-            // Such tiles of V arrive on kVPart, and this warp's arrival on kVFull hands
-            // them on: a stage is loaded again only after that, so no phase is missed.
-            uint32_t phases = 0;  // a bit for each stage
-            for (uint32_t w = blockIdx.x; w < total && ok; w += gridDim.x) {
-                const Item it = item_at(a, first, w, live);
-                for (uint32_t j = it.t0; j < it.t1; ++j, ++g) {
-                    const uint32_t left = keys_left(it, j), vs = g % C::v_stages;
-                    if (left >= kKT) continue;
-                    if (!tc::mbar_wait_suspend(&bars[kVPart + vs], (phases >> vs) & 1u, tc::kErrTimeoutFull)) {
-                        ok = false;
-                        break;
-                    }
-                    phases ^= 1u << vs;
-                    uint8_t* tile = v_ring + vs * kVPitch;
-                    if (a.v_transposed) {
-                        for (uint32_t i = lane; i < kDh * kKT; i += 32) {
-                            const uint32_t d = i / kKT, key = i % kKT;
-                            if (key >= left)
-                                *reinterpret_cast<uint16_t*>(tile + d * 128 + (((key >> 3) ^ (d & 7u)) * 16) +
-                                                             (key & 7u) * 2) = 0;
-                        }
-                    } else {
-                        for (uint32_t i = left * 8 + lane; i < kKT * 8; i += 32)
-                            *reinterpret_cast<uint4*>(tile + i * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(&bars[kVFull + vs]);
                 }
             }
         }
@@ -639,6 +618,17 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                     }
                     tc::tmem_st_wait();
                     tc::tc_fence_before();
+                }
+                if (!C::int8 && keys_left(it, j) < kKT) {
+                    // V behind the last key: 0 * NaN must not reach O.  (The stage is
+                    // not loaded again before this tile's PV, which waits for this.)
+                    const uint32_t vs = g % C::v_stages;
+                    if (!tc::mbar_wait_suspend(&bars[kVFull + vs], (g / C::v_stages) & 1u, tc::kErrTimeoutFull)) {
+                        ok = false;
+                        break;
+                    }
+                    zero_rows(v_ring + vs * kVPitch, keys_left(it, j), a.v_transposed, r);
+                    fence_proxy_async_smem();
                 }
                 tc::mbar_arrive(&bars[kPFull + sb]);
             }
@@ -942,7 +932,7 @@ uint32_t launch(const CUtensorMap (&maps)[4], const Args& a, uint32_t first, uin
     static std::atomic<uint64_t> configured{0};
     if (all_shared_once(kv_attention_kernel<KIND>, Cfg<KIND>::bytes, configured) != cudaSuccess) return DH_ERR_CUDA;
     const uint32_t grid = std::min(total, 2 * device_sms());
-    return launch_beside(kv_attention_kernel<KIND>, grid, kThreads, Cfg<KIND>::bytes, false, st, maps[0], maps[1],
+    return launch_beside(kv_attention_kernel<KIND>, grid, Cfg<KIND>::threads, Cfg<KIND>::bytes, false, st, maps[0], maps[1],
                          maps[2], maps[3], a, first, total);
 }
 
