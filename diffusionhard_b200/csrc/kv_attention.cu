@@ -24,7 +24,7 @@
 //             TMEM, where a column of ones beside V sums P
 //   warps 2-3 int8 alone: codes to f16 tiles, see convert_rows
 //   four more softmax, a thread a row: P = 2^(s c - m) over S in TMEM; O in TMEM
-//             is rescaled only when the maximum grew by more than 2^8
+//             is rescaled only when the maximum grew by more than 2^15 (2^60 for bf16)
 #include <cuda.h>
 
 #include "kv_few.h"
@@ -56,8 +56,9 @@ struct Cfg {
     static constexpr bool int8 = KIND == kInt8;
     static constexpr uint32_t threads = int8 ? 256 : 192;
     static constexpr uint32_t raw_stages = int8 ? 4 : 0;
-    static constexpr uint32_t k_stages = int8 ? 2 : 4;
-    static constexpr uint32_t v_stages = int8 ? 2 : 3;
+    // (16 bits: 4 of K and 3 of V 305 us where 2 and 2 take 302.5)
+    static constexpr uint32_t k_stages = 2;
+    static constexpr uint32_t v_stages = 2;
     static constexpr uint32_t q_at = 0;
     static constexpr uint32_t k_at = kRows * 128;
     static constexpr uint32_t v_at = k_at + k_stages * kTileBytes;
@@ -76,7 +77,7 @@ static_assert(kNumBars * 8 + 8 + 2 * kExpRing * 4 <= 512, "barrier area");
 
 DH_DEVINL void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// 2^x of two values on the FMA pipe (x <= 8): x = n + f with n = rint(x) by the
+// 2^x of two values on the FMA pipe (x < 100): x = n + f with n = rint(x) by the
 // 1.5 * 2^23 shifter, 2^f on [-0.5, 0.5] by a cubic (largest relative error
 // 7.8e-5, a third of an f16 half step), 2^n into the exponent field.  Takes a
 // quarter of the exponentials off the MUFU.
@@ -92,6 +93,11 @@ DH_DEVINL float2 exp2_poly2(float2 x) {
     return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
                        __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
+// The maximum that P is relative to stays until it grew by more than this power of
+// two, P's largest value meanwhile (f16 ends at 2^16).  32 canvases over int8, scores
+// of a few: 245 us at 8, 237 at 15; 128 x 512 queries over 1024 16-bit keys 325 and 305.
+template <int KIND>
+constexpr float kMaxGrowth = KIND == kVBf16 ? 60.f : 15.f;
 constexpr uint32_t kPolyPairMask = 0x11u;  // pairs e with bit e % 8 set
 
 // 16 codes -> 16 f16 of code * ratio * 2^-9, where f = f16(ratio * 2^15): a code
@@ -386,9 +392,10 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                         }
                         e[side] = max(exponent_of(__reduce_max_sync(0xFFFFFFFFu, peak)), -100);
                     }
-                    // O keeps one exponent of V for all tiles of an item: it only grows,
-                    // by two more than it has to, and O is rescaled when it does
-                    ev = e[1] > ev ? min(e[1] + (j == it.t0 ? 0 : 2), 126) : ev;
+                    // O keeps one exponent of V for all tiles of an item, four times what
+                    // it has to be when it is set: it only grows, and O is rescaled when
+                    // it does
+                    ev = e[1] > ev ? min(e[1] + 2, 126) : ev;
                     const float fk = pow2(15 - min(e[0], 126)), fv = pow2(15 - ev);
                     if (!tc::mbar_wait_suspend(&bars[kKEmpty + ks], ((g / C::k_stages) & 1u) ^ 1u,
                                                tc::kErrTimeoutEmpty)) {
@@ -565,7 +572,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                         m = mt;
                         ev = et;
                     } else {
-                        if (!(mt <= m + 8.0f)) {
+                        if (!(mt <= m + kMaxGrowth<KIND>)) {
                             need = true;
                             alpha = ex2_approx(m - mt);
                             m = mt;
