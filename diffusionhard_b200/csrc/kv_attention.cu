@@ -27,7 +27,7 @@
 //             is rescaled only when the maximum grew by more than 2^15 (2^60 for bf16)
 #include <cuda.h>
 
-#include "kv_few.h"
+#include "kv_kernels.h"
 #include "tmap.h"
 
 #include <algorithm>
@@ -49,11 +49,13 @@ constexpr uint32_t kExpRing = 8;                 // tiles whose exponents are ke
 
 constexpr uint32_t kMaxSplits = 64;              // parts of an item's keys
 
-enum Kind : int { kV16 = 0, kVBf16 = 1, kInt8 = 2 };
+// kWide: int8 keys that kv_widen.cu has turned into f16
+enum Kind : int { kV16 = 0, kVBf16 = 1, kInt8 = 2, kWide = 3 };
 
 template <int KIND>
 struct Cfg {
     static constexpr bool int8 = KIND == kInt8;
+    static constexpr bool scaled = int8 || KIND == kWide;  // keys carry exponents
     static constexpr uint32_t threads = int8 ? 256 : 192;
     static constexpr uint32_t raw_stages = int8 ? 4 : 0;
     // (16 bits: 4 of K and 3 of V 305 us where 2 and 2 take 302.5)
@@ -99,27 +101,6 @@ DH_DEVINL float2 exp2_poly2(float2 x) {
 template <int KIND>
 constexpr float kMaxGrowth = KIND == kVBf16 ? 60.f : 15.f;
 constexpr uint32_t kPolyPairMask = 0x11u;  // pairs e with bit e % 8 set
-
-// 16 codes -> 16 f16 of code * ratio * 2^-9, where f = f16(ratio * 2^15): a code
-// plus 128 as the bits of a subnormal f16 is (code + 128) 2^-24, so one FMA with
-// f and -f 2^-17 (exact, a power of two) takes the 128 off and scales, with one
-// rounding.
-DH_DEVINL void convert16(const uint4& codes, __half2 f, __half2 off, uint4& lo, uint4& hi) {
-    const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-    uint32_t o[8];
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t u = w[i] ^ 0x80808080u;
-#pragma unroll
-        for (uint32_t h = 0; h < 2; ++h) {
-            uint32_t p = __byte_perm(u, 0u, h ? 0x4342u : 0x4140u);
-            __half2 x = __hfma2(*reinterpret_cast<__half2*>(&p), f, off);
-            o[2 * i + h] = *reinterpret_cast<uint32_t*>(&x);
-        }
-    }
-    lo = make_uint4(o[0], o[1], o[2], o[3]);
-    hi = make_uint4(o[4], o[5], o[6], o[7]);
-}
 
 // Half of a tile's 64 rows of codes (those of this warp) into a 128-byte
 // swizzled f16 tile; `scale` holds the lane's two rows' f16 factors.
@@ -229,6 +210,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
     __syncthreads();
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_holder;
+    if constexpr (KIND == kWide) grid_wait();  // (the keys are another kernel's)
 
     if (warp == 0) {
         // ---------------------------------------------------------- loads
@@ -466,7 +448,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
         // This thread's query row from shared memory into TMEM.  Returns the
-        // factor of its scores.  int8: the row as f16 between 1/2 and 1 in
+        // factor of its scores.  int8 keys: the row as f16 between 1/2 and 1 in
         // magnitude, its exponent in the factor.
         auto copy_q = [&]() -> float {
             asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -477,7 +459,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                 qv[4 * i] = v.x, qv[4 * i + 1] = v.y, qv[4 * i + 2] = v.z, qv[4 * i + 3] = v.w;
             }
             float c = a.c;
-            if constexpr (C::int8) {
+            if constexpr (C::scaled) {
                 uint32_t peak = 0;
                 if (a.q_bf16) {
 #pragma unroll
@@ -523,7 +505,12 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
             next_item(next_w, next);
             const bool active = quad * 32 < it.rows;  // the warp has rows
             float m = 0.f;
-            int32_t ev = 0;  // exponent of O (int8)
+            int32_t ev = 0;  // exponent of O (int8 keys)
+            float2 ex0 = make_float2(1.f, 0.f), ex1 = ex0;  // of the prefix, of its own keys
+            if constexpr (KIND == kWide) {
+                if (it.len0) ex0 = a.prefix_exps[it.prefix * a.kv_heads.d + it.kv_head];
+                if (it.len1) ex1 = a.own_exps[it.own * a.kv_heads.d + it.kv_head];
+            }
             for (uint32_t j = it.t0; j < it.t1; ++j, ++g) {
                 const uint32_t sb = g & 1u;
                 if (!tc::mbar_wait_suspend(&bars[kSFull + sb], (g >> 1) & 1u, tc::kErrTimeoutAccFull)) {
@@ -541,6 +528,10 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                     if constexpr (C::int8) {
                         ct = fmaxf(c * pow2(min(exps[(g % kExpRing) * 2], 127)), kLeastFactor);
                         et = exps[(g % kExpRing) * 2 + 1];
+                    } else if constexpr (C::scaled) {
+                        const float2 ex = j < it.n0 ? ex0 : ex1;
+                        ct = fmaxf(c * ex.x, kLeastFactor);
+                        et = __float_as_int(ex.y);
                     }
                     const uint32_t left = keys_left(it, j);
                     tc::tmem_ld_wait();
@@ -578,7 +569,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                             m = mt;
                         }
                         alpha_o = alpha;
-                        if (C::int8 && et > ev) {
+                        if (C::scaled && et > ev) {
                             need = true;
                             alpha_o = alpha * pow2(max(ev - et, -126));
                             ev = et;
@@ -649,7 +640,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
             const uint64_t row = row_index(a, it, r, nullptr);
             const bool mine = r < it.rows;
             tc::tmem_ld_wait();
-            float f = C::int8 ? pow2(min(ev, 127)) : 1.f;
+            float f = C::scaled ? pow2(min(ev, 127)) : 1.f;
             float4* part = nullptr;
             if (a.part_ml) {
                 const uint64_t at = it.slot * a.total_rows + row;
@@ -768,9 +759,12 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const float2* ml,
 
 // Rows a sequence must have before its items walk the prefix by themselves.
 constexpr uint32_t kStackBelow = 128;
+// Visits of every tile of int8 keys from which they are turned into f16 first.
+constexpr uint32_t kWidenFrom = 4;
 
 struct Plan {
     Class cls[2];         // prefix of stacked rows, and each sequence's own keys
+    bool widen;           // int8 keys are turned into f16 first
     bool few[2];          // items of the kernel for few rows, on `cluster` CTAs each
     uint32_t cluster[2];
     uint32_t slots;
@@ -828,7 +822,7 @@ void split_many(Class* cls, const uint64_t* items, const uint32_t* tiles, uint32
 }
 
 Plan plan_of(uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t prefixes, uint32_t prefix_keys,
-             uint32_t own_keys, uint32_t sms) {
+             uint32_t own_keys, bool int8, uint32_t sms) {
     Plan p{};
     const uint32_t per = prefixes ? sequences / prefixes : sequences;
     const bool stacked = prefixes && per > 1 && rows < kStackBelow;
@@ -853,6 +847,12 @@ Plan plan_of(uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t pref
             many[i] = items[i];
     }
     // (beside the kernel for few rows one CTA fits an SM)
+    // Turning costs about as much as 2.5 visits of a tile.  (32 canvases, 8 visits: XXX
+    // instead of 237 us; 24 blocks behind two prefixes, 4.5: XXX and 47.)
+    const uint64_t visits = many[0] * tiles[0] + many[1] * tiles[1];
+    const uint64_t tiles_held = static_cast<uint64_t>(kv_heads) * (static_cast<uint64_t>(sequences) * t1 +
+                                                                  static_cast<uint64_t>(prefixes) * t0);
+    p.widen = int8 && !p.few[0] && !p.few[1] && visits >= kWidenFrom * tiles_held;
     if (many[0] || many[1]) split_many(p.cls, many, tiles, p.few[1] ? sms : 2 * sms, stacked);
     for (int i = 0; i < 2; ++i) {
         if (!items[i]) continue;
@@ -874,8 +874,28 @@ bool fits(uint32_t sequences, uint32_t queries, uint32_t heads, uint32_t kv_head
 
 bool misaligned(const void* p, uint32_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
 
-size_t workspace_of(uint32_t slots, uint64_t rows) {
-    return slots < 2 ? 0 : static_cast<size_t>(slots) * rows * (sizeof(float2) + kDh * sizeof(float));
+// The workspace: parts of rows, then keys as f16.
+struct Layout {
+    size_t ml, exps[2], wide[2], bytes;  // [0] of the prefixes, [1] of the sequences
+};
+
+Layout layout_of(const Plan& p, uint64_t rows, uint32_t kv_heads, const uint32_t (&entries)[2],
+                 const uint32_t (&capacity)[2]) {
+    const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    Layout l{};
+    if (p.slots > 1) {
+        l.ml = static_cast<size_t>(p.slots) * rows * kDh * sizeof(float);
+        l.bytes = up(l.ml + static_cast<size_t>(p.slots) * rows * sizeof(float2));
+    }
+    if (p.widen) {
+        for (int i = 0; i < 2; ++i) {
+            const size_t lines = static_cast<size_t>(entries[i]) * kv_heads;
+            l.exps[i] = l.bytes;
+            l.wide[i] = up(l.exps[i] + lines * sizeof(float2));
+            l.bytes = l.wide[i] + 2 * lines * capacity[i] * kDh * 2;
+        }
+    }
+    return l;
 }
 
 uint32_t check_view(const dh_kv_view& v) {
@@ -935,11 +955,12 @@ uint32_t launch_beside(Kernel kernel, uint32_t grid, uint32_t threads, uint32_t 
 }
 
 template <int KIND>
-uint32_t launch(const CUtensorMap (&maps)[4], const Args& a, uint32_t first, uint32_t total, cudaStream_t st) {
+uint32_t launch(const CUtensorMap (&maps)[4], const Args& a, uint32_t first, uint32_t total, bool beside,
+                cudaStream_t st) {
     static std::atomic<uint64_t> configured{0};
     if (all_shared_once(kv_attention_kernel<KIND>, Cfg<KIND>::bytes, configured) != cudaSuccess) return DH_ERR_CUDA;
     const uint32_t grid = std::min(total, 2 * device_sms());
-    return launch_beside(kv_attention_kernel<KIND>, grid, Cfg<KIND>::threads, Cfg<KIND>::bytes, false, st, maps[0], maps[1],
+    return launch_beside(kv_attention_kernel<KIND>, grid, Cfg<KIND>::threads, Cfg<KIND>::bytes, beside, st, maps[0], maps[1],
                          maps[2], maps[3], a, first, total);
 }
 
@@ -950,13 +971,15 @@ using namespace dh;
 
 extern "C" size_t dh_kv_attention_workspace_size(uint32_t sequences, uint32_t queries, uint32_t heads,
                                                  uint32_t kv_heads, uint32_t prefixes, uint32_t prefix_capacity,
-                                                 uint32_t own_capacity) {
+                                                 uint32_t own_capacity, uint32_t k_type) {
     if (!sequences || !queries || !heads || !kv_heads || heads % kv_heads || (prefixes && sequences % prefixes) ||
         !fits(sequences, queries, heads, kv_heads, prefixes))
         return 0;
     const Plan p = plan_of(sequences, queries * (heads / kv_heads), kv_heads, prefixes, prefix_capacity, own_capacity,
-                           device_sms());
-    return workspace_of(p.slots, static_cast<uint64_t>(sequences) * queries * heads);
+                           k_type == DH_TYPE_I8, device_sms());
+    return layout_of(p, static_cast<uint64_t>(sequences) * queries * heads, kv_heads, {prefixes, sequences},
+                     {prefix_capacity, own_capacity})
+        .bytes;
 }
 
 extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64_t* q_strides, uint32_t sequences,
@@ -982,8 +1005,9 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
     const uint32_t ratio = heads / kv_heads;
     const uint64_t rows = static_cast<uint64_t>(sequences) * queries * heads;
     const Plan p = plan_of(sequences, queries * ratio, kv_heads, prefixes, prefixes ? prefix->capacity : 0,
-                           own->capacity, device_sms());
-    const size_t need = workspace_of(p.slots, rows);
+                           own->capacity, int8, device_sms());
+    const Layout l = layout_of(p, rows, kv_heads, {prefixes, sequences}, {prefixes ? prefix->capacity : 0, own->capacity});
+    const size_t need = l.bytes;
     if (need && !workspace) return DH_ERR_NULL_POINTER;
     if (need > workspace_bytes) return DH_ERR_WORKSPACE;
     if (misaligned(workspace, 256)) return DH_ERR_ALIGNMENT;
@@ -1014,7 +1038,7 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
     a.run_rows = run_rows;
     if (p.slots > 1) {
         a.part_o = static_cast<float*>(workspace);
-        a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<size_t>(p.slots) * rows * kDh);
+        a.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + l.ml);
     }
     CUtensorMap maps[4] = {};
     if (!int8) {
@@ -1022,13 +1046,34 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
         if (prefixes && !view_maps(&maps[0], &maps[1], *prefix, prefixes, kv_heads)) return DH_ERR_CUDA;
     }
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (p.widen) {
+        WideKeys to[2];
+        for (int i = prefixes ? 0 : 1; i < 2; ++i) {
+            const uint32_t entries = i ? sequences : prefixes, capacity = i ? own->capacity : prefix->capacity;
+            uint8_t* base = static_cast<uint8_t*>(workspace);
+            to[i].exps = reinterpret_cast<float2*>(base + l.exps[i]);
+            to[i].k = reinterpret_cast<__half*>(base + l.wide[i]);
+            to[i].v = to[i].k + static_cast<size_t>(entries) * kv_heads * capacity * kDh;
+            dh_kv_view f{};
+            f.k = to[i].k, f.v = to[i].v, f.k_type = f.v_type = DH_TYPE_F16, f.capacity = capacity;
+            f.k_strides[2] = f.v_strides[2] = kDh, f.k_strides[3] = f.v_strides[3] = 1;
+            f.k_strides[1] = f.v_strides[1] = static_cast<uint64_t>(capacity) * kDh;
+            f.k_strides[0] = f.v_strides[0] = static_cast<uint64_t>(capacity) * kDh * kv_heads;
+            if (!view_maps(&maps[2 * i], &maps[2 * i + 1], f, entries, kv_heads)) return DH_ERR_CUDA;
+        }
+        a.prefix_exps = to[0].exps, a.own_exps = to[1].exps;
+        if (uint32_t status = launch_widen(a, to[0], to[1], prefixes, st)) return status;
+    }
     // Tensor-core tiles first: their few CTAs take long, and the others run beside them.
     uint32_t status = DH_OK, first = 0, total = 0;
     for (uint32_t i = 0; i < 2; ++i)
         if (!p.few[i]) total += a.cls[i].items, first += i ? 0 : a.cls[0].items;
-    if (total)
-        status = int8 ? launch<kInt8>(maps, a, first, total, st)
-                      : (v_bf16 ? launch<kVBf16>(maps, a, first, total, st) : launch<kV16>(maps, a, first, total, st));
+    if (total && p.widen)
+        status = launch<kWide>(maps, a, first, total, true, st);
+    else if (total)
+        status = int8 ? launch<kInt8>(maps, a, first, total, false, st)
+                      : (v_bf16 ? launch<kVBf16>(maps, a, first, total, false, st)
+                                : launch<kV16>(maps, a, first, total, false, st));
     bool beside = total;
     for (uint32_t i = 0; i < 2 && !status; ++i) {
         if (!p.few[i]) continue;

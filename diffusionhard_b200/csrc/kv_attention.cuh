@@ -53,6 +53,8 @@ struct Args {
     float* part_o;                           // [slots][rows][64]
     uint64_t total_rows;
     const uint32_t* run_rows;
+    const float2* prefix_exps;               // of keys turned into f16: factor of K, exponent of V
+    const float2* own_exps;
 };
 
 // Programmatic dependent launch: the next kernel may begin; all before this one have
@@ -90,6 +92,27 @@ DH_DEVINL uint32_t pack_bf16x2(float lo, float hi) {
 DH_DEVINL float pow2(int32_t n) { return __uint_as_float(static_cast<uint32_t>(n + 127) << 23); }
 // e with 2^(e - 1) <= x < 2^e for the normal fp32 with these bits
 DH_DEVINL int32_t exponent_of(uint32_t bits) { return static_cast<int32_t>((bits >> 23) & 0xFFu) - 126; }
+
+// 16 codes -> 16 f16 of code * ratio * 2^-9, where f = f16(ratio * 2^15): a code
+// plus 128 as the bits of a subnormal f16 is (code + 128) 2^-24, so one FMA with
+// f and -f 2^-17 (exact, a power of two) takes the 128 off and scales, with one
+// rounding.
+DH_DEVINL void convert16(const uint4& codes, __half2 f, __half2 off, uint4& lo, uint4& hi) {
+    const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+    uint32_t o[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t u = w[i] ^ 0x80808080u;
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+            uint32_t p = __byte_perm(u, 0u, h ? 0x4342u : 0x4140u);
+            __half2 x = __hfma2(*reinterpret_cast<__half2*>(&p), f, off);
+            o[2 * i + h] = *reinterpret_cast<uint32_t*>(&x);
+        }
+    }
+    lo = make_uint4(o[0], o[1], o[2], o[3]);
+    hi = make_uint4(o[4], o[5], o[6], o[7]);
+}
 
 struct Item {
     uint32_t seq0, kv_head, row0, rows, slot;  // rows: live rows of the tile (may be 0)

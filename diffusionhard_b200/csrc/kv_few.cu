@@ -29,7 +29,7 @@
 // it works on the last ones of the one before (`solo`).
 #include <cuda.h>
 
-#include "kv_few.h"
+#include "kv_kernels.h"
 #include "row_quant.cuh"
 
 #include <algorithm>

@@ -1,4 +1,5 @@
-// kv_few.h -- the launch of the kernel for few rows (kv_few.cu).
+// kv_kernels.h -- launches that dh_kv_attention puts together: the kernel for few rows
+// (kv_few.cu) and the one that turns int8 keys into f16 (kv_widen.cu).
 #pragma once
 
 #include <cuda.h>
@@ -27,6 +28,16 @@ inline cudaError_t all_shared_once(Kernel kernel, uint32_t bytes, std::atomic<ui
 // V (16 bits).  beside: may begin while the kernel before it in the stream runs.
 uint32_t launch_few(const CUtensorMap (&maps)[4], const Args& a, uint32_t cls, uint32_t cluster, bool int8, bool v_bf16,
                     bool beside, cudaStream_t st);
+
+// f16 rows [lines][capacity][64] of K and V, and [lines] their exponents.
+struct WideKeys {
+    __half* k = nullptr;
+    __half* v = nullptr;
+    float2* exps = nullptr;
+};
+
+// The int8 keys of a's sequences and `prefixes` prefixes.
+uint32_t launch_widen(const Args& a, const WideKeys& prefix, const WideKeys& own, uint32_t prefixes, cudaStream_t st);
 
 }  // namespace kv
 }  // namespace dh

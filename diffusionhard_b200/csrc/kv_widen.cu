@@ -1,0 +1,122 @@
+// kv_widen.cu -- an int8 K/V cache as f16 rows, for attention with many tiles of rows.
+//
+// The tensor-core kernel over int8 turns codes into f16 tiles as it goes, once for
+// every 128 rows: 32 canvases of 1024 queries and keys take 237 us that way and XXX us
+// over 16-bit keys.  Where every key is visited by at least four tiles of rows, the
+// codes are turned once, here, into the workspace.  Bound by HBM: 136 bytes in and 256
+// out for each position and K/V head.
+//
+// A line is an (entry, head).  Its K becomes code * scale * 2^-(E + 9) with E the
+// exponent of the line's largest scale, rounded once to f16 (its factor scale 2^(15 -
+// E) is rounded before, see convert16), its V likewise with an E that is at least that
+// of the sequence's prefix; both exponents go to `exps`.  Rows behind the last key
+// become zeros up to the end of its tile.
+#include "kv_kernels.h"
+
+#include <algorithm>
+
+namespace dh {
+namespace kv {
+namespace {
+
+constexpr uint32_t kThreads = 256;
+
+struct WidenArgs {
+    Segment prefix, own;
+    WideKeys out_prefix, out_own;
+    uint32_t sequences, prefixes, prefix_chunks, own_chunks, with_prefix;
+    FastDiv kv_heads, queries, per_prefix;
+    const uint32_t* run_rows;
+};
+
+// The largest magnitude (as bits) among the first n scales, for all threads.
+DH_DEVINL uint32_t largest(const float* scale, uint32_t n, uint32_t* smem) {
+    float peak = 0.f;  // (of the numbers among them)
+    for (uint32_t i = threadIdx.x * 4; i < n; i += kThreads * 4) {
+        const float4 x = *reinterpret_cast<const float4*>(scale + i);  // (lines start at 256 bytes)
+        peak = fmaxf(peak, fabsf(x.x));
+        if (i + 1 < n) peak = fmaxf(peak, fabsf(x.y));
+        if (i + 2 < n) peak = fmaxf(peak, fabsf(x.z));
+        if (i + 3 < n) peak = fmaxf(peak, fabsf(x.w));
+    }
+    const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(peak));
+    if (lane_id() == 0) smem[warp_id()] = m;
+    __syncthreads();
+    uint32_t all = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kThreads / 32; ++i) all = max(all, smem[i]);
+    __syncthreads();
+    return all;
+}
+
+DH_DEVINL int32_t exponent_in_range(uint32_t bits) { return min(max(exponent_of(bits), -100), 126); }
+
+__global__ void __launch_bounds__(kThreads) kv_widen_kernel(const __grid_constant__ WidenArgs a) {
+    __shared__ uint32_t smem[kThreads / 32];
+    grid_launch_dependents();
+    const uint32_t prefix_ctas = a.with_prefix ? a.prefixes * a.kv_heads.d * a.prefix_chunks : 0u;
+    const bool own = blockIdx.x >= prefix_ctas;
+    const uint32_t chunks = own ? a.own_chunks : a.prefix_chunks;
+    const uint32_t index = own ? blockIdx.x - prefix_ctas : blockIdx.x;
+    const uint32_t line = index / chunks, chunk = index % chunks;
+    uint32_t head = line;
+    const uint32_t entry = a.kv_heads.split(head);
+    const uint32_t live = a.run_rows ? min(a.sequences, a.queries.of(min(*a.run_rows, 0x7FFFFFFFu))) : a.sequences;
+    if ((own ? entry : entry * a.per_prefix.d) >= live) return;
+    const Segment& s = own ? a.own : a.prefix;
+    const WideKeys& to = own ? a.out_own : a.out_prefix;
+    const uint32_t len = length_of(s, entry);
+    const uint64_t at = static_cast<uint64_t>(line) * s.capacity;
+    const int32_t ek = exponent_in_range(largest(s.k_scale + at, len, smem));
+    int32_t ev = exponent_in_range(largest(s.v_scale + at, len, smem));
+    if (own && a.with_prefix) {
+        const uint32_t p = a.per_prefix.of(entry);
+        const uint64_t line0 = static_cast<uint64_t>(p) * a.kv_heads.d + head;
+        ev = max(ev, exponent_in_range(
+                         largest(a.prefix.v_scale + line0 * a.prefix.capacity, length_of(a.prefix, p), smem)));
+    }
+    if (chunk == 0 && threadIdx.x == 0)
+        to.exps[line] = make_float2(pow2(min(ek + 9, 127)), __int_as_float(ev + 9));
+    const float fk = pow2(15 - ek), fv = pow2(15 - ev);
+    const uint32_t tiles = (len + kKT - 1) / kKT;
+    const uint32_t row = threadIdx.x / 4, c = threadIdx.x & 3u;  // 16 codes of a row a thread
+    for (uint32_t t = chunk; t < tiles; t += chunks) {
+        const uint64_t pos = at + t * kKT + row;
+        const bool live_row = t * kKT + row < len;
+#pragma unroll
+        for (uint32_t side = 0; side < 2; ++side) {
+            const uint4 codes = __ldcs(reinterpret_cast<const uint4*>((side ? s.v : s.k) + pos * kDh) + c);
+            const float scale = live_row ? (side ? s.v_scale : s.k_scale)[pos] : 0.f;
+            const __half2 f = __float2half2_rn(scale * (side ? fv : fk));
+            uint4 lo, hi;
+            convert16(codes, f, __hmul2(f, __half2half2(__ushort_as_half(0x8080))), lo, hi);
+            uint4* dst = reinterpret_cast<uint4*>((side ? to.v : to.k) + pos * kDh) + 2 * c;
+            dst[0] = lo, dst[1] = hi;
+        }
+    }
+}
+
+}  // namespace
+
+uint32_t launch_widen(const Args& a, const WideKeys& prefix, const WideKeys& own, uint32_t prefixes, cudaStream_t st) {
+    WidenArgs w{};
+    w.prefix = a.prefix, w.own = a.own, w.out_prefix = prefix, w.out_own = own;
+    w.sequences = a.sequences, w.prefixes = prefixes, w.with_prefix = prefixes != 0;
+    w.kv_heads = a.kv_heads, w.queries = a.queries, w.per_prefix = a.per_prefix;
+    w.run_rows = a.run_rows;
+    // four CTAs an SM; every one reads all scales of its line
+    const auto chunks = [](uint64_t lines, uint32_t capacity) {
+        return static_cast<uint32_t>(std::min<uint64_t>((4 * device_sms() + lines - 1) / lines, capacity / kKT));
+    };
+    const uint64_t own_lines = static_cast<uint64_t>(a.sequences) * a.kv_heads.d;
+    const uint64_t prefix_lines = static_cast<uint64_t>(prefixes) * a.kv_heads.d;
+    w.own_chunks = chunks(own_lines, a.own.capacity);
+    w.prefix_chunks = prefixes ? chunks(prefix_lines, a.prefix.capacity) : 1;
+    const uint64_t ctas = own_lines * w.own_chunks + prefix_lines * w.prefix_chunks;
+    kv_widen_kernel<<<static_cast<uint32_t>(ctas), kThreads, 0, st>>>(w);
+    DH_LAUNCH_CHECK();
+    return DH_OK;
+}
+
+}  // namespace kv
+}  // namespace dh

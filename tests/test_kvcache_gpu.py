@@ -273,7 +273,7 @@ def case(batch, heads, kv_heads, n, length, kind, seed, capacity=None):
     return q, (kk, vv), length
 
 
-@pytest.mark.parametrize("n", [2, 17, 64, 127, 128, 129, 300])
+@pytest.mark.parametrize("n", [2, 8, 9, 16, 17, 64, 127, 128, 129, 300, 513])
 @pytest.mark.parametrize("kind", ["int8", "bf16", "f16", "turned"])
 def test_queries(cuda, n, kind):
     q, kv, length = case(2, 2, 2, n, 150, kind, n, capacity=200)
@@ -288,7 +288,7 @@ def test_grouped_heads(cuda, heads, kv_heads, n, kind):
 
 
 @pytest.mark.parametrize("kind", ["int8", "bf16", "turned"])
-@pytest.mark.parametrize("n", [1, 33, 140])
+@pytest.mark.parametrize("n", [1, 12, 33, 140, 600])
 def test_ragged(cuda, kind, n):
     """A length for each sequence, none, all and beyond all among them."""
     q, kv, _ = case(8, 2, 2, n, 700, kind, n, capacity=720)
@@ -301,7 +301,8 @@ def test_ragged(cuda, kind, n):
 @pytest.mark.parametrize("kind", ["int8", "bf16", "f16", "turned"])
 @pytest.mark.parametrize("groups, batch, n, prefix, own", [
     (1, 5, 1, 300, 70), (1, 130, 1, 257, 9), (2, 6, 3, 1000, 64), (3, 3, 2, 100, 100), (1, 4, 200, 130, 65),
-    (2, 4, 128, 64, 64), (1, 9, 40, 1, 1), (1, 3, 1, 5000, 2),
+    (2, 4, 128, 64, 64), (1, 9, 40, 1, 1), (1, 3, 1, 5000, 2), (2, 4, 600, 130, 65), (1, 700, 1, 70, 65),
+    (1, 7, 2, 3000, 64),
 ])
 def test_prefix(cuda, kind, groups, batch, n, prefix, own):
     q, kv, length = case(batch, 4, 2, n, own, kind, prefix, capacity=own + 5)
@@ -310,7 +311,7 @@ def test_prefix(cuda, kind, groups, batch, n, prefix, own):
 
 
 @pytest.mark.parametrize("kind", ["int8", "bf16", "turned"])
-@pytest.mark.parametrize("n", [1, 150])
+@pytest.mark.parametrize("n", [1, 150, 520])
 def test_prefix_ragged(cuda, kind, n):
     """Lengths on the device for both parts; a sequence without keys of its own,
     a group without a prefix, and both together."""
@@ -320,7 +321,7 @@ def test_prefix_ragged(cuda, kind, n):
 
 
 @pytest.mark.parametrize("kind", ["int8", "bf16"])
-@pytest.mark.parametrize("n", [1, 70])
+@pytest.mark.parametrize("n", [1, 70, 520])
 def test_peaked_and_far_scores(cuda, kind, n):
     """Scores of hundreds whose maximum keeps growing along the keys, so that the
     sums are rescaled, and rows of V whose size grows and falls by 2^30."""
@@ -334,8 +335,9 @@ def test_peaked_and_far_scores(cuda, kind, n):
     check(q * 4, kv, length)
 
 
-def test_scales(cuda):
-    q, kv, length = case(1, 2, 2, 5, 100, "int8", 9)
+@pytest.mark.parametrize("n", [5, 50, 520])
+def test_scales(cuda, n):
+    q, kv, length = case(1, 2, 2, n, 100, "int8", 9)
     for scale in (1e-3, 0.125, 1.0, 3.0):
         check(q, kv, length, scale=scale)
     # queries and keys far from 1: the scores stay the same
@@ -345,9 +347,10 @@ def test_scales(cuda):
         assert torch.equal((a.double() * by).to(BF16), b)
 
 
-def test_zero_rows(cuda):
+@pytest.mark.parametrize("n", [3, 50, 520])
+def test_zero_rows(cuda, n):
     """All-zero keys and values (scale 0) among others, and queries of zeros."""
-    q, kv, length = case(1, 2, 2, 3, 130, "int8", 10)
+    q, kv, length = case(1, 2, 2, n, 130, "int8", 10)
     kv.k[:, :, ::3], kv.k_scale[:, :, ::3] = 0, 0
     kv.v[:, :, 1::3], kv.v_scale[:, :, 1::3] = 0, 0
     q[:, :, 1] = 0
@@ -358,11 +361,12 @@ def test_zero_rows(cuda):
 
 @pytest.mark.parametrize("kind", ["int8", "bf16", "turned"])
 @pytest.mark.parametrize("at", [0, 1, 8, 9, 63, 64, 100, 129])
-def test_not_finite(cuda, kind, at):
+@pytest.mark.parametrize("n", [3, 40, 520])
+def test_not_finite(cuda, kind, at, n):
     """A key or value that is not finite shows in every row that uses it, and
     in no other."""
     for which in (0, 1):
-        q, kv, length = case(2, 2, 2, 3, 130, kind, 11)
+        q, kv, length = case(2, 2, 2, n, 130, kind, 11)
         clean = attend(q, kv, length)
         if kind == "int8":
             (kv.k_scale if which == 0 else kv.v_scale)[0, 1, at] = math.nan
@@ -380,14 +384,15 @@ def test_not_finite(cuda, kind, at):
     _lib.check_device_error()
 
 
-def test_queries_not_finite(cuda):
+@pytest.mark.parametrize("n", [5, 50, 520])
+def test_queries_not_finite(cuda, n):
     for kind in ("int8", "bf16"):
-        q, kv, length = case(1, 2, 2, 5, 90, kind, 12)
+        q, kv, length = case(1, 2, 2, n, 90, kind, 12)
         clean = attend(q, kv, length)
         q[0, 1, 2, 9], q[0, 0, 4, 0] = math.nan, math.inf
         got = attend(q, kv, length)
         assert torch.isnan(got[0, 2, 1]).all() and torch.isnan(got[0, 4, 0]).all()
-        keep = torch.ones(1, 5, 2, dtype=torch.bool, device="cuda")
+        keep = torch.ones(1, n, 2, dtype=torch.bool, device="cuda")
         keep[0, 2, 1] = keep[0, 4, 0] = False
         assert torch.equal(got[keep], clean[keep])
 
@@ -416,7 +421,7 @@ def test_layouts(cuda, kind):
 
 
 @pytest.mark.parametrize("kind", ["int8", "bf16"])
-@pytest.mark.parametrize("n", [1, 130])
+@pytest.mark.parametrize("n", [1, 130, 520])
 def test_run_rows(cuda, kind, n):
     q, kv, length = case(4, 2, 2, n, 333, kind, 14)
     _, pre, pre_length = case(1, 2, 2, 1, 500, kind, 15)
