@@ -93,25 +93,22 @@ DH_DEVINL float pow2(int32_t n) { return __uint_as_float(static_cast<uint32_t>(n
 // e with 2^(e - 1) <= x < 2^e for the normal fp32 with these bits
 DH_DEVINL int32_t exponent_of(uint32_t bits) { return static_cast<int32_t>((bits >> 23) & 0xFFu) - 126; }
 
-// 16 codes -> 16 f16 of code * ratio * 2^-9, where f = f16(ratio * 2^15): a code
-// plus 128 as the bits of a subnormal f16 is (code + 128) 2^-24, so one FMA with
-// f and -f 2^-17 (exact, a power of two) takes the 128 off and scales, with one
-// rounding.
+// 4 codes -> 4 f16 of code * ratio * 2^-9, where f = f16(ratio * 2^15): a code plus
+// 128 as the bits of a subnormal f16 is (code + 128) 2^-24, so one FMA with f and off =
+// -f 2^-17 (exact, a power of two) takes the 128 off and scales, with one rounding.
+DH_DEVINL void convert4(uint32_t codes, __half2 f, __half2 off, uint32_t& lo, uint32_t& hi) {
+    const uint32_t u = codes ^ 0x80808080u;
+    const uint32_t p = __byte_perm(u, 0u, 0x4140u), q = __byte_perm(u, 0u, 0x4342u);
+    const __half2 x = __hfma2(*reinterpret_cast<const __half2*>(&p), f, off);
+    const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&q), f, off);
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
+}
 DH_DEVINL void convert16(const uint4& codes, __half2 f, __half2 off, uint4& lo, uint4& hi) {
-    const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-    uint32_t o[8];
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t u = w[i] ^ 0x80808080u;
-#pragma unroll
-        for (uint32_t h = 0; h < 2; ++h) {
-            uint32_t p = __byte_perm(u, 0u, h ? 0x4342u : 0x4140u);
-            __half2 x = __hfma2(*reinterpret_cast<__half2*>(&p), f, off);
-            o[2 * i + h] = *reinterpret_cast<uint32_t*>(&x);
-        }
-    }
-    lo = make_uint4(o[0], o[1], o[2], o[3]);
-    hi = make_uint4(o[4], o[5], o[6], o[7]);
+    convert4(codes.x, f, off, lo.x, lo.y);
+    convert4(codes.y, f, off, lo.z, lo.w);
+    convert4(codes.z, f, off, hi.x, hi.y);
+    convert4(codes.w, f, off, hi.z, hi.w);
 }
 
 struct Item {

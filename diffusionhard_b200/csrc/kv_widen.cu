@@ -1,10 +1,10 @@
 // kv_widen.cu -- an int8 K/V cache as f16 rows, for attention with many tiles of rows.
 //
 // The tensor-core kernel over int8 turns codes into f16 tiles as it goes, once for
-// every 128 rows: 32 canvases of 1024 queries and keys take 237 us that way and XXX us
+// every 128 rows: 32 canvases of 1024 queries and keys take 237 us that way and 154 us
 // over 16-bit keys.  Where every key is visited by at least four tiles of rows, the
-// codes are turned once, here, into the workspace.  Bound by HBM: 136 bytes in and 256
-// out for each position and K/V head.
+// codes are turned once, here, into the workspace (together 196.5 us).  Bound by HBM:
+// 136 bytes in and 256 out for each position and K/V head.
 //
 // A line is an (entry, head).  Its K becomes code * scale * 2^-(E + 9) with E the
 // exponent of the line's largest scale, rounded once to f16 (its factor scale 2^(15 -
@@ -79,19 +79,37 @@ __global__ void __launch_bounds__(kThreads) kv_widen_kernel(const __grid_constan
         to.exps[line] = make_float2(pow2(min(ek + 9, 127)), __int_as_float(ev + 9));
     const float fk = pow2(15 - ek), fv = pow2(15 - ev);
     const uint32_t tiles = (len + kKT - 1) / kKT;
-    const uint32_t row = threadIdx.x / 4, c = threadIdx.x & 3u;  // 16 codes of a row a thread
-    for (uint32_t t = chunk; t < tiles; t += chunks) {
-        const uint64_t pos = at + t * kKT + row;
-        const bool live_row = t * kKT + row < len;
+    // 8 codes of a row a thread, so that a warp writes whole lines; the loads of four
+    // half tiles of K and V are under way together
+    const uint32_t row = threadIdx.x / 8, c = threadIdx.x & 7u;
+    constexpr uint32_t kAhead = 4;
+    for (uint32_t t0 = chunk; t0 < tiles; t0 += kAhead / 2 * chunks) {
+        uint2 codes[kAhead][2];
+        float scale[kAhead][2];
 #pragma unroll
-        for (uint32_t side = 0; side < 2; ++side) {
-            const uint4 codes = __ldcs(reinterpret_cast<const uint4*>((side ? s.v : s.k) + pos * kDh) + c);
-            const float scale = live_row ? (side ? s.v_scale : s.k_scale)[pos] : 0.f;
-            const __half2 f = __float2half2_rn(scale * (side ? fv : fk));
-            uint4 lo, hi;
-            convert16(codes, f, __hmul2(f, __half2half2(__ushort_as_half(0x8080))), lo, hi);
-            uint4* dst = reinterpret_cast<uint4*>((side ? to.v : to.k) + pos * kDh) + 2 * c;
-            dst[0] = lo, dst[1] = hi;
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            const uint32_t t = t0 + i / 2 * chunks, key = t * kKT + (i & 1u) * 32 + row;
+#pragma unroll
+            for (uint32_t side = 0; side < 2; ++side) {
+                codes[i][side] = make_uint2(0, 0);
+                if (t < tiles)
+                    codes[i][side] = __ldcs(reinterpret_cast<const uint2*>((side ? s.v : s.k) + (at + key) * kDh) + c);
+                scale[i][side] = t < tiles && key < len ? (side ? s.v_scale : s.k_scale)[at + key] : 0.f;
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            const uint32_t t = t0 + i / 2 * chunks, key = t * kKT + (i & 1u) * 32 + row;
+            if (t >= tiles) break;
+#pragma unroll
+            for (uint32_t side = 0; side < 2; ++side) {
+                const __half2 f = __float2half2_rn(scale[i][side] * (side ? fv : fk));
+                const __half2 off = __hmul2(f, __half2half2(__ushort_as_half(0x8080)));
+                uint4 x;
+                convert4(codes[i][side].x, f, off, x.x, x.y);
+                convert4(codes[i][side].y, f, off, x.z, x.w);
+                reinterpret_cast<uint4*>((side ? to.v : to.k) + (at + key) * kDh)[c] = x;
+            }
         }
     }
 }
@@ -104,9 +122,10 @@ uint32_t launch_widen(const Args& a, const WideKeys& prefix, const WideKeys& own
     w.sequences = a.sequences, w.prefixes = prefixes, w.with_prefix = prefixes != 0;
     w.kv_heads = a.kv_heads, w.queries = a.queries, w.per_prefix = a.per_prefix;
     w.run_rows = a.run_rows;
-    // four CTAs an SM; every one reads all scales of its line
+    // eight CTAs an SM (196.5 us for 32 canvases, 198 with four, 199.5 with 16): every one
+    // reads all scales of its line
     const auto chunks = [](uint64_t lines, uint32_t capacity) {
-        return static_cast<uint32_t>(std::min<uint64_t>((4 * device_sms() + lines - 1) / lines, capacity / kKT));
+        return static_cast<uint32_t>(std::min<uint64_t>((8 * device_sms() + lines - 1) / lines, capacity / kKT));
     };
     const uint64_t own_lines = static_cast<uint64_t>(a.sequences) * a.kv_heads.d;
     const uint64_t prefix_lines = static_cast<uint64_t>(prefixes) * a.kv_heads.d;
