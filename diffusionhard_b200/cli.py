@@ -137,6 +137,7 @@ def build_parser() -> argparse.ArgumentParser:
     turn.add_argument("--seed", type=int, default=0)
     turn.add_argument("--local-files-only", action="store_true")
     turn.add_argument("--weights-seed", type=int, default=0)
+    turn.add_argument("--int8-kv", action="store_true", help="hold the retained K/V in 8 bits")
 
     export = sub.add_parser("export-mdlm-hardware-package",
                             help="export 64-token goldens and constant-folded FP16 weights")
@@ -348,7 +349,7 @@ def main(argv: Optional[List[str]] = None) -> int:
             prefix_tokens=args.prefix_tokens, first_answer_tokens=args.first_answer_tokens,
             followup_tokens=args.followup_tokens, second_answer_tokens=args.second_answer_tokens,
             samples=args.samples, steps=args.steps, seed=args.seed, weights_seed=args.weights_seed,
-            device=args.device)
+            device=args.device, int8_kv=args.int8_kv)
         result.update(_checkpoint_note(args))
         result["dataset"] = {"id": args.dataset_id, "config": args.dataset_config, "revision": args.dataset_revision,
                              "split": args.split, "used": False,

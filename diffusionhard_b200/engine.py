@@ -68,11 +68,20 @@ class MDLMEngine:
     engine (seq_len = P, kv_len = P, offset 0: the isolated prefix) and a
     suffix engine (seq_len = S, pos_offset = P, kv_offset = P,
     kv_len = P + S): the prefix K / V are written once and never recomputed.
+
+    Two other forms of the keys run through kvcache.attend instead of
+    dh_attention.  ``int8_kv``: a kvcache.KVCacheI8 for each block holds the
+    keys; the forward quantises its rows into it at `kv_offset` and attends
+    over its first `kv_len` positions.  ``prefix_kv``: keys before those, for
+    each block K / V^T buffers as above, or with `int8_kv` KVCacheI8s, of
+    `prefix_len` positions and one entry for each group of consecutive
+    sequences (one for a prefix that the whole batch shares).
     """
 
     def __init__(self, qm: QuantizedMDLM, batch: int, seq_len: int, device: Any = "cuda", *,
                  pos_offset: int = 0, kv_len: Optional[int] = None, kv_offset: int = 0,
-                 kv_buffers: Optional[List[tuple]] = None) -> None:
+                 kv_buffers: Optional[List[tuple]] = None, int8_kv: Optional[list] = None,
+                 prefix_kv: Optional[list] = None, prefix_len: int = 0) -> None:
         import torch
 
         self.torch = torch
@@ -105,6 +114,18 @@ class MDLMEngine:
         self.act_q = torch.empty((M, 3072), dtype=torch.int8, device=d)
         self.act_scale = torch.empty(M, dtype=torch.float32, device=d)
         self.q = torch.empty((batch, H, seq_len, 64), dtype=bf16, device=d)
+        self.int8_kv, self.prefix_kv, self.prefix_len = int8_kv, prefix_kv, prefix_len
+        if int8_kv is not None:
+            if kv_buffers is not None:
+                raise ValueError("keys are held in int8_kv or in kv_buffers")
+            if len(int8_kv) != len(self.blocks) or kv_offset + seq_len > int8_kv[0].capacity or \
+                    kv_len > int8_kv[0].capacity:
+                raise ValueError("int8_kv must hold a cache of kv_len positions for each block")
+            # a forward's rows on their way into the cache, one block's at a time
+            kv_buffers = [(torch.empty((batch, H, seq_len, 64), dtype=bf16, device=d),
+                           torch.empty((batch, H, 64, seq_len), dtype=torch.float16, device=d))] * len(self.blocks)
+        if prefix_kv is not None and (len(prefix_kv) != len(self.blocks) or prefix_len <= 0):
+            raise ValueError("prefix_kv must hold the keys of each block, prefix_len of them")
         if kv_buffers is None:
             # zeros: attention reads whole 128-key tiles and needs finite V
             # past kv_len (the keys there are masked)
@@ -113,7 +134,8 @@ class MDLMEngine:
             kv_buffers = [(k, vt)] * len(self.blocks)
         self.kv_buffers = kv_buffers
         self.kv_stride = kv_buffers[0][0].shape[2]
-        if kv_offset + seq_len > self.kv_stride or kv_len > self.kv_stride:
+        self._kv_row = 0 if int8_kv is not None else kv_offset  # of the K / V^T buffers that a forward writes
+        if int8_kv is None and (kv_offset + seq_len > self.kv_stride or kv_len > self.kv_stride):
             raise ValueError("K / V buffers too short")
         self.attn = torch.empty((M, 768), dtype=bf16, device=d)
         self.mlp = torch.empty((M, 3072), dtype=bf16, device=d)
@@ -205,12 +227,32 @@ class MDLMEngine:
             _lib.call("dh_embed_gather", self._p(tok), self._p(self.embedding), self._p(self.x), self.M,
                       self.cfg.vocab_size, rr, s)
         for i, blk in enumerate(self.blocks):
-            self._forward_block(i, blk, rr, s)
+            self._forward_block(i, blk, rr, s, run_rows)
             if hook is not None:
                 hook(i)
         self._whole_forward = run_rows is None and seq_list is None
 
-    def _forward_block(self, i: int, blk: dict, rr: Any, s: Any) -> None:
+    def _attend(self, i: int, k: Any, vt: Any, rr: Any, s: Any, run_rows: Any) -> None:
+        if self.int8_kv is None and self.prefix_kv is None:
+            _lib.call("dh_attention", self._p(self.q), self._p(k), self._p(vt), self._p(self.attn), self.B, self.L,
+                      self.kv_len, self.kv_stride, rr, s)
+            return
+        from .kvcache import attend, write_kv
+
+        if run_rows is not None:
+            run_rows = run_rows.view(self.torch.int32)
+        prefix = None if self.prefix_kv is None else self.prefix_kv[i]
+        if self.int8_kv is not None:
+            keys = self.int8_kv[i]
+            write_kv(keys, k, vt.transpose(2, 3), self.kv_offset, run_rows=run_rows)
+        else:
+            keys = (k, vt.transpose(2, 3))
+            if prefix is not None:
+                prefix = (prefix[0], prefix[1].transpose(2, 3))
+        attend(self.q, keys, self.kv_len, prefix=prefix, prefix_lengths=self.prefix_len if prefix is not None else None,
+               out=self.attn, run_rows=run_rows)
+
+    def _forward_block(self, i: int, blk: dict, rr: Any, s: Any, run_rows: Any) -> None:
         M, L = self.M, self.L
         p = self._p
         call = _lib.call
@@ -219,10 +261,9 @@ class MDLMEngine:
         call("dh_ln_smooth_quant", p(self.x), p(qkv.smooth), p(qkv.inv_smooth), p(self.act_q), p(self.act_scale), M,
              None, None, rr, s)
         call("dh_gemm_qkv_rope", p(self.act_q), p(self.act_scale), p(qkv.w), p(qkv.w_scale), p(qkv.bias),
-             p(self.rope_cos), p(self.rope_sin), p(out.inv_smooth), M, L, self.pos_offset, self.kv_stride, self.kv_offset,
+             p(self.rope_cos), p(self.rope_sin), p(out.inv_smooth), M, L, self.pos_offset, self.kv_stride, self._kv_row,
              p(self.q), p(k), p(vt), rr, s)
-        call("dh_attention", p(self.q), p(k), p(vt), p(self.attn), self.B, L, self.kv_len, self.kv_stride,
-             rr, s)
+        self._attend(i, k, vt, rr, s, run_rows)
         call("dh_quant_rows_bf16", p(self.attn), None, None, p(self.act_q), p(self.act_scale), M,
              768, rr, s)
         call("dh_gemm_residual", p(self.act_q), p(self.act_scale), p(out.w), p(out.w_scale), p(out.bias),
@@ -393,6 +434,8 @@ class MDLMEngine:
         refilling sequences: as set in `compact`, else when the batch holds
         several sequences and fewer than 4 reveals per transition are expected
         (L < 4 steps), so that a sequence often goes a transition unchanged."""
+        if self.int8_kv is not None or (self.prefix_kv is not None and self.prefix_kv[0][0].shape[0] > 1):
+            return False  # (an entry of the keys belongs to its sequence, not to a packed position)
         if self.compact is not None:
             return bool(self.compact)
         return self.B > 1 and self.L < 4 * steps
@@ -454,9 +497,11 @@ class MDLMEngine:
 
     def native_loop_ok(self) -> bool:
         """Whether dh_sample_loop covers this engine's configuration: whole
-        canvases (no prefix K/V offsets), no Python hooks, and a head that is
+        canvases (no prefix K/V offsets, no int8 or shared keys), no Python hooks, and a head that is
         whole or merged over NCCL."""
         if self.pre_forward is not None or self.head_reduce is not None:
+            return False
+        if self.int8_kv is not None or self.prefix_kv is not None:
             return False
         if self.pos_offset or self.kv_offset or self.kv_len != self.L or self.kv_stride != self.L:
             return False

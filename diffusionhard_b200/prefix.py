@@ -52,21 +52,53 @@ def tensor_drift_metrics(reference: Any, changed: Any) -> Dict[str, object]:
 
 
 class PrefixConditionedGenerator:
-    """B sequences of a clean prefix (P positions) and a generated suffix (S)."""
+    """B sequences of a clean prefix (P positions) and a generated suffix (S).
+
+    ``prefixes``: how many different prefixes there are, each of B / prefixes
+    consecutive sequences (default: one a sequence).  Given, their K / V are
+    computed and held once each, apart from the suffixes', and `prefix_ids` is
+    [prefixes, P].  ``int8_kv`` (with `prefixes`): all K / V in 8 bits
+    (kvcache.KVCacheI8)."""
 
     def __init__(self, qm: QuantizedMDLM, batch: int, prefix_len: int, suffix_len: int,
-                 device: Any = "cuda") -> None:
+                 device: Any = "cuda", *, prefixes: Optional[int] = None, int8_kv: bool = False) -> None:
         self.qm = qm
         self.B, self.P, self.S = batch, prefix_len, suffix_len
+        self.prefixes = prefixes
+        if prefixes is not None:
+            if prefixes <= 0 or batch % prefixes:
+                raise ValueError(f"{prefixes} prefixes do not divide {batch} sequences")
+            self._hold_prefixes(prefixes, device, int8_kv)
+            return
+        if int8_kv:
+            raise ValueError("int8_kv needs the number of prefixes")
         self.kv = MDLMEngine.kv_cache(qm, batch, prefix_len + suffix_len, device)
         self.prefix = MDLMEngine(qm, batch, prefix_len, device, kv_len=prefix_len, kv_buffers=self.kv)
         self.suffix = MDLMEngine(qm, batch, suffix_len, device, pos_offset=prefix_len,
                                  kv_len=prefix_len + suffix_len, kv_offset=prefix_len, kv_buffers=self.kv)
         self.prefix_forwards = 0
 
+    def _hold_prefixes(self, prefixes: int, device: Any, int8_kv: bool) -> None:
+        qm, P, S = self.qm, self.P, self.S
+        if int8_kv:
+            from .kvcache import KVCacheI8
+
+            self.kv = [KVCacheI8.empty(prefixes, qm.config.heads, P, device) for _ in qm.blocks]
+            own = [KVCacheI8.empty(self.B, qm.config.heads, S, device)] * len(qm.blocks)
+            self.prefix = MDLMEngine(qm, prefixes, P, device, int8_kv=self.kv)
+            self.suffix = MDLMEngine(qm, self.B, S, device, pos_offset=P, int8_kv=own, prefix_kv=self.kv, prefix_len=P)
+        else:
+            self.kv = MDLMEngine.kv_cache(qm, prefixes, P, device)
+            self.prefix = MDLMEngine(qm, prefixes, P, device, kv_buffers=self.kv)
+            self.suffix = MDLMEngine(qm, self.B, S, device, pos_offset=P, prefix_kv=self.kv, prefix_len=P)
+        self.prefix_forwards = 0
+
     def set_prefix(self, prefix_ids: Any) -> None:
         """Compute and keep the prefix K/V of every block (one forward)."""
         import torch
+
+        if prefix_ids.numel() != self.prefix.M:
+            raise ValueError(f"prefix_ids must be [{self.prefix.B}, {self.P}]")
 
         self.prefix.tokens.copy_(prefix_ids.to(self.prefix.device, torch.int32).reshape(-1))
         self.prefix.forward()
@@ -90,6 +122,8 @@ class PrefixConditionedGenerator:
         bidirectional forward over [prefix ; suffix] gives the prefix rows."""
         import torch
 
+        if self.prefixes is not None:
+            raise ValueError("the drift report needs a prefix of every sequence's own (no `prefixes`)")
         qm, B, P, S = self.qm, self.B, self.P, self.S
         full = MDLMEngine(qm, B, P + S, self.prefix.device)
         full.tokens.copy_(torch.cat([prefix_ids, suffix_ids], dim=1).to(full.device, torch.int32).reshape(-1))

@@ -24,6 +24,10 @@ The two generate paths run the same arithmetic and must agree token for
 token.
 
 Block lengths are multiples of 32, the kernels' row granule.
+
+With ``int8_kv`` the retained K/V are held in 8 bits (kvcache.KVCacheI8), 136
+bytes for each position, head and block instead of 256: a forward quantises the
+rows it makes and attends over the cache, its own rows among them.
 """
 
 from __future__ import annotations
@@ -38,7 +42,8 @@ from .model import QuantizedMDLM
 class BlockCausalSession:
     """`batch` sequences sharing one block layout, up to `capacity` tokens."""
 
-    def __init__(self, qm: QuantizedMDLM, batch: int, capacity: int, device: Any = "cuda") -> None:
+    def __init__(self, qm: QuantizedMDLM, batch: int, capacity: int, device: Any = "cuda", *,
+                 int8_kv: bool = False) -> None:
         import torch
 
         if capacity % 32 or capacity <= 0:
@@ -46,7 +51,13 @@ class BlockCausalSession:
         if capacity > qm.config.max_positions:
             raise ValueError("session exceeds the model length")
         self.qm, self.B, self.capacity = qm, batch, capacity
-        self.kv = MDLMEngine.kv_cache(qm, batch, capacity, device)
+        self.int8_kv = int8_kv
+        if int8_kv:
+            from .kvcache import KVCacheI8
+
+            self.kv = [KVCacheI8.empty(batch, qm.config.heads, capacity, device) for _ in qm.blocks]
+        else:
+            self.kv = MDLMEngine.kv_cache(qm, batch, capacity, device)
         self.device = torch.device(device)
         self.blocks: List[Tuple[int, int, Any]] = []  # (start, end, device int32 ids [B * n])
         self._engines: Dict[Tuple[int, int], MDLMEngine] = {}
@@ -69,8 +80,8 @@ class BlockCausalSession:
         key = (start, n)
         e = self._engines.get(key)
         if e is None:
-            e = MDLMEngine(self.qm, self.B, n, self.device, pos_offset=start, kv_len=start + n, kv_offset=start,
-                           kv_buffers=self.kv)
+            held = {"int8_kv": self.kv} if self.int8_kv else {"kv_buffers": self.kv}
+            e = MDLMEngine(self.qm, self.B, n, self.device, pos_offset=start, kv_len=start + n, kv_offset=start, **held)
             self._engines[key] = e
         return e
 
@@ -130,9 +141,11 @@ class BlockCausalSession:
         return e.tokens.view(self.B, n).to(torch.long).clone(), e.metadata(steps), wall, evals
 
     def kv_bytes(self, tokens: Optional[int] = None) -> int:
-        """K (bf16) and V (f16) bytes held for `tokens` positions."""
+        """K (bf16) and V (f16), or int8 with their scales: bytes held for `tokens` positions."""
         t = self.length if tokens is None else tokens
         cfg = self.qm.config
+        if self.int8_kv:
+            return sum(c.nbytes(t) for c in self.kv)
         return 2 * cfg.blocks * self.B * t * cfg.hidden * 2
 
 
@@ -163,7 +176,7 @@ def evaluate_two_turn_mdlm_session(*, quantized: Optional[QuantizedMDLM] = None,
                                    first_answer_tokens: int = 32, followup_tokens: int = 32,
                                    second_answer_tokens: int = 32, samples: int = 3, steps: int = 64,
                                    seed: int = 0, weights_seed: int = 0, windows: Any = None,
-                                   device: Any = "cuda") -> Dict[str, object]:
+                                   device: Any = "cuda", int8_kv: bool = False) -> Dict[str, object]:
     """Two answer blocks in a block-causal session, each generated by full
     block-isolated recompute and over retained K/V; the report of
     multiturn.evaluate_two_turn_mdlm_session (multiturn.py:146-642).
@@ -173,7 +186,7 @@ def evaluate_two_turn_mdlm_session(*, quantized: Optional[QuantizedMDLM] = None,
     answer is then finalised (one forward appends its K/V), the follow-up is
     prefilled, and turn 2 is generated both ways.  The noise is keyed by
     canvas position and sequence, so the recompute and cached paths must
-    agree exactly."""
+    agree exactly.  ``int8_kv`` holds the session's K/V in 8 bits."""
     import torch
 
     from .model import MDLMConfig, build_quantized
@@ -196,7 +209,7 @@ def evaluate_two_turn_mdlm_session(*, quantized: Optional[QuantizedMDLM] = None,
     windows = torch.as_tensor(windows, dtype=torch.long)
     if tuple(windows.shape) != (samples, total):
         raise ValueError("windows must be [samples, total session tokens]")
-    sess = BlockCausalSession(qm, 1, total, device)
+    sess = BlockCausalSession(qm, 1, total, device, int8_kv=int8_kv)
     dev = sess.device
 
     results = []
@@ -276,6 +289,7 @@ def evaluate_two_turn_mdlm_session(*, quantized: Optional[QuantizedMDLM] = None,
         "windows": "seeded uniform token ids" if synthetic else "supplied",
         "session_shape": {"initial_prefix_tokens": P, "first_answer_tokens": A1, "followup_tokens": F,
                           "second_answer_tokens": A2, "final_session_tokens": total},
+        "kv_cache": "int8" if int8_kv else "16-bit",
         "steps_per_answer": steps,
         "samples": samples,
         "aggregate": {
