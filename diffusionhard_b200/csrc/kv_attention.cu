@@ -67,7 +67,8 @@ struct Cfg {
     static constexpr uint32_t ones_at = v_at + v_stages * kVPitch;
     static constexpr uint32_t raw_at = ones_at + kOnesBytes;
     static constexpr uint32_t bars_at = raw_at + raw_stages * kRawBytes;
-    static constexpr uint32_t bytes = 1024 + bars_at + 512;
+    static constexpr uint32_t order_at = bars_at + 512;  // lengths, then their order
+    static constexpr uint32_t bytes = 1024 + order_at + kOrdered * 6;
 };
 
 enum Bar : uint32_t {
@@ -143,8 +144,8 @@ DH_DEVINL void zero_rows(uint8_t* tile, uint32_t left, uint32_t transposed, uint
 
 // Item w of both classes, `first` the number of the first class's (0: they are not
 // this kernel's).
-DH_DEVINL Item item_at(const Args& a, uint32_t first, uint32_t w, uint32_t live) {
-    return w < first ? item_of(a, a.cls[0], w, live) : item_of(a, a.cls[1], w - first, live);
+DH_DEVINL Item item_at(const Args& a, uint32_t first, uint32_t w, uint32_t live, const uint16_t* order) {
+    return w < first ? item_of(a, a.cls[0], w, live, order) : item_of(a, a.cls[1], w - first, live, order);
 }
 
 template <int KIND>
@@ -167,8 +168,10 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + kNumBars);
     int32_t* exps = reinterpret_cast<int32_t*>(tmem_holder + 2);  // [kExpRing][2]: K, V of a tile
 
+    uint16_t* order = reinterpret_cast<uint16_t*>(smem + C::order_at + kOrdered * 4);
     const uint32_t warp = warp_id(), lane = lane_id();
     grid_launch_dependents();
+    if (a.cls[1].ordered) order_sequences(a, reinterpret_cast<uint32_t*>(smem + C::order_at), order);
 
     if (warp == 0 && lane == 0) {
         for (uint32_t i = 0; i < kNumBars; ++i) {
@@ -218,7 +221,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
             uint32_t g = 0;
             bool ok = true;
             for (uint32_t w = blockIdx.x; w < total && ok; w += gridDim.x) {
-                const Item it = item_at(a, first, w, live);
+                const Item it = item_at(a, first, w, live, order);
                 for (uint32_t j = it.t0; j < it.t1; ++j, ++g) {
                     const bool own = j >= it.n0;
                     const uint32_t key = (own ? j - it.n0 : j) * kKT;
@@ -297,7 +300,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
             uint32_t g = 0, n_items = 0;
             bool ok = true;
             for (uint32_t w = blockIdx.x; w < total && ok; w += gridDim.x) {
-                const Item it = item_at(a, first, w, live);
+                const Item it = item_at(a, first, w, live, order);
                 if (it.t0 == it.t1) continue;
                 if (!tc::mbar_wait_suspend(&bars[kQReady], n_items & 1u, tc::kErrTimeoutFull)) break;
                 tc::tc_fence_after();
@@ -346,7 +349,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
             // ---------------------------------------------------- conversion
             const uint32_t half = warp - 2;
             for (uint32_t w = blockIdx.x; w < total && ok; w += gridDim.x) {
-                const Item it = item_at(a, first, w, live);
+                const Item it = item_at(a, first, w, live, order);
                 int32_t ev = -1000;
                 for (uint32_t j = it.t0; j < it.t1; ++j, ++g) {
                     const uint32_t rs = g % C::raw_stages, ks = g % C::k_stages, vs = g % C::v_stages;
@@ -432,7 +435,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
         // shared memory.
         auto next_item = [&](uint32_t& w, Item& it) {
             for (; w < total; w += gridDim.x) {
-                it = item_at(a, first, w, live);
+                it = item_at(a, first, w, live, order);
                 if (it.t0 != it.t1) break;
                 if (r < it.rows) write_empty(row_index(a, it, r, nullptr), it.slot);
             }
@@ -822,7 +825,7 @@ void split_many(Class* cls, const uint64_t* items, const uint32_t* tiles, uint32
 }
 
 Plan plan_of(uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t prefixes, uint32_t prefix_keys,
-             uint32_t own_keys, bool int8, uint32_t sms) {
+             uint32_t own_keys, bool int8, bool ragged, uint32_t sms) {
     Plan p{};
     const uint32_t per = prefixes ? sequences / prefixes : sequences;
     const bool stacked = prefixes && per > 1 && rows < kStackBelow;
@@ -858,6 +861,9 @@ Plan plan_of(uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t pref
     for (int i = 0; i < 2; ++i) {
         if (!items[i]) continue;
         Class& c = p.cls[i];
+        // (where all items start at once their order does not matter)
+        const uint64_t ctas = p.few[i] ? (p.cluster[i] ? items[i] * c.splits.d * p.cluster[i] : ~0ull) : items[i] * c.splits.d;
+        c.ordered = i && ragged && sequences <= kOrdered && ctas > (p.few[i] ? 3ull : 2ull) * sms;
         c.items = static_cast<uint32_t>(items[i] * c.splits.d);
         c.slot = p.slots;
         p.slots += c.splits.d;
@@ -977,7 +983,7 @@ extern "C" size_t dh_kv_attention_workspace_size(uint32_t sequences, uint32_t qu
         !fits(sequences, queries, heads, kv_heads, prefixes))
         return 0;
     const Plan p = plan_of(sequences, queries * (heads / kv_heads), kv_heads, prefixes, prefix_capacity, own_capacity,
-                           k_type == DH_TYPE_I8, device_sms());
+                           k_type == DH_TYPE_I8, false, device_sms());
     return layout_of(p, static_cast<uint64_t>(sequences) * queries * heads, kv_heads, {prefixes, sequences},
                      {prefix_capacity, own_capacity})
         .bytes;
@@ -1006,7 +1012,7 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
     const uint32_t ratio = heads / kv_heads;
     const uint64_t rows = static_cast<uint64_t>(sequences) * queries * heads;
     const Plan p = plan_of(sequences, queries * ratio, kv_heads, prefixes, prefixes ? prefix->capacity : 0,
-                           own->capacity, int8, device_sms());
+                           own->capacity, int8, own->lengths != nullptr, device_sms());
     const Layout l = layout_of(p, rows, kv_heads, {prefixes, sequences}, {prefixes ? prefix->capacity : 0, own->capacity});
     const size_t need = l.bytes;
     if (need && !workspace) return DH_ERR_NULL_POINTER;

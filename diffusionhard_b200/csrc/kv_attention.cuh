@@ -26,6 +26,7 @@ struct Class {
     uint32_t tile_rows, items, slot;     // rows of an item; all items; the first part's slot
     FastDiv row_tiles, splits;           // items a group and K/V head; parts of the keys
     uint32_t with_prefix, with_own;
+    uint32_t ordered;                    // the longest sequences' items come first
 };
 
 struct Segment {
@@ -122,13 +123,34 @@ DH_DEVINL uint32_t length_of(const Segment& s, uint32_t entry) {
     return static_cast<uint32_t>(min(max(n, 0), static_cast<int32_t>(s.capacity)));
 }
 
+// Sequences by falling length (the lower index first among equals) into order[],
+// by the CTA's first kOrdered threads; all threads call it.  Items of long sequences
+// that start last would run alone.
+constexpr uint32_t kOrdered = 128;
+DH_DEVINL void order_sequences(const Args& a, uint32_t* lengths, uint16_t* order) {
+    const uint32_t n = a.sequences, t = threadIdx.x;
+    uint32_t mine = 0;
+    if (t < n) lengths[t] = mine = length_of(a.own, t);
+    __syncthreads();
+    if (t < n) {
+        uint32_t rank = 0;
+        for (uint32_t u = 0; u < n; ++u) {
+            const uint32_t other = lengths[u];
+            rank += other > mine || (other == mine && u < t);
+        }
+        order[rank] = static_cast<uint16_t>(t);
+    }
+    __syncthreads();
+}
+
 // Item w of a class, of the first `live` sequences.
-DH_DEVINL Item item_of(const Args& a, const Class& c, uint32_t w, uint32_t live) {
+DH_DEVINL Item item_of(const Args& a, const Class& c, uint32_t w, uint32_t live, const uint16_t* order) {
     Item it;
     uint32_t split = w, tile, head;
     tile = c.splits.split(split);
     head = c.row_tiles.split(tile);
-    const uint32_t group = a.kv_heads.split(head);
+    uint32_t group = a.kv_heads.split(head);
+    if (c.ordered) group = order[group];
     it.kv_head = head;
     it.seq0 = group * c.seqs;
     it.slot = c.slot + split;

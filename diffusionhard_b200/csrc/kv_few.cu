@@ -49,7 +49,7 @@ enum Kind : int { kV16 = 0, kVBf16 = 1, kInt8 = 2 };
 template <int KIND>
 constexpr uint32_t kStageBytes = KIND == kInt8 ? kRawBytes : 2 * kTileBytes;
 template <int KIND>
-constexpr uint32_t kSmem = 1024 + kWarps * kStages * kStageBytes<KIND> + 128;
+constexpr uint32_t kSmem = 1024 + kWarps * kStages * kStageBytes<KIND> + 128 + kOrdered * 6;
 
 template <bool BF16>
 DH_DEVINL void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -154,6 +154,9 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
     const Class& cl = a.cls[cls];
     grid_launch_dependents();
     const bool solo = cluster == 0;
+    uint32_t* lengths = reinterpret_cast<uint32_t*>(all_bars + 16);
+    uint16_t* order = reinterpret_cast<uint16_t*>(lengths + kOrdered);
+    if (cl.ordered) order_sequences(a, lengths, order);
     const uint32_t rank = cluster > 1 ? cluster_rank() : 0u;
 
     uint8_t* ring = smem + warp * kStages * kStageBytes<KIND>;
@@ -170,7 +173,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
     const uint32_t next_item = solo ? gridDim.x * kWarps : cl.items;
     const uint32_t step = solo ? 1u : kWarps;
     auto item_at = [&](uint32_t w) {
-        Item it = item_of(a, cl, w, live);
+        Item it = item_of(a, cl, w, live, order);
         if (!solo) {
             const uint32_t n = it.t1 - it.t0;
             it.t1 = it.t0 + n * (rank + 1) / cluster;
