@@ -24,7 +24,7 @@
 //             TMEM, where a column of ones beside V sums P
 //   warps 2-3 int8 alone: codes to f16 tiles, see convert_rows
 //   four more softmax, a thread a row: P = 2^(s c - m) over S in TMEM; O in TMEM
-//             is rescaled only when the maximum grew by more than 2^15 (2^60 for bf16)
+//             is rescaled only when the maximum grew by more than 2^15
 #include <cuda.h>
 
 #include "kv_kernels.h"
@@ -77,6 +77,8 @@ enum Bar : uint32_t {
     kOFree, kQReady, kDrain, kNumBars
 };
 static_assert(kNumBars * 8 + 8 + 2 * kExpRing * 4 <= 512, "barrier area");
+static_assert(Cfg<0>::bars_at >= kRows * (kSumPitch * 4 + 8) && Cfg<2>::bars_at >= kRows * (kSumPitch * 4 + 8),
+              "a CTA's sums lie below the barriers");
 
 DH_DEVINL void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -99,8 +101,7 @@ DH_DEVINL float2 exp2_poly2(float2 x) {
 // The maximum that P is relative to stays until it grew by more than this power of
 // two, P's largest value meanwhile (f16 ends at 2^16).  32 canvases over int8, scores
 // of a few: 245 us at 8, 237 at 15; 128 x 512 queries over 1024 16-bit keys 325 and 305.
-template <int KIND>
-constexpr float kMaxGrowth = KIND == kVBf16 ? 60.f : 15.f;
+constexpr float kMaxGrowth = 15.f;
 constexpr uint32_t kPolyPairMask = 0x11u;  // pairs e with bit e % 8 set
 
 // Half of a tile's 64 rows of codes (those of this warp) into a 128-byte
@@ -148,11 +149,13 @@ DH_DEVINL Item item_at(const Args& a, uint32_t first, uint32_t w, uint32_t live,
     return w < first ? item_of(a, a.cls[0], w, live, order) : item_of(a, a.cls[1], w - first, live, order);
 }
 
-template <int KIND>
+// CLUSTER: the CTAs of a cluster (`cluster` of them) have an item's parts and join them.
+template <int KIND, bool CLUSTER>
 __global__ void __launch_bounds__(Cfg<KIND>::threads, 2)
 kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ CUtensorMap tpv,
                     const __grid_constant__ CUtensorMap tok, const __grid_constant__ CUtensorMap tov,
-                    const __grid_constant__ Args a, const uint32_t first, const uint32_t total) {
+                    const __grid_constant__ Args a, const uint32_t first, const uint32_t total,
+                    const uint32_t cluster) {
     using C = Cfg<KIND>;
     const uint32_t live = a.run_rows ? min(a.sequences, a.queries.of(min(*a.run_rows, 0x7FFFFFFFu))) : a.sequences;
     if (live == 0) return;
@@ -160,6 +163,10 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~static_cast<uintptr_t>(1023));
     uint8_t* q_s = smem + C::q_at;
+    // (a cluster's CTAs join their sums through shared memory, which is theirs alone
+    // once a CTA's one item is done)
+    float* sums_s = reinterpret_cast<float*>(smem);
+    float2* ml_s = reinterpret_cast<float2*>(smem + kRows * kSumPitch * 4);
     uint8_t* k_ring = smem + C::k_at;
     uint8_t* v_ring = smem + C::v_at;
     uint8_t* ones = smem + C::ones_at;
@@ -419,8 +426,15 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
         const uint32_t lane_base = (quad * 32u) << 16;
         uint8_t* my_q = q_s + r * 128;
 
-        // Row `row` of slot `slot` has no keys.
+        // Row `row` of slot `slot` has no keys.  (Sums in shared memory: see below.)
         auto write_empty = [&](uint64_t row, uint32_t slot) {
+            if constexpr (CLUSTER) {
+                ml_s[r] = make_float2(kNoMax, 0.f);
+#pragma unroll
+                for (uint32_t i = 0; i < kDh / 4; ++i)
+                    reinterpret_cast<float4*>(sums_s + r * kSumPitch)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                return;
+            }
             if (a.part_ml) {
                 a.part_ml[slot * a.total_rows + row] = make_float2(0.f, 0.f);
                 return;
@@ -566,7 +580,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                         m = mt;
                         ev = et;
                     } else {
-                        if (!(mt <= m + kMaxGrowth<KIND>)) {
+                        if (!(mt <= m + kMaxGrowth)) {
                             need = true;
                             alpha = ex2_approx(m - mt);
                             m = mt;
@@ -645,7 +659,10 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
             tc::tmem_ld_wait();
             float f = C::scaled ? pow2(min(ev, 127)) : 1.f;
             float4* part = nullptr;
-            if (a.part_ml) {
+            if constexpr (CLUSTER) {
+                ml_s[r] = make_float2(m, l);
+                part = reinterpret_cast<float4*>(sums_s + r * kSumPitch);
+            } else if (a.part_ml) {
                 const uint64_t at = it.slot * a.total_rows + row;
                 if (mine) a.part_ml[at] = make_float2(m, l);
                 part = reinterpret_cast<float4*>(a.part_o + at * kDh);
@@ -693,6 +710,9 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
         tc::tc_fence_after();
         tc::tmem_dealloc(tmem, kTmemCols);
     }
+    if constexpr (CLUSTER)
+        join_cluster(a, item_at(a, first, blockIdx.x, live, order), smem_u32(sums_s), smem_u32(ml_s), cluster,
+                     cluster_rank(), C::threads);
 }
 
 // Joins the parts of a row, 8 lanes a row: with M = max m, w_s = 2^(m_s - M),
@@ -770,6 +790,7 @@ struct Plan {
     bool widen;           // int8 keys are turned into f16 first
     bool few[2];          // items of the kernel for few rows, on `cluster` CTAs each
     uint32_t cluster[2];
+    uint32_t many_cluster;  // CTAs an item of tensor-core tiles, 0: none share one
     uint32_t slots;
 };
 
@@ -793,11 +814,16 @@ void split_few(Class& c, uint32_t& cluster, uint64_t items, uint32_t tiles, uint
 }
 
 // Tensor-core tiles: 1 to 64 parts of the keys, by the shortest estimated time, in
-// tiles: full rounds of items on `ctas` CTAs, two tiles of start and end for each
-// item, three for a join.
-void split_many(Class* cls, const uint64_t* items, const uint32_t* tiles, uint32_t ctas, bool joined) {
+// tiles: full rounds of items on the CTAs that run at once, two tiles of start and end
+// for each item, six for a kernel that joins the parts, one for a join in a cluster
+// (at most eight parts, and an eighth of the CTAs are lost to SMs that a cluster's
+// shape leaves over: 24 x 4 items of 74 tiles took 65 us in 96 clusters of three, of
+// which not all run at once, and 47 with the kernel; 8 x 12 items of 16 tiles 17.2 us
+// in clusters of two and 16.5 with the kernel and three parts, which is another launch).
+// Returns the size of the clusters, 0: none.
+uint32_t split_many(Class* cls, const uint64_t* items, const uint32_t* tiles, uint32_t ctas, bool joined) {
     uint64_t best = ~0ull;
-    uint32_t best_splits[2] = {1, 1};
+    uint32_t best_splits[2] = {1, 1}, best_cluster = 0;
     const uint32_t most = std::max(std::max(items[0] ? tiles[0] : 0, items[1] ? tiles[1] : 0), 1u);
     for (uint32_t n = 1; n <= kMaxSplits; ++n) {
         const uint32_t chunk = ceil_div(most, n);
@@ -811,10 +837,16 @@ void split_many(Class* cls, const uint64_t* items, const uint32_t* tiles, uint32
             longest = std::max(longest, each);
         }
         const uint64_t count = items[0] * splits[0] + items[1] * splits[1];
-        uint64_t time = std::max<uint64_t>(ceil_div(count, ctas) * longest, ceil_div(work, ctas));
-        if (joined || splits[1] > 1) time += 3;
-        if (time < best) {
-            best = time;
+        const auto rounds = [&](uint32_t at_once) {
+            return std::max<uint64_t>(ceil_div(count, at_once) * longest, ceil_div(work, at_once));
+        };
+        const bool split = joined || splits[1] > 1;
+        const bool may_cluster = !joined && split && splits[1] <= kMaxCluster;
+        const uint64_t alone = rounds(ctas) + (split ? 6 : 0);
+        const uint64_t clustered = may_cluster ? rounds(ctas * 7 / 8) + 1 : ~0ull;
+        if (std::min(alone, clustered) < best) {
+            best = std::min(alone, clustered);
+            best_cluster = clustered < alone ? splits[1] : 0;
             best_splits[0] = splits[0];
             best_splits[1] = splits[1];
         }
@@ -822,6 +854,7 @@ void split_many(Class* cls, const uint64_t* items, const uint32_t* tiles, uint32
     }
     for (int i = 0; i < 2; ++i)
         if (items[i]) cls[i].splits = FastDiv(best_splits[i]);
+    return best_cluster;
 }
 
 Plan plan_of(uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t prefixes, uint32_t prefix_keys,
@@ -857,7 +890,7 @@ Plan plan_of(uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t pref
     const uint64_t tiles_held = static_cast<uint64_t>(kv_heads) * (static_cast<uint64_t>(sequences) * t1 +
                                                                   static_cast<uint64_t>(prefixes) * t0);
     p.widen = int8 && !p.few[0] && !p.few[1] && visits >= kWidenFrom * tiles_held;
-    if (many[0] || many[1]) split_many(p.cls, many, tiles, p.few[1] ? sms : 2 * sms, stacked);
+    if (many[0] || many[1]) p.many_cluster = split_many(p.cls, many, tiles, p.few[1] ? sms : 2 * sms, stacked);
     for (int i = 0; i < 2; ++i) {
         if (!items[i]) continue;
         Class& c = p.cls[i];
@@ -866,7 +899,7 @@ Plan plan_of(uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t pref
         c.ordered = i && ragged && sequences <= kOrdered && ctas > (p.few[i] ? 3ull : 2ull) * sms;
         c.items = static_cast<uint32_t>(items[i] * c.splits.d);
         c.slot = p.slots;
-        p.slots += c.splits.d;
+        p.slots += i && p.many_cluster ? 1 : c.splits.d;
     }
     return p;
 }
@@ -942,18 +975,25 @@ bool view_maps(CUtensorMap* k, CUtensorMap* v, const dh_kv_view& s, uint32_t ent
 // Launch that may begin while the kernel before it in the stream still runs
 // (`beside`; that one lets it, and the kernel itself waits before it needs or ends).
 template <class Kernel, class... A>
-uint32_t launch_beside(Kernel kernel, uint32_t grid, uint32_t threads, uint32_t smem, bool beside, cudaStream_t st,
-                       const A&... args) {
+uint32_t launch_beside(Kernel kernel, uint32_t grid, uint32_t threads, uint32_t smem, uint32_t cluster, bool beside,
+                       cudaStream_t st, const A&... args) {
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(grid);
     config.blockDim = dim3(threads);
     config.dynamicSmemBytes = smem;
     config.stream = st;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &attr;
-    config.numAttrs = beside ? 1 : 0;
+    cudaLaunchAttribute attrs[2] = {};
+    config.attrs = attrs;
+    if (cluster > 1) {
+        attrs[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attrs[config.numAttrs].val.clusterDim.x = cluster;
+        attrs[config.numAttrs].val.clusterDim.y = attrs[config.numAttrs].val.clusterDim.z = 1;
+        ++config.numAttrs;
+    }
+    if (beside) {
+        attrs[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attrs[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
     if (cudaLaunchKernelEx(&config, kernel, args...) != cudaSuccess) {
         cudaGetLastError();
         return DH_ERR_CUDA;
@@ -961,14 +1001,22 @@ uint32_t launch_beside(Kernel kernel, uint32_t grid, uint32_t threads, uint32_t 
     return DH_OK;
 }
 
-template <int KIND>
-uint32_t launch(const CUtensorMap (&maps)[4], const Args& a, uint32_t first, uint32_t total, bool beside,
-                cudaStream_t st) {
+template <int KIND, bool CLUSTER>
+uint32_t launch_one(const CUtensorMap (&maps)[4], const Args& a, uint32_t first, uint32_t total, uint32_t cluster,
+                    bool beside, cudaStream_t st) {
+    const auto kernel = kv_attention_kernel<KIND, CLUSTER>;
     static std::atomic<uint64_t> configured{0};
-    if (all_shared_once(kv_attention_kernel<KIND>, Cfg<KIND>::bytes, configured) != cudaSuccess) return DH_ERR_CUDA;
-    const uint32_t grid = std::min(total, 2 * device_sms());
-    return launch_beside(kv_attention_kernel<KIND>, grid, Cfg<KIND>::threads, Cfg<KIND>::bytes, beside, st, maps[0], maps[1],
-                         maps[2], maps[3], a, first, total);
+    if (all_shared_once(kernel, Cfg<KIND>::bytes, configured) != cudaSuccess) return DH_ERR_CUDA;
+    const uint32_t grid = CLUSTER ? total : std::min(total, 2 * device_sms());  // (a cluster has one item)
+    return launch_beside(kernel, grid, Cfg<KIND>::threads, Cfg<KIND>::bytes, cluster, beside, st, maps[0], maps[1],
+                         maps[2], maps[3], a, first, total, cluster);
+}
+
+template <int KIND>
+uint32_t launch(const CUtensorMap (&maps)[4], const Args& a, uint32_t first, uint32_t total, uint32_t cluster,
+                bool beside, cudaStream_t st) {
+    return cluster ? launch_one<KIND, true>(maps, a, first, total, cluster, beside, st)
+                   : launch_one<KIND, false>(maps, a, first, total, 0, beside, st);
 }
 
 }  // namespace
@@ -1076,11 +1124,11 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
     for (uint32_t i = 0; i < 2; ++i)
         if (!p.few[i]) total += a.cls[i].items, first += i ? 0 : a.cls[0].items;
     if (total && p.widen)
-        status = launch<kWide>(maps, a, first, total, true, st);
+        status = launch<kWide>(maps, a, first, total, p.many_cluster, true, st);
     else if (total)
-        status = int8 ? launch<kInt8>(maps, a, first, total, false, st)
-                      : (v_bf16 ? launch<kVBf16>(maps, a, first, total, false, st)
-                                : launch<kV16>(maps, a, first, total, false, st));
+        status = int8 ? launch<kInt8>(maps, a, first, total, p.many_cluster, false, st)
+                      : (v_bf16 ? launch<kVBf16>(maps, a, first, total, p.many_cluster, false, st)
+                                : launch<kV16>(maps, a, first, total, p.many_cluster, false, st));
     bool beside = total;
     for (uint32_t i = 0; i < 2 && !status; ++i) {
         if (!p.few[i]) continue;
@@ -1088,7 +1136,7 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
         beside = true;
     }
     if (status || p.slots < 2) return status;
-    return launch_beside(kv_join_kernel, ceil_div(rows, kJoinThreads / 8), kJoinThreads, 0, true, st,
+    return launch_beside(kv_join_kernel, ceil_div(rows, kJoinThreads / 8), kJoinThreads, 0, 1, true, st,
                          static_cast<const float2*>(a.part_ml), static_cast<const float*>(a.part_o), p.slots, rows,
                          a.queries, heads, a.q_bf16, a.out, lse, run_rows);
 }

@@ -190,5 +190,87 @@ DH_DEVINL uint64_t row_index(const Args& a, const Item& it, uint32_t r, const ui
     return (static_cast<uint64_t>(seq) * a.queries.d + s) * a.heads + head;
 }
 
+DH_DEVINL uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+DH_DEVINL void cluster_sync() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+DH_DEVINL uint32_t map_to(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+DH_DEVINL float2 load_remote2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+DH_DEVINL float4 load_remote4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+DH_DEVINL void add(float4& s, float f, const float4& v) {
+    s = make_float4(__fmaf_rn(f, v.x, s.x), __fmaf_rn(f, v.y, s.y), __fmaf_rn(f, v.z, s.z), __fmaf_rn(f, v.w, s.w));
+}
+
+constexpr float kNoMax = -3.0e38f;  // below every maximum, and finite
+
+// Four values (part 0..15) of row r of an item from its sums: relative to 2^top, the
+// weights' sum is `total`.
+DH_DEVINL void write_part(const Args& a, const Item& it, uint32_t r, uint32_t part, float top, float total,
+                          const float4& sum) {
+    const uint64_t row = row_index(a, it, r, nullptr);
+    if (a.part_ml) {
+        const uint64_t at = it.slot * a.total_rows + row;
+        if (part == 0) a.part_ml[at] = make_float2(top, total);
+        reinterpret_cast<float4*>(a.part_o + at * kDh)[part] = sum;
+        return;
+    }
+    const float f = total == 0.f ? 0.f : 1.f / total;
+    reinterpret_cast<uint2*>(a.out)[row * (kDh / 4) + part] =
+        a.q_bf16 ? make_uint2(pack_bf16x2(sum.x * f, sum.y * f), pack_bf16x2(sum.z * f, sum.w * f))
+                 : make_uint2(pack_f16x2(sum.x * f, sum.y * f), pack_f16x2(sum.z * f, sum.w * f));
+    if (a.lse && part == 0) a.lse[row] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.6931471805599453f;
+}
+
+// An item's rows from the sums [row][kSumPitch] and (m, l) [row] that every CTA of the
+// cluster has at these addresses of its shared memory, in the order of the CTAs; each
+// writes its share.  All threads of all of them call it.
+constexpr uint32_t kMaxCluster = 8;
+constexpr uint32_t kSumPitch = kDh + 4;
+DH_DEVINL void join_cluster(const Args& a, const Item& it, uint32_t sums_at, uint32_t ml_at, uint32_t cluster,
+                            uint32_t rank, uint32_t threads) {
+    cluster_sync();
+    for (uint32_t i = rank * threads + threadIdx.x; i < it.rows * (kDh / 4); i += cluster * threads) {
+        const uint32_t r = i / (kDh / 4), part = i % (kDh / 4);
+        float top = kNoMax, total = 0.f;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        float2 x[kMaxCluster];
+#pragma unroll
+        for (uint32_t p = 0; p < kMaxCluster; ++p) {
+            if (p >= cluster) break;
+            x[p] = load_remote2(map_to(ml_at + r * 8, p));
+            top = max_nan(top, x[p].x);
+        }
+#pragma unroll
+        for (uint32_t p = 0; p < kMaxCluster; ++p) {
+            if (p >= cluster) break;
+            const float f = ex2_approx(x[p].x - top);
+            total = __fmaf_rn(f, x[p].y, total);
+            add(sum, f, load_remote4(map_to(sums_at + (r * kSumPitch + 4 * part) * 4, p)));
+        }
+        write_part(a, it, r, part, top, total, sum);
+    }
+    cluster_sync();  // (no CTA leaves while its sums are read)
+}
+
 }  // namespace kv
 }  // namespace dh

@@ -42,7 +42,6 @@ constexpr uint32_t kWarps = 4;
 constexpr uint32_t kThreads = 32 * kWarps;
 constexpr uint32_t kStages = 2;
 constexpr int32_t kShift = 0x4B400000;  // 1.5 * 2^23 as fp32
-constexpr float kNoMax = -3.0e38f;  // below every maximum, and finite
 
 enum Kind : int { kV16 = 0, kVBf16 = 1, kInt8 = 2 };
 
@@ -90,37 +89,6 @@ DH_DEVINL uint32_t transposed(uint32_t x) {
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
-}
-
-DH_DEVINL uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-DH_DEVINL void cluster_sync() {
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-DH_DEVINL uint32_t map_to(uint32_t addr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-DH_DEVINL float2 load_remote2(uint32_t addr) {
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-    return v;
-}
-DH_DEVINL float4 load_remote4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(addr)
-                 : "memory");
-    return v;
-}
-DH_DEVINL void add(float4& s, float f, const float4& v) {
-    s = make_float4(__fmaf_rn(f, v.x, s.x), __fmaf_rn(f, v.y, s.y), __fmaf_rn(f, v.z, s.z), __fmaf_rn(f, v.w, s.w));
 }
 
 // Bytes 0 and 1 (HI: 2 and 3) of a word of codes plus 128 as an exact f16 pair of
@@ -547,11 +515,10 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
     }
 
     // ---- join the warps: [warp][row][64] sums and [warp][row] (m, l) over the rings
-    constexpr uint32_t kPitch = kDh + 4;
     constexpr uint32_t kRowsMax = 8 * NT;
     __syncthreads();
     float* sums = reinterpret_cast<float*>(smem);
-    float2* ml = reinterpret_cast<float2*>(smem + kWarps * kRowsMax * kPitch * 4);
+    float2* ml = reinterpret_cast<float2*>(smem + kWarps * kRowsMax * kSumPitch * 4);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -563,7 +530,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
             total += __shfl_xor_sync(0xFFFFFFFFu, total, 16);
             if (r >= it.rows) continue;
             if (g == 0) ml[warp * kRowsMax + r] = make_float2(m[t][e], total);
-            float* dst = sums + (warp * kRowsMax + r) * kPitch;
+            float* dst = sums + (warp * kRowsMax + r) * kSumPitch;
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
                 if constexpr (kI8) {
@@ -576,20 +543,6 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
         }
     __syncthreads();
     // four values of a row at a time
-    const auto write = [&](uint32_t r, uint32_t part, float top, float total, float4 sum) {
-        const uint64_t row = row_index(a, it, r, nullptr);
-        if (a.part_ml) {
-            const uint64_t at = it.slot * a.total_rows + row;
-            if (part == 0) a.part_ml[at] = make_float2(top, total);
-            reinterpret_cast<float4*>(a.part_o + at * kDh)[part] = sum;
-            return;
-        }
-        const float f = total == 0.f ? 0.f : 1.f / total;
-        reinterpret_cast<uint2*>(a.out)[row * (kDh / 4) + part] =
-            a.q_bf16 ? make_uint2(pack_bf16x2(sum.x * f, sum.y * f), pack_bf16x2(sum.z * f, sum.w * f))
-                     : make_uint2(pack_f16x2(sum.x * f, sum.y * f), pack_f16x2(sum.z * f, sum.w * f));
-        if (a.lse && part == 0) a.lse[row] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.6931471805599453f;
-    };
     const uint32_t parts = it.rows * (kDh / 4);
     float2* joined_ml = ml + kWarps * kRowsMax;
     for (uint32_t i = threadIdx.x; i < parts; i += kThreads) {
@@ -606,41 +559,18 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
         for (uint32_t p = 0; p < kWarps; ++p) {
             const float f = ex2_approx(x[p].x - top);
             total = __fmaf_rn(f, x[p].y, total);
-            add(sum, f, *reinterpret_cast<const float4*>(sums + (p * kRowsMax + r) * kPitch + 4 * part));
+            add(sum, f, *reinterpret_cast<const float4*>(sums + (p * kRowsMax + r) * kSumPitch + 4 * part));
         }
         if (cluster == 1) {
-            write(r, part, top, total, sum);
+            write_part(a, it, r, part, top, total, sum);
         } else {
             // (only this thread reads these values of the warps' sums)
-            *reinterpret_cast<float4*>(sums + r * kPitch + 4 * part) = sum;
+            *reinterpret_cast<float4*>(sums + r * kSumPitch + 4 * part) = sum;
             if (part == 0) joined_ml[r] = make_float2(top, total);
         }
     }
     if (cluster == 1) break;
-    // ---- join the CTAs, each writes its share
-    cluster_sync();
-    const uint32_t sums_at = smem_u32(sums), ml_at = smem_u32(joined_ml);
-    for (uint32_t i = rank * kThreads + threadIdx.x; i < parts; i += cluster * kThreads) {
-        const uint32_t r = i / (kDh / 4), part = i % (kDh / 4);
-        float top = kNoMax, total = 0.f;
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        float2 x[kMaxCluster];
-#pragma unroll
-        for (uint32_t p = 0; p < kMaxCluster; ++p) {
-            if (p >= cluster) break;
-            x[p] = load_remote2(map_to(ml_at + r * 8, p));
-            top = max_nan(top, x[p].x);
-        }
-#pragma unroll
-        for (uint32_t p = 0; p < kMaxCluster; ++p) {
-            if (p >= cluster) break;
-            const float f = ex2_approx(x[p].x - top);
-            total = __fmaf_rn(f, x[p].y, total);
-            add(sum, f, load_remote4(map_to(sums_at + (r * kPitch + 4 * part) * 4, p)));
-        }
-        write(r, part, top, total, sum);
-    }
-    cluster_sync();  // (no CTA leaves while its sums are read)
+    join_cluster(a, it, smem_u32(sums), smem_u32(joined_ml), cluster, rank, kThreads);
     }
     grid_wait();  // (what waits for this kernel waits for one that it may run beside, too)
 }

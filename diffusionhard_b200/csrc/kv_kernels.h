@@ -10,7 +10,6 @@ namespace dh {
 namespace kv {
 
 constexpr uint32_t kFewRows = 16;     // rows of an item at most
-constexpr uint32_t kMaxCluster = 8;   // CTAs that share an item's keys
 
 // smem_optin_once, with an SM's whole carve-out as shared memory: two kernels that
 // run beside each other on an SM need the same one.
