@@ -412,6 +412,11 @@ def test_layouts(cuda, kind):
     if kind == "bf16":
         k, v = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in kv)
         assert torch.equal(attend(q, (k, v), length), want)
+        # one sequence's or one head's keys for all, never copied
+        for dims in (0, 1):
+            alike = [t.narrow(dims, 0, 1) for t in kv]
+            a = attend(q, tuple(t.expand(3, 2, -1, -1) for t in alike), length)
+            assert torch.equal(a, attend(q, tuple(t.expand(3, 2, -1, -1).contiguous() for t in alike), length))
         buf = torch.full((3, 2, 130, 128), math.nan, dtype=BF16, device="cuda")
         buf[:, :, 20:120, :64], buf[:, :, 20:120, 64:] = kv[0], kv[1]
         assert torch.equal(attend(q, (buf[:, :, 20:120, :64], buf[:, :, 20:120, 64:])), want)
