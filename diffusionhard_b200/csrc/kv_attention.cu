@@ -961,15 +961,17 @@ uint32_t check_view(const dh_kv_view& v) {
     return DH_OK;
 }
 
-bool view_maps(CUtensorMap* k, CUtensorMap* v, const dh_kv_view& s, uint32_t entries, uint32_t heads) {
+// Tiles of `keys` (32 or 64) rows of K and V.
+bool view_maps(CUtensorMap* k, CUtensorMap* v, const dh_kv_view& s, uint32_t entries, uint32_t heads, uint32_t keys) {
     const auto type = [](uint32_t t) {
         return t == DH_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     };
     const bool rows = s.v_strides[3] == 1;
     return make_tmap_4d(k, s.k, type(s.k_type), kDh, s.capacity, heads, entries, s.k_strides[2] * 2,
-                        s.k_strides[1] * 2, s.k_strides[0] * 2, kKT) &&
+                        s.k_strides[1] * 2, s.k_strides[0] * 2, kDh, keys) &&
            make_tmap_4d(v, s.v, type(s.v_type), rows ? kDh : s.capacity, rows ? s.capacity : kDh, heads, entries,
-                        s.v_strides[rows ? 2 : 3] * 2, s.v_strides[1] * 2, s.v_strides[0] * 2, kKT);
+                        s.v_strides[rows ? 2 : 3] * 2, s.v_strides[1] * 2, s.v_strides[0] * 2, rows ? kDh : keys,
+                        rows ? keys : kDh);
 }
 
 // Launch that may begin while the kernel before it in the stream still runs
@@ -1095,10 +1097,14 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
         a.part_o = static_cast<float*>(workspace);
         a.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + l.ml);
     }
-    CUtensorMap maps[4] = {};
-    if (!int8) {
-        if (!view_maps(&maps[2], &maps[3], *own, sequences, kv_heads)) return DH_ERR_CUDA;
-        if (prefixes && !view_maps(&maps[0], &maps[1], *prefix, prefixes, kv_heads)) return DH_ERR_CUDA;
+    const bool any_many = p.cls[0].items && !p.few[0] ? true : !p.few[1];
+    CUtensorMap maps[4] = {}, few_maps[4] = {};
+    for (int kind = 0; kind < 2 && !int8; ++kind) {
+        if (kind ? !(p.few[0] || p.few[1]) : !any_many) continue;
+        CUtensorMap* m = kind ? few_maps : maps;
+        const uint32_t keys = kind ? kFewKeys16 : kKT;
+        if (!view_maps(&m[2], &m[3], *own, sequences, kv_heads, keys)) return DH_ERR_CUDA;
+        if (prefixes && !view_maps(&m[0], &m[1], *prefix, prefixes, kv_heads, keys)) return DH_ERR_CUDA;
     }
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (p.widen) {
@@ -1114,7 +1120,7 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
             f.k_strides[2] = f.v_strides[2] = kDh, f.k_strides[3] = f.v_strides[3] = 1;
             f.k_strides[1] = f.v_strides[1] = static_cast<uint64_t>(capacity) * kDh;
             f.k_strides[0] = f.v_strides[0] = static_cast<uint64_t>(capacity) * kDh * kv_heads;
-            if (!view_maps(&maps[2 * i], &maps[2 * i + 1], f, entries, kv_heads)) return DH_ERR_CUDA;
+            if (!view_maps(&maps[2 * i], &maps[2 * i + 1], f, entries, kv_heads, kKT)) return DH_ERR_CUDA;
         }
         a.prefix_exps = to[0].exps, a.own_exps = to[1].exps;
         if (uint32_t status = launch_widen(a, to[0], to[1], prefixes, st)) return status;
@@ -1130,9 +1136,10 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
                       : (v_bf16 ? launch<kVBf16>(maps, a, first, total, p.many_cluster, false, st)
                                 : launch<kV16>(maps, a, first, total, p.many_cluster, false, st));
     bool beside = total;
+    const uint32_t taken = total ? (int8 ? Cfg<kInt8>::bytes : Cfg<kV16>::bytes) + 1024 : 0;
     for (uint32_t i = 0; i < 2 && !status; ++i) {
         if (!p.few[i]) continue;
-        status = launch_few(maps, a, i, p.cluster[i], int8, v_bf16, beside, st);
+        status = launch_few(few_maps, a, i, p.cluster[i], int8, v_bf16, beside, taken, st);
         beside = true;
     }
     if (status || p.slots < 2) return status;

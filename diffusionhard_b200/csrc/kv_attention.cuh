@@ -143,7 +143,8 @@ DH_DEVINL void order_sequences(const Args& a, uint32_t* lengths, uint16_t* order
     __syncthreads();
 }
 
-// Item w of a class, of the first `live` sequences.
+// Item w of a class, of the first `live` sequences, in tiles of KT keys.
+template <uint32_t KT = kKT>
 DH_DEVINL Item item_of(const Args& a, const Class& c, uint32_t w, uint32_t live, const uint16_t* order) {
     Item it;
     uint32_t split = w, tile, head;
@@ -162,8 +163,8 @@ DH_DEVINL Item item_of(const Args& a, const Class& c, uint32_t w, uint32_t live,
     it.prefix = a.per_prefix.of(it.seq0);
     it.len0 = c.with_prefix ? length_of(a.prefix, it.prefix) : 0u;
     it.len1 = c.with_own ? length_of(a.own, it.own) : 0u;
-    it.n0 = (it.len0 + kKT - 1) / kKT;
-    const uint32_t n = it.n0 + (it.len1 + kKT - 1) / kKT;
+    it.n0 = (it.len0 + KT - 1) / KT;
+    const uint32_t n = it.n0 + (it.len1 + KT - 1) / KT;
     if (c.splits.d == 1) {
         it.t0 = 0, it.t1 = n;
     } else {
@@ -175,9 +176,10 @@ DH_DEVINL Item item_of(const Args& a, const Class& c, uint32_t w, uint32_t live,
     if (it.rows == 0) it.t1 = it.t0;
     return it;
 }
-// keys left from tile j on in its part (a full tile: 64 or more)
+// keys left from tile j on in its part (a full tile: KT or more)
+template <uint32_t KT = kKT>
 DH_DEVINL uint32_t keys_left(const Item& it, uint32_t j) {
-    return j < it.n0 ? it.len0 - j * kKT : it.len1 - (j - it.n0) * kKT;
+    return j < it.n0 ? it.len0 - j * KT : it.len1 - (j - it.n0) * KT;
 }
 
 // Row r of an item: its query, as an index of [sequences, queries, heads].

@@ -4,7 +4,7 @@
 //
 // With 1 to 16 rows a key costs at most 4,096 FLOP for its 136 (int8) or 256
 // (16-bit) bytes, so the cache's bytes bound it, and the kernel is built around
-// their flow: every warp streams tiles of 64 keys of its own through two buffers
+// their flow: every warp streams tiles of 64 (16 bits: 32) keys of its own through two buffers
 // in shared memory (one bulk copy for each array of codes and scales, or a TMA
 // tile), and computes on the warp's matrix instruction (16 x 8 x 16) from
 // registers: no barrier between warps, no trip of converted values through shared
@@ -45,8 +45,12 @@ constexpr int32_t kShift = 0x4B400000;  // 1.5 * 2^23 as fp32
 
 enum Kind : int { kV16 = 0, kVBf16 = 1, kInt8 = 2 };
 
+// Keys of a tile (16 bits: 3 CTAs of 64 KB an SM; with 64 keys 1 of 128 KB, and 128
+// single tokens over up to 320 keys took 18.5 us instead of 14.4).
 template <int KIND>
-constexpr uint32_t kStageBytes = KIND == kInt8 ? kRawBytes : 2 * kTileBytes;
+constexpr uint32_t kKeys = KIND == kInt8 ? kKT : kFewKeys16;
+template <int KIND>
+constexpr uint32_t kStageBytes = KIND == kInt8 ? kRawBytes : 2 * kKeys<KIND> * kDh * 2;
 template <int KIND>
 constexpr uint32_t kSmem = 1024 + kWarps * kStages * kStageBytes<KIND> + 128 + kOrdered * 6;
 
@@ -112,6 +116,8 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
               const __grid_constant__ CUtensorMap tok, const __grid_constant__ CUtensorMap tov,
               const __grid_constant__ Args a, const uint32_t cls, const uint32_t cluster) {
     constexpr bool kI8 = KIND == kInt8;
+    constexpr uint32_t kN = kKeys<KIND>, kSteps = kN / 16;
+    constexpr uint32_t kTile16 = kN * kDh * 2;  // bytes of a 16-bit tile of K
     constexpr bool kQB = QBF16 && !kI8;  // type of the first product's operands
     const uint32_t live = a.run_rows ? min(a.sequences, a.queries.of(min(*a.run_rows, 0x7FFFFFFFu))) : a.sequences;
     extern __shared__ uint8_t smem_raw[];
@@ -141,7 +147,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
     const uint32_t next_item = solo ? gridDim.x * kWarps : cl.items;
     const uint32_t step = solo ? 1u : kWarps;
     auto item_at = [&](uint32_t w) {
-        Item it = item_of(a, cl, w, live, order);
+        Item it = item_of<kN>(a, cl, w, live, order);
         if (!solo) {
             const uint32_t n = it.t1 - it.t0;
             it.t1 = it.t0 + n * (rank + 1) / cluster;
@@ -165,7 +171,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
         }
         if (ahead_w >= cl.items) return;
         const bool own = ahead_j >= ahead.n0;
-        const uint32_t key = (own ? ahead_j - ahead.n0 : ahead_j) * kKT;
+        const uint32_t key = (own ? ahead_j - ahead.n0 : ahead_j) * kN;
         const uint32_t entry = own ? ahead.own : ahead.prefix;
         uint8_t* dst = ring + st * kStageBytes<KIND>;
         uint64_t* bar = &bars[st];
@@ -185,7 +191,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
         } else if (lane < 2) {
             const bool turned = lane && a.v_transposed;
             const CUtensorMap* map = lane ? (own ? &tov : &tpv) : (own ? &tok : &tpk);
-            tc::tma_load_4d(dst + lane * kTileBytes, map, bar, turned ? key : 0, turned ? 0 : key, ahead.kv_head, entry);
+            tc::tma_load_4d(dst + lane * kTile16, map, bar, turned ? key : 0, turned ? 0 : key, ahead.kv_head, entry);
         }
         ++issued;
         ahead_j += step;
@@ -272,13 +278,13 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
         }
         uint8_t* tile = ring + st * kStageBytes<KIND>;
         const float* scales = reinterpret_cast<const float*>(tile + 2 * kKT * kDh);
-        const uint32_t left = keys_left(it, j);
+        const uint32_t left = keys_left<kN>(it, j);
 
         // scores of keys 16 i + g (x[0], x[1]) and 16 i + 8 + g (x[2], x[3]), the last
         // index through key_of for int8
-        float s[NT][4][4] = {};
+        float s[NT][kSteps][4] = {};
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
+        for (uint32_t i = 0; i < kSteps; ++i) {
             if constexpr (kI8) {
                 const uint8_t* row = tile + (16 * i + key_of(g)) * kDh + 16 * c;
                 const uint4 w0 = *reinterpret_cast<const uint4*>(row);
@@ -316,7 +322,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
                 }
             }
         }
-        float vs[4][2];  // v_scale 2^-E of this thread's keys
+        float vs[kSteps][2];  // v_scale 2^-E of this thread's keys
         float fe = 1.f;
         if constexpr (kI8) {
             float peak = 0.f;  // (of the numbers among them)
@@ -341,26 +347,26 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
             fe = pow2(max(ev - et, -126));
             ev = et;
         }
-        if (left < kKT) {
+        if (left < kN) {
             // keys behind the last one: whatever was read scores -inf; V there is zero
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i)
+                for (uint32_t i = 0; i < kSteps; ++i)
 #pragma unroll
                     for (uint32_t h = 0; h < 2; ++h)
                         if (16 * i + 8 * h + (kI8 ? key_of(g) : g) >= left) s[t][i][2 * h] = s[t][i][2 * h + 1] = -INFINITY;
             if constexpr (!kI8) {
                 if (a.v_transposed) {
-                    for (uint32_t i = lane; i < kDh * kKT; i += 32) {
-                        const uint32_t d = i / kKT, key = i % kKT;
+                    for (uint32_t i = lane; i < kDh * kN; i += 32) {  // (64-byte swizzle)
+                        const uint32_t d = i / kN, key = i % kN;
                         if (key >= left)
-                            *reinterpret_cast<uint16_t*>(tile + kTileBytes + d * 128 +
-                                                         (((key >> 3) ^ (d & 7u)) * 16) + (key & 7u) * 2) = 0;
+                            *reinterpret_cast<uint16_t*>(tile + kTile16 + d * 64 +
+                                                         (((key >> 3) ^ ((d >> 1) & 3u)) * 16) + (key & 7u) * 2) = 0;
                     }
                 } else {
-                    for (uint32_t i = left * 8 + lane; i < kKT * 8; i += 32)
-                        *reinterpret_cast<uint4*>(tile + kTileBytes + i * 16) = make_uint4(0, 0, 0, 0);
+                    for (uint32_t i = left * 8 + lane; i < kN * 8; i += 32)
+                        *reinterpret_cast<uint4*>(tile + kTile16 + i * 16) = make_uint4(0, 0, 0, 0);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (before the next load here)
                 __syncwarp();
@@ -372,8 +378,10 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
             float next[2], alpha[2];
 #pragma unroll
             for (uint32_t e = 0; e < 2; ++e) {
-                float top = max_nan(max_nan(s[t][0][e], s[t][0][e + 2], s[t][1][e]), s[t][1][e + 2],
-                                    max_nan(max_nan(s[t][2][e], s[t][2][e + 2], s[t][3][e]), s[t][3][e + 2]));
+                float top = max_nan(max_nan(s[t][0][e], s[t][0][e + 2], s[t][1][e]), s[t][1][e + 2]);
+                if constexpr (kSteps == 4)
+                    top = max_nan(top, max_nan(max_nan(s[t][2][e], s[t][2][e + 2], s[t][kSteps - 1][e]),
+                                               s[t][kSteps - 1][e + 2]));
                 top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
                 top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
                 top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
@@ -388,7 +396,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
             const float2 cr2 = make_float2(cr[t][0], cr[t][1]), nm2 = make_float2(-next[0], -next[1]);
             float2 sum = make_float2(l[t][0], l[t][1]);
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
+            for (uint32_t i = 0; i < kSteps; ++i) {
 #pragma unroll
                 for (uint32_t h = 0; h < 2; ++h) {
                     const float2 x = __ffma2_rn(make_float2(s[t][i][2 * h], s[t][i][2 * h + 1]), cr2, nm2);
@@ -409,7 +417,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
         }
         // O^T += V^T P^T, 16 keys at a time
 #pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) {
+        for (uint32_t k = 0; k < kSteps; ++k) {
             uint32_t pb[NT][2];
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -449,10 +457,10 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
                 for (uint32_t i = 0; i < 4; ++i) {
                     uint32_t va[4];
                     if (a.v_transposed)  // rows d, their keys contiguous
-                        ldmatrix4(va, smem_u32(tile) + kTileBytes + (16 * i + 8 * low + row) * 128 +
-                                          (((2 * k + high) ^ row) * 16));
+                        ldmatrix4(va, smem_u32(tile) + kTile16 + (16 * i + 8 * low + row) * 64 +
+                                          (((2 * k + high) ^ (row >> 1)) * 16));
                     else
-                        ldmatrix4_trans(va, smem_u32(tile) + kTileBytes + (16 * k + 8 * high + row) * 128 +
+                        ldmatrix4_trans(va, smem_u32(tile) + kTile16 + (16 * k + 8 * high + row) * 128 +
                                                 (((2 * i + low) ^ row) * 16));
 #pragma unroll
                     for (int t = 0; t < NT; ++t) mma_16816<KIND == kVBf16>(o[t][i], va, pb[t][0], pb[t][1]);
@@ -577,13 +585,14 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
 
 template <int KIND, bool QBF16, int NT>
 uint32_t launch(const CUtensorMap (&maps)[4], const Args& a, uint32_t cls, uint32_t cluster, bool beside,
-                cudaStream_t st) {
+                uint32_t taken, cudaStream_t st) {
     const auto kernel = kv_few_kernel<KIND, QBF16, NT>;
     static std::atomic<uint64_t> configured{0};
     if (all_shared_once(kernel, kSmem<KIND>, configured) != cudaSuccess) return DH_ERR_CUDA;
     cudaLaunchConfig_t config{};
-    // solo: as many CTAs as fit, their warps walk the items
-    const uint32_t fit = device_sms() * (227u * 1024u / (kSmem<KIND> + 1024u));
+    // solo: as many CTAs as run at once, their warps walk the items (one CTA an SM beside
+    // tensor-core tiles, with room for two, cost 40.3 us instead of 37.4)
+    const uint32_t fit = device_sms() * std::max((227u * 1024u - taken) / (kSmem<KIND> + 1024u), 1u);
     const uint32_t items = a.cls[cls].items;
     config.gridDim = dim3(cluster ? items * cluster : std::min((items + kWarps - 1) / kWarps, fit));
     config.blockDim = dim3(kThreads);
@@ -610,24 +619,24 @@ uint32_t launch(const CUtensorMap (&maps)[4], const Args& a, uint32_t cls, uint3
 
 template <int KIND, bool QBF16>
 uint32_t launch_rows(const CUtensorMap (&maps)[4], const Args& a, uint32_t cls, uint32_t cluster, bool beside,
-                cudaStream_t st) {
-    return a.cls[cls].tile_rows <= 8 ? launch<KIND, QBF16, 1>(maps, a, cls, cluster, beside, st)
-                                     : launch<KIND, QBF16, 2>(maps, a, cls, cluster, beside, st);
+                uint32_t taken, cudaStream_t st) {
+    return a.cls[cls].tile_rows <= 8 ? launch<KIND, QBF16, 1>(maps, a, cls, cluster, beside, taken, st)
+                                     : launch<KIND, QBF16, 2>(maps, a, cls, cluster, beside, taken, st);
 }
 
 template <int KIND>
 uint32_t launch_type(const CUtensorMap (&maps)[4], const Args& a, uint32_t cls, uint32_t cluster, bool beside,
-                cudaStream_t st) {
-    return a.q_bf16 ? launch_rows<KIND, true>(maps, a, cls, cluster, beside, st)
-                    : launch_rows<KIND, false>(maps, a, cls, cluster, beside, st);
+                uint32_t taken, cudaStream_t st) {
+    return a.q_bf16 ? launch_rows<KIND, true>(maps, a, cls, cluster, beside, taken, st)
+                    : launch_rows<KIND, false>(maps, a, cls, cluster, beside, taken, st);
 }
 
 }  // namespace
 
 uint32_t launch_few(const CUtensorMap (&maps)[4], const Args& a, uint32_t cls, uint32_t cluster, bool int8, bool v_bf16,
-                    bool beside, cudaStream_t st) {
-    return int8 ? launch_type<kInt8>(maps, a, cls, cluster, beside, st)
-                : (v_bf16 ? launch_type<kVBf16>(maps, a, cls, cluster, beside, st) : launch_type<kV16>(maps, a, cls, cluster, beside, st));
+                    bool beside, uint32_t taken, cudaStream_t st) {
+    return int8 ? launch_type<kInt8>(maps, a, cls, cluster, beside, taken, st)
+                : (v_bf16 ? launch_type<kVBf16>(maps, a, cls, cluster, beside, taken, st) : launch_type<kV16>(maps, a, cls, cluster, beside, taken, st));
 }
 
 }  // namespace kv

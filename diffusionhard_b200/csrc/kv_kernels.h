@@ -9,7 +9,8 @@
 namespace dh {
 namespace kv {
 
-constexpr uint32_t kFewRows = 16;     // rows of an item at most
+constexpr uint32_t kFewRows = 16;    // rows of an item at most
+constexpr uint32_t kFewKeys16 = 32;  // 16-bit keys of a tile
 
 // smem_optin_once, with an SM's whole carve-out as shared memory: two kernels that
 // run beside each other on an SM need the same one.
@@ -23,10 +24,12 @@ inline cudaError_t all_shared_once(Kernel kernel, uint32_t bytes, std::atomic<ui
     return e == cudaSuccess ? smem_optin_once(kernel, bytes, done) : e;
 }
 
-// Class `cls` of a's items on clusters of `cluster` CTAs (0: a warp an item).  maps: prefix K, V, own K,
-// V (16 bits).  beside: may begin while the kernel before it in the stream runs.
+// Class `cls` of a's items on clusters of `cluster` CTAs (0: a warp an item).  maps:
+// prefix K, V, own K, V (16 bits, tiles of kFewKeys16 keys).  beside: may begin while
+// the kernel before it in the stream runs, whose CTA on an SM has `taken` bytes of
+// shared memory.
 uint32_t launch_few(const CUtensorMap (&maps)[4], const Args& a, uint32_t cls, uint32_t cluster, bool int8, bool v_bf16,
-                    bool beside, cudaStream_t st);
+                    bool beside, uint32_t taken, cudaStream_t st);
 
 // f16 rows [lines][capacity][64] of K and V, and [lines] their exponents.
 struct WideKeys {

@@ -47,20 +47,21 @@ inline bool make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType
     return r == CUDA_SUCCESS;
 }
 
-// 4-D tensor of 16-bit elements with 128-byte swizzle: dims [d0 (contiguous), d1,
-// d2, d3], byte strides of d1..d3 multiples of 16, box [64, box_1, 1, 1].
+// 4-D tensor of 16-bit elements: dims [d0 (contiguous), d1, d2, d3], byte strides of
+// d1..d3 multiples of 16, box [box_0, box_1, 1, 1] with box_0 64 (128-byte swizzle) or
+// 32 (64-byte swizzle, see below).
 // Out-of-range elements read as zero.
 inline bool make_tmap_4d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, uint64_t d0, uint64_t d1,
-                         uint64_t d2, uint64_t d3, uint64_t s1, uint64_t s2, uint64_t s3, uint32_t box_1) {
+                         uint64_t d2, uint64_t d3, uint64_t s1, uint64_t s2, uint64_t s3, uint32_t box_0, uint32_t box_1) {
     EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return false;
     if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || ((s1 | s2 | s3) & 15u) != 0) return false;
     cuuint64_t dims[4] = {d0, d1, d2, d3};
     cuuint64_t strides[3] = {s1, s2, s3};
-    cuuint32_t box[4] = {64, box_1, 1, 1};
+    cuuint32_t box[4] = {box_0, box_1, 1, 1};
     cuuint32_t estr[4] = {1, 1, 1, 1};
-    CUresult r = fn(map, dtype, 4, const_cast<void*>(base), dims, strides, box, estr,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    CUresult r = fn(map, dtype, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    box_0 == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS;
 }
