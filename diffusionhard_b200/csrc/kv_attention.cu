@@ -102,6 +102,12 @@ DH_DEVINL float2 exp2_poly2(float2 x) {
 // two, P's largest value meanwhile (f16 ends at 2^16).  32 canvases over int8, scores
 // of a few: 245 us at 8, 237 at 15; 128 x 512 queries over 1024 16-bit keys 325 and 305.
 constexpr float kMaxGrowth = 15.f;
+// f16 loses weights below 2^-25 of the one it is relative to: together up to 2^-11 of
+// all over 2^14 keys, which is a rounding of the result.  Longer parts set the maximum
+// lower, by the headroom, and keep them down to 2^-33 (their maximum settles early:
+// with a headroom of 4 everywhere the 16 tiles of the cases above took 1.5% longer).
+constexpr uint32_t kLongTiles = 256;
+constexpr float kHeadroom = 8.f;
 constexpr uint32_t kPolyPairMask = 0x11u;  // pairs e with bit e % 8 set
 
 // Half of a tile's 64 rows of codes (those of this warp) into a 128-byte
@@ -158,7 +164,10 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                     const uint32_t cluster) {
     using C = Cfg<KIND>;
     const uint32_t live = a.run_rows ? min(a.sequences, a.queries.of(min(*a.run_rows, 0x7FFFFFFFu))) : a.sequences;
-    if (live == 0) return;
+    if (live == 0) {
+        if constexpr (KIND == kWide) grid_wait();  // (what waits for this kernel waits for that one)
+        return;
+    }
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~static_cast<uintptr_t>(1023));
@@ -521,8 +530,8 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
             uint32_t next_w = w + gridDim.x;
             next_item(next_w, next);
             const bool active = quad * 32 < it.rows;  // the warp has rows
-            float m = 0.f;
-            int32_t ev = 0;  // exponent of O (int8 keys)
+            float m = -INFINITY;
+            int32_t ev = -1000;  // exponent of O (int8 keys)
             float2 ex0 = make_float2(1.f, 0.f), ex1 = ex0;  // of the prefix, of its own keys
             if constexpr (KIND == kWide) {
                 if (it.len0) ex0 = a.prefix_exps[it.prefix * a.kv_heads.d + it.kv_head];
@@ -540,10 +549,10 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                     tc::tmem_ld_32x32b_x32(tmem + lane_base + sb * kKT, *reinterpret_cast<uint32_t(*)[32]>(&sv[0]));
                     tc::tmem_ld_32x32b_x32(tmem + lane_base + sb * kKT + 32,
                                            *reinterpret_cast<uint32_t(*)[32]>(&sv[32]));
-                    float ct = c;
+                    float ct = C::scaled ? c : a.c;
                     int32_t et = 0;
                     if constexpr (C::int8) {
-                        ct = fmaxf(c * pow2(min(exps[(g % kExpRing) * 2], 127)), kLeastFactor);
+                        ct = fmaxf(c * pow2(min(exps[(g % kExpRing) * 2], 128)), kLeastFactor);
                         et = exps[(g % kExpRing) * 2 + 1];
                     } else if constexpr (C::scaled) {
                         const float2 ex = j < it.n0 ? ex0 : ex1;
@@ -572,28 +581,25 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                                                max_nan(max_nan(pm[4], pm[5]), pm[6], pm[7]));
                     // finite (a row of -inf would give inf - inf), or NaN for an infinite
                     // score, as for one that is NaN: the row is NaN
-                    float mt = max_nan(tmax * ct, -3.0e38f);
+                    float mt = max_nan(tmax * ct, kNoMax);
                     mt = __fmaf_rn(mt, -0.f, mt);
                     float alpha = 1.f, alpha_o = 1.f;
                     bool need = false;
-                    if (j == it.t0) {
+                    if (!(mt <= m + kMaxGrowth)) {
+                        need = true;
+                        mt -= it.t1 - it.t0 > kLongTiles ? kHeadroom : 0.f;
+                        alpha = ex2_approx(m - mt);
                         m = mt;
-                        ev = et;
-                    } else {
-                        if (!(mt <= m + kMaxGrowth)) {
-                            need = true;
-                            alpha = ex2_approx(m - mt);
-                            m = mt;
-                        }
-                        alpha_o = alpha;
-                        if (C::scaled && et > ev) {
-                            need = true;
-                            alpha_o = alpha * pow2(max(ev - et, -126));
-                            ev = et;
-                        }
                     }
-                    const float2 c2 = make_float2(ct, ct);
-                    const float2 nm2 = make_float2(-m, -m);
+                    alpha_o = alpha;
+                    if (C::scaled && et > ev) {
+                        need = true;
+                        alpha_o = alpha * pow2(max(ev - et, -126));
+                        ev = et;
+                    }
+                    need = need && j != it.t0;
+                    const float damp = damping(m), cd = fmaxf(ct * damp, kLeastFactor), nm = -m * damp;
+                    const float2 c2 = make_float2(cd, cd), nm2 = make_float2(nm, nm);
                     uint32_t pk[32];
 #pragma unroll
                     for (uint32_t e = 0; e < 32; ++e) {
@@ -657,7 +663,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
             const uint64_t row = row_index(a, it, r, nullptr);
             const bool mine = r < it.rows;
             tc::tmem_ld_wait();
-            float f = C::scaled ? pow2(min(ev, 127)) : 1.f;
+            float f = C::scaled ? pow2(min(ev, 128)) : 1.f;
             float4* part = nullptr;
             if constexpr (CLUSTER) {
                 ml_s[r] = make_float2(m, l);

@@ -89,7 +89,7 @@ DH_DEVINL uint32_t pack_bf16x2(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// 2^n, -126 <= n <= 127
+// 2^n, -126 <= n <= 127; infinite for 128
 DH_DEVINL float pow2(int32_t n) { return __uint_as_float(static_cast<uint32_t>(n + 127) << 23); }
 // e with 2^(e - 1) <= x < 2^e for the normal fp32 with these bits
 DH_DEVINL int32_t exponent_of(uint32_t bits) { return static_cast<int32_t>((bits >> 23) & 0xFFu) - 126; }
@@ -223,6 +223,14 @@ DH_DEVINL void add(float4& s, float f, const float4& v) {
     s = make_float4(__fmaf_rn(f, v.x, s.x), __fmaf_rn(f, v.y, s.y), __fmaf_rn(f, v.z, s.z), __fmaf_rn(f, v.w, s.w));
 }
 
+// A weight's exponent s c - m, one FMA, is off by the rounding of m, half a step of fp32.
+// From |m| = 2^23 on that is 2^-1 and more, and at 2^28 weights would leave f16 at either
+// end.  So s c and m are taken by this power of two there, which keeps the latter below
+// 2^23: scores count to 2^-23 of their size.  1 for all others.
+DH_DEVINL float damping(float top) {
+    constexpr uint32_t kFrom = (127u + 22u) << 23;
+    return __uint_as_float(0x3F800000u + kFrom - max(__float_as_uint(top) & 0x7F800000u, kFrom));
+}
 constexpr float kNoMax = -3.0e38f;  // below every maximum, and finite
 
 // Four values (part 0..15) of row r of an item from its sums: relative to 2^top, the

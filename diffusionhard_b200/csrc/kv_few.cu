@@ -41,6 +41,9 @@ namespace {
 constexpr uint32_t kWarps = 4;
 constexpr uint32_t kThreads = 32 * kWarps;
 constexpr uint32_t kStages = 2;
+// The weights are relative to 2^m with m the maximum less this: f16 holds them down to
+// 2^-32 of the largest.
+constexpr float kHeadroom = 8.f;
 constexpr int32_t kShift = 0x4B400000;  // 1.5 * 2^23 as fp32
 
 enum Kind : int { kV16 = 0, kVBf16 = 1, kInt8 = 2 };
@@ -375,7 +378,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
         // weights, in place
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            float next[2], alpha[2];
+            float next[2], alpha[2], top2[2];
 #pragma unroll
             for (uint32_t e = 0; e < 2; ++e) {
                 float top = max_nan(max_nan(s[t][0][e], s[t][0][e + 2], s[t][1][e]), s[t][1][e + 2]);
@@ -386,14 +389,17 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
                 top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
                 top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
                 // finite, or NaN for a score that is infinite or NaN: the row is NaN
-                next[e] = max_nan(max_nan(top * cr[t][e], kNoMax), m[t][e]);
+                top2[e] = top * cr[t][e];
+                next[e] = max_nan(max_nan(top2[e] - kHeadroom, kNoMax), m[t][e]);
                 next[e] = __fmaf_rn(next[e], -0.f, next[e]);
                 alpha[e] = ex2_approx(m[t][e] - next[e]);
                 m[t][e] = next[e];
                 l[t][e] *= alpha[e];
                 alpha[e] *= fe;
             }
-            const float2 cr2 = make_float2(cr[t][0], cr[t][1]), nm2 = make_float2(-next[0], -next[1]);
+            const float damp[2] = {damping(top2[0]), damping(top2[1])};
+            const float2 cr2 = make_float2(fmaxf(cr[t][0] * damp[0], kLeastFactor), fmaxf(cr[t][1] * damp[1], kLeastFactor));
+            const float2 nm2 = make_float2(-next[0] * damp[0], -next[1] * damp[1]);
             float2 sum = make_float2(l[t][0], l[t][1]);
 #pragma unroll
             for (uint32_t i = 0; i < kSteps; ++i) {

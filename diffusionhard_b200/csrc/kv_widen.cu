@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kThreads) kv_widen_kernel(const __grid_constan
                          largest(a.prefix.v_scale + line0 * a.prefix.capacity, length_of(a.prefix, p), smem)));
     }
     if (chunk == 0 && threadIdx.x == 0)
-        to.exps[line] = make_float2(pow2(min(ek + 9, 127)), __int_as_float(ev + 9));
+        to.exps[line] = make_float2(pow2(min(ek + 9, 128)), __int_as_float(ev + 9));
     const float fk = pow2(15 - ek), fv = pow2(15 - ev);
     const uint32_t tiles = (len + kKT - 1) / kKT;
     // 8 codes of a row a thread, so that a warp writes whole lines; the loads of four

@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import functools
 import math
+import operator
 import struct
 from typing import Any, NamedTuple, Optional, Tuple, Union
 
@@ -246,7 +247,7 @@ def _view(name: str, kv: Any, lengths: Lengths, q: torch.Tensor, index: int) -> 
     elif isinstance(lengths, torch.Tensor):
         held = _ints(f"lengths of {name}", lengths, entries, index)
     else:
-        length = int(lengths)
+        length = operator.index(lengths)
         if not 0 <= length <= capacity:
             raise ValueError(f"{length} keys of {name} do not lie within its capacity of {capacity}")
     view = _pack_view(*pointers, 0 if held is None else held.data_ptr(), *ks, *vs, kt, vt, capacity, length)

@@ -335,6 +335,66 @@ def test_peaked_and_far_scores(cuda, kind, n):
     check(q * 4, kv, length)
 
 
+@pytest.mark.parametrize("kind", ["int8", "bf16", "f16", "turned"])
+@pytest.mark.parametrize("n", [1, 12, 40, 520])
+def test_scores_beyond_the_steps_of_fp32(cuda, kind, n):
+    """Scores up to 10^9 and more, of either sign, where fp32 holds no fractions: the
+    key with the largest one has all the weight."""
+    dtype = F16 if kind == "f16" else BF16
+    q, k = values((2, 2, n, DIM), 5, dtype) * 100, values((2, 2, 300, DIM), 6, dtype) * 4000
+    v = values((2, 2, 300, DIM), 7, F16 if kind == "turned" else dtype)
+    kv = cache_of(k, v) if kind == "int8" else (k, v)
+    if kind == "turned":
+        wide = torch.zeros(2, 2, DIM, 304, dtype=F16, device="cuda")
+        wide[..., :300] = v.transpose(2, 3)
+        kv = (k, wide.transpose(2, 3)[:, :, :300])
+    # roundings: the key's weight in the product, not in the divisor where rows are few
+    # (bf16 2^-8, f16 2^-11; it is a power of two only if the score's rounding is none),
+    # an int8 row twice, the output half a step
+    p_round = {"bf16": 2.0 ** -8, "int8": 2.0 ** -11 + 2.0 ** -10}.get(kind, 2.0 ** -11)
+    for scale in (1.0, 300.0):
+        out, lse = attend(q, kv, 300, scale=scale, return_lse=True)
+        out, lse = out.double().cpu(), lse.double().cpu()
+        assert torch.isfinite(out).all()
+        seen = 0
+        for b in range(2):
+            kk, vv = dense(kv, b, 300)
+            for h in range(2):
+                s = scale * (q[b, h].double().cpu() @ kk[h].T)
+                top2 = s.topk(2).values
+                # (int8 rows are rounded to f16 twice: 2^-10 of sum |q k|, 2^-7 of the largest score)
+                sure = (top2[:, 0] - top2[:, 1]) > 2.0 ** -6 * top2[:, 0].abs() + 100
+                seen += int(sure.sum())
+                want = vv[h][s.argmax(-1)]
+                err = (out[b, :, h] - want).abs()
+                limit = want.abs() * (torch.finfo(dtype).eps / 2 + p_round) + 2.0 ** -18 * vv[h].abs().max()
+                assert (err[sure] <= limit[sure]).all()
+                assert ((lse[b, :, h] - top2[:, 0]).abs() <= 2.0 ** -7 * top2[:, 0].abs()).all()
+        assert seen > 2 * n
+    _lib.check_device_error()
+
+
+@pytest.mark.parametrize("kind", ["int8", "f16"])
+@pytest.mark.parametrize("batch, n, keys", [(1200, 1, 2048), (592, 20, 20000), (74, 1000, 20000)])
+def test_many_light_keys(cuda, kind, batch, n, keys):
+    """One key with almost all the weight, and thousands with 2^-25.25 of it each, which
+    f16 relative to the largest weight would lose."""
+    k = torch.zeros(1, 1, keys, DIM, dtype=F16, device="cuda")
+    v = torch.full((1, 1, keys, DIM), 1024.0, dtype=F16, device="cuda")
+    k[0, 0, 5, 3], v[0, 0, 5] = 25.25, 0
+    q = torch.zeros(batch, 1, n, DIM, dtype=F16, device="cuda")
+    q[..., 3] = 1
+    k, v = k.expand(batch, 1, keys, DIM), v.expand(batch, 1, keys, DIM)
+    out = attend(q, cache_of(k, v) if kind == "int8" else (k, v), keys, scale=math.log(2.0)).double().cpu()
+    tail = (keys - 1) * 2.0 ** -25.25
+    # weights relative to 2^-8 of the largest, where half a step of f16 is 2^-25: 2^-33 of
+    # it, 0.47% of 2^-25.25; int8 rows of more than 16 query rows are rounded twice:
+    # 25.25 ln 2 2^-10 = 1.71%; output 2^-11
+    limit = 0.0047 + (0.0172 if kind == "int8" and n > 16 else 0) + 2.0 ** -11 + 1e-4
+    assert ((out / (1024 * tail / (1 + tail)) - 1).abs() <= limit).all()
+    _lib.check_device_error()
+
+
 @pytest.mark.parametrize("n", [5, 50, 520])
 def test_scales(cuda, n):
     q, kv, length = case(1, 2, 2, n, 100, "int8", 9)
