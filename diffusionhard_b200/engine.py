@@ -176,7 +176,8 @@ class MDLMEngine:
         self._graphs: Dict[Any, Any] = {}
         self._events = (torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True))
         self._whole_forward = False  # self.x is a forward of the whole canvas, and no generation came after it
-        self.launches_per_forward = 1 + 9 * len(self.blocks)
+        # (kvcache.attend counts as one)
+        self.launches_per_forward = 1 + (9 if int8_kv is None else 10) * len(self.blocks)
 
     def shard_head(self, v0: int, v1: int, group: Any = None, reduce: Any = None) -> None:
         """Keep only head rows [v0, v1) (vocab-sharded head).  After every head
@@ -546,6 +547,8 @@ class MDLMEngine:
         thresholds = reveal_thresholds_q32(steps, sampling_epsilon)
         native = self.native_loop_ok() if native is None else native
         self._compact_now = self.compact_for(steps)
+        if native and (self.int8_kv is not None or self.prefix_kv is not None):
+            raise ValueError("dh_sample_loop knows neither int8 nor shared keys")
         if native:
             if input_ids.numel() != self.M:
                 raise ValueError("input_ids must be [batch, seq_len]")

@@ -121,6 +121,11 @@ def test_refusals(cuda, model):
         gen.set_prefix(_ids(cuda, 4, 32, 1))
     with pytest.raises(ValueError, match="drift"):
         gen.drift_report(_ids(cuda, 2, 32, 1), _ids(cuda, 4, 32, 1))
+    for int8_kv in (False, True):
+        gen = PrefixConditionedGenerator(model, 4, 32, 32, prefixes=2, int8_kv=int8_kv)
+        with pytest.raises(ValueError, match="dh_sample_loop"):
+            gen.suffix.generate(cuda.full((4, 32), SMALL.mask_token_id), steps=4, native=True)
+    gen = PrefixConditionedGenerator(model, 4, 32, 32, prefixes=2)
     with pytest.raises(ValueError, match="int8_kv"):
         MDLMEngine(model, 1, 64, int8_kv=[])
     with pytest.raises(ValueError, match="prefix_kv"):
