@@ -40,7 +40,7 @@ using namespace kv;
 
 constexpr uint32_t kRows = 128;                  // rows per item
 constexpr uint32_t kOnesBytes = 2048;            // 16 rows of 128 bytes
-constexpr uint32_t kVPitch = kTileBytes + kOnesBytes;
+constexpr uint32_t kVPitch = kTileBytes + kOnesBytes;  // (a fine V's second tile behind it)
 constexpr uint32_t kTmemCols = 256;
 constexpr uint32_t kOCol = 128;                  // S/P buffers at 0 and 64, O at 128, l at 192
 constexpr uint32_t kQCol = 224;
@@ -49,22 +49,29 @@ constexpr uint32_t kExpRing = 8;                 // tiles whose exponents are ke
 
 constexpr uint32_t kMaxSplits = 64;              // parts of an item's keys
 
-// kWide: int8 keys that kv_widen.cu has turned into f16
-enum Kind : int { kV16 = 0, kVBf16 = 1, kInt8 = 2, kWide = 3 };
+// kWide: int8 keys that kv_widen.cu has turned into f16.  The fine forms, for queries in
+// f16, whose results show more: codes times a scale as the sum of two f16, and so the
+// products (600 f16 queries over 1000 keys: off by 1.0e-3 of the result's norm with one
+// f16, 2.4e-4 with two, 2.1e-4 of that the result's own rounding).
+enum Kind : int { kV16 = 0, kVBf16 = 1, kInt8 = 2, kWide = 3, kInt8Fine = 4, kWideFine = 5 };
 
 template <int KIND>
 struct Cfg {
-    static constexpr bool int8 = KIND == kInt8;
-    static constexpr bool scaled = int8 || KIND == kWide;  // keys carry exponents
+    static constexpr bool int8 = KIND == kInt8 || KIND == kInt8Fine;
+    static constexpr bool wide = KIND == kWide || KIND == kWideFine;
+    static constexpr bool scaled = int8 || wide;  // keys carry exponents
+    static constexpr bool fine = KIND == kInt8Fine || KIND == kWideFine;
+    static constexpr uint32_t k_bytes = fine ? 2 * kTileBytes : kTileBytes;
+    static constexpr uint32_t v_bytes = fine ? kVPitch + kTileBytes : kVPitch;
     static constexpr uint32_t threads = int8 ? 256 : 192;
-    static constexpr uint32_t raw_stages = int8 ? 4 : 0;
+    static constexpr uint32_t raw_stages = int8 ? (fine ? 2 : 4) : 0;
     // (16 bits: 4 of K and 3 of V 305 us where 2 and 2 take 302.5)
     static constexpr uint32_t k_stages = 2;
     static constexpr uint32_t v_stages = 2;
     static constexpr uint32_t q_at = 0;
     static constexpr uint32_t k_at = kRows * 128;
-    static constexpr uint32_t v_at = k_at + k_stages * kTileBytes;
-    static constexpr uint32_t ones_at = v_at + v_stages * kVPitch;
+    static constexpr uint32_t v_at = k_at + k_stages * k_bytes;
+    static constexpr uint32_t ones_at = v_at + v_stages * v_bytes;
     static constexpr uint32_t raw_at = ones_at + kOnesBytes;
     static constexpr uint32_t bars_at = raw_at + raw_stages * kRawBytes;
     static constexpr uint32_t order_at = bars_at + 512;  // lengths, then their order
@@ -110,9 +117,12 @@ constexpr uint32_t kLongTiles = 256;
 constexpr float kHeadroom = 8.f;
 constexpr uint32_t kPolyPairMask = 0x11u;  // pairs e with bit e % 8 set
 
-// Half of a tile's 64 rows of codes (those of this warp) into a 128-byte
-// swizzled f16 tile; `scale` holds the lane's two rows' f16 factors.
-DH_DEVINL void convert_rows(const uint8_t* raw, uint8_t* tile, uint32_t warp_half, uint32_t lane, __half f0, __half f1) {
+// Half of a tile's 64 rows of codes (those of this warp) into a 128-byte swizzled f16
+// tile; `factor`: of row `lane` of that half.  FINE: what it lacks into the tile `lo`
+// bytes behind it.
+template <bool FINE>
+DH_DEVINL void convert_rows(const uint8_t* raw, uint8_t* tile, uint32_t lo_at, uint32_t warp_half, uint32_t lane,
+                            float factor) {
     const uint32_t c = lane & 3u;
     uint4 codes[4];
 #pragma unroll
@@ -120,18 +130,24 @@ DH_DEVINL void convert_rows(const uint8_t* raw, uint8_t* tile, uint32_t warp_hal
         const uint32_t row = warp_half * 32 + i * 8 + (lane >> 2);
         codes[i] = *reinterpret_cast<const uint4*>(raw + row * kDh + c * 16);
     }
-    const uint32_t mine = __half_as_ushort(warp_half ? f1 : f0);
+    const uint32_t mine = __half_as_ushort(__float2half_rn(factor));
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t row = warp_half * 32 + i * 8 + (lane >> 2);
-        const __half f = __ushort_as_half(static_cast<uint16_t>(__shfl_sync(0xFFFFFFFFu, mine, i * 8 + (lane >> 2))));
-        const __half2 f2 = __half2half2(f);
-        const __half2 off = __hmul2(f2, __half2half2(__ushort_as_half(0x8080)));  // -2^-17
-        uint4 lo, hi;
-        convert16(codes[i], f2, off, lo, hi);
-        uint8_t* dst = tile + row * 128;
-        *reinterpret_cast<uint4*>(dst + (((2 * c) ^ (row & 7u)) * 16)) = lo;
-        *reinterpret_cast<uint4*>(dst + (((2 * c + 1) ^ (row & 7u)) * 16)) = hi;
+        const uint32_t row = warp_half * 32 + i * 8 + (lane >> 2), from = i * 8 + (lane >> 2);
+        const auto turn = [&](uint8_t* to, __half2 f, __half2 off) {
+            uint4 lo, hi;
+            convert16(codes[i], f, off, lo, hi);
+            *reinterpret_cast<uint4*>(to + row * 128 + (((2 * c) ^ (row & 7u)) * 16)) = lo;
+            *reinterpret_cast<uint4*>(to + row * 128 + (((2 * c + 1) ^ (row & 7u)) * 16)) = hi;
+        };
+        if constexpr (FINE) {
+            const FineFactor f = fine_factor(__shfl_sync(0xFFFFFFFFu, factor, from));
+            turn(tile, f.hi, f.off_hi);
+            turn(tile + lo_at, f.lo, f.off_lo);
+        } else {
+            const __half2 f = __half2half2(__ushort_as_half(static_cast<uint16_t>(__shfl_sync(0xFFFFFFFFu, mine, from))));
+            turn(tile, f, __hmul2(f, __half2half2(__ushort_as_half(0x8080))));  // (-2^-17)
+        }
     }
 }
 
@@ -165,7 +181,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
     using C = Cfg<KIND>;
     const uint32_t live = a.run_rows ? min(a.sequences, a.queries.of(min(*a.run_rows, 0x7FFFFFFFu))) : a.sequences;
     if (live == 0) {
-        if constexpr (KIND == kWide) grid_wait();  // (what waits for this kernel waits for that one)
+        if constexpr (C::wide) grid_wait();  // (what waits for this kernel waits for that one)
         return;
     }
     extern __shared__ uint8_t smem_raw[];
@@ -215,7 +231,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
     if (a.v_transposed) {
         for (uint32_t i = threadIdx.x; i < C::v_stages * 512; i += C::threads) {
             const uint32_t st = i / 512, w = i % 512;
-            reinterpret_cast<uint32_t*>(v_ring + st * kVPitch + kTileBytes)[w] = w < 32 ? one2 : 0u;
+            reinterpret_cast<uint32_t*>(v_ring + st * C::v_bytes + kTileBytes)[w] = w < 32 ? one2 : 0u;
         }
     } else {
         for (uint32_t i = threadIdx.x; i < 512; i += C::threads) {
@@ -229,7 +245,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
     __syncthreads();
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_holder;
-    if constexpr (KIND == kWide) grid_wait();  // (the keys are another kernel's)
+    if constexpr (C::wide) grid_wait();  // (the keys are another kernel's)
 
     if (warp == 0) {
         // ---------------------------------------------------------- loads
@@ -265,18 +281,26 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                             ok = false;
                             break;
                         }
-                        tc::mbar_arrive_expect_tx(&bars[kKFull + ks], kTileBytes);
-                        tc::tma_load_4d(k_ring + ks * kTileBytes, own ? &tok : &tpk, &bars[kKFull + ks], 0, key,
+                        tc::mbar_arrive_expect_tx(&bars[kKFull + ks], C::k_bytes);
+                        tc::tma_load_4d(k_ring + ks * C::k_bytes, own ? &tok : &tpk, &bars[kKFull + ks], 0, key,
                                         it.kv_head, entry);
+                        // (what they lack lies behind all entries)
+                        const uint32_t lo_entry = C::fine ? entry + (own ? a.sequences : a.prefixes) : 0u;
+                        if constexpr (C::fine)
+                            tc::tma_load_4d(k_ring + ks * C::k_bytes + kTileBytes, own ? &tok : &tpk,
+                                            &bars[kKFull + ks], 0, key, it.kv_head, lo_entry);
                         if (!tc::mbar_wait_suspend(&bars[kVEmpty + vs], ((g / C::v_stages) & 1u) ^ 1u,
                                                    tc::kErrTimeoutEmpty)) {
                             ++g;  // (the K tile is on its way)
                             ok = false;
                             break;
                         }
-                        tc::mbar_arrive_expect_tx(&bars[kVFull + vs], kTileBytes);
-                        tc::tma_load_4d(v_ring + vs * kVPitch, own ? &tov : &tpv, &bars[kVFull + vs],
+                        tc::mbar_arrive_expect_tx(&bars[kVFull + vs], C::fine ? 2 * kTileBytes : kTileBytes);
+                        tc::tma_load_4d(v_ring + vs * C::v_bytes, own ? &tov : &tpv, &bars[kVFull + vs],
                                         a.v_transposed ? key : 0, a.v_transposed ? 0 : key, it.kv_head, entry);
+                        if constexpr (C::fine)
+                            tc::tma_load_4d(v_ring + vs * C::v_bytes + kVPitch, own ? &tov : &tpv, &bars[kVFull + vs],
+                                            0, key, it.kv_head, lo_entry);
                     }
                 }
             }
@@ -298,17 +322,18 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
         // ------------------------------------------------------------ MMA
         if (tc::elect_one()) {
             const uint32_t o_tmem = tmem + kOCol;
+            constexpr uint32_t kIdescLo = tc::idesc_f16_f32<kRows, kDh>() | tc::kIdescBMnMajor;
             auto issue_s = [&](uint32_t g) -> bool {
                 const uint32_t ks = g % C::k_stages, sb = g & 1u;
                 if (!tc::mbar_wait_suspend(&bars[kKFull + ks], (g / C::k_stages) & 1u, tc::kErrTimeoutFull) ||
                     !tc::mbar_wait_suspend(&bars[kSPFree + sb], ((g >> 1) & 1u) ^ 1u, tc::kErrTimeoutAccEmpty))
                     return false;
                 tc::tc_fence_after();
-                const uint64_t k_desc = tc::smem_desc_sw128(k_ring + ks * kTileBytes);
+                const uint64_t k_desc = tc::smem_desc_sw128(k_ring + ks * C::k_bytes);
 #pragma unroll
-                for (uint32_t kk = 0; kk < kDh / 16; ++kk)
-                    tc::mma_f16_ts(tmem + sb * kKT, tmem + kQCol + kk * 8, tc::desc_advance(k_desc, kk * 32),
-                                   a.idesc_s, kk != 0);
+                for (uint32_t kk = 0; kk < C::k_bytes / kTileBytes * (kDh / 16); ++kk)
+                    tc::mma_f16_ts(tmem + sb * kKT, tmem + kQCol + (kk % 4) * 8,
+                                   tc::desc_advance(k_desc, kk / 4 * kTileBytes + (kk % 4) * 32), a.idesc_s, kk != 0);
                 tc::mma_commit(&bars[kSFull + sb]);
                 tc::mma_commit(&bars[kKEmpty + ks]);
                 return true;
@@ -333,7 +358,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                           tc::mbar_wait_suspend(&bars[kOFree], (n_items & 1u) ^ 1u, tc::kErrTimeoutAccEmpty));
                     if (!ok) break;
                     tc::tc_fence_after();
-                    const uint8_t* v_tile = v_ring + vs * kVPitch;
+                    const uint8_t* v_tile = v_ring + vs * C::v_bytes;
                     if (a.v_transposed) {
                         const uint64_t v_desc = tc::smem_desc_sw128(v_tile);
 #pragma unroll
@@ -347,6 +372,9 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                             tc::mma_f16_ts(o_tmem, tmem + sb * kKT + kk * 8,
                                            tc::smem_desc_mn_sw128(at, static_cast<uint32_t>(ones - at)), a.idesc_o,
                                            kk != 0 || j != it.t0);
+                            if constexpr (C::fine)
+                                tc::mma_f16_ts(o_tmem, tmem + sb * kKT + kk * 8,
+                                               tc::smem_desc_mn_sw128(at + kVPitch, kTileBytes), kIdescLo, true);
                         }
                     }
                     tc::mma_commit(&bars[kVEmpty + vs]);
@@ -407,8 +435,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                         exps[(g % kExpRing) * 2] = min(e[0], 126) + 9;
                         exps[(g % kExpRing) * 2 + 1] = ev + 9;
                     }
-                    convert_rows(raw, k_ring + ks * kTileBytes, half, lane, __float2half_rn(sc[0][0] * fk),
-                                 __float2half_rn(sc[0][1] * fk));
+                    convert_rows<C::fine>(raw, k_ring + ks * C::k_bytes, kTileBytes, half, lane, (half ? sc[0][1] : sc[0][0]) * fk);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&bars[kKFull + ks]);
@@ -417,8 +444,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                         ok = false;
                         break;
                     }
-                    convert_rows(raw + kKT * kDh, v_ring + vs * kVPitch, half, lane, __float2half_rn(sc[1][0] * fv),
-                                 __float2half_rn(sc[1][1] * fv));
+                    convert_rows<C::fine>(raw + kKT * kDh, v_ring + vs * C::v_bytes, kVPitch, half, lane, (half ? sc[1][1] : sc[1][0]) * fv);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
@@ -533,7 +559,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
             float m = -INFINITY;
             int32_t ev = -1000;  // exponent of O (int8 keys)
             float2 ex0 = make_float2(1.f, 0.f), ex1 = ex0;  // of the prefix, of its own keys
-            if constexpr (KIND == kWide) {
+            if constexpr (C::wide) {
                 if (it.len0) ex0 = a.prefix_exps[it.prefix * a.kv_heads.d + it.kv_head];
                 if (it.len1) ex1 = a.own_exps[it.own * a.kv_heads.d + it.kv_head];
             }
@@ -648,7 +674,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                         ok = false;
                         break;
                     }
-                    zero_rows(v_ring + vs * kVPitch, keys_left(it, j), a.v_transposed, r);
+                    zero_rows(v_ring + vs * C::v_bytes, keys_left(it, j), a.v_transposed, r);
                     fence_proxy_async_smem();
                 }
                 tc::mbar_arrive(&bars[kPFull + sb]);
@@ -926,7 +952,7 @@ struct Layout {
 };
 
 Layout layout_of(const Plan& p, uint64_t rows, uint32_t kv_heads, const uint32_t (&entries)[2],
-                 const uint32_t (&capacity)[2]) {
+                 const uint32_t (&capacity)[2], bool fine) {
     const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     Layout l{};
     if (p.slots > 1) {
@@ -938,7 +964,7 @@ Layout layout_of(const Plan& p, uint64_t rows, uint32_t kv_heads, const uint32_t
             const size_t lines = static_cast<size_t>(entries[i]) * kv_heads;
             l.exps[i] = l.bytes;
             l.wide[i] = up(l.exps[i] + lines * sizeof(float2));
-            l.bytes = l.wide[i] + 2 * lines * capacity[i] * kDh * 2;
+            l.bytes = l.wide[i] + (fine ? 4 : 2) * lines * capacity[i] * kDh * 2;
         }
     }
     return l;
@@ -967,15 +993,16 @@ uint32_t check_view(const dh_kv_view& v) {
     return DH_OK;
 }
 
-// Tiles of `keys` (32 or 64) rows of K and V.
-bool view_maps(CUtensorMap* k, CUtensorMap* v, const dh_kv_view& s, uint32_t entries, uint32_t heads, uint32_t keys) {
+// Tiles of `keys` (32 or 64) rows of K and V with `times` the entries.
+bool view_maps(CUtensorMap* k, CUtensorMap* v, const dh_kv_view& s, uint32_t entries, uint32_t heads, uint32_t keys,
+               uint32_t times = 1) {
     const auto type = [](uint32_t t) {
         return t == DH_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     };
     const bool rows = s.v_strides[3] == 1;
-    return make_tmap_4d(k, s.k, type(s.k_type), kDh, s.capacity, heads, entries, s.k_strides[2] * 2,
+    return make_tmap_4d(k, s.k, type(s.k_type), kDh, s.capacity, heads, times * entries, s.k_strides[2] * 2,
                         s.k_strides[1] * 2, s.k_strides[0] * 2, kDh, keys) &&
-           make_tmap_4d(v, s.v, type(s.v_type), rows ? kDh : s.capacity, rows ? s.capacity : kDh, heads, entries,
+           make_tmap_4d(v, s.v, type(s.v_type), rows ? kDh : s.capacity, rows ? s.capacity : kDh, heads, times * entries,
                         s.v_strides[rows ? 2 : 3] * 2, s.v_strides[1] * 2, s.v_strides[0] * 2, rows ? kDh : keys,
                         rows ? keys : kDh);
 }
@@ -1034,14 +1061,14 @@ using namespace dh;
 
 extern "C" size_t dh_kv_attention_workspace_size(uint32_t sequences, uint32_t queries, uint32_t heads,
                                                  uint32_t kv_heads, uint32_t prefixes, uint32_t prefix_capacity,
-                                                 uint32_t own_capacity, uint32_t k_type) {
+                                                 uint32_t own_capacity, uint32_t k_type, uint32_t q_type) {
     if (!sequences || !queries || !heads || !kv_heads || heads % kv_heads || (prefixes && sequences % prefixes) ||
         !fits(sequences, queries, heads, kv_heads, prefixes))
         return 0;
     const Plan p = plan_of(sequences, queries * (heads / kv_heads), kv_heads, prefixes, prefix_capacity, own_capacity,
                            k_type == DH_TYPE_I8, false, device_sms());
     return layout_of(p, static_cast<uint64_t>(sequences) * queries * heads, kv_heads, {prefixes, sequences},
-                     {prefix_capacity, own_capacity})
+                     {prefix_capacity, own_capacity}, q_type == DH_TYPE_F16)
         .bytes;
 }
 
@@ -1069,7 +1096,9 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
     const uint64_t rows = static_cast<uint64_t>(sequences) * queries * heads;
     const Plan p = plan_of(sequences, queries * ratio, kv_heads, prefixes, prefixes ? prefix->capacity : 0,
                            own->capacity, int8, own->lengths != nullptr, device_sms());
-    const Layout l = layout_of(p, rows, kv_heads, {prefixes, sequences}, {prefixes ? prefix->capacity : 0, own->capacity});
+    const bool fine = q_type == DH_TYPE_F16;  // (int8 keys)
+    const Layout l = layout_of(p, rows, kv_heads, {prefixes, sequences},
+                               {prefixes ? prefix->capacity : 0, own->capacity}, fine);
     const size_t need = l.bytes;
     if (need && !workspace) return DH_ERR_NULL_POINTER;
     if (need > workspace_bytes) return DH_ERR_WORKSPACE;
@@ -1086,7 +1115,7 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
     a.q = static_cast<const uint8_t*>(q);
     a.q_seq = q_strides[0] * 2, a.q_head = q_strides[1] * 2, a.q_row = q_strides[2] * 2;
     a.q_bf16 = q_type == DH_TYPE_BF16;
-    a.sequences = sequences, a.heads = heads;
+    a.sequences = sequences, a.prefixes = prefixes, a.heads = heads;
     a.queries = FastDiv(queries), a.kv_heads = FastDiv(kv_heads), a.ratio = FastDiv(ratio);
     a.per_prefix = FastDiv(prefixes ? sequences / prefixes : sequences);
     a.v_transposed = !int8 && own->v_strides[3] != 1;
@@ -1120,13 +1149,15 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
             uint8_t* base = static_cast<uint8_t*>(workspace);
             to[i].exps = reinterpret_cast<float2*>(base + l.exps[i]);
             to[i].k = reinterpret_cast<__half*>(base + l.wide[i]);
-            to[i].v = to[i].k + static_cast<size_t>(entries) * kv_heads * capacity * kDh;
+            const size_t each = static_cast<size_t>(entries) * kv_heads * capacity * kDh;
+            to[i].lo = fine ? each : 0;
+            to[i].v = to[i].k + (fine ? 2 : 1) * each;
             dh_kv_view f{};
             f.k = to[i].k, f.v = to[i].v, f.k_type = f.v_type = DH_TYPE_F16, f.capacity = capacity;
             f.k_strides[2] = f.v_strides[2] = kDh, f.k_strides[3] = f.v_strides[3] = 1;
             f.k_strides[1] = f.v_strides[1] = static_cast<uint64_t>(capacity) * kDh;
             f.k_strides[0] = f.v_strides[0] = static_cast<uint64_t>(capacity) * kDh * kv_heads;
-            if (!view_maps(&maps[2 * i], &maps[2 * i + 1], f, entries, kv_heads, kKT)) return DH_ERR_CUDA;
+            if (!view_maps(&maps[2 * i], &maps[2 * i + 1], f, entries, kv_heads, kKT, fine ? 2 : 1)) return DH_ERR_CUDA;
         }
         a.prefix_exps = to[0].exps, a.own_exps = to[1].exps;
         if (uint32_t status = launch_widen(a, to[0], to[1], prefixes, st)) return status;
@@ -1135,14 +1166,13 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
     uint32_t status = DH_OK, first = 0, total = 0;
     for (uint32_t i = 0; i < 2; ++i)
         if (!p.few[i]) total += a.cls[i].items, first += i ? 0 : a.cls[0].items;
-    if (total && p.widen)
-        status = launch<kWide>(maps, a, first, total, p.many_cluster, true, st);
-    else if (total)
-        status = int8 ? launch<kInt8>(maps, a, first, total, p.many_cluster, false, st)
-                      : (v_bf16 ? launch<kVBf16>(maps, a, first, total, p.many_cluster, false, st)
-                                : launch<kV16>(maps, a, first, total, p.many_cluster, false, st));
+    if (total) {
+        const auto go = !int8 ? (v_bf16 ? launch<kVBf16> : launch<kV16>)
+                        : p.widen ? (fine ? launch<kWideFine> : launch<kWide>) : (fine ? launch<kInt8Fine> : launch<kInt8>);
+        status = go(maps, a, first, total, p.many_cluster, p.widen, st);
+    }
     bool beside = total;
-    const uint32_t taken = total ? (int8 ? Cfg<kInt8>::bytes : Cfg<kV16>::bytes) + 1024 : 0;
+    const uint32_t taken = total ? (!int8 ? Cfg<kV16>::bytes : fine ? Cfg<kInt8Fine>::bytes : Cfg<kInt8>::bytes) + 1024 : 0;
     for (uint32_t i = 0; i < 2 && !status; ++i) {
         if (!p.few[i]) continue;
         status = launch_few(few_maps, a, i, p.cluster[i], int8, v_bf16, beside, taken, st);

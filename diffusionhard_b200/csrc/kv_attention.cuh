@@ -44,7 +44,7 @@ struct Args {
     const uint8_t* q;                        // 16-bit elements
     uint64_t q_seq, q_head, q_row;           // strides in bytes
     uint32_t q_bf16;
-    uint32_t sequences, heads;
+    uint32_t sequences, prefixes, heads;
     FastDiv queries, kv_heads, ratio, per_prefix;  // ratio: query heads of a K/V head
     uint32_t v_transposed, idesc_s, idesc_o;
     float c;                                 // scale * log2(e)
@@ -112,6 +112,19 @@ DH_DEVINL void convert16(const uint4& codes, __half2 f, __half2 off, uint4& lo, 
     convert4(codes.w, f, off, hi.z, hi.w);
 }
 
+// The same with f = hi + lo and hi of 4 bits, so that code * hi is exact: 4 f16 of code *
+// hi 2^-24 and of code * lo 2^-24, whose sum is off by 2^-15.
+struct FineFactor {
+    __half2 hi, lo, off_hi, off_lo;
+};
+DH_DEVINL FineFactor fine_factor(float f) {
+    const float hi = __uint_as_float((__float_as_uint(f) + (1u << 19)) & 0xFFF00000u);
+    const __half2 shift = __half2half2(__ushort_as_half(0x8080));  // -2^-17
+    FineFactor r;
+    r.hi = __float2half2_rn(hi), r.lo = __float2half2_rn(f - hi);
+    r.off_hi = __hmul2(r.hi, shift), r.off_lo = __hmul2(r.lo, shift);
+    return r;
+}
 struct Item {
     uint32_t seq0, kv_head, row0, rows, slot;  // rows: live rows of the tile (may be 0)
     uint32_t prefix, own;                      // cache entries

@@ -21,7 +21,9 @@
 // int8: scores are (q . codes) * scale of the key, by the integer instruction on the
 // codes as they are, with the query in two int8 parts (15 bits of its row's largest
 // value).  The weights enter the second product as f16(p * v_scale 2^-E), E an
-// exponent that only grows (one for a warp), the codes of V exact as f16.
+// exponent that only grows (one for a warp), the codes of V exact as f16; for f16
+// queries as two f16 (16 long caches 101 us in bf16 and 112 in f16; error of the
+// result 3.0e-4 with one, 2.2e-4 with two, 2.0e-4 of that its own rounding).
 //
 // An item's keys are shared by the four warps of a CTA and the CTAs of a cluster, which
 // join their sums through shared memory in a fixed order.  Where there are items
@@ -121,6 +123,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
     constexpr bool kI8 = KIND == kInt8;
     constexpr uint32_t kN = kKeys<KIND>, kSteps = kN / 16;
     constexpr uint32_t kTile16 = kN * kDh * 2;  // bytes of a 16-bit tile of K
+    constexpr bool kFine = kI8 && !QBF16;  // weights in two f16
     constexpr bool kQB = QBF16 && !kI8;  // type of the first product's operands
     const uint32_t live = a.run_rows ? min(a.sequences, a.queries.of(min(*a.run_rows, 0x7FFFFFFFu))) : a.sequences;
     extern __shared__ uint8_t smem_raw[];
@@ -424,13 +427,23 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
         // O^T += V^T P^T, 16 keys at a time
 #pragma unroll
         for (uint32_t k = 0; k < kSteps; ++k) {
-            uint32_t pb[NT][2];
+            uint32_t pb[NT][2], pl[NT][2];
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (uint32_t h = 0; h < 2; ++h)
                     pb[t][h] = transposed(KIND == kVBf16 ? pack_bf16x2(s[t][k][2 * h], s[t][k][2 * h + 1])
                                                          : pack_f16x2(s[t][k][2 * h], s[t][k][2 * h + 1]));
+            if constexpr (kFine) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; ++h) {
+                        const float x = s[t][k][2 * h], y = s[t][k][2 * h + 1];
+                        const __half2 p = __floats2half2_rn(x, y);
+                        pl[t][h] = transposed(pack_f16x2(x - __low2float(p), y - __high2float(p)));
+                    }
+            }
             if constexpr (kI8) {
                 // row g of part i is d = 8 g + 2 i, row g + 8 the next one: a thread reads
                 // d = 8 g .. 8 g + 7 of its four keys and pairs them up byte by byte
@@ -455,6 +468,10 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
                     for (int t = 0; t < NT; ++t) {
                         mma_16816<false>(o[t][2 * hw], va, pb[t][0], pb[t][1]);
                         mma_16816<false>(o[t][2 * hw + 1], vb, pb[t][0], pb[t][1]);
+                        if constexpr (kFine) {
+                            mma_16816<false>(o[t][2 * hw], va, pl[t][0], pl[t][1]);
+                            mma_16816<false>(o[t][2 * hw + 1], vb, pl[t][0], pl[t][1]);
+                        }
                     }
                 }
             } else {

@@ -31,10 +31,12 @@ inline cudaError_t all_shared_once(Kernel kernel, uint32_t bytes, std::atomic<ui
 uint32_t launch_few(const CUtensorMap (&maps)[4], const Args& a, uint32_t cls, uint32_t cluster, bool int8, bool v_bf16,
                     bool beside, uint32_t taken, cudaStream_t st);
 
-// f16 rows [lines][capacity][64] of K and V, and [lines] their exponents.
+// f16 rows [lines][capacity][64] of K and V, `lo` elements behind them (0: none) what
+// they lack, and [lines] their exponents.
 struct WideKeys {
     __half* k = nullptr;
     __half* v = nullptr;
+    size_t lo = 0;
     float2* exps = nullptr;
 };
 

@@ -51,6 +51,8 @@ DH_DEVINL uint32_t largest(const float* scale, uint32_t n, uint32_t* smem) {
 
 DH_DEVINL int32_t exponent_in_range(uint32_t bits) { return min(max(exponent_of(bits), -100), 126); }
 
+// FINE: see FineFactor.
+template <bool FINE>
 __global__ void __launch_bounds__(kThreads) kv_widen_kernel(const __grid_constant__ WidenArgs a) {
     __shared__ uint32_t smem[kThreads / 32];
     grid_launch_dependents();
@@ -103,12 +105,24 @@ __global__ void __launch_bounds__(kThreads) kv_widen_kernel(const __grid_constan
             if (t >= tiles) break;
 #pragma unroll
             for (uint32_t side = 0; side < 2; ++side) {
-                const __half2 f = __float2half2_rn(scale[i][side] * (side ? fv : fk));
-                const __half2 off = __hmul2(f, __half2half2(__ushort_as_half(0x8080)));
+                const float by = scale[i][side] * (side ? fv : fk);
+                const uint2 w = codes[i][side];
                 uint4 x;
-                convert4(codes[i][side].x, f, off, x.x, x.y);
-                convert4(codes[i][side].y, f, off, x.z, x.w);
-                reinterpret_cast<uint4*>((side ? to.v : to.k) + (at + key) * kDh)[c] = x;
+                __half* dst = (side ? to.v : to.k) + (at + key) * kDh;
+                if constexpr (FINE) {
+                    const FineFactor f = fine_factor(by);
+                    convert4(w.x, f.lo, f.off_lo, x.x, x.y);
+                    convert4(w.y, f.lo, f.off_lo, x.z, x.w);
+                    reinterpret_cast<uint4*>(dst + to.lo)[c] = x;
+                    convert4(w.x, f.hi, f.off_hi, x.x, x.y);
+                    convert4(w.y, f.hi, f.off_hi, x.z, x.w);
+                } else {
+                    const __half2 f = __float2half2_rn(by);
+                    const __half2 off = __hmul2(f, __half2half2(__ushort_as_half(0x8080)));
+                    convert4(w.x, f, off, x.x, x.y);
+                    convert4(w.y, f, off, x.z, x.w);
+                }
+                reinterpret_cast<uint4*>(dst)[c] = x;
             }
         }
     }
@@ -132,7 +146,10 @@ uint32_t launch_widen(const Args& a, const WideKeys& prefix, const WideKeys& own
     w.own_chunks = chunks(own_lines, a.own.capacity);
     w.prefix_chunks = prefixes ? chunks(prefix_lines, a.prefix.capacity) : 1;
     const uint64_t ctas = own_lines * w.own_chunks + prefix_lines * w.prefix_chunks;
-    kv_widen_kernel<<<static_cast<uint32_t>(ctas), kThreads, 0, st>>>(w);
+    if (own.lo)
+        kv_widen_kernel<true><<<static_cast<uint32_t>(ctas), kThreads, 0, st>>>(w);
+    else
+        kv_widen_kernel<false><<<static_cast<uint32_t>(ctas), kThreads, 0, st>>>(w);
     DH_LAUNCH_CHECK();
     return DH_OK;
 }

@@ -329,7 +329,7 @@ def attend(q: torch.Tensor, kv: Any, lengths: Lengths = None, *, prefix: Any = N
     run = _run_rows(run_rows, index)
     if batch and n and heads:
         size = _workspace_bytes(batch, n, heads, kv_heads, prefixes, prefix_capacity, keys.capacity,
-                                keys.v_type == _TYPE_I8, index)
+                                keys.v_type == _TYPE_I8, q_type, index)
         # (goes back to the allocator's pool of the current stream, which the
         # kernels that use it are on)
         ws = q.new_empty((size,), dtype=torch.uint8) if size else None
@@ -340,7 +340,7 @@ def attend(q: torch.Tensor, kv: Any, lengths: Lengths = None, *, prefix: Any = N
 
 @functools.lru_cache(maxsize=256)
 def _workspace_bytes(batch: int, n: int, heads: int, kv_heads: int, prefixes: int, prefix_capacity: int,
-                     capacity: int, int8: bool, index: int) -> int:
+                     capacity: int, int8: bool, q_type: int, index: int) -> int:
     with torch.cuda.device(index):
         return int(_lib.lib().dh_kv_attention_workspace_size(batch, n, heads, kv_heads, prefixes, prefix_capacity,
-                                                             capacity, _TYPE_I8 if int8 else _TYPES[torch.bfloat16]))
+                                                             capacity, _TYPE_I8 if int8 else q_type, q_type))

@@ -110,8 +110,8 @@ def test_prefixes_refused():
 
 def test_workspace():
     f = _lib.lib().dh_kv_attention_workspace_size
-    assert f(0, 1, 4, 4, 0, 0, 64, 1) == 0 and f(1, 1, 4, 3, 0, 0, 64, 1) == 0 and f(3, 1, 4, 4, 2, 64, 64, 1) == 0
-    size = f(1, 1, 4, 4, 0, 0, 1 << 16, 1)
+    assert f(0, 1, 4, 4, 0, 0, 64, 1, 1) == 0 and f(1, 1, 4, 3, 0, 0, 64, 1, 1) == 0 and f(3, 1, 4, 4, 2, 64, 64, 1, 1) == 0
+    size = f(1, 1, 4, 4, 0, 0, 1 << 16, 1, 1)
     assert 0 < size <= 64 * 4 * 264 + 256
     long = _view(capacity=1 << 16, length=1)
     args = dict(n=1, queries=1)

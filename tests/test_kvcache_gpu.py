@@ -68,6 +68,7 @@ def ref_attend(q, kv, lengths, prefix=None, prefix_lengths=None, scale=0.125):
     bound = torch.zeros_like(out)
     lse_bound = torch.zeros_like(lse)
     int8 = isinstance(kv, KVCacheI8)
+    fine = int8 and q.dtype is F16
     # (half a step of 16 bits, relative: eps / 2)
     p_round = 2.0 ** -8 if not int8 and kv[1].dtype is BF16 else 2.0 ** -11
     for b in range(batch):
@@ -88,20 +89,22 @@ def ref_attend(q, kv, lengths, prefix=None, prefix_lengths=None, scale=0.125):
             w = p / total
             o = w @ vh
             # a score: fp32 sums of 64 products; int8 rows are rounded to f16 twice
-            # (factor and product), with a floor of 2^-19 of the largest row
-            ks = (64 * 2.0 ** -24 + (2.0 ** -10 if int8 else 0)) * scale * (x.abs() @ kh.abs().T)
+            # (factor and product), for f16 queries as two f16 (2^-15 each time), with
+            # a floor of 2^-19 of the largest row
+            ks = (64 * 2.0 ** -24 + (0 if not int8 else 2.0 ** -14 if fine else 2.0 ** -10)) * scale * (x.abs() @ kh.abs().T)
             if int8:
                 ks = ks + 2.0 ** -19 * scale * x.abs().sum(-1, keepdim=True) * kh.abs().max()
                 # (a query value below 2^-14 of its row's largest is rounded to 2^-25 of that)
-                ks = ks + 2.0 ** -24 * scale * x.abs().amax(-1, keepdim=True) * kh.abs().sum(-1)[None, :]
+                # (of few rows it has 15 bits)
+                ks = ks + 2.0 ** (-15 if fine else -24) * scale * x.abs().amax(-1, keepdim=True) * kh.abs().sum(-1)[None, :]
             # a weight: its score, s c - m in fp32, the cubic for 2^x (7.8e-5), rounding
             # to 16 bits, whose smallest step is 2^-25 of a weight of 1
             e = ks + 2.0 ** -22 * ((s - m).abs().clamp(max=200) + s.abs()) + 8e-5 + p_round
             floor = (2.0 ** -25 / total).expand_as(w) if p_round < 2.0 ** -8 else torch.zeros_like(w)
             we = w * e + floor
             err = we @ vh.abs() + we.sum(-1, keepdim=True) * o.abs()
-            # V: rounded to f16 twice, with a floor; fp32 sums of the products
-            err = err + (k.shape[1] * 2.0 ** -24 + (2.0 ** -10 if int8 else 0)) * (w @ vh.abs())
+            # V: rounded to f16 twice, or to two f16, with a floor; fp32 sums of the products
+            err = err + (k.shape[1] * 2.0 ** -24 + (0 if not int8 else 2.0 ** -14 if fine else 2.0 ** -10)) * (w @ vh.abs())
             if int8:
                 err = err + 2.0 ** -19 * vh.abs().max()
             out[b, :, h], lse[b, :, h] = o, (m + torch.log(total))[:, 0]
@@ -278,6 +281,22 @@ def case(batch, heads, kv_heads, n, length, kind, seed, capacity=None):
 def test_queries(cuda, n, kind):
     q, kv, length = case(2, 2, 2, n, 150, kind, n, capacity=200)
     check(q, kv, length)
+
+
+@pytest.mark.parametrize("n, batch, length, prefix", [(1, 2, 700, 0), (16, 2, 130, 0), (17, 2, 1, 0), (40, 3, 3000, 0),
+                                                      (129, 2, 65, 200), (600, 2, 1000, 0), (520, 4, 333, 130)])
+def test_f16_queries_over_int8(cuda, n, batch, length, prefix):
+    """Whose rounding shows more than bf16's: keys and values as two f16."""
+    q, kv, _ = case(batch, 4, 2, n, length, "int8", n, capacity=length + 70)
+    pre, pre_length = None, None
+    if prefix:
+        _, pre, pre_length = case(batch // 2, 4, 2, 1, prefix, "int8", 9, capacity=prefix + 60)
+    check(q.half(), kv, length, pre, pre_length)
+    got = attend(q.half(), kv, length, prefix=pre, prefix_lengths=pre_length)
+    ref = ref_attend(q.half(), kv, [length] * batch, pre, [pre_length] * (batch // 2))[0]
+    # at random: the output and a weight each 2^-11 / sqrt(3) at most, and scores 2^-14 of
+    # a few units
+    assert float((got.double().cpu() - ref).norm() / ref.norm()) < 2.0 ** -11
 
 
 @pytest.mark.parametrize("heads, kv_heads", [(4, 1), (6, 2), (7, 7), (16, 4), (5, 1), (200, 1)])
