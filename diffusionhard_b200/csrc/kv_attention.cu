@@ -11,11 +11,12 @@
 // Work items.  A row is a (query, query head of the K/V head) pair; 128 rows
 // make a tile of the tensor core.  An item is (row tile, K/V head, a range of
 // key tiles of 64).  Rows of one sequence walk its prefix and its own keys.  With
-// few rows a sequence, the rows of all sequences of a group are stacked over the
-// prefix, which is then read once for all of them, and the sequences' own keys
-// are items of their own.  Where keys of a row fall to several items, each
-// leaves its unnormalised sums and maximum in the workspace and a second kernel
-// joins them in a fixed order.
+// fewer than 128 rows a sequence, the rows of all sequences of a group are stacked
+// over the prefix, which is then read once for all of them, and the sequences' own
+// keys are items of their own.  Items of at most 16 rows are kv_few.cu's.  Where keys of
+// a row fall to several items, the CTAs of a cluster join their sums through shared
+// memory, or each item leaves its unnormalised sums and maximum in the workspace and
+// a further kernel joins them, both in a fixed order.
 //
 // One persistent kernel, two CTAs per SM, 6 warps (int8: 8):
 //   warp 0    loads: TMA tiles of K and V (16 bits), or the contiguous codes and
@@ -25,6 +26,12 @@
 //   warps 2-3 int8 alone: codes to f16 tiles, see convert_rows
 //   four more softmax, a thread a row: P = 2^(s c - m) over S in TMEM; O in TMEM
 //             is rescaled only when the maximum grew by more than 2^15
+//
+// Bound by the softmax: 128 x 512 queries over 1024 16-bit keys take 302 us in a burst
+// (683 TFLOP/s; 350 us under the power cap), exponentials 47%, issue slots 47% and the tensor pipe 34% of the time
+// busy, with eight warps an SM that wait for one another in turn.  Tried and slower:
+// exponentials of f16 pairs (360 then, where this took 338), four CTAs an SM with
+// 128 columns of TMEM each (365), registers moved between the warps (no change).
 #include <cuda.h>
 
 #include "kv_kernels.h"
@@ -762,25 +769,11 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const float2* ml,
     if (run_rows)
         live = min(rows, static_cast<uint64_t>(queries.of(min(*run_rows, 0x7FFFFFFFu))) * queries.d * heads);
     const bool mine = row < live;  // (lanes of other rows stay for the exchanges)
-    float top = -INFINITY;
-    for (uint32_t s = c; s < slots; s += 8) {
-        const float2 x = mine ? ml[s * rows + row] : make_float2(0.f, 0.f);
-        if (x.y != 0.f) top = max_nan(top, x.x);
-    }
-#pragma unroll
-    for (uint32_t o = 1; o < 8; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    float l = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    // (all loads before their use, the first eight parts' before the maximum is known;
+    // what an empty part holds is dropped, not added)
     const float4* from = reinterpret_cast<const float4*>(part + row * kDh) + c;
-    for (uint32_t s0 = 0; s0 < slots; s0 += 8) {
-        float w = 0.f;
-        if (mine && s0 + c < slots) {
-            const float2 x = ml[(s0 + c) * rows + row];
-            w = x.y != 0.f ? ex2_approx(x.x - top) : 0.f;
-            l = __fmaf_rn(w, x.y, l);
-        }
-        // (all loads before their use: what an empty part holds is dropped, not added)
-        float4 xs[8], ys[8];
+    float4 xs[8], ys[8];
+    const auto load = [&](uint32_t s0) {
 #pragma unroll
         for (uint32_t k = 0; k < 8; ++k) {
             xs[k] = ys[k] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -789,13 +782,32 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const float2* ml,
                 xs[k] = at[0], ys[k] = at[8];
             }
         }
+    };
+    const auto stats = [&](uint32_t s) { return mine && s < slots ? ml[s * rows + row] : make_float2(0.f, 0.f); };
+    float2 x = stats(c);
+    load(0);
+    float top = x.y != 0.f ? x.x : -INFINITY;
+    for (uint32_t s = c + 8; s < slots; s += 8) {
+        const float2 other = stats(s);
+        if (other.y != 0.f) top = max_nan(top, other.x);
+    }
+#pragma unroll
+    for (uint32_t o = 1; o < 8; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    float l = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    for (uint32_t s0 = 0; s0 < slots; s0 += 8) {
+        if (s0) {
+            x = stats(s0 + c);
+            load(s0);
+        }
+        const float w = x.y != 0.f ? ex2_approx(x.x - top) : 0.f;
+        l = __fmaf_rn(w, x.y, l);
 #pragma unroll
         for (uint32_t k = 0; k < 8; ++k) {
             const float f = __shfl_sync(0xFFFFFFFFu, w, (threadIdx.x & 24u) + k);
             if (f == 0.f) continue;
-            const float4 x = xs[k], y = ys[k];
-            a = make_float4(__fmaf_rn(f, x.x, a.x), __fmaf_rn(f, x.y, a.y), __fmaf_rn(f, x.z, a.z), __fmaf_rn(f, x.w, a.w));
-            b = make_float4(__fmaf_rn(f, y.x, b.x), __fmaf_rn(f, y.y, b.y), __fmaf_rn(f, y.z, b.z), __fmaf_rn(f, y.w, b.w));
+            add(a, f, xs[k]);
+            add(b, f, ys[k]);
         }
     }
 #pragma unroll

@@ -277,13 +277,18 @@ def attend(q: torch.Tensor, kv: Any, lengths: Lengths = None, *, prefix: Any = N
 
     ``scale`` defaults to 1/8.  A query without keys gives 0.  With
     ``return_lse`` also the log of the sum of exponentials, fp32 [batch, n, heads]
-    (-inf without keys), to join results over disjoint keys.  Scores and sums are
-    fp32; the weights enter the product with V rounded to 16 bits (f16; bf16 for
-    V in bf16), int8 rows rounded to f16.  ``run_rows``: one device word, only the
-    sequences within its first rows of [batch * n] are computed.
+    (-inf without keys), to join results over disjoint keys.  ``run_rows``: one
+    device word, only the sequences within its first rows of [batch * n] are computed.
 
-    Calls that split the keys take up to 264 bytes of workspace for each query,
-    head and part."""
+    Scores and sums are fp32; the weights enter the product with V rounded to 16
+    bits (f16; bf16 for V in bf16).  Int8 rows are rounded to f16 where a K/V head
+    has more than 16 query rows; for f16 queries they are held as two f16.  A score
+    counts to 2^-23 of its size.
+
+    Calls that split the keys take 264 bytes of workspace for each query, head and
+    part (at most 64 of the prefix and 64 of the rest); calls whose queries visit
+    int8 keys many times hold those as f16, 256 bytes (f16 queries: 512) for each
+    position and K/V head."""
     index = q.get_device()
     q_type = _TYPES.get(q.dtype)
     if index < 0:

@@ -787,7 +787,15 @@ typedef struct dh_kv_view {
  *               64, or NULL
  *   run_rows    as in dh_kv_write_i8, with queries rows a sequence
  *   workspace   256-byte aligned, of the size the query returns for the current
- *               device (0: none); calls that may overlap need one each
+ *               device (0: none) from the shape, the capacities, k_type of own and
+ *               q_type; calls that may overlap need one each.  264 bytes for each
+ *               query, head and part of the keys, at most 64 parts of the prefix and
+ *               64 of the rest, and, where many queries visit int8 keys, their rows as
+ *               f16: 256 bytes (f16 queries: 512) a position and K/V head
+ * Scores and sums are fp32; weights are rounded to 16 bits (f16; bf16 for V in
+ * bf16) before the product with V; int8 rows times their scales are rounded to f16
+ * (f16 queries: held as two f16) where a K/V head has more than 16 rows.  A score
+ * counts to 2^-23 of its size.  V up to 2^90 in magnitude.
  * Results do not depend on timing: the same call gives the same bits.
  * Status: DH_ERR_*. */
 size_t dh_kv_attention_workspace_size(uint32_t sequences, uint32_t queries, uint32_t heads, uint32_t kv_heads,
