@@ -11,9 +11,9 @@
 // Work items.  A row is a (query, query head of the K/V head) pair; 128 rows
 // make a tile of the tensor core.  An item is (row tile, K/V head, a range of
 // key tiles of 64).  Rows of one sequence walk its prefix and its own keys.  With
-// fewer than 128 rows a sequence, the rows of all sequences of a group are stacked
-// over the prefix, which is then read once for all of them, and the sequences' own
-// keys are items of their own.  Items of at most 16 rows are kv_few.cu's.  Where keys of
+// few rows a sequence, those of all sequences of a group are stacked over the prefix,
+// which is then read once for all of them, and the sequences' own keys are items of
+// their own (see plan_of).  Items of at most 16 rows are kv_few.cu's.  Where keys of
 // a row fall to several items, the CTAs of a cluster join their sums through shared
 // memory, or each item leaves its unnormalised sums and maximum in the workspace and
 // a further kernel joins them, both in a fixed order.
@@ -28,8 +28,9 @@
 //             is rescaled only when the maximum grew by more than 2^15
 //
 // Bound by the softmax: 128 x 512 queries over 1024 16-bit keys take 302 us in a burst
-// (683 TFLOP/s; 350 us under the power cap), exponentials 47%, issue slots 47% and the tensor pipe 34% of the time
-// busy, with eight warps an SM that wait for one another in turn.  Tried and slower:
+// (683 TFLOP/s; 350 us under the power cap), exponentials 47%, issue slots 47% and the
+// tensor pipe 34% of the time busy, with eight warps an SM that wait for one another in
+// turn.  Tried and slower:
 // exponentials of f16 pairs (360 then, where this took 338), four CTAs an SM with
 // 128 columns of TMEM each (365), registers moved between the warps (no change).
 #include <cuda.h>
@@ -824,8 +825,6 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const float2* ml,
 
 // ------------------------------------------------------------------ plan
 
-// Rows a sequence must have before its items walk the prefix by themselves.
-constexpr uint32_t kStackBelow = 128;
 // Visits of every tile of int8 keys from which they are turned into f16 first.
 constexpr uint32_t kWidenFrom = 4;
 
@@ -836,15 +835,18 @@ struct Plan {
     uint32_t cluster[2];
     uint32_t many_cluster;  // CTAs an item of tensor-core tiles, 0: none share one
     uint32_t slots;
+    uint64_t estimate;    // of tensor-core tiles alone, in tiles
 };
 
 uint32_t ceil_div(uint64_t a, uint64_t b) { return static_cast<uint32_t>((a + b - 1) / b); }
 
-// Few rows: a warp an item where there are items enough with few tiles.  Else parts
-// of at least a tile a warp, up to eight in a cluster until the GPU has four CTAs
-// an SM, then as many clusters as that still takes.
+// Few rows: a warp an item where there are items enough with few tiles (single tokens,
+// 12 heads, int8, such warps and the other way: 40 x 128 keys 8.3 and 10.3 us, 64 x 256
+// 12.4 and 14.5, 64 x 1024 28.8 and 26.8, 100 x 1024 31.9 and 37.9, 128 x 1024 36.5 and
+// 45.3, 128 x 4096 111 and 98).  Else parts of at least a tile a warp, up to eight in a
+// cluster until the GPU has four CTAs an SM, then as many clusters as that still takes.
 void split_few(Class& c, uint32_t& cluster, uint64_t items, uint32_t tiles, uint32_t sms) {
-    if (items >= 8ull * sms && tiles <= 32) {
+    if (items >= 3ull * sms && tiles <= (items >= 8ull * sms ? 32u : 8u)) {
         cluster = 0;
         return;
     }
@@ -865,8 +867,9 @@ void split_few(Class& c, uint32_t& cluster, uint64_t items, uint32_t tiles, uint
 // which not all run at once, and 47 with the kernel; 8 x 12 items of 16 tiles 17.2 us
 // in clusters of two and 16.5 with the kernel and three parts, which is another launch).
 // Returns the size of the clusters, 0: none.
-uint32_t split_many(Class* cls, const uint64_t* items, const uint32_t* tiles, uint32_t ctas, bool joined) {
-    uint64_t best = ~0ull;
+uint32_t split_many(Class* cls, const uint64_t* items, const uint32_t* tiles, uint32_t ctas, bool joined,
+                    uint64_t& best) {
+    best = ~0ull;
     uint32_t best_splits[2] = {1, 1}, best_cluster = 0;
     const uint32_t most = std::max(std::max(items[0] ? tiles[0] : 0, items[1] ? tiles[1] : 0), 1u);
     for (uint32_t n = 1; n <= kMaxSplits; ++n) {
@@ -901,11 +904,11 @@ uint32_t split_many(Class* cls, const uint64_t* items, const uint32_t* tiles, ui
     return best_cluster;
 }
 
-Plan plan_of(uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t prefixes, uint32_t prefix_keys,
-             uint32_t own_keys, bool int8, bool ragged, uint32_t sms) {
+// stacked: a group's rows are stacked over its prefix.
+Plan plan_with(bool stacked, uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t prefixes,
+               uint32_t prefix_keys, uint32_t own_keys, bool int8, bool ragged, uint32_t sms) {
     Plan p{};
     const uint32_t per = prefixes ? sequences / prefixes : sequences;
-    const bool stacked = prefixes && per > 1 && rows < kStackBelow;
     const uint32_t t0 = ceil_div(prefix_keys, kKT), t1 = ceil_div(own_keys, kKT);
     const uint32_t tiles[2] = {stacked ? t0 : 0, t1 + (stacked || !prefixes ? 0 : t0)};
     uint64_t items[2] = {0, 0}, many[2] = {0, 0};
@@ -934,7 +937,7 @@ Plan plan_of(uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t pref
     const uint64_t tiles_held = static_cast<uint64_t>(kv_heads) * (static_cast<uint64_t>(sequences) * t1 +
                                                                   static_cast<uint64_t>(prefixes) * t0);
     p.widen = int8 && !p.few[0] && !p.few[1] && visits >= kWidenFrom * tiles_held;
-    if (many[0] || many[1]) p.many_cluster = split_many(p.cls, many, tiles, p.few[1] ? sms : 2 * sms, stacked);
+    if (many[0] || many[1]) p.many_cluster = split_many(p.cls, many, tiles, p.few[1] ? sms : 2 * sms, stacked, p.estimate);
     for (int i = 0; i < 2; ++i) {
         if (!items[i]) continue;
         Class& c = p.cls[i];
@@ -946,6 +949,25 @@ Plan plan_of(uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t pref
         p.slots += i && p.many_cluster ? 1 : c.splits.d;
     }
     return p;
+}
+
+// Rows of a group are stacked over its prefix where that saves more than the parts of
+// rows and their joining cost.  Up to 16 rows a sequence: from 17 visits an SM of the
+// prefix's tiles saved (8 single tokens behind 512 keys 10.3 us either way, behind 4000
+// 23.1 and 12.5; 16 x 4 behind 1000 20.6 and 16.8, 16 x 16 behind 500 14.4 and 16.8).
+// Else by the estimates, with a tile's time for 4000 rows of parts (64 x 32 rows behind 1000 keys 53.2 and 73.7, 8 x 96
+// behind 4000 39.1 and 53.2, 8 x 32 behind 4000 32.6 and 24.7, 2 x 20 behind 8000 26.7
+// and 20.6).
+Plan plan_of(uint32_t sequences, uint32_t rows, uint32_t kv_heads, uint32_t prefixes, uint32_t prefix_keys,
+             uint32_t own_keys, bool int8, bool ragged, uint32_t sms) {
+    const Plan p = plan_with(false, sequences, rows, kv_heads, prefixes, prefix_keys, own_keys, int8, ragged, sms);
+    if (!prefixes || sequences == prefixes) return p;
+    const Plan s = plan_with(true, sequences, rows, kv_heads, prefixes, prefix_keys, own_keys, int8, ragged, sms);
+    if (p.few[1])
+        return static_cast<uint64_t>(sequences - prefixes) * kv_heads * ceil_div(prefix_keys, kKT) >= 17ull * sms ? s : p;
+    const uint64_t all = static_cast<uint64_t>(sequences) * rows * kv_heads;
+    const auto cost = [&](const Plan& x) { return x.estimate + (x.slots > 1 ? all * x.slots / 4000 : 0); };
+    return cost(s) < cost(p) ? s : p;
 }
 
 bool fits(uint32_t sequences, uint32_t queries, uint32_t heads, uint32_t kv_heads, uint32_t prefixes) {

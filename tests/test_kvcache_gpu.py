@@ -321,7 +321,7 @@ def test_ragged(cuda, kind, n):
 @pytest.mark.parametrize("groups, batch, n, prefix, own", [
     (1, 5, 1, 300, 70), (1, 130, 1, 257, 9), (2, 6, 3, 1000, 64), (3, 3, 2, 100, 100), (1, 4, 200, 130, 65),
     (2, 4, 128, 64, 64), (1, 9, 40, 1, 1), (1, 3, 1, 5000, 2), (2, 4, 600, 130, 65), (1, 700, 1, 70, 65),
-    (1, 7, 2, 3000, 64),
+    (1, 7, 2, 3000, 64), (1, 24, 20, 1500, 64), (2, 8, 40, 2500, 130), (1, 40, 2, 900, 300),
 ])
 def test_prefix(cuda, kind, groups, batch, n, prefix, own):
     q, kv, length = case(batch, 4, 2, n, own, kind, prefix, capacity=own + 5)
