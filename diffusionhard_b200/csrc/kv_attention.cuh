@@ -138,7 +138,8 @@ DH_DEVINL uint32_t length_of(const Segment& s, uint32_t entry) {
 
 // Sequences by falling length (the lower index first among equals) into order[],
 // by the CTA's first kOrdered threads; all threads call it.  Items of long sequences
-// that start last would run alone.
+// that start last would run alone (16 single tokens over up to 32768 keys 111 us as they
+// come, 101 in this order).  kOrdered: what shared memory is set aside for.
 constexpr uint32_t kOrdered = 128;
 DH_DEVINL void order_sequences(const Args& a, uint32_t* lengths, uint16_t* order) {
     const uint32_t n = a.sequences, t = threadIdx.x;
