@@ -237,14 +237,20 @@ DH_DEVINL void add(float4& s, float f, const float4& v) {
     s = make_float4(__fmaf_rn(f, v.x, s.x), __fmaf_rn(f, v.y, s.y), __fmaf_rn(f, v.z, s.z), __fmaf_rn(f, v.w, s.w));
 }
 
-// A weight's exponent s c - m, one FMA, is off by the rounding of m, half a step of fp32.
-// From |m| = 2^23 on that is 2^-1 and more, and at 2^28 weights would leave f16 at either
-// end.  So s c and m are taken by this power of two there, which keeps the latter below
-// 2^23: scores count to 2^-23 of their size.  1 for all others.
+// A weight's exponent is one FMA, s c - m, with m the maximum rounded to fp32.  That
+// rounding is the same for all weights of a row and their sum: it cancels, and only the
+// range of the weights sees it.  From kFar on a maximum is taken as it is, without room
+// above or below it, so that the largest weight lies within 2^-8 .. 2^8 up to |m| = 2^28.
+constexpr float kFar = 4194304.f;  // 2^22
+// From there on differences to m are taken by this power of two, which keeps it below
+// 2^28 (1 for all others): what is 33 2^-27 of m below it, 2^-21 and less, is still 2^-33
+// of it.  Maxima are compared by the same measure wherever sums meet.
 DH_DEVINL float damping(float top) {
-    constexpr uint32_t kFrom = (127u + 22u) << 23;
+    constexpr uint32_t kFrom = (127u + 27u) << 23;
     return __uint_as_float(0x3F800000u + kFrom - max(__float_as_uint(top) & 0x7F800000u, kFrom));
 }
+// Sums relative to 2^m as ones relative to 2^top: their factor.
+DH_DEVINL float growth(float m, float top) { return ex2_approx((m - top) * damping(top)); }
 constexpr float kNoMax = -3.0e38f;  // below every maximum, and finite
 
 // Four values (part 0..15) of row r of an item from its sums: relative to 2^top, the
@@ -287,7 +293,7 @@ DH_DEVINL void join_cluster(const Args& a, const Item& it, uint32_t sums_at, uin
 #pragma unroll
         for (uint32_t p = 0; p < kMaxCluster; ++p) {
             if (p >= cluster) break;
-            const float f = ex2_approx(x[p].x - top);
+            const float f = growth(x[p].x, top);
             total = __fmaf_rn(f, x[p].y, total);
             add(sum, f, load_remote4(map_to(sums_at + (r * kSumPitch + 4 * part) * 4, p)));
         }

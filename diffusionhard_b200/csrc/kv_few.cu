@@ -381,7 +381,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
         // weights, in place
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            float next[2], alpha[2], top2[2];
+            float next[2], alpha[2];
 #pragma unroll
             for (uint32_t e = 0; e < 2; ++e) {
                 float top = max_nan(max_nan(s[t][0][e], s[t][0][e + 2], s[t][1][e]), s[t][1][e + 2]);
@@ -392,15 +392,15 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
                 top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
                 top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
                 // finite, or NaN for a score that is infinite or NaN: the row is NaN
-                top2[e] = top * cr[t][e];
-                next[e] = max_nan(max_nan(top2[e] - kHeadroom, kNoMax), m[t][e]);
+                const float top2 = top * cr[t][e];
+                next[e] = max_nan(max_nan(top2 - (fabsf(top2) < kFar ? kHeadroom : 0.f), kNoMax), m[t][e]);
                 next[e] = __fmaf_rn(next[e], -0.f, next[e]);
-                alpha[e] = ex2_approx(m[t][e] - next[e]);
+                alpha[e] = growth(m[t][e], next[e]);
                 m[t][e] = next[e];
                 l[t][e] *= alpha[e];
                 alpha[e] *= fe;
             }
-            const float damp[2] = {damping(top2[0]), damping(top2[1])};
+            const float damp[2] = {damping(next[0]), damping(next[1])};
             const float2 cr2 = make_float2(fmaxf(cr[t][0] * damp[0], kLeastFactor), fmaxf(cr[t][1] * damp[1], kLeastFactor));
             const float2 nm2 = make_float2(-next[0] * damp[0], -next[1] * damp[1]);
             float2 sum = make_float2(l[t][0], l[t][1]);
@@ -588,7 +588,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
         }
 #pragma unroll
         for (uint32_t p = 0; p < kWarps; ++p) {
-            const float f = ex2_approx(x[p].x - top);
+            const float f = growth(x[p].x, top);
             total = __fmaf_rn(f, x[p].y, total);
             add(sum, f, *reinterpret_cast<const float4*>(sums + (p * kRowsMax + r) * kSumPitch + 4 * part));
         }

@@ -282,8 +282,8 @@ def attend(q: torch.Tensor, kv: Any, lengths: Lengths = None, *, prefix: Any = N
 
     Scores and sums are fp32; the weights enter the product with V rounded to 16
     bits (f16; bf16 for V in bf16).  Int8 rows are rounded to f16 where a K/V head
-    has more than 16 query rows; for f16 queries they are held as two f16.  A score
-    counts to 2^-23 of its size.
+    has more than 16 query rows; for f16 queries they are held as two f16.  Scores
+    beyond 1.8e8 (2^28 log 2) count to 2^-21 of their size.
 
     Calls that split the keys take 264 bytes of workspace for each query, head and
     part (at most 64 of the prefix and 64 of the rest); calls whose queries visit

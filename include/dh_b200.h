@@ -794,8 +794,8 @@ typedef struct dh_kv_view {
  *               f16: 256 bytes (f16 queries: 512) a position and K/V head
  * Scores and sums are fp32; weights are rounded to 16 bits (f16; bf16 for V in
  * bf16) before the product with V; int8 rows times their scales are rounded to f16
- * (f16 queries: held as two f16) where a K/V head has more than 16 rows.  A score
- * counts to 2^-23 of its size.  V up to 2^90 in magnitude.
+ * (f16 queries: held as two f16) where a K/V head has more than 16 rows.  Scores
+ * beyond 1.8e8 (2^28 log 2) count to 2^-21 of their size.  V up to 2^90 in magnitude.
  * Results do not depend on timing: the same call gives the same bits.
  * Status: DH_ERR_*. */
 size_t dh_kv_attention_workspace_size(uint32_t sequences, uint32_t queries, uint32_t heads, uint32_t kv_heads,

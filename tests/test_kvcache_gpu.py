@@ -393,6 +393,90 @@ def test_scores_beyond_the_steps_of_fp32(cuda, kind, n):
     _lib.check_device_error()
 
 
+def far_keys(kind, keys, power, sign, leads):
+    """Keys whose score is sign 2^power for the best (in the middle) and `lead` fp32 steps
+    less for six others, in its tile and in tiles before and behind it; all others lie far
+    below.  V of each of them has a column of its own.  (q, kv, places, scores)"""
+    dtype = F16 if kind == "f16" else BF16
+    best = keys // 2
+    places = [best, best - 1, best + 2, keys - 1, 0, best + 75, best - 75][:1 + len(leads)]
+    half = power // 2
+    k = torch.zeros(1, 1, keys, DIM, dtype=torch.float64)
+    k[..., 0] = 0 if sign > 0 else -1.5 * 2.0 ** (power - half)
+    v = torch.zeros(1, 1, keys, DIM, dtype=torch.float64)
+    for i, p in enumerate(places):
+        k[0, 0, p, 0], k[0, 0, p, 1] = sign * 2.0 ** (power - half), -([0] + leads)[i] * 2.0 ** (power - 23)
+        v[0, 0, p, i] = 1024
+    q = torch.zeros(1, 1, 1, DIM, dtype=torch.float64)
+    q[..., 0], q[..., 1] = 2.0 ** half, 1
+    s = (q @ k.transpose(2, 3))[0, 0, 0]
+    assert torch.equal(s.float().double(), s) and all(torch.equal(t.to(dtype).double(), t) for t in (q, k, v))
+    q, k, v = (t.to(dtype).cuda() for t in (q, k, v))
+    if kind == "turned":
+        wide = torch.zeros(1, 1, DIM, (keys + 7) // 8 * 8, dtype=F16, device="cuda")
+        wide[..., :keys] = v.transpose(2, 3)
+        v = wide.transpose(2, 3)[:, :, :keys]
+    return q, (k, v), places, s
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "turned"])
+@pytest.mark.parametrize("n", [1, 12, 40, 520])
+@pytest.mark.parametrize("keys", [300, 4000])
+def test_far_scores_in_steps(cuda, kind, n, keys):
+    """Keys a few steps of fp32 below the best one, at scores where a step is half a unit
+    and more: their weights are those of the difference, in whichever tile or part."""
+    p_round = 2.0 ** -8 if kind == "bf16" else 2.0 ** -11
+    scale = math.log(2.0)
+    leads = [1, 2, 4, 8, 16, 64]
+    for power, sign in ((22, 1), (23, -1), (24, 1), (24, -1), (26, 1), (27, -1)):
+        q, kv, places, s = far_keys(kind, keys, power, sign, leads)
+        out, lse = attend(q.expand(1, 1, n, DIM), kv, scale=scale, return_lse=True)
+        got = out[0, :, 0].double().cpu() / 1024
+        want = torch.zeros(DIM, dtype=torch.float64)
+        # (scale is a float, and its product with log2(e) another: 2^-23 of a difference)
+        weights = torch.exp2(s - s.max())
+        want[:len(places)] = (weights / weights.sum())[places]
+        gap = torch.zeros(DIM, dtype=torch.float64)
+        gap[:len(places)] = (s.max() - s)[places]
+        # roundings: a weight, the sum of weights and the output to 16 bits, 2^x by a cubic
+        # (8e-5 of a weight and of the sum), the difference in fp32; the largest weight is
+        # 2^-8 at least, so the smallest step is 2^-17 of it (f16)
+        limit = want * (2 * p_round + torch.finfo(q.dtype).eps / 2 + 2e-4 + gap.clamp(max=200) * 2.0 ** -22)
+        limit += 0 if kind == "bf16" else 2.0 ** -17
+        limit += 1e-30 if q.dtype is BF16 else 2.0 ** -35
+        assert ((got - want).abs() <= limit).all(), (power, sign, float(((got - want).abs() / limit).max()))
+        want_lse = float(torch.logsumexp(s * scale, 0))
+        assert ((lse.double().cpu() - want_lse).abs() <= 2.0 ** -22 * abs(want_lse)).all()
+    # from 2^28 on a score counts to 2^-21 of its size: what lies further below has no weight
+    for power, sign in ((28, 1), (30, -1), (30, 1)):
+        q, kv, places, s = far_keys(kind, keys, power, sign, [8, 16, 64])
+        got = attend(q.expand(1, 1, n, DIM), kv, scale=scale)[0, :, 0].double().cpu() / 1024
+        assert ((got[:, 0] - 1).abs() <= 2 * p_round).all() and (got[:, 1:] <= 2.0 ** -17).all(), (power, sign)
+    _lib.check_device_error()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("n", [1, 12])
+def test_far_scores_over_int8(cuda, dtype, n):
+    """The same over int8 keys with few rows, whose scores are fp32: a score of 127 2^17 is
+    off by half a step, half a unit, in the best key and in another."""
+    c = KVCacheI8.empty(1, 1, 320)
+    for t in c:
+        t.zero_()
+    c.k[0, 0, [150, 151, 20], 0] = 127
+    c.k_scale[0, 0, [150, 151, 20]] = torch.tensor([2.0 ** 5, 2.0 ** 5 * (1 - 2.0 ** -21), 2.0 ** 5 * (1 - 2.0 ** -20)],
+                                                   device="cuda")
+    for i, p in enumerate((150, 151, 20)):
+        c.v[0, 0, p, i], c.v_scale[0, 0, p] = 127, 1
+    q = torch.zeros(1, 1, n, DIM, dtype=dtype, device="cuda")
+    q[..., 0] = 2.0 ** 12
+    got = attend(q, c, 320, scale=math.log(2.0))[0, :, 0].double().cpu() / 127
+    # differences of 127 2^-4 and 127 2^-3; the second weight is 2^-16, small for f16
+    assert ((torch.log2(got[:, 1] / got[:, 0]) + 127 / 16).abs() <= 1 + 2.0 ** -6).all()
+    assert ((got[:, 0] - 1).abs() < 2.0 ** -6).all() and (got[:, 2] <= 2.0 ** -14).all()
+    _lib.check_device_error()
+
+
 @pytest.mark.parametrize("kind", ["int8", "f16"])
 @pytest.mark.parametrize("batch, n, keys", [(1200, 1, 2048), (592, 20, 20000), (74, 1000, 20000)])
 def test_many_light_keys(cuda, kind, batch, n, keys):
