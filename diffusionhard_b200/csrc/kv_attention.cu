@@ -274,7 +274,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_consta
                             break;
                         }
                         const Segment& s = own ? a.own : a.prefix;
-                        const uint64_t at = (static_cast<uint64_t>(entry) * a.kv_heads.d + it.kv_head) * s.capacity + key;
+                        const uint64_t at = (static_cast<uint64_t>(entry) * a.kv_heads.d + it.kv_head) * s.pitch + key;
                         uint8_t* dst = raw_ring + rs * kRawBytes;
                         uint64_t* bar = &bars[kRawFull + rs];
                         tc::mbar_arrive_expect_tx(bar, kRawBytes);
@@ -1012,7 +1012,10 @@ uint32_t check_view(const dh_kv_view& v) {
         return DH_ERR_INVALID_ARGUMENT;
     if (v.k_type == DH_TYPE_I8 && v.v_type == DH_TYPE_I8) {
         if (!v.k_scale || !v.v_scale) return DH_ERR_NULL_POINTER;
-        if (v.capacity % kKT) return DH_ERR_UNSUPPORTED_SHAPE;
+        const uint64_t pitch = v.k_strides[1];
+        if (v.capacity % kKT || pitch != v.v_strides[1] || pitch % (kKT * kDh) || pitch >> 37 ||
+            (pitch && pitch < static_cast<uint64_t>(v.capacity) * kDh))
+            return DH_ERR_UNSUPPORTED_SHAPE;
         if (misaligned(v.k, 16) || misaligned(v.v, 16) || misaligned(v.k_scale, 16) || misaligned(v.v_scale, 16) ||
             misaligned(v.lengths, 4))
             return DH_ERR_ALIGNMENT;
@@ -1144,7 +1147,8 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
     a.cls[0] = p.cls[0], a.cls[1] = p.cls[1];
     const auto segment = [](const dh_kv_view& v) {
         return Segment{static_cast<const int8_t*>(v.k), static_cast<const int8_t*>(v.v), v.k_scale, v.v_scale,
-                       v.lengths, v.length, v.capacity};
+                       v.lengths, v.length, v.capacity,
+                       v.k_type == DH_TYPE_I8 && v.k_strides[1] ? static_cast<uint32_t>(v.k_strides[1] / kDh) : v.capacity};
     };
     a.own = segment(*own);
     if (prefixes) a.prefix = segment(*prefix);

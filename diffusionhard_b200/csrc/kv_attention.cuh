@@ -36,6 +36,7 @@ struct Segment {
     const float* v_scale;
     const int32_t* lengths;
     uint32_t length, capacity;
+    uint32_t pitch;                      // int8: positions from one head's rows to the next's
 };
 
 struct Args {

@@ -187,7 +187,7 @@ kv_few_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ C
         if constexpr (kI8) {
             if (lane < 4) {
                 const Segment& s = own ? a.own : a.prefix;
-                const uint64_t at = (static_cast<uint64_t>(entry) * a.kv_heads.d + ahead.kv_head) * s.capacity + key;
+                const uint64_t at = (static_cast<uint64_t>(entry) * a.kv_heads.d + ahead.kv_head) * s.pitch + key;
                 const bool is_v = lane & 1u, is_scale = lane & 2u;
                 const void* codes = (is_v ? s.v : s.k) + at * kDh;
                 const void* scales = (is_v ? s.v_scale : s.k_scale) + at;

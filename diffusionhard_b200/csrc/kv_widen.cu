@@ -69,14 +69,14 @@ __global__ void __launch_bounds__(kThreads) kv_widen_kernel(const __grid_constan
     const Segment& s = own ? a.own : a.prefix;
     const WideKeys& to = own ? a.out_own : a.out_prefix;
     const uint32_t len = length_of(s, entry);
-    const uint64_t at = static_cast<uint64_t>(line) * s.capacity;
+    const uint64_t at = static_cast<uint64_t>(line) * s.pitch, to_at = static_cast<uint64_t>(line) * s.capacity;
     const int32_t ek = exponent_in_range(largest(s.k_scale + at, len, smem));
     int32_t ev = exponent_in_range(largest(s.v_scale + at, len, smem));
     if (own && a.with_prefix) {
         const uint32_t p = a.per_prefix.of(entry);
         const uint64_t line0 = static_cast<uint64_t>(p) * a.kv_heads.d + head;
         ev = max(ev, exponent_in_range(
-                         largest(a.prefix.v_scale + line0 * a.prefix.capacity, length_of(a.prefix, p), smem)));
+                         largest(a.prefix.v_scale + line0 * a.prefix.pitch, length_of(a.prefix, p), smem)));
     }
     if (chunk == 0 && threadIdx.x == 0)
         to.exps[line] = make_float2(pow2(min(ek + 9, 128)), __int_as_float(ev + 9));
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(kThreads) kv_widen_kernel(const __grid_constan
                 const float by = scale[i][side] * (side ? fv : fk);
                 const uint2 w = codes[i][side];
                 uint4 x;
-                __half* dst = (side ? to.v : to.k) + (at + key) * kDh;
+                __half* dst = (side ? to.v : to.k) + (to_at + key) * kDh;
                 if constexpr (FINE) {
                     const FineFactor f = fine_factor(by);
                     convert4(w.x, f.lo, f.off_lo, x.x, x.y);

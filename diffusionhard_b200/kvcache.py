@@ -33,6 +33,12 @@ from .scoring import _TYPES, _current_device, _ptr, _raw_stream
 HEAD_DIM = 64
 CAPACITY_STEP = 64
 _TYPE_I8 = 3
+# Work and workspace go by the capacity of a view.  Of caches with more positions than
+# this, a call whose length the host knows shows only as many keys as that (8 x 512
+# queries, 12 heads, over 500 of 32768 int8 keys: 49.2 us and 19 MB, whole 54.8 and 851;
+# one over 33 of 2048 4.4 and 7.0 us).  In smaller ones lengths on the host and on the
+# device give the same bits.
+_WHOLE_KEYS = 512
 
 Lengths = Union[int, torch.Tensor, None]
 
@@ -202,7 +208,7 @@ class _Keys(NamedTuple):
     view: bytes          # dh_kv_view
     entries: int
     heads: int
-    capacity: int
+    capacity: int        # as in the view
     v_type: int          # with `turned`: what a prefix must have alike
     turned: bool         # V's columns are contiguous
     held: Any            # a tensor the view points into
@@ -214,7 +220,7 @@ def _view(name: str, kv: Any, lengths: Lengths, q: torch.Tensor, index: int) -> 
         k, k_scale, v, v_scale = kv
         entries, heads, capacity, _ = _check_cache(name, kv, index)
         kt = vt = _TYPE_I8
-        ks = vs = (0, 0, 0, 0)
+        ks = vs = (0, capacity * HEAD_DIM, 0, 0)
         pointers = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
     else:
         k, v = kv
@@ -250,6 +256,9 @@ def _view(name: str, kv: Any, lengths: Lengths, q: torch.Tensor, index: int) -> 
         length = operator.index(lengths)
         if not 0 <= length <= capacity:
             raise ValueError(f"{length} keys of {name} do not lie within its capacity of {capacity}")
+        if capacity > _WHOLE_KEYS:
+            step = CAPACITY_STEP if kt == _TYPE_I8 else 1
+            capacity = max(-(-length // step), 1) * step
     view = _pack_view(*pointers, 0 if held is None else held.data_ptr(), *ks, *vs, kt, vt, capacity, length)
     return _Keys(view, entries, heads, capacity, vt, turned, held)
 
@@ -288,7 +297,8 @@ def attend(q: torch.Tensor, kv: Any, lengths: Lengths = None, *, prefix: Any = N
     Calls that split the keys take 264 bytes of workspace for each query, head and
     part (at most 64 of the prefix and 64 of the rest); calls whose queries visit
     int8 keys many times hold those as f16, 256 bytes (f16 queries: 512) for each
-    position and K/V head."""
+    position and K/V head.  Parts and positions are those of the capacity or, for
+    caches of more than 512 positions, of `lengths` as an int."""
     index = q.get_device()
     q_type = _TYPES.get(q.dtype)
     if index < 0:
@@ -333,8 +343,8 @@ def attend(q: torch.Tensor, kv: Any, lengths: Lengths = None, *, prefix: Any = N
     lse = q.new_empty((batch, n, heads), dtype=torch.float32) if return_lse else None
     run = _run_rows(run_rows, index)
     if batch and n and heads:
-        size = _workspace_bytes(batch, n, heads, kv_heads, prefixes, prefix_capacity, keys.capacity,
-                                keys.v_type == _TYPE_I8, q_type, index)
+        size = _workspace_bytes(batch, n, heads, kv_heads, prefixes, -(-prefix_capacity // CAPACITY_STEP),
+                                -(-keys.capacity // CAPACITY_STEP), keys.v_type == _TYPE_I8, q_type, index)
         # (goes back to the allocator's pool of the current stream, which the
         # kernels that use it are on)
         ws = q.new_empty((size,), dtype=torch.uint8) if size else None
@@ -344,8 +354,10 @@ def attend(q: torch.Tensor, kv: Any, lengths: Lengths = None, *, prefix: Any = N
 
 
 @functools.lru_cache(maxsize=256)
-def _workspace_bytes(batch: int, n: int, heads: int, kv_heads: int, prefixes: int, prefix_capacity: int,
-                     capacity: int, int8: bool, q_type: int, index: int) -> int:
+def _workspace_bytes(batch: int, n: int, heads: int, kv_heads: int, prefixes: int, prefix_tiles: int,
+                     tiles: int, int8: bool, q_type: int, index: int) -> int:
+    # (the same for all capacities of a number of tiles)
     with torch.cuda.device(index):
-        return int(_lib.lib().dh_kv_attention_workspace_size(batch, n, heads, kv_heads, prefixes, prefix_capacity,
-                                                             capacity, _TYPE_I8 if int8 else q_type, q_type))
+        return int(_lib.lib().dh_kv_attention_workspace_size(
+            batch, n, heads, kv_heads, prefixes, prefix_tiles * CAPACITY_STEP, tiles * CAPACITY_STEP,
+            _TYPE_I8 if int8 else q_type, q_type))

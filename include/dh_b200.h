@@ -751,14 +751,17 @@ uint32_t dh_kv_read_i8(const int8_t* k_codes, const float* k_scale, const int8_t
 
 /* Keys and values of dh_kv_attention: entries x kv_heads x capacity rows of 64.
  *   DH_TYPE_I8 (k and v): a cache of dh_kv_write_i8, contiguous, 16-byte aligned,
- *               capacity a multiple of 64
+ *               capacity a multiple of 64; or the first `capacity` positions of every
+ *               head of a larger one, 64 times whose capacity is then both k_strides[1]
+ *               and v_strides[1] (0: 64 times `capacity`; the others are not used)
  *   16 bits     k of the queries' type, v DH_TYPE_BF16 or _F16, strides (entry,
  *               head, row, element) in elements; k's rows contiguous, v's rows or
  *               v's columns (a transposed V); starts and all other strides at
  *               multiples of 16 bytes
  * length: the keys of every entry (the first ones of its capacity), or lengths:
  * device [entries], clamped to [0, capacity].  What lies behind them is not used,
- * whatever it holds. */
+ * whatever it holds.  Work is laid out, and workspace taken, for `capacity` keys: who
+ * knows a smaller number gives that as the capacity. */
 typedef struct dh_kv_view {
     const void* k;
     const void* v;

@@ -131,3 +131,15 @@ def test_functions_refuse_host_tensors():
     for bad in ((0, 1, 1), (1, 0, 1), (1, 1, 0), (1, 1, -64)):
         with pytest.raises(ValueError, match="positive"):
             kvcache.KVCacheI8.empty(*bad, device="cpu")
+
+
+@pytest.mark.parametrize("strides", [(4096, 8192), (0, 4096), (4032, 4032), (2048, 2048), (1 << 37, 1 << 37),
+                                     (4097, 4097)])
+def test_int8_pitch_refused(strides):
+    """Heads of int8 keys that lie closer than their capacity, not in whole tiles, or
+    differently for K and V."""
+    k, v = (U64x4(0, s, 0, 0) for s in strides)
+    bad = dict(I8, k_strides=k, v_strides=v)
+    assert _attend(_view(**bad)) == SHAPE
+    good = dict(I8, k_strides=U64x4(0, 8192, 0, 0), v_strides=U64x4(0, 8192, 0, 0))
+    assert _attend(_view(**good), prefix=_view(**bad)) == SHAPE

@@ -616,6 +616,38 @@ def test_split_and_whole_agree(cuda):
     check(q, kv)
 
 
+@pytest.mark.parametrize("kind", ["int8", "bf16", "turned"])
+@pytest.mark.parametrize("n", [1, 32, 300])
+def test_length_known_to_the_host(cuda, kind, n):
+    """Keys that are a small part of a cache cost what they cost in a small one: the same
+    bits, so the same parts, and no more memory."""
+    torch = cuda
+
+    def peak(call):
+        out = call()
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        again = call()
+        torch.cuda.synchronize()
+        used = torch.cuda.max_memory_allocated() - before
+        assert torch.equal(out, again)
+        return out, used
+
+    for length, prefix_length in ((600, None), (150, None), (1, None), (64, 600), (0, 128), (700, 0), (0, 0)):
+        q, small, _ = case(4, 4, 2, n, max(length, 1), kind, n)
+        _, large, _ = case(4, 4, 2, n, max(length, 1), kind, n, capacity=8000)
+        kws = [{}, {}]
+        if prefix_length is not None:
+            kws = [dict(prefix=case(2, 4, 2, 1, max(prefix_length, 1), kind, n + 5, capacity=cap)[1],
+                        prefix_lengths=prefix_length) for cap in (None, 9000)]
+        a, used = peak(lambda: attend(q, small, length, **kws[0]))
+        b, most = peak(lambda: attend(q, large, length, **kws[1]))
+        assert torch.equal(a, b) and most <= used
+        check(q, large, length, kws[1].get("prefix"), kws[1].get("prefix_lengths"))
+    _lib.check_device_error()
+
+
 def test_same_bits(cuda):
     """The same call gives the same bits, alone or beside others on two streams."""
     for kind in ("int8", "bf16"):
