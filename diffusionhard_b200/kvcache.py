@@ -308,7 +308,7 @@ def attend(q: torch.Tensor, kv: Any, lengths: Lengths = None, *, prefix: Any = N
     batch, heads, n, _ = q.shape
     qs = _strides(q)
     if qs[3] != 1 or (qs[0] | qs[1] | qs[2]) % 8 or q.data_ptr() & 15:
-        q = q.contiguous()
+        q = q.clone(memory_format=torch.contiguous_format)
         qs = _strides(q)
     keys = _view("kv", kv, lengths, q, index)
     kv_heads = keys.heads

@@ -589,6 +589,18 @@ def test_layouts(cuda, kind):
 
 
 @pytest.mark.parametrize("kind", ["int8", "bf16"])
+@pytest.mark.parametrize("at", [1, 4])
+def test_queries_that_start_anywhere(cuda, kind, at):
+    """Contiguous queries whose first element lies at no 16-byte boundary."""
+    q, kv, length = case(2, 2, 2, 6, 100, kind, 13)
+    flat = torch.zeros(q.numel() + 8, dtype=BF16, device="cuda")
+    flat[at:at + q.numel()] = q.reshape(-1)
+    moved = flat[at:at + q.numel()].view(q.shape)
+    assert moved.is_contiguous() and moved.data_ptr() % 16
+    assert torch.equal(attend(moved, kv, length), attend(q, kv, length))
+
+
+@pytest.mark.parametrize("kind", ["int8", "bf16"])
 @pytest.mark.parametrize("n", [1, 130, 520])
 def test_run_rows(cuda, kind, n):
     q, kv, length = case(4, 2, 2, n, 333, kind, 14)
