@@ -1111,6 +1111,18 @@ extern "C" size_t dh_kv_attention_workspace_size(uint32_t sequences, uint32_t qu
         .bytes;
 }
 
+extern "C" uint32_t dh_kv_attention_launches(uint32_t sequences, uint32_t queries, uint32_t heads, uint32_t kv_heads,
+                                             uint32_t prefixes, uint32_t prefix_capacity, uint32_t own_capacity,
+                                             uint32_t k_type) {
+    if (!sequences || !queries || !heads || !kv_heads || heads % kv_heads || (prefixes && sequences % prefixes) ||
+        !fits(sequences, queries, heads, kv_heads, prefixes))
+        return 0;
+    const Plan p = plan_of(sequences, queries * (heads / kv_heads), kv_heads, prefixes, prefix_capacity, own_capacity,
+                           k_type == DH_TYPE_I8, false, device_sms());
+    const bool many = (p.cls[0].items && !p.few[0]) || !p.few[1];
+    return p.widen + many + p.few[0] + p.few[1] + (p.slots > 1);
+}
+
 extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64_t* q_strides, uint32_t sequences,
                                     uint32_t queries, uint32_t heads, uint32_t kv_heads, const dh_kv_view* own,
                                     const dh_kv_view* prefix, uint32_t prefixes, float scale, void* out, float* lse,

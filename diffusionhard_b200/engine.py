@@ -176,8 +176,7 @@ class MDLMEngine:
         self._graphs: Dict[Any, Any] = {}
         self._events = (torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True))
         self._whole_forward = False  # self.x is a forward of the whole canvas, and no generation came after it
-        # (kvcache.attend counts as one)
-        self.launches_per_forward = 1 + (9 if int8_kv is None else 10) * len(self.blocks)
+        self.launches_per_forward = 1 + (8 + self._attend_launches()) * len(self.blocks)
 
     def shard_head(self, v0: int, v1: int, group: Any = None, reduce: Any = None) -> None:
         """Keep only head rows [v0, v1) (vocab-sharded head).  After every head
@@ -232,6 +231,20 @@ class MDLMEngine:
             if hook is not None:
                 hook(i)
         self._whole_forward = run_rows is None and seq_list is None
+
+    def _attend_launches(self) -> int:
+        """Kernels of a block's attention, the write of its K / V into an int8 cache included."""
+        int8, prefix = self.int8_kv, self.prefix_kv
+        if int8 is None and prefix is None:
+            return 1
+        from .kvcache import attend_launches
+
+        held = {} if prefix is None else {"prefixes": prefix[0][0].shape[0], "prefix_capacity": prefix[0][0].shape[2],
+                                          "prefix_length": self.prefix_len}
+        capacity = self.kv_stride if int8 is None else int8[0].capacity
+        heads = self.q.shape[1]
+        return (int8 is not None) + attend_launches(self.B, self.L, heads, heads, capacity, self.kv_len,
+                                                    int8=int8 is not None, device=self.device, **held)
 
     def _attend(self, i: int, k: Any, vt: Any, rr: Any, s: Any, run_rows: Any) -> None:
         if self.int8_kv is None and self.prefix_kv is None:

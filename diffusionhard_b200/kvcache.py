@@ -214,6 +214,14 @@ class _Keys(NamedTuple):
     held: Any            # a tensor the view points into
 
 
+def _shown(capacity: int, length: int, int8: bool) -> int:
+    """The capacity that a call shows of a cache with `length` keys."""
+    if capacity <= _WHOLE_KEYS:
+        return capacity
+    step = CAPACITY_STEP if int8 else 1
+    return max(-(-length // step), 1) * step
+
+
 def _view(name: str, kv: Any, lengths: Lengths, q: torch.Tensor, index: int) -> _Keys:
     turned = False
     if isinstance(kv, KVCacheI8):
@@ -256,9 +264,7 @@ def _view(name: str, kv: Any, lengths: Lengths, q: torch.Tensor, index: int) -> 
         length = operator.index(lengths)
         if not 0 <= length <= capacity:
             raise ValueError(f"{length} keys of {name} do not lie within its capacity of {capacity}")
-        if capacity > _WHOLE_KEYS:
-            step = CAPACITY_STEP if kt == _TYPE_I8 else 1
-            capacity = max(-(-length // step), 1) * step
+        capacity = _shown(capacity, length, kt == _TYPE_I8)
     view = _pack_view(*pointers, 0 if held is None else held.data_ptr(), *ks, *vs, kt, vt, capacity, length)
     return _Keys(view, entries, heads, capacity, vt, turned, held)
 
@@ -351,6 +357,16 @@ def attend(q: torch.Tensor, kv: Any, lengths: Lengths = None, *, prefix: Any = N
         _call_on("dh_kv_attention", index, q.data_ptr(), q_type, _pack4(*qs), batch, n, heads, kv_heads, keys.view,
                  prefix_view, prefixes, scale, out.data_ptr(), _ptr(lse), run, _ptr(ws), size)
     return (out, lse) if return_lse else out
+
+
+def attend_launches(batch: int, n: int, heads: int, kv_heads: int, capacity: int, length: int, *, int8: bool,
+                    prefixes: int = 0, prefix_capacity: int = 0, prefix_length: int = 0, device: Any = "cuda") -> int:
+    """Kernels that :func:`attend` launches for queries [batch, heads, n, 64] over
+    `length` keys (an int) of a cache, behind `prefix_length` keys of `prefixes` others."""
+    with torch.cuda.device(device):
+        return int(_lib.lib().dh_kv_attention_launches(
+            batch, n, heads, kv_heads, prefixes, _shown(prefix_capacity, prefix_length, int8) if prefixes else 0,
+            _shown(capacity, length, int8), _TYPE_I8 if int8 else _TYPES[torch.bfloat16]))
 
 
 @functools.lru_cache(maxsize=256)

@@ -804,6 +804,9 @@ typedef struct dh_kv_view {
 size_t dh_kv_attention_workspace_size(uint32_t sequences, uint32_t queries, uint32_t heads, uint32_t kv_heads,
                                       uint32_t prefixes, uint32_t prefix_capacity, uint32_t own_capacity,
                                       uint32_t k_type, uint32_t q_type);
+/* The kernels that such a call launches: one to three (0: a shape that is refused). */
+uint32_t dh_kv_attention_launches(uint32_t sequences, uint32_t queries, uint32_t heads, uint32_t kv_heads,
+                                  uint32_t prefixes, uint32_t prefix_capacity, uint32_t own_capacity, uint32_t k_type);
 uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64_t* q_strides, uint32_t sequences,
                          uint32_t queries, uint32_t heads, uint32_t kv_heads, const dh_kv_view* own,
                          const dh_kv_view* prefix, uint32_t prefixes, float scale, void* out, float* lse,

@@ -143,3 +143,11 @@ def test_int8_pitch_refused(strides):
     assert _attend(_view(**bad)) == SHAPE
     good = dict(I8, k_strides=U64x4(0, 8192, 0, 0), v_strides=U64x4(0, 8192, 0, 0))
     assert _attend(_view(**good), prefix=_view(**bad)) == SHAPE
+
+
+def test_launches():
+    f = _lib.lib().dh_kv_attention_launches
+    assert f(0, 1, 4, 4, 0, 0, 64, 1) == 0 and f(1, 1, 4, 3, 0, 0, 64, 1) == 0 and f(3, 1, 4, 4, 2, 64, 64, 1) == 0
+    assert f(1, 1, 12, 12, 0, 0, 64, 3) == 1  # one kernel, no parts
+    assert f(32, 1024, 12, 12, 0, 0, 1024, 3) == 2  # keys turned into f16 first
+    assert 2 <= f(128, 1, 12, 12, 1, 8192, 320, 1) <= 3

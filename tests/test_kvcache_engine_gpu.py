@@ -130,3 +130,38 @@ def test_refusals(cuda, model):
         MDLMEngine(model, 1, 64, int8_kv=[])
     with pytest.raises(ValueError, match="prefix_kv"):
         MDLMEngine(model, 1, 64, prefix_kv=gen.kv)
+
+
+def _captured_kernels(torch, enqueue):
+    from cuda.bindings import runtime as rt
+
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(g):
+        enqueue()
+    graph = rt.cudaGraph_t(init_value=g.raw_cuda_graph())
+    err, _, count = rt.cudaGraphGetNodes(graph, 0)
+    assert err == rt.cudaError_t.cudaSuccess
+    err, nodes, count = rt.cudaGraphGetNodes(graph, count)
+    assert err == rt.cudaError_t.cudaSuccess
+    kinds = [rt.cudaGraphNodeGetType(node)[1] for node in nodes[:count]]
+    return sum(kind == rt.cudaGraphNodeType.cudaGraphNodeTypeKernel for kind in kinds)
+
+
+@pytest.mark.parametrize("make", [
+    lambda m: BlockCausalSession(m, 8, 1024, int8_kv=True).engine(960, 32),
+    lambda m: BlockCausalSession(m, 1, 1024, int8_kv=True).engine(0, 64),
+    lambda m: BlockCausalSession(m, 32, 1024, int8_kv=True).engine(0, 1024),
+    lambda m: BlockCausalSession(m, 2, 256).engine(128, 32),
+    lambda m: PrefixConditionedGenerator(m, 4, 512, 32, prefixes=1).suffix,
+    lambda m: PrefixConditionedGenerator(m, 4, 512, 512, prefixes=2, int8_kv=True).suffix,
+    lambda m: PrefixConditionedGenerator(m, 4, 512, 512, prefixes=4).suffix,
+    lambda m: PrefixConditionedGenerator(m, 4, 512, 512).suffix,
+])
+def test_launch_count_is_the_captured_kernel_count(cuda, model, make):
+    """launches_per_forward against the kernel nodes of a captured forward."""
+    eng = make(model)
+    eng.tokens.zero_()
+    eng.forward()
+    cuda.cuda.synchronize()
+    assert _captured_kernels(cuda, eng.forward) == eng.launches_per_forward
+    _lib.check_device_error()
