@@ -329,6 +329,32 @@ def test_prefix(cuda, kind, groups, batch, n, prefix, own):
     check(q, kv, length, pre, pre_length)
 
 
+@pytest.mark.parametrize("v_dtype", [BF16, F16])
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("n", [1, 12, 40, 300])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_types_of_v(cuda, dtype, v_dtype, turned, n):
+    """V in either 16-bit type by rows or columns, for queries and keys of either type,
+    alone and behind a prefix, with NaN behind the last key."""
+
+    def keys(entries, length, seed):
+        cap = length + 11
+        k = torch.full((entries, 2, cap, DIM), math.nan, dtype=dtype, device="cuda")
+        k[:, :, :length] = values((entries, 2, length, DIM), seed, dtype)
+        v = torch.full((entries, 2, (cap + 7) // 8 * 8, DIM), math.nan, dtype=v_dtype, device="cuda")
+        v[:, :, :length] = values((entries, 2, length, DIM), seed + 1, v_dtype)
+        if turned:
+            v = v.transpose(2, 3).contiguous().transpose(2, 3)
+        return k, v[:, :, :cap]
+
+    q = values((4, 4, n, DIM), n, dtype)
+    own, prefix = keys(4, 150, 21), keys(2, 333, 31)
+    check(q, own, 150)
+    check(q, own, dev_ints([150, 0, 65, 1]))
+    check(q, own, 150, prefix, 333)
+    check(q, own, dev_ints([150, 0, 65, 1]), prefix, dev_ints([333, 64]))
+
+
 @pytest.mark.parametrize("kind", ["int8", "bf16", "turned"])
 @pytest.mark.parametrize("n", [1, 150, 520])
 def test_prefix_ragged(cuda, kind, n):
