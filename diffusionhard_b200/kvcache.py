@@ -296,9 +296,14 @@ def attend(q: torch.Tensor, kv: Any, lengths: Lengths = None, *, prefix: Any = N
     device word, only the sequences within its first rows of [batch * n] are computed.
 
     Scores and sums are fp32; the weights enter the product with V rounded to 16
-    bits (f16; bf16 for V in bf16).  Int8 rows are rounded to f16 where a K/V head
-    has more than 16 query rows; for f16 queries they are held as two f16.  Scores
-    beyond 1.8e8 (2^28 log 2) count to 2^-21 of their size.
+    bits (f16; bf16 for V in bf16).  Scores beyond 1.8e8 (2^28 log 2) count to 2^-21
+    of their size.  V, and K in 8 bits, may be up to 2^90 in magnitude.
+    Over int8 keys, where a K/V head has at most 16 query rows, a query is held in 15
+    bits: an element is off by up to 1/32512 of its row's largest (all of a row
+    below 2^-100 counts as zero).  With more rows a query is f16 relative to its
+    row's largest value, and K and V are rounded to f16, factor and product, 2^-11 of
+    themselves each (f16 queries: two f16, 2^-15), but not below 2^-19 of the largest
+    value that the keys of the sequence and its prefix hold at this head.
 
     Calls that split the keys take 264 bytes of workspace for each query, head and
     part (at most 64 of the prefix and 64 of the rest); calls whose queries visit

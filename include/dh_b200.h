@@ -796,9 +796,14 @@ typedef struct dh_kv_view {
  *               64 of the rest, and, where many queries visit int8 keys, their rows as
  *               f16: 256 bytes (f16 queries: 512) a position and K/V head
  * Scores and sums are fp32; weights are rounded to 16 bits (f16; bf16 for V in
- * bf16) before the product with V; int8 rows times their scales are rounded to f16
- * (f16 queries: held as two f16) where a K/V head has more than 16 rows.  Scores
- * beyond 1.8e8 (2^28 log 2) count to 2^-21 of their size.  V up to 2^90 in magnitude.
+ * bf16) before the product with V.  Scores beyond 1.8e8 (2^28 log 2) count to 2^-21
+ * of their size.  V, and K in 8 bits, up to 2^90 in magnitude.
+ * Int8 keys, at most 16 rows a K/V head: a query is held in 15 bits, its elements off
+ * by up to 1/32512 of the row's largest (a row below 2^-100 counts as zero).  More
+ * rows: a query is f16 relative to its row's largest value; K and V are rounded to
+ * f16, the scale and the product with a code, 2^-11 of themselves each (f16 queries:
+ * two f16, 2^-15), but not below 2^-19 of the largest value that the keys of the
+ * sequence and its prefix hold at this head.
  * Results do not depend on timing: the same call gives the same bits.
  * Status: DH_ERR_*. */
 size_t dh_kv_attention_workspace_size(uint32_t sequences, uint32_t queries, uint32_t heads, uint32_t kv_heads,
