@@ -1129,8 +1129,10 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
                                     const uint32_t* run_rows, void* workspace, size_t workspace_bytes, void* stream) {
     if (!q || !q_strides || !own || !out || (prefixes && !prefix)) return DH_ERR_NULL_POINTER;
     if ((q_type != DH_TYPE_BF16 && q_type != DH_TYPE_F16) || !sequences || !queries || !heads || !kv_heads ||
-        heads % kv_heads || (prefixes && sequences % prefixes) || !(scale > 0.f) || !std::isfinite(scale))
+        heads % kv_heads || (prefixes && sequences % prefixes))
         return DH_ERR_INVALID_ARGUMENT;
+    const float c = scale * 1.4426950408889634f;  // log2(e)
+    if (!(c >= kLeastFactor && std::isfinite(c))) return DH_ERR_INVALID_ARGUMENT;
     if (!fits(sequences, queries, heads, kv_heads, prefixes)) return DH_ERR_UNSUPPORTED_SHAPE;
     if (uint32_t st = check_view(*own)) return st;
     const bool int8 = own->k_type == DH_TYPE_I8;
@@ -1175,7 +1177,7 @@ extern "C" uint32_t dh_kv_attention(const void* q, uint32_t q_type, const uint64
     const bool v_bf16 = own->v_type == DH_TYPE_BF16;
     a.idesc_o = (v_bf16 ? tc::idesc_bf16_f32<kRows, kPvN>() : tc::idesc_f16_f32<kRows, kPvN>()) |
                 (a.v_transposed ? 0u : tc::kIdescBMnMajor);
-    a.c = std::max(scale * 1.4426950408889634f, kLeastFactor);
+    a.c = c;
     a.out = static_cast<uint8_t*>(out);
     a.lse = lse;
     a.total_rows = rows;

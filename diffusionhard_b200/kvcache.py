@@ -20,7 +20,6 @@ are not, but are kept inside the cache.  Results carry no gradients, and an
 from __future__ import annotations
 
 import functools
-import math
 import operator
 import struct
 from typing import Any, NamedTuple, Optional, Tuple, Union
@@ -290,7 +289,7 @@ def attend(q: torch.Tensor, kv: Any, lengths: Lengths = None, *, prefix: Any = N
     batch: 1 for a prefix of the whole batch), ``prefix_lengths`` as `lengths`
     for them.
 
-    ``scale`` defaults to 1/8.  A query without keys gives 0.  With
+    ``scale`` (2^-126 to 2^127) defaults to 1/8.  A query without keys gives 0.  With
     ``return_lse`` also the log of the sum of exponentials, fp32 [batch, n, heads]
     (-inf without keys), to join results over disjoint keys.  ``run_rows``: one
     device word, only the sequences within its first rows of [batch * n] are computed.
@@ -344,8 +343,8 @@ def attend(q: torch.Tensor, kv: Any, lengths: Lengths = None, *, prefix: Any = N
         raise ValueError("prefix_lengths without a prefix")
     if scale is None:
         scale = 0.125
-    elif not (scale > 0 and math.isfinite(scale)):
-        raise ValueError("scale must be positive and finite")
+    elif not 2.0 ** -126 <= scale <= 2.0 ** 127:
+        raise ValueError("scale must be positive and finite (2^-126 to 2^127)")
     if out is None:
         out = q.new_empty((batch, n, heads, HEAD_DIM))
     elif _on("out", out, index).numel() != batch * n * heads * HEAD_DIM or out.dtype is not q.dtype \

@@ -786,6 +786,7 @@ typedef struct dh_kv_view {
  *               for each K/V head
  *   prefix      NULL (prefixes 0), or `prefixes` entries: of consecutive sequences,
  *               each sequences / prefixes share one.  Types and layout of V as in own
+ *   scale       positive; it and scale * log2(e) normal in fp32
  *   out         [sequences, queries, heads, 64] of q_type; lse the same without the
  *               64, or NULL
  *   run_rows    as in dh_kv_write_i8, with queries rows a sequence

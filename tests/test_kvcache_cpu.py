@@ -151,3 +151,9 @@ def test_launches():
     assert f(1, 1, 12, 12, 0, 0, 64, 3) == 1  # one kernel, no parts
     assert f(32, 1024, 12, 12, 0, 0, 1024, 3) == 2  # keys turned into f16 first
     assert 2 <= f(128, 1, 12, 12, 1, 8192, 320, 1) <= 3
+
+
+@pytest.mark.parametrize("scale", [3e38, 2.0 ** 127.9, 1e-39, 1e-45, -0.0])
+def test_scales_out_of_range(scale):
+    """Whose factor of scores, scale * log2(e), overflows, or lies below the normal floats."""
+    assert _attend(scale=scale) == ARG
