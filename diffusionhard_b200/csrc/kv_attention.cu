@@ -27,8 +27,8 @@
 //   four more softmax, a thread a row: P = 2^(s c - m) over S in TMEM; O in TMEM
 //             is rescaled only when the maximum grew by more than 2^15
 //
-// Bound by the softmax: 128 x 512 queries over 1024 16-bit keys take 302 us in a burst
-// (683 TFLOP/s; 350 us under the power cap), exponentials 47%, issue slots 47% and the
+// Bound by the softmax: 128 x 512 queries over 1024 16-bit keys take 305 us in a burst
+// (676 TFLOP/s; 350 us under the power cap), exponentials 47%, issue slots 47% and the
 // tensor pipe 34% of the time busy, with eight warps an SM that wait for one another in
 // turn.  Tried and slower:
 // exponentials of f16 pairs (360 then, where this took 338), four CTAs an SM with
@@ -73,7 +73,7 @@ struct Cfg {
     static constexpr uint32_t v_bytes = fine ? kVPitch + kTileBytes : kVPitch;
     static constexpr uint32_t threads = int8 ? 256 : 192;
     static constexpr uint32_t raw_stages = int8 ? (fine ? 2 : 4) : 0;
-    // (16 bits: 4 of K and 3 of V 305 us where 2 and 2 take 302.5)
+    // (16 bits: 4 of K and 3 of V 305 us where 2 and 2 took 302.5)
     static constexpr uint32_t k_stages = 2;
     static constexpr uint32_t v_stages = 2;
     static constexpr uint32_t q_at = 0;
@@ -115,7 +115,7 @@ DH_DEVINL float2 exp2_poly2(float2 x) {
 }
 // The maximum that P is relative to stays until it grew by more than this power of
 // two, P's largest value meanwhile (f16 ends at 2^16).  32 canvases over int8, scores
-// of a few: 245 us at 8, 237 at 15; 128 x 512 queries over 1024 16-bit keys 325 and 305.
+// of a few: 245 us at 8, 237 at 15; 128 x 512 queries over 1024 16-bit keys 325 and 305 then.
 constexpr float kMaxGrowth = 15.f;
 // f16 loses weights below 2^-25 of the one it is relative to: together up to 2^-11 of
 // all over 2^14 keys, which is a rounding of the result.  Longer parts set the maximum

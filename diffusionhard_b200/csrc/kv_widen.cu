@@ -3,7 +3,7 @@
 // The tensor-core kernel over int8 turns codes into f16 tiles as it goes, once for
 // every 128 rows: 32 canvases of 1024 queries and keys take 237 us that way and 154 us
 // over 16-bit keys.  Where every key is visited by at least four tiles of rows, the
-// codes are turned once, here, into the workspace (together 195 us).  Bound by HBM:
+// codes are turned once, here, into the workspace (together 198 us).  Bound by HBM:
 // 136 bytes in and 256 out for each position and K/V head (f16 queries: 512, see
 // FineFactor; 260 us).
 //

@@ -61,6 +61,24 @@ def test_session_generation_in_8_bits(cuda, model):
     _lib.check_device_error()
 
 
+def test_session_generation_in_a_large_cache(cuda, model):
+    """The same where lengths are a small part of the cache, of which calls show no more,
+    and as in a cache that has no more."""
+    torch = cuda
+    outs = []
+    for capacity in (1024, 640):
+        s = BlockCausalSession(model, 2, capacity, int8_kv=True)
+        s.append(_ids(torch, 2, 64, 2))
+        for n in (32, 480):
+            a, _, _, _ = s.generate(n, steps=8, seed=5, recompute=True)
+            b, _, _, _ = s.generate(n, steps=8, seed=5)
+            assert torch.equal(a, b)
+            s.append(b)
+            outs.append(b)
+    assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3])
+    _lib.check_device_error()
+
+
 def test_two_turns_in_8_bits(cuda, model):
     r = evaluate_two_turn_mdlm_session(quantized=model, samples=2, steps=16, int8_kv=True)
     assert r["aggregate"]["exact_turn_1_sequences"] == r["aggregate"]["exact_turn_2_sequences"] == 2
